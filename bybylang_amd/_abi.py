@@ -15,6 +15,9 @@ BYHIP_UNSUPPORTED = 1
 BYHIP_ERROR = -1
 
 F32, F16, BF16, MXFP4_KM = 0, 1, 2, 3
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
+NORM_RMS, NORM_LAYER = 0, 1
 
 
 class HipBackendError(RuntimeError):
@@ -38,6 +41,36 @@ class Q4WInfo(C.Structure):
                 ("groups_per_row", C.c_int), ("scale_is_f16", C.c_int),
                 ("zero_uniform", C.c_int), ("zero_value", C.c_float),
                 ("device_bytes", C.c_size_t), ("f16_safe", C.c_int)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("pages", C.c_int),
+                ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("starts", C.c_void_p), ("lens", C.c_void_p),
+                ("batch", C.c_int), ("table_stride", C.c_int), ("rows", C.c_int)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("layout", C.c_int), ("rot_dim", C.c_int), ("magnitude", C.c_float),
+                ("steps", C.c_void_p)]
+
+
+class Attn(C.Structure):
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_int),
+                ("slopes", C.c_void_p), ("prefix", C.c_void_p)]
+
+
+class KvPool(C.Structure):
+    _fields_ = [("caches", C.POINTER(KvCache)), ("n_caches", C.c_int), ("refs", C.c_void_p),
+                ("table", C.c_void_p), ("lens", C.c_void_p), ("slots", C.c_int),
+                ("table_stride", C.c_int), ("status", C.c_void_p)]
+
+
+class Norm(C.Structure):
+    _fields_ = [("kind", C.c_int), ("eps", C.c_float), ("weight", C.c_void_p), ("bias", C.c_void_p)]
 
 
 _VP, _SZ, _I, _U8P, _FP = C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p
@@ -96,6 +129,19 @@ SIGNATURES = {
     "byhip_tile_gemm_ready": (_I, [_I, _I]),
     "byhip_program_dispatch": (_I, [C.POINTER(C.c_uint32), _I, _VP, _SZ, _VP, _SZ, _VP, _SZ,
                                     _VP, _SZ, _I]),
+    "byhip_rope_steps": (_I, [_I, C.c_double, _I, C.c_double, C.c_double, C.c_double, C.c_double, _VP,
+                              C.POINTER(C.c_float)]),
+    "byhip_rope_append": (_I, [_VP, _SZ, _VP, _SZ, _VP, _SZ, _I, _I, _I, C.POINTER(Rope),
+                               C.POINTER(KvCache), C.POINTER(KvBatch), _VP, _SZ, _I]),
+    "byhip_paged_attention": (_I, [_VP, _SZ, _I, _I, C.POINTER(Attn), C.POINTER(KvCache),
+                                   C.POINTER(KvBatch), _VP, _SZ, _I]),
+    "byhip_cache_fork": (_I, [C.POINTER(KvPool), _VP, _VP, _I]),
+    "byhip_cache_free": (_I, [C.POINTER(KvPool), _VP, _I]),
+    "byhip_cache_grow": (_I, [C.POINTER(KvPool), _VP, _VP, _I]),
+    "byhip_cache_compact": (_I, [C.POINTER(KvPool), _VP, _VP]),
+    "byhip_cache_copy": (_I, [C.POINTER(KvPool), _VP, _VP, _I]),
+    "byhip_norm_block": (_I, [_VP, _SZ, _I, _I, _I, C.POINTER(Norm), _VP, _SZ, _VP, _SZ, C.c_float,
+                              _VP, _SZ, _I, C.POINTER(Norm), _VP, _SZ, _I]),
     "byhip_debug_unpack_q4": (_I, [_VP, _U8P, _FP, _FP]),
     "byhip_debug_unpack_fp4km": (_I, [_U8P, _SZ, _FP, _SZ, _I, _I, _U8P, _FP]),
     "byhip_debug_copy": (_I, [_VP, _VP, _SZ]),

@@ -1,0 +1,121 @@
+// byhip_attn.hip - attention of new rows over a paged cache: the entry point and the general kernel (gfx950).
+//
+// For row t of sequence b at position p and head h, over the keys j that the masks let it see:
+//   s_j = scale q . k_j, capped to softcap tanh(s / softcap), less slope_h |p - j|
+//   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m), m the largest s_j
+// in one pass: m, the sum and the output are kept as of the keys seen so far, and scaled down when m grows.
+#include "byhip_attn.h"
+
+namespace byhip {
+namespace {
+
+constexpr int kGeneralMaxDim = 2048;  // queries and sums of 4 waves in 64 KB of LDS
+
+// One wave per row and head, 64 keys at a time, a key per lane for the scores and a value per lane for the
+// sums. It takes heads of any size.
+template <int CT>
+__global__ __launch_bounds__(256) void attn_general(AttnArgs a) {
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const size_t item = (size_t)blockIdx.x * 4 + wave;
+    if (item >= (size_t)a.s.rows * a.heads) return;
+    const int t = __builtin_amdgcn_readfirstlane((int)(item / a.heads)), h = __builtin_amdgcn_readfirstlane((int)(item % a.heads));
+    const int b = find_sequence(a.s.starts, a.s.batch, t);
+    if (b >= a.s.batch) return;
+    const SeqInfo s = seq_info(a, b);
+    const int pos = s.first_pos + t - a.s.starts[b];
+    const int D = a.c.dim, kvh = h / (a.heads / a.c.kv_heads);
+    const float slope = a.slopes ? a.slopes[h] : 0.0f;
+    float* q = lds + wave * 2 * D;
+    float* acc = q + D;
+    for (int d = lane; d < D; d += 64) {
+        const size_t i = (size_t)t * a.q_stride + (size_t)h * D + d;
+        q[d] = a.q_dtype == BYHIP_F32 ? load1<BYHIP_F32>(a.q, i) : load1<CT>(a.q, i);
+        acc[d] = 0.0f;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave reads its lanes' queries
+    __builtin_amdgcn_wave_barrier();
+    float m = -INFINITY, sum = 0.0f;
+    for (int j0 = 0; j0 < s.len; j0 += 64) {
+        const int j = j0 + lane;
+        bool see = sees(a, s, pos, j);
+        if (__ballot(see) == 0) continue;
+        const int col = j / a.c.page_size;
+        const int page = see ? a.s.table[(size_t)b * a.s.stride + col] : -1;
+        see = page >= 0 && page < a.c.pages;
+        const size_t row = ((size_t)page * a.c.kv_heads + kvh) * a.c.page_size + (j - col * a.c.page_size);
+        float sc = -INFINITY;
+        if (see) {
+            float dot = 0.0f;
+            for (int d = 0; d < D; ++d) dot = fmaf(q[d], load1<CT>(a.c.k, row * D + d), dot);
+            sc = dot * a.scale;
+            if (a.softcap > 0.0f) sc = a.softcap * tanhf(sc / a.softcap);
+            sc -= slope * fabsf((float)(pos - j));
+        }
+        float top = sc;
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        const float grown = fmaxf(m, top);
+        const bool nan = __ballot(sc != sc) != 0;
+        if (grown == -INFINITY && !nan) continue;
+        const float base = grown == -INFINITY ? 0.0f : grown;
+        const float w = see ? expf(sc - base) : 0.0f;
+        const float fade = expf(m - base);
+        sum = sum * fade + wave_sum(w);
+        for (int d = lane; d < D; d += 64) acc[d] *= fade;
+        m = grown;
+        for (uint64_t left = __ballot(see); left; left &= left - 1) {
+            const int l = __ffsll((unsigned long long)left) - 1;
+            const float wj = __shfl(w, l, 64);
+            const size_t rj = (size_t)__shfl((long long)row, l, 64);
+            for (int d = lane; d < D; d += 64) acc[d] = fmaf(wj, load1<CT>(a.c.v, rj * D + d), acc[d]);
+        }
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int d = lane; d < D; d += 64) {
+        const float o[1] = {sum == 0.0f ? 0.0f : acc[d] * f};
+        store_vec<1>(a.out, (size_t)t * a.out_stride + (size_t)h * D + d, o, a.out_dtype);
+    }
+}
+
+void launch_general(const AttnArgs& a) {
+    if (a.c.dim > kGeneralMaxDim) unsupported("byhip: attention heads of %d values (at most %d)", a.c.dim, kGeneralMaxDim);
+    const size_t items = (size_t)a.s.rows * a.heads;
+    const dim3 grid((unsigned)((items + 3) / 4));
+    const size_t lds = (size_t)8 * a.c.dim * sizeof(float);
+    if (a.cache_dtype == BYHIP_F16) launch("attn_general", attn_general<BYHIP_F16>, grid, dim3(256), lds, a);
+    else launch("attn_general", attn_general<BYHIP_BF16>, grid, dim3(256), lds, a);
+    BYHIP_LAUNCHED("attn_general");
+}
+
+}  // namespace
+}  // namespace byhip
+
+using namespace byhip;
+
+extern "C" int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype, int heads, const byhip_attn* attn,
+                                     const byhip_kv_cache* cache, const byhip_kv_batch* batch, void* out,
+                                     size_t out_stride, int out_dtype) {
+    return guard([&] {
+        enter_compute();
+        if (!attn) fail("byhip: null attention options");
+        AttnArgs a{};
+        a.c = cache_args(cache);
+        a.s = batch_args(batch);
+        if (heads <= 0 || heads % a.c.kv_heads) fail("byhip: %d heads over %d key heads", heads, a.c.kv_heads);
+        if (q_dtype != BYHIP_F32 && (q_dtype == BYHIP_F16 || q_dtype == BYHIP_BF16) && q_dtype != cache->dtype)
+            unsupported("byhip: 16-bit queries have the cache's dtype (%d, cache %d)", q_dtype, cache->dtype);
+        const size_t width = (size_t)heads * a.c.dim;
+        check_rows(q, a.s.rows, width, q_stride, q_dtype, "queries");
+        check_rows(out, a.s.rows, width, out_stride, out_dtype, "attention output");
+        if (!(attn->softcap >= 0.0f)) fail("byhip: softcap %g", (double)attn->softcap);
+        if (attn->slopes) check_span(attn->slopes, (size_t)heads * 4, "slopes");
+        if (attn->prefix) check_span(attn->prefix, (size_t)a.s.batch * 4, "prefix lengths");
+        if (a.s.rows == 0 || a.s.batch == 0) return;
+        a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride;
+        a.q_dtype = q_dtype; a.out_dtype = out_dtype; a.cache_dtype = cache->dtype; a.heads = heads;
+        a.scale = attn->scale; a.softcap = attn->softcap; a.window = attn->window;
+        a.slopes = attn->slopes; a.prefix = attn->prefix;
+        note_device_write(out);
+        launch_general(a);
+    });
+}

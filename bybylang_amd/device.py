@@ -10,12 +10,17 @@ import ctypes as C
 import numpy as np
 
 from . import _abi
-from ._abi import BF16, F16, F32, MXFP4_KM, HipBackendError, HipUnsupported, check, load
+from ._abi import (BF16, F16, F32, MXFP4_KM, NORM_LAYER, NORM_RMS, ROPE_BASE, ROPE_HALVES,
+                   ROPE_LINEAR, ROPE_PAIRS, ROPE_PARTS, ROPE_PLAIN, HipBackendError, HipUnsupported,
+                   check, load)
 
 __all__ = ["DeviceBuffer", "Q4Weights", "init", "device_info", "synchronize", "stream",
            "q4_matmul", "fp4km_tile_gemm", "mxfp4_gemm", "f16_tile_gemm", "program_dispatch",
            "tile_gemm_ready", "F32", "F16", "BF16", "MXFP4_KM", "HipBackendError",
-           "HipUnsupported", "dtype_code", "np_dtype"]
+           "HipUnsupported", "dtype_code", "np_dtype", "KvCache", "KvBatch", "KvPool", "Rope", "Attn",
+           "Norm", "rope_steps", "rope_append", "paged_attention", "cache_fork", "cache_free",
+           "cache_grow", "cache_compact", "cache_copy", "norm_block", "ROPE_HALVES", "ROPE_PAIRS",
+           "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_BASE", "ROPE_PARTS", "NORM_RMS", "NORM_LAYER"]
 
 _NP = {F32: np.float32, F16: np.float16, BF16: np.uint16}
 
@@ -217,3 +222,120 @@ def tile_gemm_ready(f16: bool, tensor_core: bool = True) -> bool:
     if rc < 0:
         check(rc, "byhip_tile_gemm_ready")
     return rc == 1
+
+
+# ── attention over a paged cache ────────────────────────────────────────────────────────────
+#
+# The descriptors below are made once per cache, batch layout or option set; they keep the buffers they
+# point into alive. Buffers are anything with a `ptr` (DeviceBuffer, or a caller's own device memory).
+
+
+def _ptr(b):
+    return None if b is None else b.ptr
+
+
+class _Struct:
+    def __init__(self, value, *keep):
+        self.value, self.ref, self.keep = value, C.byref(value), keep
+
+
+class KvCache(_Struct):
+    """One layer's cache (byhip_kv_cache): k and v [pages][kv_heads][page_size][head_dim]."""
+
+    def __init__(self, k, v, dtype: int, pages: int, page_size: int, kv_heads: int, head_dim: int):
+        super().__init__(_abi.KvCache(k.ptr, v.ptr, dtype, pages, page_size, kv_heads, head_dim), k, v)
+
+
+class KvBatch(_Struct):
+    """The sequences of a call (byhip_kv_batch): int32 page tables [batch][table_stride], row starts
+    [batch + 1] and lengths [batch] on the device."""
+
+    def __init__(self, table, table_stride: int, starts, lens, batch: int, rows: int):
+        super().__init__(_abi.KvBatch(table.ptr, starts.ptr, lens.ptr, batch, table_stride, rows),
+                         table, starts, lens)
+
+
+class KvPool(_Struct):
+    """The layers' caches with their shared page table, reference counts and lengths (byhip_kv_pool)."""
+
+    def __init__(self, caches, refs, table, table_stride: int, lens, slots: int, status):
+        arr = (_abi.KvCache * len(caches))(*[c.value for c in caches])
+        super().__init__(_abi.KvPool(arr, len(caches), refs.ptr, table.ptr, lens.ptr, slots, table_stride,
+                                     status.ptr), arr, caches, refs, table, lens, status)
+
+
+class Rope(_Struct):
+    """Rotary positions (byhip_rope); `steps` holds rope_steps' uint64 values on the device."""
+
+    def __init__(self, layout: int, rot_dim: int, steps, magnitude: float = 1.0):
+        super().__init__(_abi.Rope(layout, rot_dim, magnitude, steps.ptr), steps)
+
+
+class Attn(_Struct):
+    """How scores become weights (byhip_attn)."""
+
+    def __init__(self, scale: float, softcap: float = 0.0, window: int = 0, slopes=None, prefix=None):
+        super().__init__(_abi.Attn(scale, softcap, window, _ptr(slopes), _ptr(prefix)), slopes, prefix)
+
+
+class Norm(_Struct):
+    """A norm's kind, eps, weight and bias (byhip_norm)."""
+
+    def __init__(self, kind: int, eps: float, weight=None, bias=None):
+        super().__init__(_abi.Norm(kind, eps, _ptr(weight), _ptr(bias)), weight, bias)
+
+
+def _ref(s):
+    return None if s is None else s.ref
+
+
+def rope_steps(rot_dim: int, base: float = 10000.0, scaling: int = ROPE_PLAIN, factor: float = 1.0,
+               original_len: float = 0.0, slow: float = 1.0, fast: float = 32.0):
+    """(steps [rot_dim / 2] uint64, magnitude) of byhip_rope_steps, on the host."""
+    steps = np.zeros(max(rot_dim // 2, 1), np.uint64)
+    mag = C.c_float(1.0)
+    check(load().byhip_rope_steps(rot_dim, base, scaling, factor, original_len, slow, fast,
+                                  steps.ctypes.data, C.byref(mag)), "byhip_rope_steps")
+    return steps[:rot_dim // 2], mag.value
+
+
+def rope_append(q, q_stride: int, k, k_stride: int, v, v_stride: int, x_dtype: int, heads: int,
+                rope: Rope | None, cache: KvCache | None, batch: KvBatch, q_out, q_out_stride: int,
+                q_out_dtype: int, head_dim: int = 0) -> None:
+    check(load().byhip_rope_append(q.ptr, q_stride, _ptr(k), k_stride, _ptr(v), v_stride, x_dtype, heads,
+                                   head_dim, _ref(rope), _ref(cache), batch.ref, q_out.ptr, q_out_stride,
+                                   q_out_dtype), "byhip_rope_append")
+
+
+def paged_attention(q, q_stride: int, q_dtype: int, heads: int, attn: Attn, cache: KvCache,
+                    batch: KvBatch, out, out_stride: int, out_dtype: int) -> None:
+    check(load().byhip_paged_attention(q.ptr, q_stride, q_dtype, heads, attn.ref, cache.ref, batch.ref,
+                                       out.ptr, out_stride, out_dtype), "byhip_paged_attention")
+
+
+def cache_fork(pool: KvPool, parents, rows, n: int) -> None:
+    check(load().byhip_cache_fork(pool.ref, parents.ptr, rows.ptr, n), "byhip_cache_fork")
+
+
+def cache_free(pool: KvPool, rows, n: int) -> None:
+    check(load().byhip_cache_free(pool.ref, rows.ptr, n), "byhip_cache_free")
+
+
+def cache_grow(pool: KvPool, rows, add, n: int) -> None:
+    check(load().byhip_cache_grow(pool.ref, rows.ptr, add.ptr, n), "byhip_cache_grow")
+
+
+def cache_compact(pool: KvPool, table_out=None, refs_out=None) -> None:
+    check(load().byhip_cache_compact(pool.ref, _ptr(table_out), _ptr(refs_out)), "byhip_cache_compact")
+
+
+def cache_copy(pool: KvPool, src, dst, n: int) -> None:
+    check(load().byhip_cache_copy(pool.ref, src.ptr, dst.ptr, n), "byhip_cache_copy")
+
+
+def norm_block(x, x_stride: int, x_dtype: int, M: int, N: int, post: Norm | None, gate, gate_stride: int,
+               res, res_stride: int, res_scale: float, h, h_stride: int, h_dtype: int, pre: Norm | None,
+               y, y_stride: int, y_dtype: int) -> None:
+    check(load().byhip_norm_block(x.ptr, x_stride, x_dtype, M, N, _ref(post), _ptr(gate), gate_stride,
+                                  _ptr(res), res_stride, res_scale, _ptr(h), h_stride, h_dtype, _ref(pre),
+                                  _ptr(y), y_stride, y_dtype), "byhip_norm_block")

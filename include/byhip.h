@@ -286,6 +286,142 @@ int byhip_program_dispatch(const uint32_t* words, int n_words, void* mem, size_t
                            const void* u8, size_t u8_len, const void* lut, size_t lut_len,
                            const void* input, size_t input_len, int rows);
 
+/* ── Attention over a paged cache ─────────────────────────────────────────────────────────────
+ *
+ * The half of a decoder layer between the QKV and the O projection, and the norms around it, with no
+ * counterpart in the reference's backends. Everything lives on the device: the cache, the page tables,
+ * the lengths and the reference counts, so a step that grows, forks or frees sequences can be recorded
+ * with the calls that use them. Kernels check every page id, row and position they take from device memory
+ * against the sizes given here and leave out what lies outside. */
+
+/* One layer's cache, in the caller's memory: keys and values each [pages][kv_heads][page_size][head_dim],
+ * dtype BYHIP_F16 or BYHIP_BF16. */
+typedef struct byhip_kv_cache {
+    void* k;
+    void* v;
+    int dtype;
+    int pages, page_size, kv_heads, head_dim;
+} byhip_kv_cache;
+
+/* The sequences of a call. Sequence b holds lens[b] tokens, this call's own among them, in pages
+ * table[b * table_stride ..]; this call's rows starts[b] .. starts[b + 1] - 1 are its last tokens, so row i of
+ * them has position lens[b] - (starts[b + 1] - starts[b]) + i. Device arrays; starts[0] = 0, ascending,
+ * at most `rows`. */
+typedef struct byhip_kv_batch {
+    const int* table;
+    const int* starts;  /* [batch + 1] */
+    const int* lens;    /* [batch] */
+    int batch, table_stride, rows;
+} byhip_kv_batch;
+
+enum byhip_rope_layout {
+    BYHIP_ROPE_HALVES = 0,  /* value i turns with value i + rot_dim / 2 */
+    BYHIP_ROPE_PAIRS = 1    /* value 2 i turns with value 2 i + 1 */
+};
+enum byhip_rope_scaling {
+    BYHIP_ROPE_PLAIN = 0,   /* turns per position base^(-2 i / rot_dim) / (2 pi) */
+    BYHIP_ROPE_LINEAR = 1,  /* the same over `factor` (position interpolation) */
+    BYHIP_ROPE_BASE = 2,    /* base * factor^(rot_dim / (rot_dim - 2)): the slowest pair slows by `factor` */
+    BYHIP_ROPE_PARTS = 3    /* pairs that turn fewer than `slow` times in original_len positions slow by
+                             * `factor`, those of more than `fast` turns stay, a linear ramp between;
+                             * magnitude 0.1 ln(factor) + 1 */
+};
+/* Rotary positions of the first rot_dim values of a head (even; the others pass through): steps[i] (device,
+ * rot_dim / 2) is pair i's turn per position in units of 2^-64 of a whole turn, so that position * step
+ * modulo 2^64 is the angle at any position without rounding. Rotated values are multiplied by `magnitude`. */
+typedef struct byhip_rope {
+    int layout;
+    int rot_dim;
+    float magnitude;
+    const uint64_t* steps;
+} byhip_rope;
+
+/* Fills steps[rot_dim / 2] and *magnitude (host memory) for a base and scaling. Needs no device. */
+int byhip_rope_steps(int rot_dim, double base, int scaling, double factor, double original_len, double slow,
+                     double fast, uint64_t* steps, float* magnitude);
+
+/* Rotary positions and the cache's append in one pass: rows of `heads` query heads, kv_heads key heads and
+ * kv_heads value heads (x_dtype F32 / F16 / BF16, row strides in elements, so the three may lie in one QKV
+ * buffer). The rotated queries go to q_out; rotated keys and values go to their positions in the
+ * cache's pages, rounded once to its dtype. rope NULL: no rotation. cache NULL: queries only (k, v unused;
+ * head_dim then comes from `head_dim`, which otherwise must be 0 or the cache's). q_out may be q itself where
+ * the types and strides agree. */
+int byhip_rope_append(const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v,
+                      size_t v_stride, int x_dtype, int heads, int head_dim, const byhip_rope* rope,
+                      const byhip_kv_cache* cache, const byhip_kv_batch* batch, void* q_out,
+                      size_t q_out_stride, int q_out_dtype);
+
+/* How scores become weights: s = scale * q . k; softcap > 0: s = softcap * tanh(s / softcap); slopes
+ * (device, [heads], or NULL): s -= slopes[head] * |position - j|. Key j < lens[b] is seen from position p where
+ * j <= p and (window <= 0 or p - j < window), or j < prefix[b] (device, [batch], or NULL). */
+typedef struct byhip_attn {
+    float scale;
+    float softcap;
+    int window;
+    const float* slopes;
+    const int* prefix;
+} byhip_attn;
+
+/* Attention of the call's rows (a token each, a chunk, or any mixture) over the cache: q and out are rows of
+ * `heads` heads (heads % kv_heads == 0, neighbouring heads share a key head). Rows that see no key, or
+ * whose scores are all -inf, give zeros; what the masks hide has no influence, whatever it holds.
+ * q_dtype F32, or the cache's dtype; out_dtype F32, F16 or BF16. fp32 on either side keeps fp32's
+ * precision throughout; with 16-bit q and out the weights are rounded once to the cache's dtype before they
+ * multiply the values. Sums and softmax statistics are fp32. */
+int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype, int heads, const byhip_attn* attn,
+                          const byhip_kv_cache* cache, const byhip_kv_batch* batch, void* out,
+                          size_t out_stride, int out_dtype);
+
+/* The pages of all layers' caches (a host array of descriptors of equal geometry), which share one page table:
+ * sequence slot r holds lens[r] tokens in pages table[r * table_stride ..]; refs[p] counts the slots that
+ * hold page p (0: free). All device arrays. status (device, 4 ints, cleared by the caller) adds up over
+ * calls: [0] slots refused for want of pages or table columns, [1] entries refused as invalid (a slot or parent out of
+ * range or named twice), [2] pages copied, [3] pages newly taken. A refused entry changes nothing else. */
+typedef struct byhip_kv_pool {
+    const byhip_kv_cache* caches;
+    int n_caches;
+    int* refs;
+    int* table;
+    int* lens;
+    int slots, table_stride;
+    int* status;
+} byhip_kv_pool;
+
+/* Slot rows[i] becomes a fork of slot parents[i]: what it held is released, the parent's pages are shared. A
+ * parent that is itself among `rows` is refused. n <= 1024. */
+int byhip_cache_fork(const byhip_kv_pool* pool, const int* parents, const int* rows, int n);
+/* Slots rows[i] release their pages; their lengths become 0. n <= 1024. */
+int byhip_cache_free(const byhip_kv_pool* pool, const int* rows, int n);
+/* Slot rows[i] gets room for add[i] >= 0 more tokens and counts them in lens: the lowest free pages, in the
+ * order of i. A partly filled last page that others still hold is copied first, so that a slot only ever
+ * appends to pages of its own. Slots past the first that does not fit are refused. n <= 1024. */
+int byhip_cache_grow(const byhip_kv_pool* pool, const int* rows, const int* add, int n);
+/* Moves live pages to the front: the i-th free page below the number of live ones receives the i-th live page
+ * above it. refs and all tables follow; refs_out / table_out (or NULL: in place) receive them. */
+int byhip_cache_compact(const byhip_kv_pool* pool, int* table_out, int* refs_out);
+/* Page src[i] of every layer is copied to page dst[i] (device arrays; no dst twice or among src; pairs
+ * outside the pool are left out). */
+int byhip_cache_copy(const byhip_kv_pool* pool, const int* src, const int* dst, int n);
+
+enum byhip_norm_kind { BYHIP_NORM_RMS = 0, BYHIP_NORM_LAYER = 1 };
+/* v / sqrt(mean(v^2) + eps), or (v - mean) / sqrt(variance + eps); then * weight + bias (device, fp32, each
+ * may be NULL). */
+typedef struct byhip_norm {
+    int kind;
+    float eps;
+    const float* weight;
+    const float* bias;
+} byhip_norm;
+
+/* Between two blocks, M rows of N values: h = res_scale * res + gate * post(x), y = pre(h). post NULL: x
+ * itself; gate (fp32, gate_stride between rows, 0: one row for all) NULL: 1; res NULL: 0; h NULL: not
+ * stored; pre NULL: no y. res and h have h_dtype and may be the same rows. y is formed from h before its rounding.
+ * Row strides in elements. */
+int byhip_norm_block(const void* x, size_t x_stride, int x_dtype, int M, int N, const byhip_norm* post,
+                     const float* gate, size_t gate_stride, const void* res, size_t res_stride,
+                     float res_scale, void* h, size_t h_stride, int h_dtype, const byhip_norm* pre, void* y,
+                     size_t y_stride, int y_dtype);
+
 /* ── Debug (bit-exact unpack checks) ──────────────────────────────────────────────────────── */
 
 /* Unpacks resident Q4 weights on the device into host arrays: codes [N*K] (0..15), scales and
