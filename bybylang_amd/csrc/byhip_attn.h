@@ -1,4 +1,5 @@
-// byhip_attn.h - arguments and masks shared by the kernels of byhip_paged_attention.
+// byhip_attn.h - what the kernels of byhip_paged_attention share: arguments, masks, the division of the work
+// among blocks and the layout of partial results.
 #pragma once
 
 #include "byhip_cache.h"
@@ -15,24 +16,168 @@ struct AttnArgs {
     const int* prefix;
     CacheArgs c;
     BatchArgs s;
+    int group;       // query heads per key head
+    int q_vec;       // query rows can be read 16 bytes at a time
+    int out_vec;     // output rows can be written 4 values at a time
+    int min_rows, max_rows;  // rows (tokens x group) of the sequences this launch takes
+    float* part;     // partial results
+    int4* joins;     // one description per block
 };
 
-// Keys of sequence b that exist, and how many of them every row sees (the open prefix).
+// Sequence b as a launch sees it.
 struct SeqInfo {
-    int len, first_pos, prefix;  // first_pos: position of the call's first row
+    int len, first_pos, prefix;  // keys that can be read; position of the first row; keys that every row sees
+    int rows;                    // tokens x group, 0 when the launch does not take the sequence
 };
 
 __device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, int b) {
     SeqInfo s;
-    const int len = a.s.lens[b];
-    s.first_pos = len - (a.s.starts[b + 1] - a.s.starts[b]);
-    s.len = seq_len(a.s, a.c, b);
-    s.prefix = a.prefix ? min(a.prefix[b], s.len) : 0;
+    const int n = a.s.starts[b + 1] - a.s.starts[b];
+    s.first_pos = a.s.lens[b] - n;
+    s.len = max(0, seq_len(a.s, a.c, b));
+    s.prefix = a.prefix ? max(0, min(a.prefix[b], s.len)) : 0;
+    const long long rows = (long long)n * a.group;
+    s.rows = rows < a.min_rows || rows > a.max_rows ? 0 : (int)rows;
     return s;
 }
 
 __device__ __forceinline__ bool sees(const AttnArgs& a, const SeqInfo& s, int pos, int j) {
     return j < s.len && ((j <= pos && (a.window <= 0 || pos - j < a.window)) || j < s.prefix);
+}
+
+// The same for 32 keys j0 .. as bits, of those `there`. Formed without branches.
+__device__ __forceinline__ uint32_t low_bits(int n) { return (uint32_t)((1ull << max(0, min(n, 32))) - 1); }
+__device__ __forceinline__ uint32_t seen_keys(const AttnArgs& a, const SeqInfo& s, int pos, int j0, uint32_t there) {
+    const uint32_t gone = a.window > 0 ? low_bits(pos - a.window + 1 - j0) : 0u;
+    return there & ((low_bits(pos + 1 - j0) & ~gone) | low_bits(s.prefix - j0));
+}
+
+// The key tiles (of T keys) that rows at positions p0 .. p1 need: first those of the open prefix below
+// the window, then those from the window's start to the last key. At least one, so that every row is written.
+template <int T>
+struct TileRange {
+    int prefix_tiles, start, tiles;
+    __device__ __forceinline__ TileRange(const AttnArgs& a, const SeqInfo& s, int p0, int p1) {
+        start = a.window > 0 ? max(0, p0 - a.window + 1) / T * T : 0;
+        const int end = max(0, max(min(s.len, p1 + 1), s.prefix));
+        start = min(start, end / T * T);
+        prefix_tiles = min((s.prefix + T - 1) / T, start / T);
+        tiles = max(1, prefix_tiles + (end - start + T - 1) / T);
+    }
+    __device__ __forceinline__ int key(int t) const { return t < prefix_tiles ? t * T : start + (t - prefix_tiles) * T; }
+};
+
+constexpr int kAttnBatch = 1024;  // sequences per launch: their prefix sums lie in LDS
+
+// A block whose share ends inside an item leaves {last block of the item, sequence, row tile, head}; .x = 0: none.
+// Slot 2 w holds block w's part of an item that began before it, slot 2 w + 1 its part of one that goes on after it: R x DIM
+// unnormalised sums, then R maxima (log2) and R sums of weights.
+template <int R, int DIM>
+__device__ __forceinline__ float* part_slot(float* part, int slot) {
+    return part + (size_t)slot * R * (DIM + 2);
+}
+
+// 1 when a launch takes these arguments.
+bool attn_rows_takes(const AttnArgs& a);
+void launch_attn_rows(AttnArgs a);
+
+// Joins the parts of items of R rows that several blocks worked on. Grid: blocks x row groups; 16 lanes hold a row's
+// values, 16 groups of lanes walk over its parts.
+template <int R, int DIM>
+__global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
+    constexpr int V = DIM / 16;
+    const int w = blockIdx.x;
+    const int4 d = a.joins[w];
+    if (d.x == 0) return;
+    __shared__ float red[16][DIM + 2];
+    const int b = d.y, rt = d.z, h = d.w;
+    const int group = threadIdx.x >> 4, col = (threadIdx.x & 15) * V;
+    const SeqInfo s = seq_info(a, b);
+    const int rows = min(R, s.rows - rt * R), parts = d.x - w + 1;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        float acc[V] = {}, m = -INFINITY, l = 0.0f;
+        for (int i = group; i < parts; i += 16) {
+            const float* p = part_slot<R, DIM>(a.part, i == 0 ? 2 * w + 1 : 2 * (w + i));
+            const float pm = p[R * DIM + r], pl = p[R * DIM + R + r];
+            float x[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(p + r * DIM + col + e);
+                x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
+            }
+            const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
+            const float fo = __builtin_amdgcn_exp2f(m - base), fn = __builtin_amdgcn_exp2f(pm - base);
+            l = l * fo + pl * fn;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] = acc[e] * fo + x[e] * fn;
+            m = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) red[group][col + e] = acc[e];
+        if (col == 0) { red[group][DIM] = m; red[group][DIM + 1] = l; }
+        __syncthreads();
+        if (threadIdx.x < DIM && (int)threadIdx.x < a.c.dim) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, red[i][DIM]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f, o = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float f = __builtin_amdgcn_exp2f(red[i][DIM] - base);
+                sum += red[i][DIM + 1] * f;
+                o += red[i][threadIdx.x] * f;
+            }
+            const float v[1] = {sum == 0.0f ? 0.0f : o / sum};
+            const int q = rt * R + r, t = a.s.starts[b] + q / a.group;
+            store_vec<1>(a.out, (size_t)t * a.out_stride + (size_t)(h * a.group + q % a.group) * a.c.dim + threadIdx.x, v, a.out_dtype);
+        }
+    }
+}
+
+// The cache's 16-bit type in registers and the matrix instructions on it.
+template <int CT> struct Half8;
+template <> struct Half8<BYHIP_F16> {
+    typedef _Float16 vec __attribute__((ext_vector_type(8)));
+    typedef _Float16 one;
+};
+template <> struct Half8<BYHIP_BF16> {
+    typedef __bf16 vec __attribute__((ext_vector_type(8)));
+    typedef __bf16 one;
+};
+typedef float f16v __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f4 mfma16(Half8<BYHIP_F16>::vec x, Half8<BYHIP_F16>::vec y, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mfma16(Half8<BYHIP_BF16>::vec x, Half8<BYHIP_BF16>::vec y, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+__device__ __forceinline__ f16v mfma32(Half8<BYHIP_F16>::vec x, Half8<BYHIP_F16>::vec y, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0); }
+__device__ __forceinline__ f16v mfma32(Half8<BYHIP_BF16>::vec x, Half8<BYHIP_BF16>::vec y, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0); }
+
+// x as NP terms of the cache's type, each the rounding of what the ones before it leave.
+template <int CT, int NP>
+__device__ __forceinline__ void split_terms(float x, typename Half8<CT>::one (&t)[NP]) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        t[p] = (typename Half8<CT>::one)x;
+        if (p + 1 < NP) x -= (float)t[p];
+    }
+}
+
+constexpr float kLog2e = 1.44269504f;
+
+// tanh. Near 0 its Taylor sum (to y^15 below 1/2: remainder under 2e-8 of it), else 1 - 2 / (1 + e^2y).
+template <bool PRECISE>
+__device__ __forceinline__ float soft_tanh(float y) {
+    const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
+    const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+    if constexpr (!PRECISE) return far;
+    const float z = y * y;
+    float s = fmaf(z, -1.45583439e-3f, 3.59212804e-3f);
+    s = fmaf(z, s, -8.86323553e-3f);
+    s = fmaf(z, s, 2.18694885e-2f);
+    s = fmaf(z, s, -5.39682540e-2f);
+    s = fmaf(z, s, 1.33333333e-1f);
+    s = fmaf(z, s, -3.33333333e-1f);
+    return fabsf(y) < 0.5f ? fmaf(y * z, s, y) : far;
 }
 
 }  // namespace byhip

@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256) void attn_general(AttnArgs a) {
     if (b >= a.s.batch) return;
     const SeqInfo s = seq_info(a, b);
     const int pos = s.first_pos + t - a.s.starts[b];
-    const int D = a.c.dim, kvh = h / (a.heads / a.c.kv_heads);
+    const int D = a.c.dim, kvh = h / a.group;
     const float slope = a.slopes ? a.slopes[h] : 0.0f;
     float* q = lds + wave * 2 * D;
     float* acc = q + D;
@@ -115,7 +115,13 @@ extern "C" int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype
         a.q_dtype = q_dtype; a.out_dtype = out_dtype; a.cache_dtype = cache->dtype; a.heads = heads;
         a.scale = attn->scale; a.softcap = attn->softcap; a.window = attn->window;
         a.slopes = attn->slopes; a.prefix = attn->prefix;
+        a.group = heads / a.c.kv_heads;
+        a.min_rows = 1;
+        a.max_rows = 0x7FFFFFFF;
+        a.q_vec = q_stride * dtype_bytes(q_dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+        a.out_vec = aligned4(out, out_stride, out_dtype);
         note_device_write(out);
-        launch_general(a);
+        if (attn_rows_takes(a)) launch_attn_rows(a);
+        else launch_general(a);
     });
 }

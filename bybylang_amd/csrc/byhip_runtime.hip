@@ -30,6 +30,7 @@ struct State {
     hipDeviceProp_t prop{};
     std::unordered_map<const void*, Alloc> allocs;
     void* workspace = nullptr;  // kWorkspaceBytes, allocated by byhip_init, kept until exit
+    void* attn_workspace = nullptr;  // kAttnWorkspaceBytes, the same
     // session
     bool session_open = false;
     std::vector<void*> deferred_frees;
@@ -122,6 +123,7 @@ void enter_compute() {
 hipStream_t stream() { return st().stream; }
 int compute_units() { return st().prop.multiProcessorCount; }
 void* workspace() { return st().workspace; }
+void* attn_workspace() { return st().attn_workspace; }
 bool session_open() { return st().session_open || st().recording; }
 bool keeping_launches() { return st().recording && st().direct_open; }
 void keep_launch(Relaunch l) { st().kept.push_back(std::move(l)); }
@@ -277,8 +279,9 @@ int byhip_init(int device) {
         BYHIP_HIP(hipDeviceGetAttribute(&khz, hipDeviceAttributeWallClockRate, device));
         s.realtime_hz = khz * 1e3;
         BYHIP_HIP(hipMalloc(&s.workspace, kWorkspaceBytes));
+        BYHIP_HIP(hipMalloc(&s.attn_workspace, kAttnWorkspaceBytes));
         BYHIP_HIP(hipMalloc(reinterpret_cast<void**>(&s.flags), 64 * sizeof(int)));
-        g_alloc_count.fetch_add(2);
+        g_alloc_count.fetch_add(3);
         BYHIP_HIP(hipHostMalloc(reinterpret_cast<void**>(&s.gate), sizeof(int), hipHostMallocCoherent));
         *s.gate = 0;
         static_scratch_setup(device);
