@@ -67,6 +67,7 @@ struct TileRange {
     __device__ __forceinline__ int key(int t) const { return t < prefix_tiles ? t * T : start + (t - prefix_tiles) * T; }
 };
 
+constexpr size_t kAttnJoinBytes = 65536;  // at the start of the workspace
 constexpr int kAttnBatch = 1024;  // sequences per launch: their prefix sums lie in LDS
 
 // A block whose share ends inside an item leaves {last block of the item, sequence, row tile, head}; .x = 0: none.
@@ -77,9 +78,19 @@ __device__ __forceinline__ float* part_slot(float* part, int slot) {
     return part + (size_t)slot * R * (DIM + 2);
 }
 
-// 1 when a launch takes these arguments.
-bool attn_rows_takes(const AttnArgs& a);
-void launch_attn_rows(AttnArgs a);
+// The launches, per type of the cache; `precise`: fp32 queries or outputs.
+void launch_attn_rows_f16(const AttnArgs& a, bool precise);
+void launch_attn_rows_bf16(const AttnArgs& a, bool precise);
+void launch_attn_chunk_f16(const AttnArgs& a, bool precise);
+void launch_attn_chunk_bf16(const AttnArgs& a, bool precise);
+
+// What block w leaves when its share ends inside an item it began: the block that holds the item's last unit.
+__device__ __forceinline__ int4 join_of(long long last, long long blocks, long long total, int b, int rt, int h) {
+    int w = (int)((last * blocks + blocks - 1) / total);
+    while ((long long)w * total / blocks > last) --w;
+    while ((long long)(w + 1) * total / blocks <= last) ++w;
+    return make_int4(w, b, rt, h);
+}
 
 // Joins the parts of items of R rows that several blocks worked on. Grid: blocks x row groups; 16 lanes hold a row's
 // values, 16 groups of lanes walk over its parts.

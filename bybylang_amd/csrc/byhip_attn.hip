@@ -4,6 +4,8 @@
 //   s_j = scale q . k_j, capped to softcap tanh(s / softcap), less slope_h |p - j|
 //   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m), m the largest s_j
 // in one pass: m, the sum and the output are kept as of the keys seen so far, and scaled down when m grows.
+#include <algorithm>
+
 #include "byhip_attn.h"
 
 namespace byhip {
@@ -87,6 +89,40 @@ void launch_general(const AttnArgs& a) {
     BYHIP_LAUNCHED("attn_general");
 }
 
+// Rows per key head from which attn_chunk reads a sequence: attn_rows reads its keys once per 16 rows.
+constexpr int kChunkRows = 33;
+
+// Whether the kernels on matrix instructions take the cache: whole 16-byte pieces of a head, cache rows that 32 bits count.
+bool takes(const AttnArgs& a) {
+    return a.c.dim % 8 == 0 && a.c.dim <= 256 && reinterpret_cast<uintptr_t>(a.c.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.c.v) % 16 == 0 &&
+           (double)a.c.pages * a.c.kv_heads * a.c.page_size < 4294967295.0;
+}
+
+void launch_tiled(AttnArgs a) {
+    a.joins = static_cast<int4*>(attn_workspace());
+    a.part = reinterpret_cast<float*>(static_cast<char*>(attn_workspace()) + kAttnJoinBytes);
+    const bool precise = a.q_dtype == BYHIP_F32 || a.out_dtype == BYHIP_F32, f16 = a.cache_dtype == BYHIP_F16;
+    // The lengths are on the device: one sequence has all rows; as many rows as sequences are decoding; else
+    // sequences of few rows and of many go to a launch each, which passes over the others.
+    const long long rows = (long long)a.s.rows * a.group;
+    const bool one = a.s.batch == 1;
+    const bool few = !one || rows < kChunkRows, many = one ? rows >= kChunkRows : a.s.rows > a.s.batch;
+    const AttnArgs whole = a;
+    for (int b0 = 0; b0 < whole.s.batch; b0 += kAttnBatch) {
+        a.s.table = whole.s.table + (size_t)b0 * whole.s.stride;
+        a.s.starts = whole.s.starts + b0;
+        a.s.lens = whole.s.lens + b0;
+        a.s.batch = std::min(kAttnBatch, whole.s.batch - b0);
+        a.prefix = whole.prefix ? whole.prefix + b0 : nullptr;
+        a.min_rows = 1;
+        a.max_rows = many ? kChunkRows - 1 : 0x7FFFFFFF;
+        if (few) (f16 ? launch_attn_rows_f16 : launch_attn_rows_bf16)(a, precise);
+        a.min_rows = few ? kChunkRows : 1;
+        a.max_rows = 0x7FFFFFFF;
+        if (many) (f16 ? launch_attn_chunk_f16 : launch_attn_chunk_bf16)(a, precise);
+    }
+}
+
 }  // namespace
 }  // namespace byhip
 
@@ -116,12 +152,11 @@ extern "C" int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype
         a.scale = attn->scale; a.softcap = attn->softcap; a.window = attn->window;
         a.slopes = attn->slopes; a.prefix = attn->prefix;
         a.group = heads / a.c.kv_heads;
-        a.min_rows = 1;
         a.max_rows = 0x7FFFFFFF;
         a.q_vec = q_stride * dtype_bytes(q_dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
         a.out_vec = aligned4(out, out_stride, out_dtype);
         note_device_write(out);
-        if (attn_rows_takes(a)) launch_attn_rows(a);
+        if (takes(a)) launch_tiled(a);
         else launch_general(a);
     });
 }

@@ -1,4 +1,4 @@
-// byhip_attn_rows.hip - attention of few rows per sequence over a paged cache: decoding (gfx950).
+// byhip_attn_rows.h - attention of few rows per sequence over a paged cache: decoding (gfx950).
 //
 // A sequence's rows that share a key head (tokens x group) form tiles of 16. A wave takes 32 keys at a
 // time, straight from memory into the registers the matrix instructions read:
@@ -18,6 +18,8 @@
 //
 // fp32 queries or outputs: the queries as two fp16 terms (scaled per row to fp16's range) or three bf16 terms, the
 // weights likewise, one matrix instruction per term; the memory still bounds it.
+#pragma once
+
 #include "byhip_attn.h"
 
 namespace byhip {
@@ -420,12 +422,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
                 }
             }
         }
-        if (begins && !ends) {  // the blocks up to the item's last unit hold the rest
-            const long long last = u - t0 + range.tiles - 1;
-            join = make_int4((int)((last * blocks + blocks - 1) / total), b, rt, h);
-            while ((long long)join.x * total / blocks > last) --join.x;
-            while ((long long)(join.x + 1) * total / blocks <= last) ++join.x;
-        }
+        if (begins && !ends) join = join_of(u - t0 + range.tiles - 1, blocks, total, b, rt, h);
         u += t1 - t0;
     }
     if (tid == 0) a.joins[w] = join;
@@ -441,42 +438,12 @@ void launch_rows(const AttnArgs& a, unsigned blocks) {
 }
 
 template <int CT, int NP>
-void launch_rows_dim(const AttnArgs& a, unsigned blocks) {
+void launch_rows_dim(const AttnArgs& a) {
+    const unsigned blocks = (unsigned)compute_units() * 2;  // two are resident per CU
     if (a.c.dim <= 64) launch_rows<CT, NP, 64>(a, blocks);
     else if (a.c.dim <= 128) launch_rows<CT, NP, 128>(a, blocks);
     else launch_rows<CT, NP, 256>(a, blocks);
 }
 
 }  // namespace
-
-bool attn_rows_takes(const AttnArgs& a) {
-    // whole 16-byte pieces of a head, and cache rows that 32 bits count
-    return a.c.dim % 8 == 0 && a.c.dim <= 256 && reinterpret_cast<uintptr_t>(a.c.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.c.v) % 16 == 0 &&
-           (double)a.c.pages * a.c.kv_heads * a.c.page_size < 4294967295.0;
-}
-
-void launch_attn_rows(AttnArgs a) {
-    // two blocks per CU are resident
-    const unsigned blocks = (unsigned)compute_units() * 2;
-    a.joins = static_cast<int4*>(attn_workspace());
-    a.part = reinterpret_cast<float*>(a.joins + 4096);
-    const bool precise = a.q_dtype == BYHIP_F32 || a.out_dtype == BYHIP_F32;
-    const BatchArgs whole = a.s;
-    const int* prefix = a.prefix;
-    for (int b0 = 0; b0 < whole.batch; b0 += kAttnBatch) {
-        a.s.table = whole.table + (size_t)b0 * whole.stride;
-        a.s.starts = whole.starts + b0;
-        a.s.lens = whole.lens + b0;
-        a.s.batch = whole.batch - b0 < kAttnBatch ? whole.batch - b0 : kAttnBatch;
-        a.prefix = prefix ? prefix + b0 : nullptr;
-        if (a.cache_dtype == BYHIP_F16) {
-            if (precise) launch_rows_dim<BYHIP_F16, 2>(a, blocks);
-            else launch_rows_dim<BYHIP_F16, 1>(a, blocks);
-        } else {
-            if (precise) launch_rows_dim<BYHIP_BF16, 3>(a, blocks);
-            else launch_rows_dim<BYHIP_BF16, 1>(a, blocks);
-        }
-    }
-}
-
 }  // namespace byhip
