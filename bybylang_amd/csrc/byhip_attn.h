@@ -19,10 +19,18 @@ struct AttnArgs {
     int group;       // query heads per key head
     int q_vec;       // query rows can be read 16 bytes at a time
     int out_vec;     // output rows can be written 4 values at a time
+    uint32_t page_mul;   // key / page_size as a product's high bits
+    int page_shift;      // -1: pages of one key
     int min_rows, max_rows;  // rows (tokens x group) of the sequences this launch takes
     float* part;     // partial results
     int4* joins;     // one description per block
 };
+
+// Column of key j (below 2^31) in its table row. With l = ceil(log2(page size)) and page_mul = ceil(2^(31 + l) / page size),
+// the product's error is under j / 2^(31 + l) < 1 / page size.
+__device__ __forceinline__ int page_col(const AttnArgs& a, int j) {
+    return a.page_shift < 0 ? j : (int)(__umulhi((uint32_t)j, a.page_mul) >> a.page_shift);
+}
 
 // Sequence b as a launch sees it.
 struct SeqInfo {
@@ -92,57 +100,87 @@ __device__ __forceinline__ int4 join_of(long long last, long long blocks, long l
     return make_int4(w, b, rt, h);
 }
 
-// Joins the parts of items of R rows that several blocks worked on. Grid: blocks x row groups; 16 lanes hold a row's
-// values, 16 groups of lanes walk over its parts.
-template <int R, int DIM>
+// Joins the parts of items of R rows that several blocks worked on. Grid: blocks x row groups. 16 lanes hold a row's values;
+// the 4 lane groups of a wave, and with WAVES 4 those of the block's 4 waves, walk over its parts. With WAVES 1 each wave has rows of its own.
+template <int R, int DIM, int WAVES>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
-    constexpr int V = DIM / 16;
+    constexpr int V = DIM / 16, GROUPS = 4 * WAVES, OWN = 4 / WAVES;
     const int w = blockIdx.x;
     const int4 d = a.joins[w];
     if (d.x == 0) return;
-    __shared__ float red[16][DIM + 2];
-    const int b = d.y, rt = d.z, h = d.w;
-    const int group = threadIdx.x >> 4, col = (threadIdx.x & 15) * V;
+    __shared__ float red[WAVES == 4 ? 4 : 1][DIM + 2];
+    const int b = d.y, rt = d.z, h = d.w, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int group = WAVES == 4 ? threadIdx.x >> 4 : lane >> 4, col = (lane & 15) * V;
     const SeqInfo s = seq_info(a, b);
     const int rows = min(R, s.rows - rt * R), parts = d.x - w + 1;
-    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (int r = blockIdx.y * OWN + (WAVES == 4 ? 0 : wave); r < rows; r += gridDim.y * OWN) {
         float acc[V] = {}, m = -INFINITY, l = 0.0f;
-        for (int i = group; i < parts; i += 16) {
-            const float* p = part_slot<R, DIM>(a.part, i == 0 ? 2 * w + 1 : 2 * (w + i));
-            const float pm = p[R * DIM + r], pl = p[R * DIM + R + r];
-            float x[V];
-#pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(p + r * DIM + col + e);
-                x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
-            }
+        const auto add = [&](float pm, float pl, const float (&x)[V]) {
             const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
             const float fo = __builtin_amdgcn_exp2f(m - base), fn = __builtin_amdgcn_exp2f(pm - base);
             l = l * fo + pl * fn;
 #pragma unroll
             for (int e = 0; e < V; ++e) acc[e] = acc[e] * fo + x[e] * fn;
             m = top;
-        }
-        __syncthreads();
+        };
+#pragma unroll 2
+        for (int i = group; i < parts; i += GROUPS) {
+            const float* p = part_slot<R, DIM>(a.part, i == 0 ? 2 * w + 1 : 2 * (w + i));
+            float x[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) red[group][col + e] = acc[e];
-        if (col == 0) { red[group][DIM] = m; red[group][DIM + 1] = l; }
-        __syncthreads();
-        if (threadIdx.x < DIM && (int)threadIdx.x < a.c.dim) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, red[i][DIM]);
-            const float base = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f, o = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float f = __builtin_amdgcn_exp2f(red[i][DIM] - base);
-                sum += red[i][DIM + 1] * f;
-                o += red[i][threadIdx.x] * f;
+            for (int e = 0; e < V; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(p + r * DIM + col + e);
+                x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
             }
-            const float v[1] = {sum == 0.0f ? 0.0f : o / sum};
-            const int q = rt * R + r, t = a.s.starts[b] + q / a.group;
-            store_vec<1>(a.out, (size_t)t * a.out_stride + (size_t)(h * a.group + q % a.group) * a.c.dim + threadIdx.x, v, a.out_dtype);
+            add(p[R * DIM + r], p[R * DIM + R + r], x);
+        }
+#pragma unroll
+        for (int lanes = 16; lanes < 64; lanes <<= 1) {
+            float x[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = __shfl_xor(acc[e], lanes, 64);
+            add(__shfl_xor(m, lanes, 64), __shfl_xor(l, lanes, 64), x);
+        }
+        if constexpr (WAVES == 4) {
+            __syncthreads();
+            if (lane < 16) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) red[wave][col + e] = acc[e];
+                if (lane == 0) { red[wave][DIM] = m; red[wave][DIM + 1] = l; }
+            }
+            __syncthreads();
+            m = -INFINITY;
+            l = 0.0f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float x[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[e] = red[i][col + e];
+                add(red[i][DIM], red[i][DIM + 1], x);
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int q = rt * R + r, t = a.s.starts[b] + q / a.group;
+        const size_t out = (size_t)t * a.out_stride + (size_t)(h * a.group + q % a.group) * a.c.dim + col;
+        if (threadIdx.x < 16 || (WAVES == 1 && lane < 16)) {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                if (col + e >= a.c.dim) continue;
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : acc[e + k] * inv;
+                if (a.out_vec) {
+                    store_vec<4>(a.out, out + e, v, a.out_dtype);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float one[1] = {v[k]};
+                        store_vec<1>(a.out, out + e + k, one, a.out_dtype);
+                    }
+                }
+            }
         }
     }
 }
@@ -171,6 +209,12 @@ __device__ __forceinline__ void split_terms(float x, typename Half8<CT>::one (&t
         t[p] = (typename Half8<CT>::one)x;
         if (p + 1 < NP) x -= (float)t[p];
     }
+}
+
+// Two 16-bit values, those that are not finite (all exponent bits `exp` set) as 0.
+__device__ __forceinline__ uint32_t finite_only(uint32_t x, uint32_t exp) {
+    x &= (x & exp) == exp ? 0xFFFF0000u : ~0u;
+    return x & ((x >> 16 & exp) == exp ? 0xFFFFu : ~0u);
 }
 
 constexpr float kLog2e = 1.44269504f;

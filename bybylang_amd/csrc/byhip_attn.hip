@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void attn_general(AttnArgs a) {
         const int j = j0 + lane;
         bool see = sees(a, s, pos, j);
         if (__ballot(see) == 0) continue;
-        const int col = j / a.c.page_size;
+        const int col = page_col(a, j);
         const int page = see ? a.s.table[(size_t)b * a.s.stride + col] : -1;
         see = page >= 0 && page < a.c.pages;
         const size_t row = ((size_t)page * a.c.kv_heads + kvh) * a.c.page_size + (j - col * a.c.page_size);
@@ -153,6 +153,10 @@ extern "C" int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype
         a.slopes = attn->slopes; a.prefix = attn->prefix;
         a.group = heads / a.c.kv_heads;
         a.max_rows = 0x7FFFFFFF;
+        int log = 0;
+        while ((1ll << log) < a.c.page_size) ++log;
+        a.page_shift = log - 1;
+        a.page_mul = log ? (uint32_t)(((1ull << (31 + log)) + a.c.page_size - 1) / a.c.page_size) : 0u;
         a.q_vec = q_stride * dtype_bytes(q_dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
         a.out_vec = aligned4(out, out_stride, out_dtype);
         note_device_write(out);

@@ -27,16 +27,21 @@ namespace {
 
 constexpr int kChunkKeys = 64;
 constexpr int kXcds = 8;
+// What cutting an item costs the blocks that share it, in key tiles: the part's way to the workspace and back.
+constexpr int kCutTiles = 8;
+// Key tiles a block should at least get before another one takes part.
+constexpr int kShareTiles = 4;
 __device__ __attribute__((aligned(64))) uint32_t zero_piece[16];  // what keys and values outside the cache read as
 
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
-typedef float f8v __attribute__((ext_vector_type(8)));
 
-// Workgroup barrier once this wave's direct loads have landed and its LDS reads are done.
-__device__ __forceinline__ void tile_barrier() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// Workgroup barrier after this wave's LDS reads, and with LOADS also once its direct loads have landed.
+template <bool LOADS>
+__device__ __forceinline__ void phase_barrier() {
+    if constexpr (LOADS) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 template <int CT, int NP, int DIM, int WAVES, bool EXTRA>
@@ -46,12 +51,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     constexpr int STEPS = DIM / 16, DT = DIM / 32, PIECES = DIM / 8, SW = (PIECES < 16 ? PIECES : 16) - 1;
     constexpr int ROW = DIM * 2, TILE = T * ROW;                  // bytes of a key, of a tile
     constexpr int NI = TILE / 1024 / WAVES, RPI = 1024 / ROW;     // direct loads per wave and tile, keys per load
-    constexpr float kShift = CT == BYHIP_F16 ? 7.0f : 0.0f;       // log2 of the weights' factor
-    constexpr float kRaise = 8.0f;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];  // K, V of one tile, then of the next
-    __shared__ int row_tiles[kAttnBatch + 1];                         // row tiles of the sequences before each
-    __shared__ long long units_before[NT + 1];                        // key tiles of the row tiles before each thread's run
+    constexpr bool PAIRED = WAVES == 8;                           // two waves per SIMD, half a tile apart
+    constexpr int BUFS = PAIRED ? 3 : 2;
+    constexpr float kShift = CT == BYHIP_F16 ? 4.0f : 0.0f;       // log2 of the weights' factor
+    constexpr float kLimit = 32768.0f;                            // a lane's weights of a tile may add up to this
+    constexpr uint32_t kExp = CT == BYHIP_F16 ? 0x7C00u : 0x7F80u;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BUFS * TILE];  // BUFS tiles of K, then of V
+    __shared__ int row_tiles[kAttnBatch + 1];                                // row tiles of the sequences before each
+    __shared__ long long units_before[NT + 1];                               // key tiles of the row tiles before each thread's run
     __shared__ long long wave_total[WAVES];
+    __shared__ int longest;                                                  // key tiles of the largest item
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, hf = lane >> 5;
 
@@ -105,22 +114,31 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     };
     {
         long long sum = 0;
-        int b;
-        for (int x = tid * run; x < min((tid + 1) * run, all_row_tiles); ++x) sum += tiles_at(x, b);
+        int b, top = 0;
+        if (tid == 0) longest = 0;
+        for (int x = tid * run; x < min((tid + 1) * run, all_row_tiles); ++x) {
+            const int n = tiles_at(x, b);
+            sum += n;
+            top = max(top, n);
+        }
         const long long base = scan(sum);
+        if (top) atomicMax(&longest, top);
         units_before[tid] = base;
         if (tid == NT - 1) units_before[NT] = base + sum;
         __syncthreads();
     }
     const long long per_head = units_before[NT], total = per_head * a.c.kv_heads;
-    const long long blocks = min((long long)gridDim.x, total);
+    const long long items = (long long)all_row_tiles * a.c.kv_heads;
+    // Whole items where the fullest block then has no more than with equal shares and their cuts.
+    const bool whole = (items + gridDim.x - 1) / gridDim.x * longest <= max((long long)kShareTiles, total / gridDim.x) + kCutTiles;
+    const long long blocks = min((long long)gridDim.x, whole ? items : max(1LL, total / kShareTiles));
     int w = blockIdx.x;
     if (blocks == (long long)gridDim.x && gridDim.x % kXcds == 0) w = (w % kXcds) * (gridDim.x / kXcds) + w / kXcds;
-    if (w >= blocks) {
+    if (w >= blocks || total == 0) {
         if (tid == 0) a.joins[w] = make_int4(0, 0, 0, 0);
         return;
     }
-    const long long u0 = total * w / blocks, u1 = total * (w + 1) / blocks;
+    const long long u0 = whole ? w : total * w / blocks, u1 = whole ? items : total * (w + 1) / blocks;
     int4 join = make_int4(0, 0, 0, 0);
 
     // this lane's places in the LDS tiles
@@ -133,35 +151,45 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int key = 8 * j + 4 * hf + (lane & 15) / 4, piece = 4 * dt + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
-            v_at[dt][j] = key * ROW + ((piece ^ (key & SW)) << 4) + 8 * (lane & 1);
+            v_at[dt][j] = key * ROW + ((piece ^ (2 * key & SW)) << 4) + 8 * (lane & 1);
         }
     // and its share of the direct loads: key (wave NI + i) RPI + lane / PIECES, the piece that belongs at lane % PIECES
     const int load_key = wave * NI * RPI + lane / PIECES;
     lds_byte* const lds3 = (lds_byte*)lds;
 
     for (long long u = u0; u < u1;) {
-        const int h = __builtin_amdgcn_readfirstlane((int)(u / per_head));
-        long long in_head = u - h * per_head;
-        int lo = 0, hi = NT - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (units_before[mid] <= in_head) lo = mid;
-            else hi = mid - 1;
+        int h, b, rt, t0, t1;
+        if (whole) {
+            h = __builtin_amdgcn_readfirstlane((int)(u / all_row_tiles));
+            const int x = __builtin_amdgcn_readfirstlane((int)(u % all_row_tiles));
+            b = __builtin_amdgcn_readfirstlane(sequence_of(x));
+            rt = x - row_tiles[b];
+            t0 = 0;
+        } else {
+            h = __builtin_amdgcn_readfirstlane((int)(u / per_head));
+            long long in_head = u - h * per_head;
+            int lo = 0, hi = NT - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (units_before[mid] <= in_head) lo = mid;
+                else hi = mid - 1;
+            }
+            in_head -= units_before[lo];
+            int x = lo * run, n_tiles = tiles_at(x, b);
+            while (in_head >= n_tiles) {
+                in_head -= n_tiles;
+                n_tiles = tiles_at(++x, b);
+            }
+            b = __builtin_amdgcn_readfirstlane(b);
+            rt = __builtin_amdgcn_readfirstlane(x) - row_tiles[b];
+            t0 = __builtin_amdgcn_readfirstlane((int)in_head);
         }
-        in_head -= units_before[lo];
-        int x = lo * run, b, n_tiles = tiles_at(x, b);
-        while (in_head >= n_tiles) {
-            in_head -= n_tiles;
-            n_tiles = tiles_at(++x, b);
-        }
-        x = __builtin_amdgcn_readfirstlane(x);
-        b = __builtin_amdgcn_readfirstlane(b);
-        const int rt = x - row_tiles[b], t0 = __builtin_amdgcn_readfirstlane((int)in_head);
+        rt = __builtin_amdgcn_readfirstlane(rt);
         const SeqInfo s = seq_info(a, b);
         int p0, p1;
         positions(s, rt, p0, p1);
         const TileRange<T> range(a, s, p0, p1);
-        const int t1 = __builtin_amdgcn_readfirstlane((int)min((long long)range.tiles, t0 + (u1 - u)));
+        t1 = whole ? range.tiles : __builtin_amdgcn_readfirstlane((int)min((long long)range.tiles, t0 + (u1 - u)));
 
         // 2. the wave's rows
         const int row0 = rt * R + wave * 32, row = row0 + c;
@@ -189,10 +217,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 for (int st = 0; st < STEPS; ++st) {
                     const int d = 16 * st + 8 * hf;
                     const bool in = valid && d < a.c.dim;
+                    float f[8] = {};
+                    if (in) {
+                        if (a.q_vec) {
+                            const float4 x = *reinterpret_cast<const float4*>(p + d), y = *reinterpret_cast<const float4*>(p + d + 4);
+                            f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+                            f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) f[e] = p[d + e];
+                        }
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         typename Half8<CT>::one t[NP];
-                        split_terms<CT, NP>(in ? ldexpf(p[in ? d + e : 0], shift) : 0.0f, t);
+                        split_terms<CT, NP>(ldexpf(f[e], shift), t);
 #pragma unroll
                         for (int i = 0; i < NP; ++i) q[i][st][e] = t[i];
                     }
@@ -226,61 +265,80 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
 
-        // 3. key tiles
+        // 3. key tiles. A tile's work is two phases with a barrier after each: products (O^T += V^T P^T of the tile
+        // before, S^T = K Q^T of this one) and weights (exponentials of S^T; the direct loads of K two tiles and V one tile
+        // ahead). Of two waves on a SIMD one runs a phase behind the other, so that one's products go with the other's weights.
+        const int n = t1 - t0;
         const auto page_of = [&](int t) {  // the page of key `lane` of tile t
             const int j = range.key(t) + lane, at = max(0, min(j, s.len - 1));
-            return a.s.table[(size_t)b * a.s.stride + at / a.c.page_size];
+            return a.s.table[(size_t)b * a.s.stride + page_col(a, at)];
         };
-        const auto load = [&](int t, int page, int buf, uint64_t& there) {
+        struct Keys {
+            uint32_t row[NI];  // the cache rows this lane loads, ~0: none
+            uint64_t there;    // bit j: key j exists
+        };
+        const auto keys_of = [&](int t, int page) {
+            Keys k;
             const int j = range.key(t) + lane, at = max(0, min(j, s.len - 1));
             const bool is = (j < s.len) & (page >= 0) & (page < a.c.pages);
-            there = __ballot(is);
-            const uint32_t key_row = is ? ((uint32_t)page * a.c.kv_heads + h) * a.c.page_size + at % a.c.page_size : ~0u;
+            k.there = __ballot(is);
+            const uint32_t row = is ? ((uint32_t)page * a.c.kv_heads + h) * a.c.page_size + (at - page_col(a, at) * a.c.page_size) : ~0u;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) k.row[i] = (uint32_t)__shfl((int)row, load_key + i * RPI, 64);
+            return k;
+        };
+        const auto load = [&](const uint16_t* base, const Keys& k, int to, bool values) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int key = load_key + i * RPI;
-                const uint32_t from = (uint32_t)__shfl((int)key_row, key, 64);
-                const int piece = (lane % PIECES) ^ (key & SW);
-                const bool in = (from != ~0u) & (8 * piece < a.c.dim);
-                const size_t off = (size_t)from * a.c.dim + 8 * piece;
-                const uint16_t* zero = reinterpret_cast<const uint16_t*>(zero_piece);
-                const uint16_t* kp = in ? a.c.k + off : zero;
-                const uint16_t* vp = in ? a.c.v + off : zero;
-                lds_byte* dst = lds3 + buf * 2 * TILE + (wave * NI + i) * 1024;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp, (lds_void*)dst, 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp, (lds_void*)(dst + TILE), 16, 0, 0);
+                const int piece = (lane % PIECES) ^ ((values ? 2 * key : key) & SW);
+                const bool in = (k.row[i] != ~0u) & (8 * piece < a.c.dim);
+                const uint16_t* p = in ? base + (size_t)k.row[i] * a.c.dim + 8 * piece : reinterpret_cast<const uint16_t*>(zero_piece);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (lds_void*)(lds3 + to + (wave * NI + i) * 1024),
+                                                 16, 0, 0);
             }
         };
-        uint64_t there = 0, next_there = 0;
-        int page = page_of(t0);
-        tile_barrier();  // the item before may still be reading its last tile
-        load(t0, page, 0, there);
-        if (t0 + 1 < t1) page = page_of(t0 + 1);
-        for (int t = t0; t < t1; ++t) {
-            const int buf = (t - t0) & 1, j0 = range.key(t);
-            tile_barrier();
-            if (t + 1 < t1) load(t + 1, page, buf ^ 1, next_there);
-            if (t + 2 < t1) page = page_of(t + 2);
-            const uint8_t* kt = lds + buf * 2 * TILE;
-            const uint8_t* vt = kt + TILE;
-            const auto full = [&](int lo_pos, int hi_pos) {
-                return there == ~0ull && ((j0 + T - 1 <= lo_pos && (a.window <= 0 || hi_pos - j0 < a.window)) || j0 + T <= s.prefix);
-            };
-            // values that are not finite and that a row does not see (or that meet weights of several terms) are added apart
-            constexpr uint32_t kExp = CT == BYHIP_F16 ? 0x7C00u : 0x7F80u;
-            bool odd = false;
-            if (NP > 1 || !full(p0, p1)) {
-                uint32_t any = 0;
+        const auto k_tile = [&](int i) { return i % BUFS * TILE; };
+        const auto v_tile = [&](int i) { return (BUFS + i % BUFS) * TILE; };
+        Keys ahead = keys_of(t0, page_of(t0));  // the newest tile whose keys are known: K loaded, V not yet
+        uint64_t there = ahead.there, next_there = 0;
+        int page = n > 1 ? page_of(t0 + 1) : 0;
+        phase_barrier<true>();  // the item before has been read
+        load(a.c.k, ahead, k_tile(0), false);
+        load(a.c.v, ahead, v_tile(0), true);
+        if (n > 1) {
+            ahead = keys_of(t0 + 1, page);
+            next_there = ahead.there;
+            load(a.c.k, ahead, k_tile(1), false);
+            if (n > 2) page = page_of(t0 + 2);
+        }
+        phase_barrier<true>();
+        if (PAIRED && wave >= WAVES / 2) phase_barrier<false>();
+
+        f16v sc[2];
+        vec wt[NP][4];
+        bool weighed = false, odd = false;  // the tile before left weights; its V holds values that are not finite
+        uint32_t see[2] = {~0u, ~0u};
+        for (int i = 0; i <= n; ++i) {
+            const int j0 = range.key(min(t0 + i, t1 - 1));
+            // products
+            if (weighed) {
+                lds_byte* vt = lds3 + v_tile(i - 1);
 #pragma unroll
-                for (int i = 0; i < TILE / 16 / NT; ++i) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vt + (i * NT + tid) * 16);
-                    for (const uint32_t x : {v.x, v.y, v.z, v.w}) any |= (uint32_t)((x & kExp) == kExp) | (uint32_t)((x >> 16 & kExp) == kExp);
-                }
-                odd = __syncthreads_or(any != 0);
+                for (int st = 0; st < 4; ++st)
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vt + v_at[dt][0] + st * 16 * ROW));
+                        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vt + v_at[dt][1] + st * 16 * ROW));
+                        uint4 v = __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                        if (odd) { v.x = finite_only(v.x, kExp); v.y = finite_only(v.y, kExp); v.z = finite_only(v.z, kExp); v.w = finite_only(v.w, kExp); }
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; --p) o[dt] = mfma32(__builtin_bit_cast(vec, v), wt[p][st], o[dt]);
+                    }
             }
-            const bool works = row0 < s.rows && (j0 <= wp1 || j0 < s.prefix);  // some row of the wave may see the tile
-            f16v sc[2];
+            const bool works = i < n && row0 < s.rows && (j0 <= wp1 || j0 < s.prefix);  // some row of the wave may see the tile
             if (works) {
+                const uint8_t* kt = lds + k_tile(i);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
@@ -289,35 +347,91 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                     for (int st = 0; st < STEPS; ++st) {
                         const vec k = *reinterpret_cast<const vec*>(kt + k_at[st] + kb * 32 * ROW);
 #pragma unroll
-                        for (int i = NP - 1; i >= 0; --i) sc[kb] = mfma32(k, q[i][st], sc[kb]);
+                        for (int p = NP - 1; p >= 0; --p) sc[kb] = mfma32(k, q[p][st], sc[kb]);
                     }
                 }
-                if constexpr (EXTRA) {
+            }
+            if (i == n) break;
+            phase_barrier<true>();
+
+            // weights
+            uint64_t far_there = 0;
+            if (i + 1 < n) load(a.c.v, ahead, v_tile(i + 1), true);
+            if (i + 2 < n) {
+                ahead = keys_of(t0 + i + 2, page);
+                far_there = ahead.there;
+                load(a.c.k, ahead, k_tile(i + 2), false);
+                if (i + 3 < n) page = page_of(t0 + i + 3);
+            }
+            weighed = works;
+            if (works) {
+                if constexpr (EXTRA) {  // to capped and biased scores (log2)
+                    if (a.softcap > 0.0f && NP == 1) {
+                        const float f = factor * (2.0f * kLog2e / a.softcap), top = a.softcap * kLog2e;
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
+                        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float v = sc[kb][e] * factor;
-                            if (a.softcap > 0.0f) v = a.softcap * soft_tanh<(NP > 1)>(v / a.softcap);
-                            sc[kb][e] = v * kLog2e - slope * fabsf((float)(pos - (j0 + 32 * kb + 8 * (e / 4) + 4 * hf + e % 4)));
-                        }
+                            for (int e = 0; e < 16; ++e)
+                                sc[kb][e] = fmaf(-2.0f * top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[kb][e] * f)), top);
+                    } else if (a.softcap > 0.0f) {
+                        const float f = factor / a.softcap, top = a.softcap * kLog2e;
+#pragma unroll
+                        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) sc[kb][e] = top * soft_tanh<true>(sc[kb][e] * f);
+                    } else {
+                        const float f = factor * kLog2e;
+#pragma unroll
+                        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) sc[kb][e] *= f;
+                    }
+                    if (a.slopes) {
+                        const float back = (float)(pos - j0 - 4 * hf);
+#pragma unroll
+                        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) sc[kb][e] = fmaf(-slope, fabsf(back - (float)(32 * kb + 8 * (e / 4) + e % 4)), sc[kb][e]);
+                    }
                 }
-                uint32_t see[2] = {~0u, ~0u};
-                if (!full(wp0, wp1)) {
+                const bool full = there == ~0ull && ((j0 + T - 1 <= wp0 && (a.window <= 0 || wp1 - j0 < a.window)) || j0 + T <= s.prefix);
+                if (!full) {  // without branches: all 64 lanes take part in what follows
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb) {
                         see[kb] = seen_keys(a, s, pos, j0 + 32 * kb, (uint32_t)(there >> (32 * kb)));
 #pragma unroll
                         for (int e = 0; e < 16; ++e) sc[kb][e] = see[kb] >> (8 * (e / 4) + e % 4) >> (4 * hf) & 1u ? sc[kb][e] : -INFINITY;
                     }
+                } else {
+                    see[0] = see[1] = ~0u;
                 }
-                float top = -INFINITY;
+                // Weights against the row's reference. Their sum bounds the largest of them: only where it passes the limit
+                // (or the row has no reference yet) is a maximum looked for, the reference raised and the sums scaled down.
+                float sum;
+                const auto weigh = [&]() {
+                    const float base = m == -INFINITY ? 0.0f : m - kShift;
+                    sum = 0.0f;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                    for (int st = 0; st < 4; ++st)
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(sc[kb][e], sc[kb][e + 1]));
-                if (!EXTRA) top *= factor;
-                if (__ballot(top > m + kRaise || (m == -INFINITY && top > m))) {
+                        for (int e = 0; e < 8; ++e) {
+                            const float x = sc[st / 2][8 * (st & 1) + e];
+                            const float v = __builtin_amdgcn_exp2f(EXTRA ? x - base : fmaf(x, factor, -base));
+                            sum += v;
+                            typename Half8<CT>::one t[NP];
+                            split_terms<CT, NP>(v, t);
+#pragma unroll
+                            for (int p = 0; p < NP; ++p) wt[p][st][e] = t[p];
+                        }
+                };
+                weigh();
+                if (__ballot((sum > kLimit) | (m == -INFINITY))) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[kb][e]);
+                    if (!EXTRA) top *= factor;
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
                     const float raised = fmaxf(m, top);
                     const float fade = raised == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
@@ -327,7 +441,26 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[dt][e] *= fade;
+                    weigh();
                 }
+                l += sum;
+            }
+            phase_barrier<false>();
+            // Values that are not finite and that a row does not see would spoil its sums (0 times infinity), and so would
+            // seen ones where weights have several terms: they are added apart, and the products pass over them.
+            odd = false;
+            if (works && (NP > 1 || __ballot((see[0] & see[1]) != ~0u))) {
+                const uint8_t* vt = lds + v_tile(i);
+                uint32_t any = 0;
+#pragma unroll 4
+                for (int e = 0; e < TILE / 1024; ++e) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(vt + (e * 64 + lane) * 16);
+                    any |= v.x ^ finite_only(v.x, kExp);
+                    any |= v.y ^ finite_only(v.y, kExp);
+                    any |= v.z ^ finite_only(v.z, kExp);
+                    any |= v.w ^ finite_only(v.w, kExp);
+                }
+                odd = __ballot(any != 0) != 0;
                 if (odd) {
                     for (int key = 0; key < T; ++key) {
                         const uint32_t mine = (key < 32 ? see[0] >> key : see[1] >> (key - 32)) & 1u;
@@ -335,7 +468,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                             for (int g = 0; g < 4; ++g) {  // dimensions 32 dt + 8 g + 4 hf .. + 3
-                                const int piece = (4 * dt + g) ^ (key & SW);
+                                const int piece = (4 * dt + g) ^ (2 * key & SW);
                                 const uint2 v = *reinterpret_cast<const uint2*>(vt + key * ROW + piece * 16 + 8 * hf);
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
@@ -346,54 +479,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                             }
                     }
                 }
-                // weights, packed into the operands of the products with V
-                const float base = m == -INFINITY ? 0.0f : m - kShift;
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        sc[kb][e] = __builtin_amdgcn_exp2f(EXTRA ? sc[kb][e] - base : fmaf(sc[kb][e], factor, -base));
-                        l += sc[kb][e];
-                    }
-            }
-            if (odd) {  // every wave has added what it sees of them: the tile's odd values become 0
-                tile_barrier();
-#pragma unroll
-                for (int i = 0; i < TILE / 16 / NT; ++i) {
-                    uint32_t* v = reinterpret_cast<uint32_t*>(lds + buf * 2 * TILE + TILE + (i * NT + tid) * 16);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t x = v[e];
-                        x &= (x & kExp) == kExp ? 0xFFFF0000u : ~0u;
-                        x &= (x >> 16 & kExp) == kExp ? 0xFFFFu : ~0u;
-                        v[e] = x;
-                    }
-                }
-                tile_barrier();
-            }
-            if (works) {
-#pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    vec wt[NP];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        typename Half8<CT>::one t[NP];
-                        split_terms<CT, NP>(sc[st / 2][8 * (st & 1) + i], t);
-#pragma unroll
-                        for (int n = 0; n < NP; ++n) wt[n][i] = t[n];
-                    }
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(lds3 + (buf * 2 + 1) * TILE + v_at[dt][0] + st * 16 * ROW));
-                        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(lds3 + (buf * 2 + 1) * TILE + v_at[dt][1] + st * 16 * ROW));
-                        const vec v = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                        for (int n = NP - 1; n >= 0; --n) o[dt] = mfma32(v, wt[n], o[dt]);
-                    }
-                }
             }
             there = next_there;
+            next_there = far_there;
         }
+        if (PAIRED && wave < WAVES / 2) phase_barrier<false>();
 
         // 4. the wave's rows leave, whole or as a part
         const bool begins = t0 == 0, ends = t1 == range.tiles;
@@ -438,7 +528,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                         (f4){o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
         }
         if (begins && !ends) join = join_of(u - t0 + range.tiles - 1, blocks, total, b, rt, h);
-        u += t1 - t0;
+        u += whole ? blocks : t1 - t0;
     }
     if (tid == 0) a.joins[w] = join;
 }
@@ -451,7 +541,7 @@ void launch_chunk(const AttnArgs& a) {
     if (a.softcap > 0.0f || a.slopes || !(a.scale > 0.0f)) launch("attn_chunk", (attn_chunk<CT, NP, DIM, WAVES, true>), dim3(blocks), dim3(64 * WAVES), 0, a);
     else launch("attn_chunk", (attn_chunk<CT, NP, DIM, WAVES, false>), dim3(blocks), dim3(64 * WAVES), 0, a);
     BYHIP_LAUNCHED("attn_chunk");
-    launch("attn_join", (attn_join<32 * WAVES, DIM>), dim3(blocks, 64), dim3(256), 0, a);
+    launch("attn_join", (attn_join<32 * WAVES, DIM, 1>), dim3(blocks, 16), dim3(256), 0, a);
     BYHIP_LAUNCHED("attn_join");
 }
 

@@ -64,7 +64,7 @@ struct Rows {
     // all 64 lanes take part in what follows.
     __device__ __forceinline__ uint32_t key_row(int b, int j0, uint32_t& there) const {
         const int j = j0 + (lane & 31);
-        const int at = max(0, min(j, s.len - 1)), col = at / a.c.page_size;
+        const int at = max(0, min(j, s.len - 1)), col = page_col(a, at);
         const int page = a.s.table[(size_t)b * a.s.stride + col];
         const bool is = (j < s.len) & (page >= 0) & (page < a.c.pages);
         there = (uint32_t)__ballot(is);
@@ -268,8 +268,7 @@ struct Rows {
             }
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) {
-                v[i][e] &= (v[i][e] & kExp) == kExp ? 0xFFFF0000u : ~0u;
-                v[i][e] &= (v[i][e] >> 16 & kExp) == kExp ? 0xFFFFu : ~0u;
+                v[i][e] = finite_only(v[i][e], kExp);
             }
         }
     }
@@ -433,7 +432,7 @@ void launch_rows(const AttnArgs& a, unsigned blocks) {
     if (a.softcap > 0.0f || a.slopes) launch("attn_rows", (attn_rows<CT, NP, DIM, true>), dim3(blocks), dim3(256), 0, a);
     else launch("attn_rows", (attn_rows<CT, NP, DIM, false>), dim3(blocks), dim3(256), 0, a);
     BYHIP_LAUNCHED("attn_rows");
-    launch("attn_join", (attn_join<kRows, DIM>), dim3(blocks, kRows), dim3(256), 0, a);
+    launch("attn_join", (attn_join<kRows, DIM, 4>), dim3(blocks, kRows), dim3(256), 0, a);
     BYHIP_LAUNCHED("attn_join");
 }
 
