@@ -92,6 +92,15 @@ void launch_attn_rows_bf16(const AttnArgs& a, bool precise);
 void launch_attn_chunk_f16(const AttnArgs& a, bool precise);
 void launch_attn_chunk_bf16(const AttnArgs& a, bool precise);
 
+// Values that are the same in every lane, as the compiler cannot see where they come through LDS: loops over them then
+// run on scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long long uniform(long long v) {
+    return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+__device__ __forceinline__ uint32_t bit_mask(bool b) { return 0u - (uint32_t)b; }
+
 // What block w leaves when its share ends inside an item it began: the block that holds the item's last unit.
 __device__ __forceinline__ int4 join_of(long long last, long long blocks, long long total, int b, int rt, int h) {
     int w = (int)((last * blocks + blocks - 1) / total);

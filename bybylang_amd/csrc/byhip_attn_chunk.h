@@ -25,6 +25,7 @@
 namespace byhip {
 namespace {
 
+#define INLINE __attribute__((always_inline))
 constexpr int kChunkKeys = 64;
 constexpr int kXcds = 8;
 // What cutting an item costs the blocks that share it, in key tiles: the part's way to the workspace and back.
@@ -42,6 +43,22 @@ template <bool LOADS>
 __device__ __forceinline__ void phase_barrier() {
     if constexpr (LOADS) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// 16 bytes per lane from memory to LDS byte `to` + 16 lane. Written as assembly because the compiler makes every later LDS
+// read wait for such loads, which here belong to tiles still ahead; it has no output register, phase_barrier<true> waits for
+// it, and a wait of the compiler's own that counts it among its loads only waits longer.
+__device__ __forceinline__ void load_to_lds(const void* p, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory");
+}
+
+template <int I> struct Index { static constexpr int value = I; };
+template <int I, int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    if constexpr (I < N) {
+        f(Index<I>{});
+        unrolled<I + 1, N>(f);
+    }
 }
 
 template <int CT, int NP, int DIM, int WAVES, bool EXTRA>
@@ -94,7 +111,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
         if (tid == NT - 1) row_tiles[a.s.batch] = base + sum;
         __syncthreads();
     }
-    const int all_row_tiles = row_tiles[a.s.batch];
+    const int all_row_tiles = uniform(row_tiles[a.s.batch]);
     const int run = (all_row_tiles + NT - 1) / NT;
     const auto sequence_of = [&](int x) {  // the last one with row tiles before it <= x
         int lo = 0, hi = a.s.batch - 1;
@@ -127,10 +144,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
         if (tid == NT - 1) units_before[NT] = base + sum;
         __syncthreads();
     }
-    const long long per_head = units_before[NT], total = per_head * a.c.kv_heads;
+    const long long per_head = uniform(units_before[NT]), total = per_head * a.c.kv_heads;
     const long long items = (long long)all_row_tiles * a.c.kv_heads;
     // Whole items where the fullest block then has no more than with equal shares and their cuts.
-    const bool whole = (items + gridDim.x - 1) / gridDim.x * longest <= max((long long)kShareTiles, total / gridDim.x) + kCutTiles;
+    const bool whole = (items + gridDim.x - 1) / gridDim.x * uniform(longest) <= max((long long)kShareTiles, total / gridDim.x) + kCutTiles;
     const long long blocks = min((long long)gridDim.x, whole ? items : max(1LL, total / kShareTiles));
     int w = blockIdx.x;
     if (blocks == (long long)gridDim.x && gridDim.x % kXcds == 0) w = (w % kXcds) * (gridDim.x / kXcds) + w / kXcds;
@@ -141,32 +158,28 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     const long long u0 = whole ? w : total * w / blocks, u1 = whole ? items : total * (w + 1) / blocks;
     int4 join = make_int4(0, 0, 0, 0);
 
-    // this lane's places in the LDS tiles
-    int k_at[STEPS];  // pieces 2 st + hf of key c
-#pragma unroll
-    for (int st = 0; st < STEPS; ++st) k_at[st] = c * ROW + (((2 * st + hf) ^ (c & SW)) << 4);
-    int v_at[DT][2];  // keys 8 j + 4 hf + (lane % 16) / 4, values 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4)
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int key = 8 * j + 4 * hf + (lane & 15) / 4, piece = 4 * dt + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
-            v_at[dt][j] = key * ROW + ((piece ^ (2 * key & SW)) << 4) + 8 * (lane & 1);
-        }
-    // and its share of the direct loads: key (wave NI + i) RPI + lane / PIECES, the piece that belongs at lane % PIECES
+    // This lane's places in the LDS tiles: pieces 2 st + hf of key c at k_at ^ 32 st (K's piece i of key j lies at i ^ j), and
+    // keys 4 hf + (lane % 16) / 4 (+ 8 j + 16 st), values 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) at v_at ^ 64 dt (V's
+    // piece i of key j at i ^ 2 j, so that the 4 keys of a transposing read fall on different banks).
+    const int k_at = c * ROW + ((hf ^ (c & SW)) << 4);
+    const int v_key = 4 * hf + (lane & 15) / 4;
+    const int v_at = v_key * ROW + (((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ (2 * v_key & SW)) << 4) + 8 * (lane & 1);
+    // and its share of the direct loads: keys load_key + i RPI, whose bits do not overlap, the piece that belongs at lane % PIECES
     const int load_key = wave * NI * RPI + lane / PIECES;
+    const int k_piece = (lane % PIECES) ^ (load_key & SW), v_piece = (lane % PIECES) ^ (2 * load_key & SW);
     lds_byte* const lds3 = (lds_byte*)lds;
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds3);
 
     for (long long u = u0; u < u1;) {
         int h, b, rt, t0, t1;
         if (whole) {
-            h = __builtin_amdgcn_readfirstlane((int)(u / all_row_tiles));
-            const int x = __builtin_amdgcn_readfirstlane((int)(u % all_row_tiles));
-            b = __builtin_amdgcn_readfirstlane(sequence_of(x));
-            rt = x - row_tiles[b];
+            h = (int)(u / all_row_tiles);
+            const int x = (int)(u % all_row_tiles);
+            b = uniform(sequence_of(x));
+            rt = x - uniform(row_tiles[b]);
             t0 = 0;
         } else {
-            h = __builtin_amdgcn_readfirstlane((int)(u / per_head));
+            h = (int)(u / per_head);
             long long in_head = u - h * per_head;
             int lo = 0, hi = NT - 1;
             while (lo < hi) {
@@ -180,16 +193,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 in_head -= n_tiles;
                 n_tiles = tiles_at(++x, b);
             }
-            b = __builtin_amdgcn_readfirstlane(b);
-            rt = __builtin_amdgcn_readfirstlane(x) - row_tiles[b];
-            t0 = __builtin_amdgcn_readfirstlane((int)in_head);
+            b = uniform(b);
+            rt = uniform(x - row_tiles[b]);
+            t0 = uniform((int)in_head);
         }
-        rt = __builtin_amdgcn_readfirstlane(rt);
         const SeqInfo s = seq_info(a, b);
         int p0, p1;
         positions(s, rt, p0, p1);
         const TileRange<T> range(a, s, p0, p1);
-        t1 = whole ? range.tiles : __builtin_amdgcn_readfirstlane((int)min((long long)range.tiles, t0 + (u1 - u)));
+        t1 = whole ? range.tiles : (int)min((long long)range.tiles, t0 + (u1 - u));
 
         // 2. the wave's rows
         const int row0 = rt * R + wave * 32, row = row0 + c;
@@ -259,17 +271,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
             factor = ldexpf(EXTRA ? a.scale : a.scale * kLog2e, -shift);
         }
         float m = -INFINITY, l = 0.0f;
+        // O^T as whole vectors throughout: a loop over its elements would have the compiler carry 16 scalars per vector and
+        // copy them together for every product
         f16v o[DT];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+        for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v)(0.0f);
 
         // 3. key tiles. A tile's work is two phases with a barrier after each: products (O^T += V^T P^T of the tile
         // before, S^T = K Q^T of this one) and weights (exponentials of S^T; the direct loads of K two tiles and V one tile
         // ahead). Of two waves on a SIMD one runs a phase behind the other, so that one's products go with the other's weights.
         const int n = t1 - t0;
-        const auto page_of = [&](int t) {  // the page of key `lane` of tile t
+        const auto page_of = [&](int t) INLINE {  // the page of key `lane` of tile t
             const int j = range.key(t) + lane, at = max(0, min(j, s.len - 1));
             return a.s.table[(size_t)b * a.s.stride + page_col(a, at)];
         };
@@ -277,25 +289,26 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
             uint32_t row[NI];  // the cache rows this lane loads, ~0: none
             uint64_t there;    // bit j: key j exists
         };
-        const auto keys_of = [&](int t, int page) {
+        const auto keys_of = [&](int t, int page) INLINE {
             Keys k;
             const int j = range.key(t) + lane, at = max(0, min(j, s.len - 1));
             const bool is = (j < s.len) & (page >= 0) & (page < a.c.pages);
             k.there = __ballot(is);
-            const uint32_t row = is ? ((uint32_t)page * a.c.kv_heads + h) * a.c.page_size + (at - page_col(a, at) * a.c.page_size) : ~0u;
+            const uint32_t row = ((uint32_t)page * a.c.kv_heads + h) * a.c.page_size + (at - page_col(a, at) * a.c.page_size) | ~bit_mask(is);
 #pragma unroll
             for (int i = 0; i < NI; ++i) k.row[i] = (uint32_t)__shfl((int)row, load_key + i * RPI, 64);
             return k;
         };
-        const auto load = [&](const uint16_t* base, const Keys& k, int to, bool values) {
+        const auto load = [&](const uint16_t* base, const Keys& k, int to, bool values) INLINE {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int key = load_key + i * RPI;
-                const int piece = (lane % PIECES) ^ ((values ? 2 * key : key) & SW);
-                const bool in = (k.row[i] != ~0u) & (8 * piece < a.c.dim);
-                const uint16_t* p = in ? base + (size_t)k.row[i] * a.c.dim + 8 * piece : reinterpret_cast<const uint16_t*>(zero_piece);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (lds_void*)(lds3 + to + (wave * NI + i) * 1024),
-                                                 16, 0, 0);
+                const int piece = values ? v_piece ^ (2 * i * RPI & SW) : k_piece ^ (i * RPI & SW);
+                // selected with masks, not with branches: a divergent branch in the loop would keep it off scalar control flow
+                const uint32_t in = bit_mask(k.row[i] != ~0u) & bit_mask(8 * piece < a.c.dim);
+                const uint64_t there_at = reinterpret_cast<uint64_t>(base) + ((uint64_t)k.row[i] * a.c.dim + 8 * piece) * 2;
+                const uint64_t keep = (uint64_t)in << 32 | in;
+                const void* p = reinterpret_cast<const void*>((there_at & keep) | (reinterpret_cast<uint64_t>(zero_piece) & ~keep));
+                load_to_lds(p, lds_base + to + (wave * NI + i) * 1024);
             }
         };
         const auto k_tile = [&](int i) { return i % BUFS * TILE; };
@@ -317,205 +330,264 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
 
         f16v sc[2];
         vec wt[NP][4];
-        bool weighed = false, odd = false;  // the tile before left weights; its V holds values that are not finite
-        uint32_t see[2] = {~0u, ~0u};
-        for (int i = 0; i <= n; ++i) {
-            const int j0 = range.key(min(t0 + i, t1 - 1));
-            // products
-            if (weighed) {
-                lds_byte* vt = lds3 + v_tile(i - 1);
+        constexpr int LEAD = 4, NV = 4 * DT, NK = 2 * STEPS;  // operands read ahead of their use; operands of a tile's V and K
+        const auto v_operand = [&](int tile, int k) INLINE {
+            lds_byte* at = (lds_byte*)((uintptr_t)(lds3 + (v_at + tile)) ^ (64 * (k % DT)));
+            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + k / DT * 16 * ROW));
+            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + k / DT * 16 * ROW + 8 * ROW));
+            return __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        const auto k_operand = [&](int tile, int k) INLINE {
+            typedef __attribute__((address_space(3))) vec lds_vec;
+            return *(lds_vec*)(((uintptr_t)(lds3 + (k_at + tile)) ^ (32 * (k / 2))) + k % 2 * 32 * ROW);
+        };
+        // O^T += V^T P^T of the tile at vt, then S^T = K Q^T of the tile at kt, in one run of reads and products
+        const auto products = [&](int vt, int kt, auto with_v, auto with_k) INLINE {
+            constexpr int V0 = decltype(with_v)::value ? 0 : NV, N = decltype(with_k)::value ? NV + NK : NV;
+            vec ring[LEAD + 1];
+            const auto read = [&](auto k) INLINE {
+                constexpr int K = decltype(k)::value;
+                if constexpr (K < NV) ring[K % (LEAD + 1)] = v_operand(vt, K);
+                else ring[K % (LEAD + 1)] = k_operand(kt, K - NV);
+            };
+            unrolled<V0, (V0 + LEAD < N ? V0 + LEAD : N)>(read);
+            unrolled<V0, N>([&](auto k) INLINE {
+                constexpr int K = decltype(k)::value;
+                if constexpr (K + LEAD < N) read(Index<K + LEAD>{});
+                __builtin_amdgcn_sched_barrier(0);
+                const vec x = ring[K % (LEAD + 1)];
+                if constexpr (K < NV) {
 #pragma unroll
-                for (int st = 0; st < 4; ++st)
+                    for (int p = NP - 1; p >= 0; --p) o[K % DT] = mfma32(x, wt[p][K / DT], o[K % DT]);
+                } else {
+                    constexpr int E = K - NV;
+                    if constexpr (E / 2 == 0) sc[E % 2] = (f16v)(0.0f);
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vt + v_at[dt][0] + st * 16 * ROW));
-                        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vt + v_at[dt][1] + st * 16 * ROW));
-                        uint4 v = __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                        if (odd) { v.x = finite_only(v.x, kExp); v.y = finite_only(v.y, kExp); v.z = finite_only(v.z, kExp); v.w = finite_only(v.w, kExp); }
-#pragma unroll
-                        for (int p = NP - 1; p >= 0; --p) o[dt] = mfma32(__builtin_bit_cast(vec, v), wt[p][st], o[dt]);
-                    }
-            }
-            const bool works = i < n && row0 < s.rows && (j0 <= wp1 || j0 < s.prefix);  // some row of the wave may see the tile
-            if (works) {
-                const uint8_t* kt = lds + k_tile(i);
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) sc[kb][e] = 0.0f;
-#pragma unroll
-                    for (int st = 0; st < STEPS; ++st) {
-                        const vec k = *reinterpret_cast<const vec*>(kt + k_at[st] + kb * 32 * ROW);
-#pragma unroll
-                        for (int p = NP - 1; p >= 0; --p) sc[kb] = mfma32(k, q[p][st], sc[kb]);
-                    }
+                    for (int p = NP - 1; p >= 0; --p) sc[E % 2] = mfma32(x, q[p][E / 2], sc[E % 2]);
                 }
-            }
-            if (i == n) break;
-            phase_barrier<true>();
-
-            // weights
-            uint64_t far_there = 0;
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        const auto loads = [&](int i) INLINE {  // K of tile i + 2, V of tile i + 1
+            uint64_t far = 0;
             if (i + 1 < n) load(a.c.v, ahead, v_tile(i + 1), true);
             if (i + 2 < n) {
                 ahead = keys_of(t0 + i + 2, page);
-                far_there = ahead.there;
+                far = ahead.there;
                 load(a.c.k, ahead, k_tile(i + 2), false);
                 if (i + 3 < n) page = page_of(t0 + i + 3);
             }
-            weighed = works;
-            if (works) {
-                if constexpr (EXTRA) {  // to capped and biased scores (log2)
-                    if (a.softcap > 0.0f && NP == 1) {
-                        const float f = factor * (2.0f * kLog2e / a.softcap), top = a.softcap * kLog2e;
-#pragma unroll
-                        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                sc[kb][e] = fmaf(-2.0f * top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[kb][e] * f)), top);
-                    } else if (a.softcap > 0.0f) {
-                        const float f = factor / a.softcap, top = a.softcap * kLog2e;
-#pragma unroll
-                        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) sc[kb][e] = top * soft_tanh<true>(sc[kb][e] * f);
-                    } else {
-                        const float f = factor * kLog2e;
-#pragma unroll
-                        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) sc[kb][e] *= f;
-                    }
-                    if (a.slopes) {
-                        const float back = (float)(pos - j0 - 4 * hf);
-#pragma unroll
-                        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) sc[kb][e] = fmaf(-slope, fabsf(back - (float)(32 * kb + 8 * (e / 4) + e % 4)), sc[kb][e]);
-                    }
-                }
-                const bool full = there == ~0ull && ((j0 + T - 1 <= wp0 && (a.window <= 0 || wp1 - j0 < a.window)) || j0 + T <= s.prefix);
-                if (!full) {  // without branches: all 64 lanes take part in what follows
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) {
-                        see[kb] = seen_keys(a, s, pos, j0 + 32 * kb, (uint32_t)(there >> (32 * kb)));
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) sc[kb][e] = see[kb] >> (8 * (e / 4) + e % 4) >> (4 * hf) & 1u ? sc[kb][e] : -INFINITY;
-                    }
-                } else {
-                    see[0] = see[1] = ~0u;
-                }
-                // Weights against the row's reference. Their sum bounds the largest of them: only where it passes the limit
-                // (or the row has no reference yet) is a maximum looked for, the reference raised and the sums scaled down.
-                float sum;
-                const auto weigh = [&]() {
-                    const float base = m == -INFINITY ? 0.0f : m - kShift;
-                    sum = 0.0f;
-#pragma unroll
-                    for (int st = 0; st < 4; ++st)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float x = sc[st / 2][8 * (st & 1) + e];
-                            const float v = __builtin_amdgcn_exp2f(EXTRA ? x - base : fmaf(x, factor, -base));
-                            sum += v;
-                            typename Half8<CT>::one t[NP];
-                            split_terms<CT, NP>(v, t);
-#pragma unroll
-                            for (int p = 0; p < NP; ++p) wt[p][st][e] = t[p];
-                        }
-                };
-                weigh();
-                if (__ballot((sum > kLimit) | (m == -INFINITY))) {
-                    float top = -INFINITY;
+            return far;
+        };
+        if (row0 >= s.rows) {  // a wave without rows brings its share of the tiles
+            for (int i = 0; i < n; ++i) {
+                phase_barrier<true>();
+                (void)loads(i);
+                phase_barrier<false>();
+            }
+            if (PAIRED && wave < WAVES / 2) phase_barrier<false>();
+            u += whole ? blocks : n;
+            continue;
+        }
+        uint32_t see[2];
+        uint64_t far_there = 0;
+        const auto begin_weights = [&](int i) INLINE {  // the second phase, up to scores (log2, or raw ones that `factor` scales)
+            const int j0 = range.key(t0 + i);
+            phase_barrier<true>();
+            far_there = loads(i);
+            see[0] = see[1] = ~0u;
+            if constexpr (EXTRA) {  // to capped and biased scores (log2)
+                if (a.softcap > 0.0f && NP == 1) {
+                    const float f = factor * (2.0f * kLog2e / a.softcap), top = a.softcap * kLog2e;
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[kb][e]);
-                    if (!EXTRA) top *= factor;
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float raised = fmaxf(m, top);
-                    const float fade = raised == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
-                    m = raised;
-                    l *= fade;
+                        for (int e = 0; e < 16; ++e)
+                            sc[kb][e] = fmaf(-2.0f * top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[kb][e] * f)), top);
+                } else if (a.softcap > 0.0f) {
+                    const float f = factor / a.softcap, top = a.softcap * kLog2e;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
+                    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[dt][e] *= fade;
-                    weigh();
+                        for (int e = 0; e < 16; ++e) sc[kb][e] = top * soft_tanh<true>(sc[kb][e] * f);
+                } else {
+                    const float f = factor * kLog2e;
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sc[kb][e] *= f;
                 }
-                l += sum;
+                if (a.slopes) {
+                    const float back = (float)(pos - j0 - 4 * hf);
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sc[kb][e] = fmaf(-slope, fabsf(back - (float)(32 * kb + 8 * (e / 4) + e % 4)), sc[kb][e]);
+                }
             }
-            phase_barrier<false>();
-            // Values that are not finite and that a row does not see would spoil its sums (0 times infinity), and so would
-            // seen ones where weights have several terms: they are added apart, and the products pass over them.
-            odd = false;
-            if (works && (NP > 1 || __ballot((see[0] & see[1]) != ~0u))) {
-                const uint8_t* vt = lds + v_tile(i);
-                uint32_t any = 0;
+            const bool full = there == ~0ull && ((j0 + T - 1 <= wp0 && (a.window <= 0 || wp1 - j0 < a.window)) || j0 + T <= s.prefix);
+            if (!full) {  // without branches: all 64 lanes take part in what follows
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    see[kb] = seen_keys(a, s, pos, j0 + 32 * kb, (uint32_t)(there >> (32 * kb)));
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sc[kb][e] = see[kb] >> (8 * (e / 4) + e % 4) >> (4 * hf) & 1u ? sc[kb][e] : -INFINITY;
+                }
+            }
+        };
+        // Weights against the row's reference. Their sum bounds the largest of them: only where it passes the limit (or the row
+        // has no reference yet) is a maximum looked for, the reference raised and the sums scaled down.
+        float sum = 0.0f;
+        const auto weigh = [&]() INLINE {
+            const float base = m == -INFINITY ? 0.0f : m - kShift;
+            sum = 0.0f;
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = sc[st / 2][8 * (st & 1) + e];
+                    const float v = __builtin_amdgcn_exp2f(EXTRA ? x - base : fmaf(x, factor, -base));
+                    sum += v;
+                    typename Half8<CT>::one t[NP];
+                    split_terms<CT, NP>(v, t);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) wt[p][st][e] = t[p];
+                }
+        };
+        const auto past_limit = [&]() INLINE { return (int)__builtin_amdgcn_readfirstlane(__ballot((sum > kLimit) | (m == -INFINITY)) != 0); };
+        const auto raise_reference = [&]() INLINE {
+            float top = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[kb][e]);
+            if (!EXTRA) top *= factor;
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float raised = fmaxf(m, top);
+            const float fade = raised == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
+            m = raised;
+            l *= fade;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = o[dt] * (f16v)(fade);
+        };
+        // Values that are not finite and that a row does not see would spoil its sums (0 times infinity), and so would seen
+        // ones where weights have several terms: whether the tile holds any such.
+        const auto find_odd = [&](int i) INLINE {
+            if (NP == 1 && !__builtin_amdgcn_readfirstlane(__ballot((see[0] & see[1]) != ~0u) != 0)) return 0;
+            const uint8_t* vt = lds + v_tile(i);
+            uint32_t any = 0;
 #pragma unroll 4
-                for (int e = 0; e < TILE / 1024; ++e) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vt + (e * 64 + lane) * 16);
-                    any |= v.x ^ finite_only(v.x, kExp);
-                    any |= v.y ^ finite_only(v.y, kExp);
-                    any |= v.z ^ finite_only(v.z, kExp);
-                    any |= v.w ^ finite_only(v.w, kExp);
-                }
-                odd = __ballot(any != 0) != 0;
-                if (odd) {
-                    for (int key = 0; key < T; ++key) {
-                        const uint32_t mine = (key < 32 ? see[0] >> key : see[1] >> (key - 32)) & 1u;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int g = 0; g < 4; ++g) {  // dimensions 32 dt + 8 g + 4 hf .. + 3
-                                const int piece = (4 * dt + g) ^ (2 * key & SW);
-                                const uint2 v = *reinterpret_cast<const uint2*>(vt + key * ROW + piece * 16 + 8 * hf);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const uint32_t bits = (e < 2 ? v.x : v.y) >> (16 * (e & 1)) & 0xFFFFu;
-                                    const float val = CT == BYHIP_F16 ? (float)bits_h((uint16_t)bits) : __builtin_bit_cast(float, bits << 16);
-                                    o[dt][4 * g + e] += mine & (uint32_t)((bits & kExp) == kExp) ? val : 0.0f;
-                                }
-                            }
-                    }
-                }
+            for (int e = 0; e < TILE / 1024; ++e) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vt + (e * 64 + lane) * 16);
+                any |= v.x ^ finite_only(v.x, kExp);
+                any |= v.y ^ finite_only(v.y, kExp);
+                any |= v.z ^ finite_only(v.z, kExp);
+                any |= v.w ^ finite_only(v.w, kExp);
             }
+            return (int)__builtin_amdgcn_readfirstlane(__ballot(any != 0) != 0);
+        };
+        const auto weights = [&](int i) INLINE {
+            begin_weights(i);
+            weigh();
+            if (past_limit()) {
+                raise_reference();
+                weigh();
+            }
+            l += sum;
+            phase_barrier<false>();
+        };
+        const auto odd_values = [&](int i) INLINE {  // they are added to the rows that see them, and the products pass over them
+            const uint8_t* vt = lds + v_tile(i);
+            for (int key = 0; key < T; ++key) {
+                const uint32_t mine = (key < 32 ? see[0] >> key : see[1] >> (key - 32)) & 1u;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    f16v add;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {  // dimensions 32 dt + 8 g + 4 hf .. + 3
+                        const int piece = (4 * dt + g) ^ (2 * key & SW);
+                        const uint2 v = *reinterpret_cast<const uint2*>(vt + key * ROW + piece * 16 + 8 * hf);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t bits = (e < 2 ? v.x : v.y) >> (16 * (e & 1)) & 0xFFFFu;
+                            const float val = CT == BYHIP_F16 ? (float)bits_h((uint16_t)bits) : __builtin_bit_cast(float, bits << 16);
+                            add[4 * g + e] = mine & (uint32_t)((bits & kExp) == kExp) ? val : 0.0f;
+                        }
+                    }
+                    o[dt] = o[dt] + add;
+                }
+                }
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const uint4 v = __builtin_bit_cast(uint4, v_operand(v_tile(i), k));
+                const vec x = __builtin_bit_cast(vec, make_uint4(finite_only(v.x, kExp), finite_only(v.y, kExp), finite_only(v.z, kExp), finite_only(v.w, kExp)));
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) o[k % DT] = mfma32(x, wt[p][k / DT], o[k % DT]);
+            }
+        };
+        // A loop with one exit and no choice but the rare raise in it: with more, the compiler carries all sums twice. A tile
+        // with odd values, and the last one, end it; what then remains runs in a loop of its own.
+        int i = 0;
+        products(0, k_tile(0), Index<0>{}, Index<1>{});
+        weights(0);
+        int odd = find_odd(0);
+        const auto next = [&]() INLINE {
             there = next_there;
             next_there = far_there;
+            weights(++i);
+            odd = find_odd(i);
+        };
+        while ((i < n - 1) & (odd == 0)) {
+            products(v_tile(i), k_tile(i + 1), Index<1>{}, Index<1>{});
+            next();
         }
+        while (i < n - 1) {
+            if (odd) odd_values(i);
+            else products(v_tile(i), 0, Index<1>{}, Index<0>{});
+            products(0, k_tile(i + 1), Index<0>{}, Index<1>{});
+            next();
+        }
+        if (odd) odd_values(i);
+        else products(v_tile(i), 0, Index<1>{}, Index<0>{});
         if (PAIRED && wave < WAVES / 2) phase_barrier<false>();
+
 
         // 4. the wave's rows leave, whole or as a part
         const bool begins = t0 == 0, ends = t1 == range.tiles;
         l += __shfl_xor(l, 32, 64);
         if (begins && ends) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (valid) {
-                const size_t out = (size_t)(a.s.starts[b] + token) * a.out_stride + (size_t)hq * a.c.dim;
+            const size_t at = (size_t)(a.s.starts[b] + token) * a.out_stride + (size_t)hq * a.c.dim + 4 * hf;
+            const auto leave = [&](auto dtype, auto vector) {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const int d = 32 * dt + 8 * g + 4 * hf;
+                        const int d = 32 * dt + 8 * g;
+                        if (d >= a.c.dim) continue;  // the same for all lanes: heads are multiples of 8
                         float x[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = l == 0.0f ? 0.0f : o[dt][4 * g + e] * inv;
-                        if (d < a.c.dim) {
-                            if (a.out_vec) {
-                                store_vec<4>(a.out, out + d, x, a.out_dtype);
-                            } else {
+                        if constexpr (decltype(vector)::value) {
+                            store_vec<4>(a.out, at + d, x, decltype(dtype)::value);
+                        } else {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const float one[1] = {x[e]};
-                                    store_vec<1>(a.out, out + d + e, one, a.out_dtype);
-                                }
-                            }
+                            for (int e = 0; e < 4; ++e) store_y<decltype(dtype)::value>(a.out, at + d + e, x[e]);
                         }
                     }
+            };
+            const auto leave_as = [&](auto dtype) {
+                if (a.out_vec) leave(dtype, Index<1>{});
+                else leave(dtype, Index<0>{});
+            };
+            if (valid) {
+                if (a.out_dtype == BYHIP_F32) leave_as(Index<BYHIP_F32>{});
+                else if (a.out_dtype == BYHIP_F16) leave_as(Index<BYHIP_F16>{});
+                else leave_as(Index<BYHIP_BF16>{});
             }
-        } else {
-            float* slot = part_slot<R, DIM>(a.part, begins ? 2 * w + 1 : 2 * w);
+        } else if (valid) {
             const int r = wave * 32 + c;
+            float* slot = part_slot<R, DIM>(a.part, begins ? 2 * w + 1 : 2 * w);
             if (hf == 0) {
                 slot[R * DIM + r] = m;
                 slot[R * DIM + R + r] = l;

@@ -68,7 +68,7 @@ struct Rows {
         const int page = a.s.table[(size_t)b * a.s.stride + col];
         const bool is = (j < s.len) & (page >= 0) & (page < a.c.pages);
         there = (uint32_t)__ballot(is);
-        return is ? ((uint32_t)page * a.c.kv_heads + head) * a.c.page_size + (at - col * a.c.page_size) : 0u;
+        return (((uint32_t)page * a.c.kv_heads + head) * a.c.page_size + (at - col * a.c.page_size)) & bit_mask(is);
     }
     __device__ __forceinline__ void load_k(KTile& k, uint32_t rows) const {
 #pragma unroll
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
         if (tid == 255) before[a.s.batch] = base + sum;
         __syncthreads();
     }
-    const long long per_head = before[a.s.batch], total = per_head * a.c.kv_heads;
+    const long long per_head = uniform(before[a.s.batch]), total = per_head * a.c.kv_heads;
     // 2. this block's run of units
     const long long blocks = min((long long)gridDim.x, max(1LL, (total + kWaves - 1) / kWaves));
     const int w = blockIdx.x;
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
 
     Rows<CT, NP, DIM, EXTRA> r(a);
     for (long long u = u0; u < u1;) {
-        const int h = __builtin_amdgcn_readfirstlane((int)(u / per_head));
+        const int h = (int)(u / per_head);
         const long long in_head = u - h * per_head;
         int lo = 0, hi = a.s.batch - 1;
         while (lo < hi) {
@@ -327,12 +327,12 @@ __global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
             if (before[mid] <= in_head) lo = mid;
             else hi = mid - 1;
         }
-        const int b = __builtin_amdgcn_readfirstlane(lo);
-        const long long local = in_head - before[b];
+        const int b = uniform(lo);
+        const long long local = in_head - uniform(before[b]);
         SeqInfo s = seq_info(a, b);
         const auto range = tiles_of(s);
-        const int rt = __builtin_amdgcn_readfirstlane((int)(local / range.tiles)), t0 = __builtin_amdgcn_readfirstlane((int)(local % range.tiles));
-        const int t1 = __builtin_amdgcn_readfirstlane((int)min((long long)range.tiles, t0 + (u1 - u)));
+        const int rt = (int)(local / range.tiles), t0 = (int)(local % range.tiles);
+        const int t1 = (int)min((long long)range.tiles, t0 + (u1 - u));
         r.begin(b, h, rt);
         const int p0 = s.first_pos + rt * kRows / a.group, p1 = s.first_pos + (min(s.rows, (rt + 1) * kRows) - 1) / a.group;
 
