@@ -24,6 +24,7 @@ struct AttnArgs {
     int min_rows, max_rows;  // rows (tokens x group) of the sequences this launch takes
     float* part;     // partial results
     int4* joins;     // one description per block
+    const void* zeros;  // 16 zero bytes: what keys and values outside the cache read as
 };
 
 // Column of key j (below 2^31) in its table row. With l = ceil(log2(page size)) and page_mul = ceil(2^(31 + l) / page size),

@@ -100,6 +100,7 @@ bool takes(const AttnArgs& a) {
 
 void launch_tiled(AttnArgs a) {
     a.joins = static_cast<int4*>(attn_workspace());
+    a.zeros = static_cast<char*>(attn_workspace()) + kAttnWorkspaceBytes;
     a.part = reinterpret_cast<float*>(static_cast<char*>(attn_workspace()) + kAttnJoinBytes);
     const bool precise = a.q_dtype == BYHIP_F32 || a.out_dtype == BYHIP_F32, f16 = a.cache_dtype == BYHIP_F16;
     // The lengths are on the device: one sequence has all rows; as many rows as sequences are decoding; else

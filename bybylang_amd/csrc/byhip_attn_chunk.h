@@ -32,7 +32,6 @@ constexpr int kXcds = 8;
 constexpr int kCutTiles = 8;
 // Key tiles a block should at least get before another one takes part.
 constexpr int kShareTiles = 4;
-__device__ __attribute__((aligned(64))) uint32_t zero_piece[16];  // what keys and values outside the cache read as
 
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -307,24 +306,27 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 const uint32_t in = bit_mask(k.row[i] != ~0u) & bit_mask(8 * piece < a.c.dim);
                 const uint64_t there_at = reinterpret_cast<uint64_t>(base) + ((uint64_t)k.row[i] * a.c.dim + 8 * piece) * 2;
                 const uint64_t keep = (uint64_t)in << 32 | in;
-                const void* p = reinterpret_cast<const void*>((there_at & keep) | (reinterpret_cast<uint64_t>(zero_piece) & ~keep));
+                const void* p = reinterpret_cast<const void*>((there_at & keep) | (reinterpret_cast<uint64_t>(a.zeros) & ~keep));
                 load_to_lds(p, lds_base + to + (wave * NI + i) * 1024);
             }
         };
         const auto k_tile = [&](int i) { return i % BUFS * TILE; };
         const auto v_tile = [&](int i) { return (BUFS + i % BUFS) * TILE; };
-        Keys ahead = keys_of(t0, page_of(t0));  // the newest tile whose keys are known: K loaded, V not yet
-        uint64_t there = ahead.there, next_there = 0;
+        // V of tile i + 1 and K of tile i + 2 are loaded together; the keys of tile i + 3 are looked up meanwhile, from the page
+        // that was asked for a tile before
+        Keys v_keys = keys_of(t0, page_of(t0)), k_keys = v_keys;
+        uint64_t there = v_keys.there, next_there = 0;
         int page = n > 1 ? page_of(t0 + 1) : 0;
         phase_barrier<true>();  // the item before has been read
-        load(a.c.k, ahead, k_tile(0), false);
-        load(a.c.v, ahead, v_tile(0), true);
+        load(a.c.k, v_keys, k_tile(0), false);
+        load(a.c.v, v_keys, v_tile(0), true);
         if (n > 1) {
-            ahead = keys_of(t0 + 1, page);
-            next_there = ahead.there;
-            load(a.c.k, ahead, k_tile(1), false);
-            if (n > 2) page = page_of(t0 + 2);
+            v_keys = keys_of(t0 + 1, page);
+            next_there = v_keys.there;
+            load(a.c.k, v_keys, k_tile(1), false);
         }
+        if (n > 2) k_keys = keys_of(t0 + 2, page_of(t0 + 2));
+        if (n > 3) page = page_of(t0 + 3);
         phase_barrier<true>();
         if (PAIRED && wave >= WAVES / 2) phase_barrier<false>();
 
@@ -368,21 +370,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        const auto loads = [&](int i) INLINE {  // K of tile i + 2, V of tile i + 1
-            uint64_t far = 0;
-            if (i + 1 < n) load(a.c.v, ahead, v_tile(i + 1), true);
-            if (i + 2 < n) {
-                ahead = keys_of(t0 + i + 2, page);
-                far = ahead.there;
-                load(a.c.k, ahead, k_tile(i + 2), false);
-                if (i + 3 < n) page = page_of(t0 + i + 3);
-            }
-            return far;
+        const auto loads = [&](int i) INLINE {  // at the start of the second phase
+            if (i + 1 < n) load(a.c.v, v_keys, v_tile(i + 1), true);
+            if (i + 2 < n) load(a.c.k, k_keys, k_tile(i + 2), false);
+        };
+        const auto look_up = [&](int i) INLINE {  // at its end
+            v_keys = k_keys;
+            if (i + 3 < n) k_keys = keys_of(t0 + i + 3, page);
+            if (i + 4 < n) page = page_of(t0 + i + 4);
         };
         if (row0 >= s.rows) {  // a wave without rows brings its share of the tiles
             for (int i = 0; i < n; ++i) {
                 phase_barrier<true>();
-                (void)loads(i);
+                loads(i);
+                look_up(i);
                 phase_barrier<false>();
             }
             if (PAIRED && wave < WAVES / 2) phase_barrier<false>();
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
         const auto begin_weights = [&](int i) INLINE {  // the second phase, up to scores (log2, or raw ones that `factor` scales)
             const int j0 = range.key(t0 + i);
             phase_barrier<true>();
-            far_there = loads(i);
+            loads(i);
             see[0] = see[1] = ~0u;
             if constexpr (EXTRA) {  // to capped and biased scores (log2)
                 if (a.softcap > 0.0f && NP == 1) {
@@ -494,6 +495,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 weigh();
             }
             l += sum;
+            far_there = k_keys.there;
+            look_up(i);
             phase_barrier<false>();
         };
         const auto odd_values = [&](int i) INLINE {  // they are added to the rows that see them, and the products pass over them

@@ -81,7 +81,7 @@ int compute_units();
 // stream uses it in stream order.
 constexpr size_t kWorkspaceBytes = 32u << 20;
 void* workspace();
-// The same for the partial results of attention over a paged cache.
+// The same for the partial results of attention over a paged cache; 256 zero bytes follow it.
 constexpr size_t kAttnWorkspaceBytes = (size_t)80 << 20;
 void* attn_workspace();
 // Takes the device address of byhip_q4_matmul_static's scratch array on `device` (current).
