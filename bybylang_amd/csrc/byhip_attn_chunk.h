@@ -37,18 +37,23 @@ typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-// Workgroup barrier after this wave's LDS reads, and with LOADS also once its direct loads have landed.
-template <bool LOADS>
+// Workgroup barrier after this wave's LDS reads, and unless LATEST < 0 once all its direct loads but the LATEST last ones have
+// landed (they land in order; loads of the compiler's own among the last only make it wait for more).
+template <int LATEST>
 __device__ __forceinline__ void phase_barrier() {
-    if constexpr (LOADS) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if constexpr (LATEST >= 0) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATEST) : "memory");
     else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // 16 bytes per lane from memory to LDS byte `to` + 16 lane. Written as assembly because the compiler makes every later LDS
-// read wait for such loads, which here belong to tiles still ahead; it has no output register, phase_barrier<true> waits for
+// read wait for such loads, which here belong to tiles still ahead; it has no output register, phase_barrier waits for
 // it, and a wait of the compiler's own that counts it among its loads only waits longer.
 __device__ __forceinline__ void load_to_lds(const void* p, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory");
+}
+// The same for 4 bytes per lane.
+__device__ __forceinline__ void word_to_lds(const void* p, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(to) : "memory");
 }
 
 template <int I> struct Index { static constexpr int value = I; };
@@ -68,14 +73,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     constexpr int ROW = DIM * 2, TILE = T * ROW;                  // bytes of a key, of a tile
     constexpr int NI = TILE / 1024 / WAVES, RPI = 1024 / ROW;     // direct loads per wave and tile, keys per load
     constexpr bool PAIRED = WAVES == 8;                           // two waves per SIMD, half a tile apart
-    constexpr int BUFS = PAIRED ? 3 : 2;
+    constexpr int AHEAD = DIM <= 128 ? 2 : 1;                     // tiles between the loads of one and its use
+    constexpr int BUFS = AHEAD + (PAIRED ? 2 : 1);
+    constexpr int SLOTS = 2 * AHEAD;                              // page lookups on their way and in use
+    constexpr int BATCH = 2 * NI + 1;                             // a wave's direct loads per tile
     constexpr float kShift = CT == BYHIP_F16 ? 4.0f : 0.0f;       // log2 of the weights' factor
     constexpr float kLimit = 32768.0f;                            // a lane's weights of a tile may add up to this
     constexpr uint32_t kExp = CT == BYHIP_F16 ? 0x7C00u : 0x7F80u;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BUFS * TILE];  // BUFS tiles of K, then of V
+    __shared__ __attribute__((aligned(256))) int looked_up[WAVES][SLOTS][64];  // each wave's pages of the keys of tiles ahead
     __shared__ int row_tiles[kAttnBatch + 1];                                // row tiles of the sequences before each
     __shared__ long long units_before[NT + 1];                               // key tiles of the row tiles before each thread's run
     __shared__ long long wave_total[WAVES];
+    __shared__ int not_finite;                                               // the last pass whose sums were not
     __shared__ int longest;                                                  // key tiles of the largest item
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, hf = lane >> 5;
@@ -131,7 +141,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     {
         long long sum = 0;
         int b, top = 0;
-        if (tid == 0) longest = 0;
+        if (tid == 0) longest = not_finite = 0;
         for (int x = tid * run; x < min((tid + 1) * run, all_row_tiles); ++x) {
             const int n = tiles_at(x, b);
             sum += n;
@@ -156,6 +166,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     }
     const long long u0 = whole ? w : total * w / blocks, u1 = whole ? items : total * (w + 1) / blocks;
     int4 join = make_int4(0, 0, 0, 0);
+    int pass = 0;
 
     // This lane's places in the LDS tiles: pieces 2 st + hf of key c at k_at ^ 32 st (K's piece i of key j lies at i ^ j), and
     // keys 4 hf + (lane % 16) / 4 (+ 8 j + 16 st), values 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) at v_at ^ 64 dt (V's
@@ -167,6 +178,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     const int load_key = wave * NI * RPI + lane / PIECES;
     const int k_piece = (lane % PIECES) ^ (load_key & SW), v_piece = (lane % PIECES) ^ (2 * load_key & SW);
     lds_byte* const lds3 = (lds_byte*)lds;
+    const uint32_t pages_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_byte*)looked_up[wave][0]);
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds3);
 
     for (long long u = u0; u < u1;) {
@@ -201,6 +213,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
         positions(s, rt, p0, p1);
         const TileRange<T> range(a, s, p0, p1);
         t1 = whole ? range.tiles : (int)min((long long)range.tiles, t0 + (u1 - u));
+
+        const auto page_at = [&](int t) INLINE {  // the table's entry of key `lane` of tile t
+            const int at = max(0, min(range.key(t) + lane, s.len - 1));
+            return a.s.table + (size_t)b * a.s.stride + page_col(a, at);
+        };
+        int first_pages[AHEAD + 2];
+#pragma unroll
+        for (int i = 0; i < AHEAD + 2; ++i) first_pages[i] = *page_at(t0 + i);
 
         // 2. the wave's rows
         const int row0 = rt * R + wave * 32, row = row0 + c;
@@ -269,29 +289,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
             }
             factor = ldexpf(EXTRA ? a.scale : a.scale * kLog2e, -shift);
         }
-        float m = -INFINITY, l = 0.0f;
+        float m, l;
         // O^T as whole vectors throughout: a loop over its elements would have the compiler carry 16 scalars per vector and
         // copy them together for every product
         f16v o[DT];
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v)(0.0f);
 
         // 3. key tiles. A tile's work is two phases with a barrier after each: products (O^T += V^T P^T of the tile
         // before, S^T = K Q^T of this one) and weights (exponentials of S^T; the direct loads of K two tiles and V one tile
         // ahead). Of two waves on a SIMD one runs a phase behind the other, so that one's products go with the other's weights.
         const int n = t1 - t0;
-        const auto page_of = [&](int t) INLINE {  // the page of key `lane` of tile t
-            const int j = range.key(t) + lane, at = max(0, min(j, s.len - 1));
-            return a.s.table[(size_t)b * a.s.stride + page_col(a, at)];
-        };
         struct Keys {
             uint32_t row[NI];  // the cache rows this lane loads, ~0: none
-            uint64_t there;    // bit j: key j exists
+            uint64_t there;    // bit j: key j exists; none past the share's last tile, whose loads are of zeros
         };
         const auto keys_of = [&](int t, int page) INLINE {
             Keys k;
             const int j = range.key(t) + lane, at = max(0, min(j, s.len - 1));
-            const bool is = (j < s.len) & (page >= 0) & (page < a.c.pages);
+            const bool is = (t < t1) & (j < s.len) & (page >= 0) & (page < a.c.pages);
             k.there = __ballot(is);
             const uint32_t row = ((uint32_t)page * a.c.kv_heads + h) * a.c.page_size + (at - page_col(a, at) * a.c.page_size) | ~bit_mask(is);
 #pragma unroll
@@ -312,24 +326,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
         };
         const auto k_tile = [&](int i) { return i % BUFS * TILE; };
         const auto v_tile = [&](int i) { return (BUFS + i % BUFS) * TILE; };
-        // V of tile i + 1 and K of tile i + 2 are loaded together; the keys of tile i + 3 are looked up meanwhile, from the page
-        // that was asked for a tile before
-        Keys v_keys = keys_of(t0, page_of(t0)), k_keys = v_keys;
-        uint64_t there = v_keys.there, next_there = 0;
-        int page = n > 1 ? page_of(t0 + 1) : 0;
-        phase_barrier<true>();  // the item before has been read
-        load(a.c.k, v_keys, k_tile(0), false);
-        load(a.c.v, v_keys, v_tile(0), true);
-        if (n > 1) {
-            v_keys = keys_of(t0 + 1, page);
-            next_there = v_keys.there;
-            load(a.c.k, v_keys, k_tile(1), false);
-        }
-        if (n > 2) k_keys = keys_of(t0 + 2, page_of(t0 + 2));
-        if (n > 3) page = page_of(t0 + 3);
-        phase_barrier<true>();
-        if (PAIRED && wave >= WAVES / 2) phase_barrier<false>();
-
+        // Phase i loads a batch: V of tile i + AHEAD, K of tile i + AHEAD + 1 and the pages of tile i + 2 AHEAD + 2. Batch
+        // i - AHEAD has landed when phase i begins.
+        Keys v_keys, k_keys;
+        uint64_t there[AHEAD + 1];  // of tiles i ..
+        const auto look_up_to = [&](int t, int slot) INLINE { word_to_lds(page_at(t), pages_base + slot * 256); };
+        const auto loads = [&](int i) INLINE {
+            load(a.c.v, v_keys, v_tile(i + AHEAD), true);
+            load(a.c.k, k_keys, k_tile(i + AHEAD + 1), false);
+            look_up_to(t0 + i + 2 * AHEAD + 2, (i + AHEAD) % SLOTS);
+        };
+        const auto look_up = [&](int i) INLINE {  // at its end
+            v_keys = k_keys;
+            k_keys = keys_of(t0 + i + AHEAD + 2, looked_up[wave][i % SLOTS][lane]);
+        };
         f16v sc[2];
         vec wt[NP][4];
         constexpr int LEAD = 4, NV = 4 * DT, NK = 2 * STEPS;  // operands read ahead of their use; operands of a tile's V and K
@@ -370,31 +380,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        const auto loads = [&](int i) INLINE {  // at the start of the second phase
-            if (i + 1 < n) load(a.c.v, v_keys, v_tile(i + 1), true);
-            if (i + 2 < n) load(a.c.k, k_keys, k_tile(i + 2), false);
-        };
-        const auto look_up = [&](int i) INLINE {  // at its end
-            v_keys = k_keys;
-            if (i + 3 < n) k_keys = keys_of(t0 + i + 3, page);
-            if (i + 4 < n) page = page_of(t0 + i + 4);
-        };
-        if (row0 >= s.rows) {  // a wave without rows brings its share of the tiles
-            for (int i = 0; i < n; ++i) {
-                phase_barrier<true>();
-                loads(i);
-                look_up(i);
-                phase_barrier<false>();
-            }
-            if (PAIRED && wave < WAVES / 2) phase_barrier<false>();
-            u += whole ? blocks : n;
-            continue;
-        }
         uint32_t see[2];
-        uint64_t far_there = 0;
         const auto begin_weights = [&](int i) INLINE {  // the second phase, up to scores (log2, or raw ones that `factor` scales)
             const int j0 = range.key(t0 + i);
-            phase_barrier<true>();
+            phase_barrier<(AHEAD - 1) * BATCH>();
             loads(i);
             see[0] = see[1] = ~0u;
             if constexpr (EXTRA) {  // to capped and biased scores (log2)
@@ -426,11 +415,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                         for (int e = 0; e < 16; ++e) sc[kb][e] = fmaf(-slope, fabsf(back - (float)(32 * kb + 8 * (e / 4) + e % 4)), sc[kb][e]);
                 }
             }
-            const bool full = there == ~0ull && ((j0 + T - 1 <= wp0 && (a.window <= 0 || wp1 - j0 < a.window)) || j0 + T <= s.prefix);
+            const bool full = there[0] == ~0ull && ((j0 + T - 1 <= wp0 && (a.window <= 0 || wp1 - j0 < a.window)) || j0 + T <= s.prefix);
             if (!full) {  // without branches: all 64 lanes take part in what follows
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
-                    see[kb] = seen_keys(a, s, pos, j0 + 32 * kb, (uint32_t)(there >> (32 * kb)));
+                    see[kb] = seen_keys(a, s, pos, j0 + 32 * kb, (uint32_t)(there[0] >> (32 * kb)));
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sc[kb][e] = see[kb] >> (8 * (e / 4) + e % 4) >> (4 * hf) & 1u ? sc[kb][e] : -INFINITY;
                 }
@@ -471,22 +460,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt] = o[dt] * (f16v)(fade);
         };
-        // Values that are not finite and that a row does not see would spoil its sums (0 times infinity), and so would seen
-        // ones where weights have several terms: whether the tile holds any such.
-        const auto find_odd = [&](int i) INLINE {
-            if (NP == 1 && !__builtin_amdgcn_readfirstlane(__ballot((see[0] & see[1]) != ~0u) != 0)) return 0;
-            const uint8_t* vt = lds + v_tile(i);
-            uint32_t any = 0;
-#pragma unroll 4
-            for (int e = 0; e < TILE / 1024; ++e) {
-                const uint4 v = *reinterpret_cast<const uint4*>(vt + (e * 64 + lane) * 16);
-                any |= v.x ^ finite_only(v.x, kExp);
-                any |= v.y ^ finite_only(v.y, kExp);
-                any |= v.z ^ finite_only(v.z, kExp);
-                any |= v.w ^ finite_only(v.w, kExp);
-            }
-            return (int)__builtin_amdgcn_readfirstlane(__ballot(any != 0) != 0);
-        };
         const auto weights = [&](int i) INLINE {
             begin_weights(i);
             weigh();
@@ -495,11 +468,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 weigh();
             }
             l += sum;
-            far_there = k_keys.there;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) there[k] = there[k + 1];
+            there[AHEAD] = k_keys.there;
             look_up(i);
-            phase_barrier<false>();
+            phase_barrier<-1>();
         };
-        const auto odd_values = [&](int i) INLINE {  // they are added to the rows that see them, and the products pass over them
+        const auto odd_values = [&](int i) INLINE {  // O^T += V^T P^T of the finite values, and the others where they are seen
             const uint8_t* vt = lds + v_tile(i);
             for (int key = 0; key < T; ++key) {
                 const uint32_t mine = (key < 32 ? see[0] >> key : see[1] >> (key - 32)) & 1u;
@@ -519,7 +494,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                     }
                     o[dt] = o[dt] + add;
                 }
-                }
+            }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const uint4 v = __builtin_bit_cast(uint4, v_operand(v_tile(i), k));
@@ -528,32 +503,66 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 for (int p = NP - 1; p >= 0; --p) o[k % DT] = mfma32(x, wt[p][k / DT], o[k % DT]);
             }
         };
-        // A loop with one exit and no choice but the rare raise in it: with more, the compiler carries all sums twice. A tile
-        // with odd values, and the last one, end it; what then remains runs in a loop of its own.
-        int i = 0;
-        products(0, k_tile(0), Index<0>{}, Index<1>{});
-        weights(0);
-        int odd = find_odd(0);
-        const auto next = [&]() INLINE {
-            there = next_there;
-            next_there = far_there;
-            weights(++i);
-            odd = find_odd(i);
-        };
-        while ((i < n - 1) & (odd == 0)) {
-            products(v_tile(i), k_tile(i + 1), Index<1>{}, Index<1>{});
-            next();
+        // Values that are not finite spoil the sums of rows that do not see them (0 times infinity), and of rows that do where
+        // weights have several terms (infinity less infinity). That shows in the sums, so the tiles are not searched for them: a block
+        // whose sums are not finite works through them once more, carefully, adding such values only where they are seen.
+        bool careful = false;
+        for (;;) {
+            m = -INFINITY;
+            l = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v)(0.0f);
+            phase_barrier<0>();  // the item before has been read
+            k_keys = keys_of(t0, first_pages[0]);
+            load(a.c.k, k_keys, k_tile(0), false);
+#pragma unroll
+            for (int i = -AHEAD; i < 0; ++i) {
+                there[i + AHEAD] = k_keys.there;
+                v_keys = k_keys;
+                k_keys = keys_of(t0 + i + AHEAD + 1, first_pages[i + AHEAD + 1]);
+                loads(i);
+            }
+            there[AHEAD] = k_keys.there;
+            v_keys = k_keys;
+            k_keys = keys_of(t0 + AHEAD + 1, first_pages[AHEAD + 1]);
+            phase_barrier<AHEAD * BATCH>();
+            if (PAIRED && wave >= WAVES / 2) phase_barrier<-1>();
+            if (row0 >= s.rows) {  // a wave without rows brings its share of the tiles
+                for (int i = 0; i < n; ++i) {
+                    phase_barrier<(AHEAD - 1) * BATCH>();
+                    loads(i);
+                    look_up(i);
+                    phase_barrier<-1>();
+                }
+            } else if (!careful) {  // a loop with one exit and no choice but the rare raise in it: with more, the compiler carries all sums twice
+                products(0, k_tile(0), Index<0>{}, Index<1>{});
+                weights(0);
+                int i = 0;
+                while (i < n - 1) {
+                    products(v_tile(i), k_tile(i + 1), Index<1>{}, Index<1>{});
+                    weights(++i);
+                }
+                products(v_tile(i), 0, Index<1>{}, Index<0>{});
+            } else {
+                for (int i = 0; i < n; ++i) {
+                    products(0, k_tile(i), Index<0>{}, Index<1>{});
+                    weights(i);
+                    odd_values(i);
+                }
+            }
+            if (PAIRED && wave < WAVES / 2) phase_barrier<-1>();
+            if (careful) break;
+            uint32_t odd = 0;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) odd |= bit_mask(!(fabsf(o[dt][e]) < INFINITY));
+            ++pass;
+            if (__ballot(odd != 0 && valid) != 0 && lane == 0) not_finite = pass;
+            phase_barrier<-1>();
+            careful = uniform(not_finite) == pass;
+            if (!careful) break;
         }
-        while (i < n - 1) {
-            if (odd) odd_values(i);
-            else products(v_tile(i), 0, Index<1>{}, Index<0>{});
-            products(0, k_tile(i + 1), Index<0>{}, Index<1>{});
-            next();
-        }
-        if (odd) odd_values(i);
-        else products(v_tile(i), 0, Index<1>{}, Index<0>{});
-        if (PAIRED && wave < WAVES / 2) phase_barrier<false>();
-
 
         // 4. the wave's rows leave, whole or as a part
         const bool begins = t0 == 0, ends = t1 == range.tiles;
@@ -606,6 +615,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
         u += whole ? blocks : t1 - t0;
     }
     if (tid == 0) a.joins[w] = join;
+    phase_barrier<0>();  // no load on its way to LDS that is given back
 }
 
 template <int CT, int NP, int DIM, int WAVES>
