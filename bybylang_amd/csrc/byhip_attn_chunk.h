@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     constexpr int ROW = DIM * 2, TILE = T * ROW;                  // bytes of a key, of a tile
     constexpr int NI = TILE / 1024 / WAVES, RPI = 1024 / ROW;     // direct loads per wave and tile, keys per load
     constexpr bool PAIRED = WAVES == 8;                           // two waves per SIMD, half a tile apart
-    constexpr int AHEAD = DIM <= 128 ? 2 : 1;                     // tiles between the loads of one and its use
+    constexpr int AHEAD = PAIRED ? 2 : 1;                         // tiles between the loads of one and its use
     constexpr int BUFS = AHEAD + (PAIRED ? 2 : 1);
     constexpr int SLOTS = 2 * AHEAD;                              // page lookups on their way and in use
     constexpr int BATCH = 2 * NI + 1;                             // a wave's direct loads per tile
