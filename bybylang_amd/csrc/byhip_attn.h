@@ -20,7 +20,7 @@ struct AttnArgs {
     int q_vec;       // query rows can be read 16 bytes at a time
     int out_vec;     // output rows can be written 4 values at a time
     uint32_t page_mul;   // key / page_size as a product's high bits
-    int page_shift;      // -1: pages of one key
+    int page_shift;
     int min_rows, max_rows;  // rows (tokens x group) of the sequences this launch takes
     float* part;     // partial results
     int4* joins;     // one description per block
@@ -30,7 +30,7 @@ struct AttnArgs {
 // Column of key j (below 2^31) in its table row. With l = ceil(log2(page size)) and page_mul = ceil(2^(31 + l) / page size),
 // the product's error is under j / 2^(31 + l) < 1 / page size.
 __device__ __forceinline__ int page_col(const AttnArgs& a, int j) {
-    return a.page_shift < 0 ? j : (int)(__umulhi((uint32_t)j, a.page_mul) >> a.page_shift);
+    return (int)(__umulhi(2u * (uint32_t)j, a.page_mul) >> a.page_shift);
 }
 
 // Sequence b as a launch sees it.

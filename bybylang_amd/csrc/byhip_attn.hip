@@ -156,8 +156,8 @@ extern "C" int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype
         a.max_rows = 0x7FFFFFFF;
         int log = 0;
         while ((1ll << log) < a.c.page_size) ++log;
-        a.page_shift = log - 1;
-        a.page_mul = log ? (uint32_t)(((1ull << (31 + log)) + a.c.page_size - 1) / a.c.page_size) : 0u;
+        a.page_shift = log;
+        a.page_mul = (uint32_t)(((1ull << (31 + log)) + a.c.page_size - 1) / a.c.page_size);
         a.q_vec = q_stride * dtype_bytes(q_dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
         a.out_vec = aligned4(out, out_stride, out_dtype);
         note_device_write(out);

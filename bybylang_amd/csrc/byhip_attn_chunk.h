@@ -74,8 +74,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     constexpr int NI = TILE / 1024 / WAVES, RPI = 1024 / ROW;     // direct loads per wave and tile, keys per load
     constexpr bool PAIRED = WAVES == 8;                           // two waves per SIMD, half a tile apart
     constexpr int AHEAD = PAIRED ? 2 : 1;                         // tiles between the loads of one and its use
-    constexpr int BUFS = AHEAD + (PAIRED ? 2 : 1);
-    constexpr int SLOTS = 2 * AHEAD;                              // page lookups on their way and in use
+    // Loads go out between the products where those take less time than the weights (64 values: 146 us from 158, 4 x 700
+    // rows x 4000 keys), else with the weights (128 values: 1.02 ms, from 1.04 between the products).
+    constexpr bool EARLY = DIM <= 64;
+    constexpr int BUFS = AHEAD + (EARLY || PAIRED ? 2 : 1);
+    constexpr int SLOTS = 4;                                      // page lookups on their way and in use
     constexpr int BATCH = 2 * NI + 1;                             // a wave's direct loads per tile
     constexpr float kShift = CT == BYHIP_F16 ? 4.0f : 0.0f;       // log2 of the weights' factor
     constexpr float kLimit = 32768.0f;                            // a lane's weights of a tile may add up to this
@@ -312,34 +315,38 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
             for (int i = 0; i < NI; ++i) k.row[i] = (uint32_t)__shfl((int)row, load_key + i * RPI, 64);
             return k;
         };
-        const auto load = [&](const uint16_t* base, const Keys& k, int to, bool values) INLINE {
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int piece = values ? v_piece ^ (2 * i * RPI & SW) : k_piece ^ (i * RPI & SW);
-                // selected with masks, not with branches: a divergent branch in the loop would keep it off scalar control flow
-                const uint32_t in = bit_mask(k.row[i] != ~0u) & bit_mask(8 * piece < a.c.dim);
-                const uint64_t there_at = reinterpret_cast<uint64_t>(base) + ((uint64_t)k.row[i] * a.c.dim + 8 * piece) * 2;
-                const uint64_t keep = (uint64_t)in << 32 | in;
-                const void* p = reinterpret_cast<const void*>((there_at & keep) | (reinterpret_cast<uint64_t>(a.zeros) & ~keep));
-                load_to_lds(p, lds_base + to + (wave * NI + i) * 1024);
-            }
+        const auto load = [&](const uint16_t* base, const Keys& k, int to, auto index, auto values) INLINE {
+            constexpr int i = decltype(index)::value;
+            const int piece = decltype(values)::value ? v_piece ^ (2 * i * RPI & SW) : k_piece ^ (i * RPI & SW);
+            // selected with masks, not with branches: a divergent branch in the loop would keep it off scalar control flow
+            const uint32_t in = bit_mask(k.row[i] != ~0u) & bit_mask(8 * piece < a.c.dim);
+            const uint64_t there_at = reinterpret_cast<uint64_t>(base) + ((uint64_t)k.row[i] * a.c.dim + 8 * piece) * 2;
+            const uint64_t keep = (uint64_t)in << 32 | in;
+            const void* p = reinterpret_cast<const void*>((there_at & keep) | (reinterpret_cast<uint64_t>(a.zeros) & ~keep));
+            load_to_lds(p, lds_base + to + (wave * NI + i) * 1024);
         };
         const auto k_tile = [&](int i) { return i % BUFS * TILE; };
         const auto v_tile = [&](int i) { return (BUFS + i % BUFS) * TILE; };
-        // Phase i loads a batch: V of tile i + AHEAD, K of tile i + AHEAD + 1 and the pages of tile i + 2 AHEAD + 2. Batch
-        // i - AHEAD has landed when phase i begins.
+        // With tile i goes a batch of loads: V of tile i + AHEAD, K of tile i + AHEAD + 1 and the pages of tile i + 2 AHEAD + 3.
+        // The weights of tile i wait for batch i - AHEAD.
+        constexpr int WAIT = EARLY ? AHEAD * BATCH : (AHEAD - 1) * BATCH;
         Keys v_keys, k_keys;
         uint64_t there[AHEAD + 1];  // of tiles i ..
-        const auto look_up_to = [&](int t, int slot) INLINE { word_to_lds(page_at(t), pages_base + slot * 256); };
-        const auto loads = [&](int i) INLINE {
-            load(a.c.v, v_keys, v_tile(i + AHEAD), true);
-            load(a.c.k, k_keys, k_tile(i + AHEAD + 1), false);
-            look_up_to(t0 + i + 2 * AHEAD + 2, (i + AHEAD) % SLOTS);
-        };
-        const auto look_up = [&](int i) INLINE {  // at its end
+        const auto look_up = [&](int i) INLINE { word_to_lds(page_at(t0 + i + 2 * AHEAD + 3), pages_base + (i + AHEAD + 1) % SLOTS * 256); };
+        const auto next_keys = [&](int i) INLINE {  // where the next batch's loads are
             v_keys = k_keys;
             k_keys = keys_of(t0 + i + AHEAD + 2, looked_up[wave][i % SLOTS][lane]);
         };
+        constexpr int PARTS = 2 * NI + 2;
+        const auto load_part = [&](int i, auto part) INLINE {
+            constexpr int P = decltype(part)::value;
+            if constexpr (P < NI) load(a.c.v, v_keys, v_tile(i + AHEAD), Index<P>{}, Index<1>{});
+            else if constexpr (P < 2 * NI) load(a.c.k, k_keys, k_tile(i + AHEAD + 1), Index<P - NI>{}, Index<0>{});
+            else if constexpr (P == 2 * NI) look_up(i);
+            else next_keys(i);
+        };
+        const auto load_batch = [&](int i) INLINE { unrolled<0, PARTS>([&](auto part) INLINE { load_part(i, part); }); };
+
         f16v sc[2];
         vec wt[NP][4];
         constexpr int LEAD = 4, NV = 4 * DT, NK = 2 * STEPS;  // operands read ahead of their use; operands of a tile's V and K
@@ -353,8 +360,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
             typedef __attribute__((address_space(3))) vec lds_vec;
             return *(lds_vec*)(((uintptr_t)(lds3 + (k_at + tile)) ^ (32 * (k / 2))) + k % 2 * 32 * ROW);
         };
-        // O^T += V^T P^T of the tile at vt, then S^T = K Q^T of the tile at kt, in one run of reads and products
-        const auto products = [&](int vt, int kt, auto with_v, auto with_k) INLINE {
+        // O^T += V^T P^T of the tile at vt, then S^T = K Q^T of the tile at kt, in one run of reads and products, with batch `batch` of the loads spread between the products (where they are early)
+        const auto products = [&](int vt, int kt, int batch, auto with_v, auto with_k) INLINE {
             constexpr int V0 = decltype(with_v)::value ? 0 : NV, N = decltype(with_k)::value ? NV + NK : NV;
             vec ring[LEAD + 1];
             const auto read = [&](auto k) INLINE {
@@ -378,13 +385,32 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                     for (int p = NP - 1; p >= 0; --p) sc[E % 2] = mfma32(x, q[p][E / 2], sc[E % 2]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
+                if constexpr (EARLY && decltype(with_k)::value) {  // part P follows product V0 + (P + 1) (N - V0) / (PARTS + 1)
+                    static_assert(PARTS < NK, "");
+                    constexpr int P = ((K + 1 - V0) * (PARTS + 1) + N - V0 - 1) / (N - V0) - 1;
+                    if constexpr (P < PARTS && (P + 1) * (N - V0) / (PARTS + 1) == K + 1 - V0) {
+                        load_part(batch, Index<P>{});
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
             });
         };
         uint32_t see[2];
+        uint64_t here;  // of the tile at hand
+        const auto next_there = [&]() INLINE {
+            here = there[0];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) there[k] = there[k + 1];
+            there[AHEAD] = v_keys.there;
+        };
         const auto begin_weights = [&](int i) INLINE {  // the second phase, up to scores (log2, or raw ones that `factor` scales)
             const int j0 = range.key(t0 + i);
-            phase_barrier<(AHEAD - 1) * BATCH>();
-            loads(i);
+            if constexpr (EARLY) next_there();
+            phase_barrier<WAIT>();
+            if constexpr (!EARLY) {
+                load_batch(i);
+                next_there();
+            }
             see[0] = see[1] = ~0u;
             if constexpr (EXTRA) {  // to capped and biased scores (log2)
                 if (a.softcap > 0.0f && NP == 1) {
@@ -415,13 +441,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                         for (int e = 0; e < 16; ++e) sc[kb][e] = fmaf(-slope, fabsf(back - (float)(32 * kb + 8 * (e / 4) + e % 4)), sc[kb][e]);
                 }
             }
-            const bool full = there[0] == ~0ull && ((j0 + T - 1 <= wp0 && (a.window <= 0 || wp1 - j0 < a.window)) || j0 + T <= s.prefix);
+            const bool full = here == ~0ull && ((j0 + T - 1 <= wp0 && (a.window <= 0 || wp1 - j0 < a.window)) || j0 + T <= s.prefix);
             if (!full) {  // without branches: all 64 lanes take part in what follows
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
-                    see[kb] = seen_keys(a, s, pos, j0 + 32 * kb, (uint32_t)(there[0] >> (32 * kb)));
+                    see[kb] = seen_keys(a, s, pos, j0 + 32 * kb, (uint32_t)(here >> (32 * kb)));
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) sc[kb][e] = see[kb] >> (8 * (e / 4) + e % 4) >> (4 * hf) & 1u ? sc[kb][e] : -INFINITY;
+                    for (int e = 0; e < 16; ++e) sc[kb][e] = (int)(see[kb] >> (4 * hf) << (31 - 8 * (e / 4) - e % 4)) < 0 ? sc[kb][e] : -INFINITY;
                 }
             }
         };
@@ -468,10 +494,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 weigh();
             }
             l += sum;
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) there[k] = there[k + 1];
-            there[AHEAD] = k_keys.there;
-            look_up(i);
             phase_barrier<-1>();
         };
         const auto odd_values = [&](int i) INLINE {  // O^T += V^T P^T of the finite values, and the others where they are seen
@@ -513,14 +535,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v)(0.0f);
             phase_barrier<0>();  // the item before has been read
+            look_up(-AHEAD - 1);
             k_keys = keys_of(t0, first_pages[0]);
-            load(a.c.k, k_keys, k_tile(0), false);
+            unrolled<0, NI>([&](auto part) INLINE { load(a.c.k, k_keys, k_tile(0), part, Index<0>{}); });
 #pragma unroll
             for (int i = -AHEAD; i < 0; ++i) {
                 there[i + AHEAD] = k_keys.there;
                 v_keys = k_keys;
                 k_keys = keys_of(t0 + i + AHEAD + 1, first_pages[i + AHEAD + 1]);
-                loads(i);
+                unrolled<0, PARTS - 1>([&](auto part) INLINE { load_part(i, part); });
             }
             there[AHEAD] = k_keys.there;
             v_keys = k_keys;
@@ -529,23 +552,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
             if (PAIRED && wave >= WAVES / 2) phase_barrier<-1>();
             if (row0 >= s.rows) {  // a wave without rows brings its share of the tiles
                 for (int i = 0; i < n; ++i) {
-                    phase_barrier<(AHEAD - 1) * BATCH>();
-                    loads(i);
-                    look_up(i);
+                    if constexpr (EARLY) load_batch(i);
+                    phase_barrier<WAIT>();
+                    if constexpr (!EARLY) load_batch(i);
                     phase_barrier<-1>();
                 }
             } else if (!careful) {  // a loop with one exit and no choice but the rare raise in it: with more, the compiler carries all sums twice
-                products(0, k_tile(0), Index<0>{}, Index<1>{});
+                products(0, k_tile(0), 0, Index<0>{}, Index<1>{});
                 weights(0);
                 int i = 0;
                 while (i < n - 1) {
-                    products(v_tile(i), k_tile(i + 1), Index<1>{}, Index<1>{});
+                    products(v_tile(i), k_tile(i + 1), i + 1, Index<1>{}, Index<1>{});
                     weights(++i);
                 }
-                products(v_tile(i), 0, Index<1>{}, Index<0>{});
+                products(v_tile(i), 0, 0, Index<1>{}, Index<0>{});
             } else {
                 for (int i = 0; i < n; ++i) {
-                    products(0, k_tile(i), Index<0>{}, Index<1>{});
+                    products(0, k_tile(i), i, Index<0>{}, Index<1>{});
                     weights(i);
                     odd_values(i);
                 }
