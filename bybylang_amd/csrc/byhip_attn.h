@@ -111,19 +111,23 @@ __device__ __forceinline__ int4 join_of(long long last, long long blocks, long l
 }
 
 // Joins the parts of items of R rows that several blocks worked on. Grid: blocks x row groups. 16 lanes hold a row's values;
-// the 4 lane groups of a wave, and with WAVES 4 those of the block's 4 waves, walk over its parts. With WAVES 1 each wave has rows of its own.
+// the 4 lane groups of a wave, and with WAVES 4 those of the block's 4 waves, walk over its parts. With WAVES 1 each wave has
+// rows of its own, and each lane group where the parts are few (the usual two: 17 us, 34 MB, with a wave per row, 8.6 us with a group).
 template <int R, int DIM, int WAVES>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
-    constexpr int V = DIM / 16, GROUPS = 4 * WAVES, OWN = 4 / WAVES;
+    constexpr int V = DIM / 16;
     const int w = blockIdx.x;
     const int4 d = a.joins[w];
     if (d.x == 0) return;
     __shared__ float red[WAVES == 4 ? 4 : 1][DIM + 2];
     const int b = d.y, rt = d.z, h = d.w, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int group = WAVES == 4 ? threadIdx.x >> 4 : lane >> 4, col = (lane & 15) * V;
+    const int col = (lane & 15) * V;
     const SeqInfo s = seq_info(a, b);
     const int rows = min(R, s.rows - rt * R), parts = d.x - w + 1;
-    for (int r = blockIdx.y * OWN + (WAVES == 4 ? 0 : wave); r < rows; r += gridDim.y * OWN) {
+    const bool alone = WAVES == 1 && parts <= 4;  // a lane group has its row alone
+    const int groups = alone ? 1 : 4 * WAVES, group = alone ? 0 : WAVES == 4 ? threadIdx.x >> 4 : lane >> 4;
+    const int own = WAVES == 4 ? 1 : alone ? 16 : 4, first = WAVES == 4 ? 0 : alone ? threadIdx.x >> 4 : wave;
+    for (int r = blockIdx.y * own + first; r < rows; r += gridDim.y * own) {
         float acc[V] = {}, m = -INFINITY, l = 0.0f;
         const auto add = [&](float pm, float pl, const float (&x)[V]) {
             const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
@@ -134,7 +138,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
             m = top;
         };
 #pragma unroll 2
-        for (int i = group; i < parts; i += GROUPS) {
+        for (int i = group; i < parts; i += groups) {
             const float* p = part_slot<R, DIM>(a.part, i == 0 ? 2 * w + 1 : 2 * (w + i));
             float x[V];
 #pragma unroll
@@ -144,8 +148,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
             }
             add(p[R * DIM + r], p[R * DIM + R + r], x);
         }
-#pragma unroll
-        for (int lanes = 16; lanes < 64; lanes <<= 1) {
+        for (int lanes = 16; !alone && lanes < 64; lanes <<= 1) {
             float x[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) x[e] = __shfl_xor(acc[e], lanes, 64);
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const int q = rt * R + r, t = a.s.starts[b] + q / a.group;
         const size_t out = (size_t)t * a.out_stride + (size_t)(h * a.group + q % a.group) * a.c.dim + col;
-        if (threadIdx.x < 16 || (WAVES == 1 && lane < 16)) {
+        if (threadIdx.x < 16 || (WAVES == 1 && (alone || lane < 16))) {
 #pragma unroll
             for (int e = 0; e < V; e += 4) {
                 if (col + e >= a.c.dim) continue;

@@ -65,11 +65,12 @@ __device__ __forceinline__ void unrolled(F&& f) {
     }
 }
 
-template <int CT, int NP, int DIM, int WAVES, bool EXTRA>
+// DIM: values a row takes in LDS and in a part, at least the head's; USED of them are multiplied.
+template <int CT, int NP, int DIM, int USED, int WAVES, bool EXTRA>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) {
     typedef typename Half8<CT>::vec vec;
     constexpr int R = 32 * WAVES, T = kChunkKeys, NT = 64 * WAVES;
-    constexpr int STEPS = DIM / 16, DT = DIM / 32, PIECES = DIM / 8, SW = (PIECES < 16 ? PIECES : 16) - 1;
+    constexpr int STEPS = USED / 16, DT = USED / 32, PIECES = DIM / 8, SW = (PIECES < 16 ? PIECES : 16) - 1;
     constexpr int ROW = DIM * 2, TILE = T * ROW;                  // bytes of a key, of a tile
     constexpr int NI = TILE / 1024 / WAVES, RPI = 1024 / ROW;     // direct loads per wave and tile, keys per load
     constexpr bool PAIRED = WAVES == 8;                           // two waves per SIMD, half a tile apart
@@ -641,13 +642,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     phase_barrier<0>();  // no load on its way to LDS that is given back
 }
 
-template <int CT, int NP, int DIM, int WAVES>
+template <int CT, int NP, int DIM, int USED, int WAVES>
 void launch_chunk(const AttnArgs& a) {
     constexpr size_t kSlots = (size_t)2 * 32 * WAVES * (DIM + 2) * sizeof(float);  // one block's
     const size_t room = (kAttnWorkspaceBytes - kAttnJoinBytes) / kSlots;
     const unsigned blocks = (unsigned)std::min<size_t>(room, compute_units());
-    if (a.softcap > 0.0f || a.slopes || !(a.scale > 0.0f)) launch("attn_chunk", (attn_chunk<CT, NP, DIM, WAVES, true>), dim3(blocks), dim3(64 * WAVES), 0, a);
-    else launch("attn_chunk", (attn_chunk<CT, NP, DIM, WAVES, false>), dim3(blocks), dim3(64 * WAVES), 0, a);
+    if (a.softcap > 0.0f || a.slopes || !(a.scale > 0.0f)) launch("attn_chunk", (attn_chunk<CT, NP, DIM, USED, WAVES, true>), dim3(blocks), dim3(64 * WAVES), 0, a);
+    else launch("attn_chunk", (attn_chunk<CT, NP, DIM, USED, WAVES, false>), dim3(blocks), dim3(64 * WAVES), 0, a);
     BYHIP_LAUNCHED("attn_chunk");
     launch("attn_join", (attn_join<32 * WAVES, DIM, 1>), dim3(blocks, 16), dim3(256), 0, a);
     BYHIP_LAUNCHED("attn_join");
@@ -656,9 +657,10 @@ void launch_chunk(const AttnArgs& a) {
 // Blocks of 8 waves where two waves per SIMD have the registers they need, else of 4.
 template <int CT, int NP>
 void launch_chunk_dim(const AttnArgs& a) {
-    if (a.c.dim <= 64) launch_chunk<CT, NP, 64, NP == 1 ? 8 : 4>(a);
-    else if (a.c.dim <= 128) launch_chunk<CT, NP, 128, NP == 1 ? 8 : 4>(a);
-    else launch_chunk<CT, NP, 256, 4>(a);
+    if (a.c.dim <= 64) launch_chunk<CT, NP, 64, 64, NP == 1 ? 8 : 4>(a);
+    else if (a.c.dim <= 96) launch_chunk<CT, NP, 128, 96, NP == 1 ? 8 : 4>(a);
+    else if (a.c.dim <= 128) launch_chunk<CT, NP, 128, 128, NP == 1 ? 8 : 4>(a);
+    else launch_chunk<CT, NP, 256, 256, 4>(a);
 }
 
 }  // namespace
