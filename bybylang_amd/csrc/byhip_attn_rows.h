@@ -45,6 +45,7 @@ struct Rows {
     int koff[STEPS], voff[(V + 7) / 8];  // this lane's values of a key (those past the head's end read its first)
     uint32_t kmask[STEPS];     // 0 for those past the end
     float slope, factor;       // factor: scale (and the row's power of two), with log2 e unless EXTRA
+    float inv_cap;
     vec q[NP][STEPS];
     float m, l;                // reference (log2) of row c; this lane's sum of weights
     f4 o[V];
@@ -162,6 +163,7 @@ struct Rows {
                 for (int p = 1; p < NP; ++p) q[p][st] = __builtin_bit_cast(vec, make_uint4(0, 0, 0, 0));
             }
         }
+        inv_cap = EXTRA && a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
         factor = ldexpf(EXTRA ? a.scale : a.scale * kLog2e, -shift);
         m = -INFINITY;
         l = 0.0f;
@@ -169,8 +171,9 @@ struct Rows {
         for (int t = 0; t < V; ++t) o[t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // One tile of keys j0 ..; `there`: bit j of the keys that exist.
-    __device__ __forceinline__ void tile(const KTile& k, VTile& v, int j0, uint32_t there, int p0, int p1) {
+    // One tile of keys j0 ..; `there`: bit j of the keys that exist; `read`: called once k has been read.
+    template <typename F>
+    __device__ __forceinline__ void tile(const KTile& k, VTile& v, int j0, uint32_t there, int p0, int p1, F&& read) {
         float x[8];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -184,10 +187,11 @@ struct Rows {
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[4 * kb + r] = acc[r] * factor;
         }
+        read();
         if constexpr (EXTRA) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (a.softcap > 0.0f) x[i] = a.softcap * soft_tanh<(NP > 1)>(x[i] / a.softcap);
+                if (a.softcap > 0.0f) x[i] = a.softcap * soft_tanh<(NP > 1)>(x[i] * inv_cap);
                 x[i] = x[i] * kLog2e - slope * fabsf((float)(pos - (j0 + 16 * (i / 4) + 4 * g + i % 4)));
             }
         }
@@ -274,8 +278,12 @@ struct Rows {
     }
 };
 
+// Blocks resident per CU: two, but one where 256 registers per lane would not hold a tile (heads of 256 values at one sequence
+// of 65536 keys x 4: 373 us with one, 754 with two; fp32 473 and 1631).
+constexpr int rows_blocks(int dim) { return dim > 128 ? 1 : 2; }
+
 template <int CT, int NP, int DIM, bool EXTRA>
-__global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
+__global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
     constexpr int V = DIM / 16, kPitch = DIM + 4;
     __shared__ long long before[kAttnBatch + 1];  // units (tiles of 32 keys x row tiles) of the sequences before each
     __shared__ long long wave_sum_of[kWaves];
@@ -346,11 +354,14 @@ __global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
         if (t + kWaves < t1) next = r.key_row(b, range.key(t + kWaves), next_there);
         if (t < t1) r.load_k(ka, rows);
         const auto step = [&](auto& cur, auto& ahead) {
+            constexpr bool kOneTile = DIM > 128;  // registers for one tile of keys: the next one's follow its last use
             r.load_v(v, rows);
             uint32_t after = 0, after_there = 0;
             if (t + 2 * kWaves < t1) after = r.key_row(b, range.key(t + 2 * kWaves), after_there);
-            if (t + kWaves < t1) r.load_k(ahead, next);
-            r.tile(cur, v, range.key(t), there, p0, p1);
+            if (!kOneTile && t + kWaves < t1) r.load_k(ahead, next);
+            r.tile(cur, v, range.key(t), there, p0, p1, [&] {
+                if (kOneTile) r.load_k(cur, next);  // row 0 after the last tile
+            });
             rows = next;
             there = next_there;
             next = after;
@@ -359,6 +370,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
         };
         while (t < t1) {
             step(ka, kb);
+            if (DIM > 128) continue;
             if (t >= t1) break;
             step(kb, ka);
         }
@@ -428,7 +440,8 @@ __global__ __launch_bounds__(256, 2) void attn_rows(AttnArgs a) {
 }
 
 template <int CT, int NP, int DIM>
-void launch_rows(const AttnArgs& a, unsigned blocks) {
+void launch_rows(const AttnArgs& a) {
+    const unsigned blocks = (unsigned)(compute_units() * rows_blocks(DIM));
     if (a.softcap > 0.0f || a.slopes) launch("attn_rows", (attn_rows<CT, NP, DIM, true>), dim3(blocks), dim3(256), 0, a);
     else launch("attn_rows", (attn_rows<CT, NP, DIM, false>), dim3(blocks), dim3(256), 0, a);
     BYHIP_LAUNCHED("attn_rows");
@@ -438,10 +451,9 @@ void launch_rows(const AttnArgs& a, unsigned blocks) {
 
 template <int CT, int NP>
 void launch_rows_dim(const AttnArgs& a) {
-    const unsigned blocks = (unsigned)compute_units() * 2;  // two are resident per CU
-    if (a.c.dim <= 64) launch_rows<CT, NP, 64>(a, blocks);
-    else if (a.c.dim <= 128) launch_rows<CT, NP, 128>(a, blocks);
-    else launch_rows<CT, NP, 256>(a, blocks);
+    if (a.c.dim <= 64) launch_rows<CT, NP, 64>(a);
+    else if (a.c.dim <= 128) launch_rows<CT, NP, 128>(a);
+    else launch_rows<CT, NP, 256>(a);
 }
 
 }  // namespace
