@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
         if (t + kWaves < t1) next = r.key_row(b, range.key(t + kWaves), next_there);
         if (t < t1) r.load_k(ka, rows);
         const auto step = [&](auto& cur, auto& ahead) {
-            constexpr bool kOneTile = DIM > 128;  // registers for one tile of keys: the next one's follow its last use
+            constexpr bool kOneTile = DIM > 128 || (DIM > 64 && NP > 1);  // registers for one tile of keys: the next one's follow its last use
             r.load_v(v, rows);
             uint32_t after = 0, after_there = 0;
             if (t + 2 * kWaves < t1) after = r.key_row(b, range.key(t + 2 * kWaves), after_there);
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
         };
         while (t < t1) {
             step(ka, kb);
-            if (DIM > 128) continue;
+            if (DIM > 128 || (DIM > 64 && NP > 1)) continue;
             if (t >= t1) break;
             step(kb, ka);
         }
