@@ -1,8 +1,8 @@
 // byhip_norm.hip - the residual stream between two blocks (gfx950): h = res_scale res + gate . post(x),
 // y = pre(h), post and pre RMS or layer norms.
 //
-// Every input is read once and every output written once: a row's values stay in its block's registers (4 CH
-// per thread) from the first norm to the last store. Sums are fp32; a variance is the mean of the squared
+// Every input is read once and every output written once: a row's values stay in its block's registers (at most
+// 32 per thread) from the first norm to the last store. Sums are fp32; a variance is the mean of the squared
 // deviations from the mean already formed, not a difference of two large sums. Rows too long for the registers
 // of 1024 threads pass over x again for each sum.
 #include <algorithm>
@@ -25,20 +25,23 @@ struct NormArgs {
     float res_scale;
 };
 
-// Sum over the block's threads (TH of them, in waves), the same value in every thread.
-template <int TH>
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_sum(v);
-    if constexpr (TH > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+// Sums over the block's threads, the same value in every thread. One barrier each: successive sums use the halves of `red`
+// in turn, and a half is written again only after the barrier of the sum between.
+struct BlockSum {
+    float (*red)[16];
+    int turn = 0;
+    __device__ __forceinline__ float operator()(float v) {
+        v = wave_sum(v);
+        const int waves = blockDim.x >> 6;
+        if (waves == 1) return v;
+        if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = v;
         __syncthreads();
         v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < TH / 64; ++i) v += red[i];
+        for (int i = 0; i < waves; ++i) v += red[turn][i];
+        turn ^= 1;
+        return v;
     }
-    return v;
-}
+};
 
 // Loads, scales and stores of 4 values at column i, those past N left out (read as 0).
 template <int DT>
@@ -63,9 +66,10 @@ __device__ __forceinline__ void write4(void* p, size_t row, int i, int N, int ve
     }
 }
 
-// One norm over the row held in v (columns 4 (TH c + thread) ..).
-template <int TH, int CH>
-__device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n, int N, int vec, int tid, float* red) {
+// One norm over the row held in v (columns 4 (threads c + thread) ..).
+template <int CH>
+__device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n, int N, int vec, int tid, BlockSum& block_sum) {
+    const int TH = blockDim.x;
     float mean = 0.0f;
     if (n.kind == BYHIP_NORM_LAYER) {
         float s = 0.0f;
@@ -73,7 +77,7 @@ __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n,
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s += v[c][e];  // 0 past N
-        mean = block_sum<TH>(s, red) / N;
+        mean = block_sum(s) / N;
     }
     float s = 0.0f;
 #pragma unroll
@@ -83,7 +87,7 @@ __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n,
             const float d = 4 * (TH * c + tid) + e < N ? v[c][e] - mean : 0.0f;
             s += d * d;
         }
-    const float f = 1.0f / sqrtf(block_sum<TH>(s, red) / N + n.eps);
+    const float f = 1.0f / sqrtf(block_sum(s) / N + n.eps);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = 4 * (TH * c + tid);
@@ -95,10 +99,11 @@ __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n,
     }
 }
 
-template <int XT, int HT, int TH, int CH>
-__global__ __launch_bounds__(TH) void norm_block(NormArgs a) {
-    __shared__ float red[TH / 64 + 1];
-    const int tid = threadIdx.x;
+template <int XT, int HT, int CH>
+__global__ __launch_bounds__(1024) void norm_block(NormArgs a) {
+    __shared__ float red[2][16];
+    BlockSum block_sum{red};
+    const int tid = threadIdx.x, TH = blockDim.x;
     const size_t row = blockIdx.x;
     float v[CH][4], r[CH][4];
 #pragma unroll
@@ -107,7 +112,7 @@ __global__ __launch_bounds__(TH) void norm_block(NormArgs a) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) read4<HT>(a.res, row * a.res_stride, 4 * (TH * c + tid), a.N, a.vec, r[c]);
     }
-    if (a.has_post) norm_row<TH, CH>(v, a.post, a.N, a.vec, tid, red);
+    if (a.has_post) norm_row<CH>(v, a.post, a.N, a.vec, tid, block_sum);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = 4 * (TH * c + tid);
@@ -126,7 +131,7 @@ __global__ __launch_bounds__(TH) void norm_block(NormArgs a) {
         if (a.h) write4(a.h, row * a.h_stride, i, a.N, a.vec, v[c], HT);
     }
     if (!a.has_pre) return;
-    norm_row<TH, CH>(v, a.pre, a.N, a.vec, tid, red);
+    norm_row<CH>(v, a.pre, a.N, a.vec, tid, block_sum);
 #pragma unroll
     for (int c = 0; c < CH; ++c) write4(a.y, row * a.y_stride, 4 * (TH * c + tid), a.N, a.vec, v[c], a.y_dtype);
 }
@@ -134,7 +139,8 @@ __global__ __launch_bounds__(TH) void norm_block(NormArgs a) {
 // Rows of any length: each sum walks over x (and res) again. h may be res's rows, so it is written last.
 template <int XT, int HT>
 __global__ __launch_bounds__(1024) void norm_block_long(NormArgs a) {
-    __shared__ float red[17];
+    __shared__ float red[2][16];
+    BlockSum block_sum{red};
     const int tid = threadIdx.x;
     const size_t row = blockIdx.x;
     const float inv = 1.0f / a.N;
@@ -142,7 +148,7 @@ __global__ __launch_bounds__(1024) void norm_block_long(NormArgs a) {
     auto sum = [&](auto&& value) {
         float s = 0.0f;
         for (int i = tid; i < a.N; i += 1024) s += value(i);
-        return block_sum<1024>(s, red);
+        return block_sum(s);
     };
     auto x = [&](int i) { return load1<XT>(a.x, row * a.x_stride + i); };
     if (a.has_post) {
@@ -170,25 +176,20 @@ __global__ __launch_bounds__(1024) void norm_block_long(NormArgs a) {
     }
 }
 
-template <int XT, int HT, int TH>
-bool try_norm(const NormArgs& a, int ch) {
-    switch (ch) {
-    case 1: launch("norm_block", (norm_block<XT, HT, TH, 1>), dim3(a.M), dim3(TH), 0, a); return true;
-    case 2: launch("norm_block", (norm_block<XT, HT, TH, 2>), dim3(a.M), dim3(TH), 0, a); return true;
-    case 3: case 4: launch("norm_block", (norm_block<XT, HT, TH, 4>), dim3(a.M), dim3(TH), 0, a); return true;
-    case 5: case 6: case 7: case 8: launch("norm_block", (norm_block<XT, HT, TH, 8>), dim3(a.M), dim3(TH), 0, a); return true;
-    default: return false;
-    }
-}
-
 template <int XT, int HT>
 void launch_norm(const NormArgs& a) {
-    const auto chunks = [&](int threads) { return (int)std::min<long long>(99, ((long long)a.N + 4LL * threads - 1) / (4LL * threads)); };
-    bool done = false;
-    if (a.N <= 512) done = try_norm<XT, HT, 64>(a, chunks(64));
-    else if (a.N <= 8192) done = try_norm<XT, HT, 256>(a, chunks(256));
-    else done = try_norm<XT, HT, 1024>(a, chunks(1024));
-    if (!done) launch("norm_block_long", (norm_block_long<XT, HT>), dim3(a.M), dim3(1024), 0, a);
+    // Values per thread: many rows fill the card by themselves, and 16 per thread cost the fewest barriers per value; few rows take
+    // all the threads they can have.
+    const bool few = a.M <= 2 * compute_units();
+    const long long fours = ((long long)a.N + 3) / 4;
+    const int ch = fours <= (few ? 1024 : 64) ? 1 : fours <= (few ? 2048 : 128) ? 2 : fours <= 4096 ? 4 : 8;
+    const long long threads = ((fours + ch - 1) / ch + 63) / 64 * 64;
+    const dim3 grid(a.M), block((unsigned)threads);
+    if (threads > 1024) launch("norm_block_long", (norm_block_long<XT, HT>), grid, dim3(1024), 0, a);
+    else if (ch == 1) launch("norm_block", (norm_block<XT, HT, 1>), grid, block, 0, a);
+    else if (ch == 2) launch("norm_block", (norm_block<XT, HT, 2>), grid, block, 0, a);
+    else if (ch == 4) launch("norm_block", (norm_block<XT, HT, 4>), grid, block, 0, a);
+    else launch("norm_block", (norm_block<XT, HT, 8>), grid, block, 0, a);
     BYHIP_LAUNCHED("norm_block");
 }
 
