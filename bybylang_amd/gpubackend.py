@@ -97,6 +97,10 @@ class SessionHandle:
     probeBytes: int = 0
     extra: dict = field(default_factory=dict)
 
+    @property
+    def ptr(self):  # so that device.KvCache and its kin take session handles
+        return self.hipHandle
+
 
 def sessionBegin(backend: GpuBackend) -> bool:
     """sessionBegin, gpubackend.nim:1042: False when a session is already open or on failure."""
@@ -380,6 +384,80 @@ def gpuMatmulQ4(backend: GpuBackend, a, wq, scales, zeros, m: int, k: int, n: in
         if cpuFallback is None:
             raise
         return cpuFallback(a, wq, sc, ze, m, k, n, groupSize, nGroupsPerRow)
+
+
+# ── attention over a paged cache ────────────────────────────────────────────────────────────
+#
+# The reference keeps no cache of keys and values on the GPU; these procs follow its session
+# conventions: fp32 handles of dense rows, False when the library does not take the arguments, an
+# exception on an error. Caches, batches and options are the descriptors of device.py, over session
+# handles (sessionUploadBytes for int32 tables, sessionAllocScratch for the rest).
+
+
+def _encoded(rc: int, what: str) -> bool:
+    if rc == _abi.BYHIP_UNSUPPORTED:
+        return False
+    check(rc, what)
+    return True
+
+
+def _opt(x):
+    return None if x is None else x.ref
+
+
+def sessionRopeAppend(backend: GpuBackend, q: SessionHandle, k: SessionHandle, v: SessionHandle,
+                      heads: int, rope, cache, batch, qOut: SessionHandle) -> bool:
+    """qOut = the rotated queries; the rotated keys and the values go to their rows of the cache."""
+    _require_hip(backend)
+    c = cache.value
+    D, N = c.head_dim, c.head_dim * c.kv_heads
+    return _encoded(load().byhip_rope_append(q.hipHandle, heads * D, k.hipHandle, N, v.hipHandle, N, _abi.F32, heads,
+                                             D, _opt(rope), cache.ref, batch.ref, qOut.hipHandle, heads * D,
+                                             _abi.F32), "sessionRopeAppend")
+
+
+def sessionPagedAttention(backend: GpuBackend, q: SessionHandle, heads: int, attn, cache, batch,
+                          out: SessionHandle) -> bool:
+    """out = attention of the batch's rows over their sequences in the cache."""
+    _require_hip(backend)
+    N = heads * cache.value.head_dim
+    return _encoded(load().byhip_paged_attention(q.hipHandle, N, _abi.F32, heads, attn.ref, cache.ref, batch.ref,
+                                                 out.hipHandle, N, _abi.F32), "sessionPagedAttention")
+
+
+def sessionNormBlock(backend: GpuBackend, x: SessionHandle, M: int, N: int, post, gate: SessionHandle | None,
+                     res: SessionHandle | None, resScale: float, h: SessionHandle | None, pre,
+                     y: SessionHandle | None) -> bool:
+    """h = resScale res + gate . post(x), y = pre(h); what is None is left out."""
+    _require_hip(backend)
+    ptr = lambda b: None if b is None else b.hipHandle  # noqa: E731
+    return _encoded(load().byhip_norm_block(x.hipHandle, N, _abi.F32, M, N, _opt(post), ptr(gate), N, ptr(res), N,
+                                            resScale, ptr(h), N, _abi.F32, _opt(pre), ptr(y), N, _abi.F32),
+                    "sessionNormBlock")
+
+
+def sessionCacheFork(backend: GpuBackend, pool, parents: SessionHandle, rows: SessionHandle, n: int) -> bool:
+    """Slot rows[i] continues slot parents[i]'s sequence, sharing its pages."""
+    _require_hip(backend)
+    return _encoded(load().byhip_cache_fork(pool.ref, parents.hipHandle, rows.hipHandle, n), "sessionCacheFork")
+
+
+def sessionCacheFree(backend: GpuBackend, pool, rows: SessionHandle, n: int) -> bool:
+    """The slots' sequences end; pages no other slot shares are free again."""
+    _require_hip(backend)
+    return _encoded(load().byhip_cache_free(pool.ref, rows.hipHandle, n), "sessionCacheFree")
+
+
+def sessionCacheGrow(backend: GpuBackend, pool, rows: SessionHandle, add: SessionHandle, n: int) -> bool:
+    """Room for add[i] more tokens in slot rows[i] (negative: that many are dropped)."""
+    _require_hip(backend)
+    return _encoded(load().byhip_cache_grow(pool.ref, rows.hipHandle, add.hipHandle, n), "sessionCacheGrow")
+
+
+def sessionCacheCompact(backend: GpuBackend, pool) -> bool:
+    """Moves the pages in use to the pool's front."""
+    _require_hip(backend)
+    return _encoded(load().byhip_cache_compact(pool.ref, None, None), "sessionCacheCompact")
 
 
 # ── FP4-KM / FP16 tile GEMM (gpubackend.nim:1442-1488) ───────────────────────────────────────
