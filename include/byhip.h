@@ -392,8 +392,8 @@ typedef struct byhip_kv_pool {
 int byhip_cache_fork(const byhip_kv_pool* pool, const int* parents, const int* rows, int n);
 /* Slots rows[i] release their pages; their lengths become 0. n <= 1024. */
 int byhip_cache_free(const byhip_kv_pool* pool, const int* rows, int n);
-/* Slot rows[i] gets room for add[i] >= 0 more tokens and counts them in lens: the lowest free pages, in the
- * order of i. A partly filled last page that others still hold is copied first, so that a slot only ever
+/* Slot rows[i] gets room for add[i] more tokens and counts them in lens: the lowest free pages, in the
+ * order of i. A negative add[i] drops that many tokens (at most all) and releases the pages that then hold none. A partly filled last page that others still hold is copied first, so that a slot only ever
  * appends to pages of its own. Slots past the first that does not fit are refused. n <= 1024. */
 int byhip_cache_grow(const byhip_kv_pool* pool, const int* rows, const int* add, int n);
 /* Moves live pages to the front: the i-th free page below the number of live ones receives the i-th live page

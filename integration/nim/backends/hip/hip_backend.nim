@@ -24,6 +24,33 @@ const
   BYHIP_BF16* = 2.cint
   BYHIP_MXFP4_KM* = 3.cint
 
+# Attention over a paged cache: the descriptors of include/byhip.h, field by field.
+type
+  ByhipKvCache* {.bycopy.} = object
+    k*, v*: pointer
+    dtype*, pages*, pageSize*, kvHeads*, headDim*: cint
+  ByhipKvBatch* {.bycopy.} = object
+    table*, starts*, lens*: pointer
+    batch*, tableStride*, rows*: cint
+  ByhipRope* {.bycopy.} = object
+    layout*, rotDim*: cint
+    magnitude*: cfloat
+    steps*: pointer
+  ByhipAttn* {.bycopy.} = object
+    scale*, softcap*: cfloat
+    window*: cint
+    slopes*, prefix*: pointer
+  ByhipKvPool* {.bycopy.} = object
+    caches*: ptr ByhipKvCache
+    nCaches*: cint
+    refs*, table*, lens*: pointer
+    slots*, tableStride*: cint
+    status*: pointer
+  ByhipNorm* {.bycopy.} = object
+    kind*: cint
+    eps*: cfloat
+    weight*, bias*: pointer
+
 {.push importc, cdecl, dynlib: HipLib.}
 proc byhip_init*(device: cint): cint
 proc byhip_last_error*(): cstring
@@ -76,6 +103,24 @@ proc byhip_tile_gemm_ready*(f16, tensorCore: cint): cint
 proc byhip_program_dispatch*(words: ptr uint32, nWords: cint, mem: pointer, memLen: csize_t,
                              u8: pointer, u8Len: csize_t, lut: pointer, lutLen: csize_t,
                              input: pointer, inputLen: csize_t, rows: cint): cint
+proc byhip_rope_steps*(rotDim: cint, base: cdouble, scaling: cint, factor, originalLen, slow,
+                       fast: cdouble, steps: ptr uint64, magnitude: ptr cfloat): cint
+proc byhip_rope_append*(q: pointer, qStride: csize_t, k: pointer, kStride: csize_t, v: pointer,
+                        vStride: csize_t, xDtype, heads, headDim: cint, rope: ptr ByhipRope,
+                        cache: ptr ByhipKvCache, batch: ptr ByhipKvBatch, qOut: pointer,
+                        qOutStride: csize_t, qOutDtype: cint): cint
+proc byhip_paged_attention*(q: pointer, qStride: csize_t, qDtype, heads: cint, attn: ptr ByhipAttn,
+                            cache: ptr ByhipKvCache, batch: ptr ByhipKvBatch, outp: pointer,
+                            outStride: csize_t, outDtype: cint): cint
+proc byhip_cache_fork*(pool: ptr ByhipKvPool, parents, rows: pointer, n: cint): cint
+proc byhip_cache_free*(pool: ptr ByhipKvPool, rows: pointer, n: cint): cint
+proc byhip_cache_grow*(pool: ptr ByhipKvPool, rows, add: pointer, n: cint): cint
+proc byhip_cache_compact*(pool: ptr ByhipKvPool, tableOut, refsOut: pointer): cint
+proc byhip_cache_copy*(pool: ptr ByhipKvPool, src, dst: pointer, n: cint): cint
+proc byhip_norm_block*(x: pointer, xStride: csize_t, xDtype, M, N: cint, post: ptr ByhipNorm,
+                       gate: pointer, gateStride: csize_t, res: pointer, resStride: csize_t,
+                       resScale: cfloat, h: pointer, hStride: csize_t, hDtype: cint,
+                       pre: ptr ByhipNorm, y: pointer, yStride: csize_t, yDtype: cint): cint
 {.pop.}
 
 proc hipCheck*(rc: cint, what: string) =
@@ -203,3 +248,51 @@ proc hipSessionF16GemmTile*(a, w: pointer, wHalves: int, c: pointer, M, K, N: in
 
 proc hipSessionTileGemmReady*(f16, tensorCore: bool): bool =
   byhip_tile_gemm_ready(f16.cint, tensorCore.cint) == 1
+
+# ── Attention over a paged cache (no counterpart in gpubackend.nim) ──────────────────────────
+
+proc hipSessionRopeAppend*(q, k, v: pointer, heads: int, rope: var ByhipRope, cache: var ByhipKvCache,
+                           batch: var ByhipKvBatch, qOut: pointer): bool =
+  ## fp32 handles of dense rows, like the other session ops
+  let d = cache.headDim.int
+  let rc = byhip_rope_append(q, csize_t(heads * d), k, csize_t(cache.kvHeads.int * d), v,
+                             csize_t(cache.kvHeads.int * d), BYHIP_F32, heads.cint, d.cint, addr rope,
+                             addr cache, addr batch, qOut, csize_t(heads * d), BYHIP_F32)
+  hipCheck(rc, "sessionRopeAppend")
+  rc == BYHIP_OK
+
+proc hipSessionPagedAttention*(q: pointer, heads: int, attn: var ByhipAttn, cache: var ByhipKvCache,
+                               batch: var ByhipKvBatch, outp: pointer): bool =
+  let n = csize_t(heads * cache.headDim.int)
+  let rc = byhip_paged_attention(q, n, BYHIP_F32, heads.cint, addr attn, addr cache, addr batch, outp, n,
+                                 BYHIP_F32)
+  hipCheck(rc, "sessionPagedAttention")
+  rc == BYHIP_OK
+
+proc hipSessionNormBlock*(x: pointer, M, N: int, post: ptr ByhipNorm, gate, res: pointer,
+                          resScale: float32, h: pointer, pre: ptr ByhipNorm, y: pointer): bool =
+  let rc = byhip_norm_block(x, csize_t(N), BYHIP_F32, M.cint, N.cint, post, gate, csize_t(N), res,
+                            csize_t(N), resScale.cfloat, h, csize_t(N), BYHIP_F32, pre, y, csize_t(N),
+                            BYHIP_F32)
+  hipCheck(rc, "sessionNormBlock")
+  rc == BYHIP_OK
+
+proc hipSessionCacheFork*(pool: var ByhipKvPool, parents, rows: pointer, n: int): bool =
+  let rc = byhip_cache_fork(addr pool, parents, rows, n.cint)
+  hipCheck(rc, "sessionCacheFork")
+  rc == BYHIP_OK
+
+proc hipSessionCacheFree*(pool: var ByhipKvPool, rows: pointer, n: int): bool =
+  let rc = byhip_cache_free(addr pool, rows, n.cint)
+  hipCheck(rc, "sessionCacheFree")
+  rc == BYHIP_OK
+
+proc hipSessionCacheGrow*(pool: var ByhipKvPool, rows, add: pointer, n: int): bool =
+  let rc = byhip_cache_grow(addr pool, rows, add, n.cint)
+  hipCheck(rc, "sessionCacheGrow")
+  rc == BYHIP_OK
+
+proc hipSessionCacheCompact*(pool: var ByhipKvPool): bool =
+  let rc = byhip_cache_compact(addr pool, nil, nil)
+  hipCheck(rc, "sessionCacheCompact")
+  rc == BYHIP_OK
