@@ -2,6 +2,8 @@
 // among blocks and the layout of partial results.
 #pragma once
 
+#include <algorithm>
+
 #include "byhip_cache.h"
 
 namespace byhip {
@@ -86,6 +88,9 @@ template <int R, int DIM>
 __device__ __forceinline__ float* part_slot(float* part, int slot) {
     return part + (size_t)slot * R * (DIM + 2);
 }
+
+// Keys that a table's row has room for.
+inline long long key_room(const AttnArgs& a) { return std::max(1LL, (long long)a.s.stride * a.c.page_size); }
 
 // The launches, per type of the cache; `precise`: fp32 queries or outputs.
 void launch_attn_rows_f16(const AttnArgs& a, bool precise);

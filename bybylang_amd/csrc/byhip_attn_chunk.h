@@ -646,7 +646,10 @@ template <int CT, int NP, int DIM, int USED, int WAVES>
 void launch_chunk(const AttnArgs& a) {
     constexpr size_t kSlots = (size_t)2 * 32 * WAVES * (DIM + 2) * sizeof(float);  // one block's
     const size_t room = (kAttnWorkspaceBytes - kAttnJoinBytes) / kSlots;
-    const unsigned blocks = (unsigned)std::min<size_t>(room, compute_units());
+    // no more than the tiles that the tables have room for
+    const long long items = (a.s.batch + (long long)a.s.rows * a.group / (32 * WAVES)) * a.c.kv_heads;
+    const long long tiles = items * ((key_room(a) + kChunkKeys - 1) / kChunkKeys);
+    const unsigned blocks = (unsigned)std::min<long long>(std::min<long long>((long long)room, compute_units()), std::max(1LL, tiles));
     if (a.softcap > 0.0f || a.slopes || !(a.scale > 0.0f)) launch("attn_chunk", (attn_chunk<CT, NP, DIM, USED, WAVES, true>), dim3(blocks), dim3(64 * WAVES), 0, a);
     else launch("attn_chunk", (attn_chunk<CT, NP, DIM, USED, WAVES, false>), dim3(blocks), dim3(64 * WAVES), 0, a);
     BYHIP_LAUNCHED("attn_chunk");

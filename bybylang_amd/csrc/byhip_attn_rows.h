@@ -20,6 +20,8 @@
 // weights likewise, one matrix instruction per term; the memory still bounds it.
 #pragma once
 
+#include <algorithm>
+
 #include "byhip_attn.h"
 
 namespace byhip {
@@ -292,8 +294,13 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
 
     const auto tiles_of = [&](const SeqInfo& s) { return TileRange<kKeys>(a, s, s.first_pos, s.first_pos + s.rows / a.group - 1); };
-    // 1. units before each sequence: a run of sequences per thread, then a scan over the block
-    {
+    // 1. units before each sequence: a run of sequences per thread, then a scan over the block (1.2 us, so not for one)
+    const bool one = a.s.batch == 1;
+    long long all_units = 0;
+    if (one) {
+        const SeqInfo s = seq_info(a, 0);
+        if (s.rows) all_units = (long long)((s.rows + kRows - 1) / kRows) * tiles_of(s).tiles;
+    } else {
         const int per = (a.s.batch + 255) / 256, b0 = min(tid * per, a.s.batch), b1 = min(b0 + per, a.s.batch);
         long long sum = 0;
         for (int b = b0; b < b1; ++b) {
@@ -313,8 +320,9 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
         for (int b = b0; b < b1; ++b) before[b] += base;
         if (tid == 255) before[a.s.batch] = base + sum;
         __syncthreads();
+        all_units = before[a.s.batch];
     }
-    const long long per_head = uniform(before[a.s.batch]), total = per_head * a.c.kv_heads;
+    const long long per_head = uniform(all_units), total = per_head * a.c.kv_heads;
     // 2. this block's run of units
     const long long blocks = min((long long)gridDim.x, max(1LL, (total + kWaves - 1) / kWaves));
     const int w = blockIdx.x;
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
             else hi = mid - 1;
         }
         const int b = uniform(lo);
-        const long long local = in_head - uniform(before[b]);
+        const long long local = one ? in_head : in_head - uniform(before[b]);
         SeqInfo s = seq_info(a, b);
         const auto range = tiles_of(s);
         const int rt = (int)(local / range.tiles), t0 = (int)(local % range.tiles);
@@ -441,11 +449,16 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
 
 template <int CT, int NP, int DIM>
 void launch_rows(const AttnArgs& a) {
-    const unsigned blocks = (unsigned)(compute_units() * rows_blocks(DIM));
+    // no more than the units that the tables have room for
+    const long long row_tiles = a.s.batch + (long long)a.s.rows * a.group / kRows;
+    const long long units = row_tiles * ((key_room(a) + kKeys - 1) / kKeys) * a.c.kv_heads;
+    const unsigned blocks = (unsigned)std::min<long long>(compute_units() * rows_blocks(DIM), std::max(1LL, (units + kWaves - 1) / kWaves));
+    // a token per sequence, as a rule, where there are no more rows than sequences: a tile then has the group's rows
+    const unsigned join_rows = (unsigned)(a.s.rows <= a.s.batch ? std::min(kRows, a.group) : kRows);
     if (a.softcap > 0.0f || a.slopes) launch("attn_rows", (attn_rows<CT, NP, DIM, true>), dim3(blocks), dim3(256), 0, a);
     else launch("attn_rows", (attn_rows<CT, NP, DIM, false>), dim3(blocks), dim3(256), 0, a);
     BYHIP_LAUNCHED("attn_rows");
-    launch("attn_join", (attn_join<kRows, DIM, 4>), dim3(blocks, kRows), dim3(256), 0, a);
+    launch("attn_join", (attn_join<kRows, DIM, 4>), dim3(blocks, join_rows), dim3(256), 0, a);
     BYHIP_LAUNCHED("attn_join");
 }
 
