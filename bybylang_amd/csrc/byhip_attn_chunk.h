@@ -172,15 +172,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     int4 join = make_int4(0, 0, 0, 0);
     int pass = 0;
 
-    // This lane's places in the LDS tiles: pieces 2 st + hf of key c at k_at ^ 32 st (K's piece i of key j lies at i ^ j), and
-    // keys 4 hf + (lane % 16) / 4 (+ 8 j + 16 st), values 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) at v_at ^ 64 dt (V's
-    // piece i of key j at i ^ 2 j, so that the 4 keys of a transposing read fall on different banks).
-    const int k_at = c * ROW + ((hf ^ (c & SW)) << 4);
+    // A key's pieces are turned within its row in LDS, so that what one cycle reads, 256 bytes, lies on different banks: K's, of
+    // which 16 lanes read a piece each of 16 keys, and V's, of which 32 lanes read 64 bytes each of 4 keys. K's piece i of key j
+    // lies at i ^ k_turn(j), V's at i ^ v_turn(j); turns of keys whose bits do not overlap combine.
+    const auto k_turn = [](int j) INLINE { return (PIECES >= 16 ? j : j >> 1) & SW; };
+    const auto v_turn = [](int j) INLINE { return (PIECES >= 16 ? 4 * j : 2 * j) & SW; };
+    // This lane's places: pieces 2 st + hf of key c at k_at ^ 32 st, and keys 4 hf + (lane % 16) / 4 (+ 8 j + 16 st), values
+    // 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) at v_at ^ 64 dt.
+    const int k_at = c * ROW + ((hf ^ k_turn(c)) << 4);
     const int v_key = 4 * hf + (lane & 15) / 4;
-    const int v_at = v_key * ROW + (((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ (2 * v_key & SW)) << 4) + 8 * (lane & 1);
+    const int v_at = v_key * ROW + (((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ v_turn(v_key)) << 4) + 8 * (lane & 1);
     // and its share of the direct loads: keys load_key + i RPI, whose bits do not overlap, the piece that belongs at lane % PIECES
     const int load_key = wave * NI * RPI + lane / PIECES;
-    const int k_piece = (lane % PIECES) ^ (load_key & SW), v_piece = (lane % PIECES) ^ (2 * load_key & SW);
+    const int k_piece = (lane % PIECES) ^ k_turn(load_key), v_piece = (lane % PIECES) ^ v_turn(load_key);
     lds_byte* const lds3 = (lds_byte*)lds;
     const uint32_t pages_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_byte*)looked_up[wave][0]);
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds3);
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
         };
         const auto load = [&](const uint16_t* base, const Keys& k, int to, auto index, auto values) INLINE {
             constexpr int i = decltype(index)::value;
-            const int piece = decltype(values)::value ? v_piece ^ (2 * i * RPI & SW) : k_piece ^ (i * RPI & SW);
+            const int piece = decltype(values)::value ? v_piece ^ v_turn(i * RPI) : k_piece ^ k_turn(i * RPI);
             // selected with masks, not with branches: a divergent branch in the loop would keep it off scalar control flow
             const uint32_t in = bit_mask(k.row[i] != ~0u) & bit_mask(8 * piece < a.c.dim);
             const uint64_t there_at = reinterpret_cast<uint64_t>(base) + ((uint64_t)k.row[i] * a.c.dim + 8 * piece) * 2;
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                     f16v add;
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {  // dimensions 32 dt + 8 g + 4 hf .. + 3
-                        const int piece = (4 * dt + g) ^ (2 * key & SW);
+                        const int piece = (4 * dt + g) ^ v_turn(key);
                         const uint2 v = *reinterpret_cast<const uint2*>(vt + key * ROW + piece * 16 + 8 * hf);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
