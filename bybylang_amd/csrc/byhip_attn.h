@@ -43,7 +43,8 @@ struct SeqInfo {
 
 __device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, int b) {
     SeqInfo s;
-    const int n = a.s.starts[b + 1] - a.s.starts[b];
+    const int from = a.s.starts[b], to = a.s.starts[b + 1];
+    const int n = from >= 0 && to <= a.s.rows ? max(0, to - from) : 0;  // rows outside the call's are no rows
     s.first_pos = a.s.lens[b] - n;
     s.len = max(0, seq_len(a.s, a.c, b));
     s.prefix = a.prefix ? max(0, min(a.prefix[b], s.len)) : 0;

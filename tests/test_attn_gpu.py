@@ -92,6 +92,13 @@ def test_heads_of_other_sizes(hip, D):
     Case(hip, [40, 9], [3, 9], 4, 2, D, 8, F16, F32, F32, seed=D).check()
 
 
+@pytest.mark.parametrize("D", [8, 72, 80, 96, 104, 136, 200])
+@pytest.mark.parametrize("ct,qt", [(F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)])
+def test_heads_that_do_not_fill_their_tiles(hip, D, ct, qt):
+    """Prompts, chunks and single tokens of heads between the sizes that the kernels on matrix instructions are made for."""
+    Case(hip, [130, 300, 77], [130, 50, 1], 6, 2, D, 16, ct, qt, qt, seed=D).check()
+
+
 @pytest.mark.parametrize("H,Hk", [(1, 1), (5, 1), (7, 7), (12, 4), (16, 1), (40, 2), (33, 1)])
 def test_groups(hip, H, Hk):
     Case(hip, [130, 65], [1, 40], H, Hk, 64, 16, BF16, seed=H).check()
@@ -134,6 +141,23 @@ def test_rows_outside_the_starts_stay(hip):
 
 MASKS = [dict(window=1), dict(window=20), dict(window=64), dict(cap=5.0), dict(slopes=True), dict(prefix=[0, 40, 90]), dict(prefix=[500, 1, 70], window=16),
          dict(cap=20.0, window=33, slopes=True, prefix=[10, 60, 5]), dict(cap=30.0, slopes=True), dict(window=1000, prefix=[3, 3, 3])]
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [1, 60, 40]])
+def test_sequences_with_rows_past_the_calls_are_left_out(hip, new):
+    """`rows` below the last start: the sequence whose rows pass it keeps its outputs as they were, the others have theirs."""
+    c = Case(hip, [90, 70, 80], new, 4, 2, 64, 16, F16, F32, F32)
+    up = hip.DeviceBuffer.from_array
+    bufs = [up(a) for a in (c.q, c.kv[0], c.kv[1], c.table, c.starts, np.array(c.lens, np.int32))]
+    q, k, v, t, s, n = bufs
+    out = up(np.full((c.T, c.W), 77.0, np.float32))  # room for all rows; the call is told of fewer
+    rows = int(c.starts[2])
+    hip.paged_attention(q, c.W, F32, 4, hip.Attn(c.scale), hip.KvCache(k, v, F16, c.pages, 16, 2, 64),
+                        hip.KvBatch(t, c.table.shape[1], s, n, 3, rows), out, c.W, F32)
+    got = out.read(np.float32, c.T * c.W).reshape(c.T, 4, 64)
+    assert np.all(got[rows:] == 77.0)
+    c.new = new[:2] + [0]
+    c.check(got.astype(np.float64))
 
 
 @pytest.mark.parametrize("kw", MASKS, ids=[",".join(k) + str(i) for i, k in enumerate(MASKS)])
