@@ -5,7 +5,7 @@
 // host round trip, and can be recorded. What has to be decided in order (which free page goes to whom, which
 // of several sharers keeps a page) is decided by one block with prefix sums, so the outcome never depends on
 // scheduling; the bytes then move in one copy kernel over all layers, at the rate of a plain copy (841 MB of live pages
-// in 163 us, 5.2 TB/s; the planning block 10 us, a chain of prefix sums).
+// in 163 us, 5.2 TB/s; the planning blocks 8 to 10 us, a chain of reads and prefix sums).
 #include <algorithm>
 
 #include "byhip_cache.h"
@@ -37,22 +37,24 @@ __device__ __forceinline__ int pages_of(int tokens, int page_size) {
     return tokens <= 0 ? 0 : (int)(((long long)tokens + page_size - 1) / page_size);
 }
 
-// Exclusive prefix sum over the block's threads; the total in every thread.
-__device__ __forceinline__ int block_prefix(int v, int* red, int& total) {
+// Exclusive prefix sum over the block's threads; the total in every thread. `red`: one value per wave.
+template <typename T>
+__device__ __forceinline__ T block_prefix(T v, T* red, T& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int s = v;
+    T s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(s, o, 64);
+        const T u = __shfl_up(s, o, 64);
         if (lane >= o) s += u;
     }
     __syncthreads();
     if (lane == 63) red[wave] = s;
     __syncthreads();
-    int before = 0;
+    T before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < kPlanThreads / 64; ++w) {
-        if (w == wave) before = total;
+        before += w < wave ? red[w] : 0;
         total += red[w];
     }
     return before + s - v;
@@ -90,8 +92,9 @@ __global__ __launch_bounds__(256) void cache_assign(PoolArgs p, const int* paren
 // One block: room for add[i] more tokens in slot rows[i].
 __global__ __launch_bounds__(kPlanThreads) void cache_grow_plan(PoolArgs p, const int* rows, const int* add, int n, int* free_list,
                                                                 MoveList copies) {
-    __shared__ int row_of[kMaxRows], last_of[kMaxRows], first_of[kMaxRows], sum_before[kMaxRows + 1], shares[kMaxRows];
+    __shared__ int row_of[kMaxRows], last_of[kMaxRows], first_of[kMaxRows], sum_before[kMaxRows + 1];
     __shared__ int red[kPlanThreads / 64];
+    __shared__ unsigned long long red_counts[kPlanThreads / 64];
     const int i = threadIdx.x;
     const int row = i < n ? rows[i] : -1, more = i < n ? add[i] : 0;
     row_of[i] = row;
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(kPlanThreads) void cache_grow_plan(PoolArgs p, cons
         for (int e = 0; e < kPerThread; ++e)
             if (at + e < p.pages && p.refs[at + e] <= 0) mask |= 1u << e;
         int here;
-        int rank = found + block_prefix(__popc(mask), red, here);
+        int rank = found + block_prefix((int)__popc(mask), red, here);
 #pragma unroll
         for (int e = 0; e < kPerThread; ++e)
             if (mask >> e & 1) {
@@ -144,12 +147,14 @@ __global__ __launch_bounds__(kPlanThreads) void cache_grow_plan(PoolArgs p, cons
         found += here;
     }
     // 4. slots are served up to the first that does not fit
-    const bool served = grows && before + need <= found;
-    shares[i] = served ? need : 0;
+    const bool served = grows && before + need <= found, refused = too_long || (grows && !served);
     __threadfence_block();
-    __syncthreads();
-    int taken;
-    block_prefix(shares[i], red, taken);
+    // one sum for all counts: copies, refused and bad slots (11 bits each), pages taken (31)
+    unsigned long long counts;
+    const unsigned long long mine_before = block_prefix(
+        (unsigned long long)(served && copy) | (unsigned long long)refused << 11 | (unsigned long long)(bad && i < n) << 22 |
+            (unsigned long long)(served ? need : 0) << 33, red_counts, counts);
+    const int copied = (int)(counts & 2047), n_refused = (int)(counts >> 11 & 2047), n_bad = (int)(counts >> 22 & 2047), taken = (int)(counts >> 33);
     for (int k = i; k < taken; k += kPlanThreads) {
         int lo = 0, hi = n - 1;  // the last slot whose sum before it is <= k and that takes pages
         while (lo < hi) {
@@ -162,8 +167,7 @@ __global__ __launch_bounds__(kPlanThreads) void cache_grow_plan(PoolArgs p, cons
         p.table[(size_t)row_of[lo] * p.stride + col] = page;
         p.refs[page] = 1;
     }
-    int copied;
-    const int slot = block_prefix(served && copy, red, copied);
+    const int slot = (int)(mine_before & 2047);
     if (served && copy) {
         copies.src[slot] = last;
         copies.dst[slot] = free_list[before];
@@ -181,10 +185,6 @@ __global__ __launch_bounds__(kPlanThreads) void cache_grow_plan(PoolArgs p, cons
         }
         p.lens[row] = keep;
     }
-    const bool refused = too_long || (grows && !served);
-    int n_refused, n_bad;
-    block_prefix(refused, red, n_refused);
-    block_prefix(bad && i < n, red, n_bad);
     if (i == 0) {
         *copies.count = copied;
         if (n_refused) atomicAdd(&p.status[0], n_refused);
@@ -215,16 +215,16 @@ __global__ __launch_bounds__(kPlanThreads) void cache_compact_plan(PoolArgs p, i
                 remap[at + e] = at + e;
                 if (refs_out != p.refs) refs_out[at + e] = r;
             }
-        int h, m;
-        int hr = holes + block_prefix(__popc(hole), red, h);
-        int mr = movers + block_prefix(__popc(mover), red, m);
+        int both;  // a turn has at most 8192 of each: one sum for the two
+        const int before = block_prefix((int)(__popc(hole) | __popc(mover) << 16), red, both);
+        int hr = holes + (before & 0xFFFF), mr = movers + (before >> 16);
 #pragma unroll
         for (int e = 0; e < kPerThread; ++e) {
             if (hole >> e & 1) moves.dst[hr++] = at + e;
             if (mover >> e & 1) moves.src[mr++] = at + e;
         }
-        holes += h;
-        movers += m;
+        holes += both & 0xFFFF;
+        movers += both >> 16;
     }
     __threadfence_block();
     __syncthreads();
