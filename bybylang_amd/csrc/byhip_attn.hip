@@ -89,8 +89,14 @@ void launch_general(const AttnArgs& a) {
     BYHIP_LAUNCHED("attn_general");
 }
 
-// Rows per key head from which attn_chunk reads a sequence: attn_rows reads its keys once per 16 rows.
-constexpr int kChunkRows = 33;
+// Rows per key head from which attn_chunk reads a sequence. attn_rows reads its keys once per 16 rows; attn_chunk reads them once
+// per 256 but starts 10 us later, which is 56 MB at attn_rows' rate. 16 sequences of 4096 keys, 8 key heads of 128 values (268 MB),
+// 16 rows: 64 us with attn_rows, 68 with attn_chunk; 32 rows: 100 and 68; one sequence of 600 keys, 32 rows: 15 and 25. With fp32
+// rows, whose terms attn_chunk multiplies for 128 rows at least, 32 rows take 110 and 117 on bf16 (256 values: 240 and 403).
+int chunk_rows(const AttnArgs& a, bool precise) {
+    const double bytes = (double)a.s.batch * key_room(a) * a.c.kv_heads * a.c.dim * 4.0;  // keys and values there is room for
+    return !precise && bytes >= 56e6 ? 17 : 33;
+}
 
 // Whether the kernels on matrix instructions take the cache: whole 16-byte pieces of a head, cache rows that 32 bits count.
 bool takes(const AttnArgs& a) {
@@ -107,7 +113,8 @@ void launch_tiled(AttnArgs a) {
     // sequences of few rows and of many go to a launch each, which passes over the others.
     const long long rows = (long long)a.s.rows * a.group;
     const bool one = a.s.batch == 1;
-    const bool few = !one || rows < kChunkRows, many = one ? rows >= kChunkRows : a.s.rows > a.s.batch;
+    const int from = chunk_rows(a, precise);
+    const bool few = !one || rows < from, many = one ? rows >= from : a.s.rows > a.s.batch;
     const AttnArgs whole = a;
     for (int b0 = 0; b0 < whole.s.batch; b0 += kAttnBatch) {
         a.s.table = whole.s.table + (size_t)b0 * whole.s.stride;
@@ -116,9 +123,9 @@ void launch_tiled(AttnArgs a) {
         a.s.batch = std::min(kAttnBatch, whole.s.batch - b0);
         a.prefix = whole.prefix ? whole.prefix + b0 : nullptr;
         a.min_rows = 1;
-        a.max_rows = many ? kChunkRows - 1 : 0x7FFFFFFF;
+        a.max_rows = many ? from - 1 : 0x7FFFFFFF;
         if (few) (f16 ? launch_attn_rows_f16 : launch_attn_rows_bf16)(a, precise);
-        a.min_rows = few ? kChunkRows : 1;
+        a.min_rows = few ? from : 1;
         a.max_rows = 0x7FFFFFFF;
         if (many) (f16 ? launch_attn_chunk_f16 : launch_attn_chunk_bf16)(a, precise);
     }

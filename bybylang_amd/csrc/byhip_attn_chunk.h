@@ -164,7 +164,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     }
     const long long per_head = uniform(units_before[NT]), total = per_head * a.c.kv_heads;
     const long long items = (long long)all_row_tiles * a.c.kv_heads;
-    // Whole items where the fullest block then has no more than with equal shares and their cuts.
+    // Whole items where the fullest block then has no more than with equal shares and their cuts (64 values, 255 rows x 1024
+    // keys: 240 items whole 47 us, cut 62; 264 items 71 and 64; 4 x 2100 rows x 4000 keys, 288 items: 182 and 129).
     const bool whole = (items + gridDim.x - 1) / gridDim.x * uniform(longest) <= max((long long)kShareTiles, total / gridDim.x) + kCutTiles;
     const long long blocks = min((long long)gridDim.x, whole ? items : max(1LL, total / kShareTiles));
     int w = blockIdx.x;

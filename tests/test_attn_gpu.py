@@ -223,6 +223,13 @@ def test_equal_runs_and_batches(hip):
     assert np.array_equal(c.run()[31:], a[31:])
 
 
+@pytest.mark.parametrize("ct", [F16, BF16])
+def test_rows_beside_long_tables(hip, ct):
+    """Tables with room for many keys, whatever the sequences hold: 4 to 24 rows per key head and single tokens."""
+    Case(hip, [300, 90, 17, 200, 1000], [12, 1, 8, 2, 9], 4, 2, 64, 16, ct, ct, ct, cols=4000).check()
+    Case(hip, [300], [11], 4, 2, 64, 16, ct, ct, ct, cols=16000).check()
+
+
 def test_cache_past_4_gib(hip):
     g = synth.rng(6400)
     Hk, page, D, pages = 8, 64, 128, 34000  # 4.46 GB each of keys and values
