@@ -16,7 +16,7 @@
 // order, so that blocks on one XCD read the same head's keys through its L2.
 //
 // What bounds it: the two phases of a tile, products and exponentials, which two waves per SIMD run in turn. 4096 rows x 16384
-// keys, 32 heads of 128 values, bf16: 0.94 to 0.97 ms, 1 PFLOP/s, matrix instructions busy 49% of the cycles. With 64 values the
+// keys, 32 heads of 128 values, bf16: 0.94 to 1.05 ms by the clock of the card, 920 to 1020 TFLOP/s, matrix instructions busy 49% of the cycles. With 64 values the
 // exponentials outweigh the products (4 x 700 rows x 4000 keys: 138 us, 455 TFLOP/s; capped 180 us).
 //
 // fp32 queries or outputs: two fp16 or three bf16 terms of queries and weights, a matrix instruction each, in blocks of 4
