@@ -50,7 +50,8 @@ class KvCache(C.Structure):
 
 class KvBatch(C.Structure):
     _fields_ = [("table", C.c_void_p), ("starts", C.c_void_p), ("lens", C.c_void_p),
-                ("batch", C.c_int), ("table_stride", C.c_int), ("rows", C.c_int)]
+                ("batch", C.c_int), ("table_stride", C.c_int), ("rows", C.c_int),
+                ("granted", C.c_void_p)]
 
 
 class Rope(C.Structure):
@@ -66,7 +67,7 @@ class Attn(C.Structure):
 class KvPool(C.Structure):
     _fields_ = [("caches", C.POINTER(KvCache)), ("n_caches", C.c_int), ("refs", C.c_void_p),
                 ("table", C.c_void_p), ("lens", C.c_void_p), ("slots", C.c_int),
-                ("table_stride", C.c_int), ("status", C.c_void_p)]
+                ("table_stride", C.c_int), ("status", C.c_void_p), ("granted", C.c_void_p)]
 
 
 class Norm(C.Structure):

@@ -120,6 +120,7 @@ void launch_tiled(AttnArgs a) {
         a.s.table = whole.s.table + (size_t)b0 * whole.s.stride;
         a.s.starts = whole.s.starts + b0;
         a.s.lens = whole.s.lens + b0;
+        a.s.granted = whole.s.granted ? whole.s.granted + b0 : nullptr;
         a.s.batch = std::min(kAttnBatch, whole.s.batch - b0);
         a.prefix = whole.prefix ? whole.prefix + b0 : nullptr;
         a.min_rows = 1;

@@ -19,6 +19,7 @@ struct BatchArgs {
     const int* table;
     const int* starts;
     const int* lens;
+    const int* granted;
     int batch, stride, rows;
 };
 
@@ -34,6 +35,10 @@ __device__ __forceinline__ int seq_len(const BatchArgs& s, const CacheArgs& c, i
     const int len = s.lens[b];
     return len > room ? (int)room : len;
 }
+
+// Whether sequence b has room for the n rows that it brings: those of a refused cache_grow have no position, or they would be
+// placed over the tokens before them.
+__device__ __forceinline__ bool has_room(const BatchArgs& s, int b, int n) { return !s.granted || s.granted[b] >= n; }
 
 // The sequence of row t: the number of entries of starts[1 .. batch] that are <= t, `batch` when t belongs to
 // none. The 64 lanes of a wave look at 64 entries at a time, so 4096 sequences take two dependent loads.

@@ -23,6 +23,7 @@ struct PoolArgs {
     int* table;
     int* lens;
     int* status;
+    int* granted;
     int slots, stride, pages, page_size;
 };
 
@@ -174,6 +175,7 @@ __global__ __launch_bounds__(kPlanThreads) void cache_grow_plan(PoolArgs p, cons
         atomicSub(&p.refs[last], 1);
     }
     if (served) p.lens[row] = (int)want;
+    if (p.granted && !bad) p.granted[row] = served ? more : 0;
     // 5. slots that shrink release the pages past their new end
     if (!bad && more < 0) {
         const int keep = want < 0 ? 0 : (int)want;
@@ -315,11 +317,12 @@ Pool pool_args(const byhip_kv_pool* pool, bool needs_caches) {
     check_span(pool->table, (size_t)pool->slots * pool->table_stride * 4, "page table");
     check_span(pool->lens, (size_t)pool->slots * 4, "lengths");
     check_span(pool->status, 16, "pool status");
-    a.p.refs = pool->refs; a.p.table = pool->table; a.p.lens = pool->lens; a.p.status = pool->status;
+    if (pool->granted) check_span(pool->granted, (size_t)pool->slots * 4, "granted tokens");
+    a.p.refs = pool->refs; a.p.table = pool->table; a.p.lens = pool->lens; a.p.status = pool->status; a.p.granted = pool->granted;
     a.p.slots = pool->slots; a.p.stride = pool->table_stride; a.p.pages = first.pages; a.p.page_size = first.page_size;
     a.page_bytes = (size_t)first.kv_heads * first.page_size * first.head_dim * 2;
     a.wide = a.wide && a.page_bytes % 16 == 0;
-    for (void* w : {(void*)pool->refs, (void*)pool->table, (void*)pool->lens, (void*)pool->status}) note_device_write(w);
+    for (void* w : {(void*)pool->refs, (void*)pool->table, (void*)pool->lens, (void*)pool->status, (void*)pool->granted}) note_device_write(w);
     return a;
 }
 

@@ -64,8 +64,8 @@ __global__ __launch_bounds__(256) void rope_append(RopeArgs a, int units, int he
     const int t = blockIdx.x;
     const int b = find_sequence(a.s.starts, a.s.batch, t);
     if (b >= a.s.batch) return;
-    const int pos = a.s.lens[b] - a.s.starts[b + 1] + t;
-    if (pos < 0) return;
+    const int to = a.s.starts[b + 1], pos = a.s.lens[b] - to + t;
+    if (pos < 0 || !has_room(a.s, b, to - a.s.starts[b])) return;
     // the token's place in the pages
     size_t place = 0;
     bool in_cache = false;
@@ -172,8 +172,9 @@ BatchArgs batch_args(const byhip_kv_batch* b) {
     check_span(b->table, (size_t)b->batch * b->table_stride * 4, "page table");
     check_span(b->starts, ((size_t)b->batch + 1) * 4, "row starts");
     check_span(b->lens, (size_t)b->batch * 4, "lengths");
+    if (b->granted) check_span(b->granted, (size_t)b->batch * 4, "granted tokens");
     BatchArgs a;
-    a.table = b->table; a.starts = b->starts; a.lens = b->lens;
+    a.table = b->table; a.starts = b->starts; a.lens = b->lens; a.granted = b->granted;
     a.batch = b->batch; a.stride = b->table_stride; a.rows = b->rows;
     return a;
 }

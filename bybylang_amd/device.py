@@ -248,20 +248,21 @@ class KvCache(_Struct):
 
 class KvBatch(_Struct):
     """The sequences of a call (byhip_kv_batch): int32 page tables [batch][table_stride], row starts
-    [batch + 1] and lengths [batch] on the device."""
+    [batch + 1], lengths [batch] and, where grows may be refused, the tokens they got [batch] on the device."""
 
-    def __init__(self, table, table_stride: int, starts, lens, batch: int, rows: int):
-        super().__init__(_abi.KvBatch(table.ptr, starts.ptr, lens.ptr, batch, table_stride, rows),
-                         table, starts, lens)
+    def __init__(self, table, table_stride: int, starts, lens, batch: int, rows: int, granted=None):
+        super().__init__(_abi.KvBatch(table.ptr, starts.ptr, lens.ptr, batch, table_stride, rows, _ptr(granted)),
+                         table, starts, lens, granted)
 
 
 class KvPool(_Struct):
-    """The layers' caches with their shared page table, reference counts and lengths (byhip_kv_pool)."""
+    """The layers' caches with their shared page table, reference counts and lengths (byhip_kv_pool); `granted`
+    [slots] receives the tokens that each slot's last grow got."""
 
-    def __init__(self, caches, refs, table, table_stride: int, lens, slots: int, status):
+    def __init__(self, caches, refs, table, table_stride: int, lens, slots: int, status, granted=None):
         arr = (_abi.KvCache * len(caches))(*[c.value for c in caches])
         super().__init__(_abi.KvPool(arr, len(caches), refs.ptr, table.ptr, lens.ptr, slots, table_stride,
-                                     status.ptr), arr, caches, refs, table, lens, status)
+                                     status.ptr, _ptr(granted)), arr, caches, refs, table, lens, status, granted)
 
 
 class Rope(_Struct):

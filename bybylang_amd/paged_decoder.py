@@ -3,7 +3,8 @@ positions, and a cache whose sequences grow, fork, end and are compacted.
 
 `python -m bybylang_amd.paged_decoder` runs it: ragged prompts, beams that share their prompt's pages,
 recorded decode steps. A step reads its lengths from the device and grows them itself, so that one
-recording, replayed, is every further step.
+recording, replayed, is every further step. A slot that finds no room (no free page, or `max_len` reached) keeps
+its tokens and brings none: its rows of the output hold the stream without attention, and `granted` says so.
 """
 from __future__ import annotations
 
@@ -45,7 +46,8 @@ class PagedDecoder:
                        for _ in layers]
         self.table = _ints(np.full(slots * self.stride, -1))
         self.lens, self.refs, self.status = _ints([0] * slots), _ints([0] * pages), _ints([0] * 4)
-        self.pool = dev.KvPool(self.caches, self.refs, self.table, self.stride, self.lens, slots, self.status)
+        self.room = _ints([0] * slots)
+        self.pool = dev.KvPool(self.caches, self.refs, self.table, self.stride, self.lens, slots, self.status, self.room)
         self.starts, self.add, self.all_rows = _ints([0] * (slots + 1)), _ints([0] * slots), _ints(range(slots))
         self.some, self.others = _ints([0] * slots), _ints([0] * slots)
         steps, magnitude = dev.rope_steps(head_dim, rope_base)
@@ -67,13 +69,14 @@ class PagedDecoder:
         self.rows = int(sum(counts))
         self._set(self.starts, np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
         self._set(self.add, np.asarray(counts, np.int32))
-        self.batch = dev.KvBatch(self.table, self.stride, self.starts, self.lens, self.slots, self.rows)
+        self.batch = dev.KvBatch(self.table, self.stride, self.starts, self.lens, self.slots, self.rows, self.room)
 
     def set_input(self, x) -> None:
         self._set(self.x, np.asarray(x, np.float32).reshape(self.rows, self.width))
 
     def encode(self) -> None:
-        """The blocks over the rows of self.x, to self.y; the slots' sequences are longer by their rows afterwards."""
+        """The blocks over the rows of self.x, to self.y; the slots' sequences are longer by their rows afterwards, unless
+        there is no room for them."""
         T, E = self.rows, self.width
         ok = g.sessionCacheGrow(gbHip, self.pool, self.all_rows, self.add, self.slots)
         ok &= g.sessionNormBlock(gbHip, self.x, T, E, None, None, None, 1.0, self.h, self.norms[0], self.y)
@@ -121,8 +124,12 @@ class PagedDecoder:
     def lengths(self) -> np.ndarray:
         return g.sessionRead(gbHip, self.lens, self.slots).view(np.int32)
 
+    def granted(self) -> np.ndarray:
+        """The tokens that each slot's last step took: its rows, or 0 where there was no room for them."""
+        return g.sessionRead(gbHip, self.room, self.slots).view(np.int32)
+
     def refused(self) -> int:
-        """Tokens' rows that found no free page, since the start."""
+        """How many times a slot found no room for its rows, since the start."""
         return int(g.sessionRead(gbHip, self.status, 4).view(np.int32)[0])
 
 

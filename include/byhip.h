@@ -312,6 +312,10 @@ typedef struct byhip_kv_batch {
     const int* starts;  /* [batch + 1] */
     const int* lens;    /* [batch] */
     int batch, table_stride, rows;
+    const int* granted; /* [batch] or NULL: tokens that sequence b's last cache_grow got (byhip_kv_pool). Where it brings more
+                         * rows than that, they have no position: nothing is appended for them, and their attention is 0. A
+                         * caller whose grows may be refused passes it: lens then does not count the refused rows, and without
+                         * it they would take the places of the tokens before them, in pages that others may share. */
 } byhip_kv_batch;
 
 enum byhip_rope_layout {
@@ -376,7 +380,8 @@ int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype, int heads
  * sequence slot r holds lens[r] tokens in pages table[r * table_stride ..]; refs[p] counts the slots that
  * hold page p (0: free). All device arrays. status (device, 4 ints, cleared by the caller) adds up over
  * calls: [0] slots refused for want of pages or table columns, [1] entries refused as invalid (a slot or parent out of
- * range or named twice), [2] pages copied, [3] pages newly taken. A refused entry changes nothing else. */
+ * range or named twice), [2] pages copied, [3] pages newly taken. A refused entry changes nothing else but granted
+ * (device, [slots], or NULL): cache_grow writes there how many tokens a slot got, 0 where it was refused or shrank. */
 typedef struct byhip_kv_pool {
     const byhip_kv_cache* caches;
     int n_caches;
@@ -385,6 +390,7 @@ typedef struct byhip_kv_pool {
     int* lens;
     int slots, table_stride;
     int* status;
+    int* granted;
 } byhip_kv_pool;
 
 /* Slot rows[i] becomes a fork of slot parents[i]: what it held is released, the parent's pages are shared. A

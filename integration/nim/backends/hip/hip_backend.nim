@@ -32,6 +32,7 @@ type
   ByhipKvBatch* {.bycopy.} = object
     table*, starts*, lens*: pointer
     batch*, tableStride*, rows*: cint
+    granted*: pointer
   ByhipRope* {.bycopy.} = object
     layout*, rotDim*: cint
     magnitude*: cfloat
@@ -45,7 +46,7 @@ type
     nCaches*: cint
     refs*, table*, lens*: pointer
     slots*, tableStride*: cint
-    status*: pointer
+    status*, granted*: pointer
   ByhipNorm* {.bycopy.} = object
     kind*: cint
     eps*: cfloat
