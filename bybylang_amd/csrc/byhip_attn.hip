@@ -25,6 +25,7 @@ __global__ __launch_bounds__(256) void attn_general(AttnArgs a) {
     const int b = find_sequence(a.s.starts, a.s.batch, t);
     if (b >= a.s.batch) return;
     const SeqInfo s = seq_info(a, b);
+    if (s.rows == 0) return;  // its rows pass the call's
     const int pos = s.first_pos + t - a.s.starts[b];
     const int D = a.c.dim, kvh = h / a.group;
     const float slope = a.slopes ? a.slopes[h] : 0.0f;

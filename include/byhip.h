@@ -306,7 +306,7 @@ typedef struct byhip_kv_cache {
 /* The sequences of a call. Sequence b holds lens[b] tokens, this call's own among them, in pages
  * table[b * table_stride ..]; this call's rows starts[b] .. starts[b + 1] - 1 are its last tokens, so row i of
  * them has position lens[b] - (starts[b + 1] - starts[b]) + i. Device arrays; starts[0] = 0, ascending,
- * at most `rows`. */
+ * at most `rows`: a sequence whose rows pass them is left out. */
 typedef struct byhip_kv_batch {
     const int* table;
     const int* starts;  /* [batch + 1] */
