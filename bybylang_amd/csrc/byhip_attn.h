@@ -231,6 +231,12 @@ __device__ __forceinline__ void split_terms(float x, typename Half8<CT>::one (&t
     }
 }
 
+// The power of two by which a row of fp32 queries is multiplied before it is split into fp16 terms: its largest value `top` comes
+// to [2^14, 2^15). At most 2^100, so that scale / 2^shift stays a normal number (0 times a masked score of -infinity would be NaN):
+// rows of zeros, and rows below 2^-86, whose terms then end at 2^-125 or so, far below what a weight can show.
+__device__ __forceinline__ int query_shift(float top) { return min(fp16_range_shift(top), 100); }
+constexpr float kLeastScale = 0x1p-20f;  // smaller scales (and those that are not positive) are applied before the masks
+
 // Two 16-bit values, those that are not finite (all exponent bits `exp` set) as 0.
 __device__ __forceinline__ uint32_t finite_only(uint32_t x, uint32_t exp) {
     x &= (x & exp) == exp ? 0xFFFF0000u : ~0u;

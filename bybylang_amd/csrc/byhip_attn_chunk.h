@@ -256,7 +256,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
 #pragma unroll
                         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(p[d + e]));
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    shift = fp16_range_shift(top);
+                    shift = query_shift(top);
                 }
 #pragma unroll
                 for (int st = 0; st < STEPS; ++st) {
@@ -660,7 +660,7 @@ void launch_chunk(const AttnArgs& a) {
     const long long items = (a.s.batch + (long long)a.s.rows * a.group / (32 * WAVES)) * a.c.kv_heads;
     const long long tiles = items * ((key_room(a) + kChunkKeys - 1) / kChunkKeys);
     const unsigned blocks = (unsigned)std::min<long long>(std::min<long long>((long long)room, compute_units()), std::max(1LL, tiles));
-    if (a.softcap > 0.0f || a.slopes || !(a.scale > 0.0f)) launch("attn_chunk", (attn_chunk<CT, NP, DIM, USED, WAVES, true>), dim3(blocks), dim3(64 * WAVES), 0, a);
+    if (a.softcap > 0.0f || a.slopes || !(a.scale >= kLeastScale)) launch("attn_chunk", (attn_chunk<CT, NP, DIM, USED, WAVES, true>), dim3(blocks), dim3(64 * WAVES), 0, a);
     else launch("attn_chunk", (attn_chunk<CT, NP, DIM, USED, WAVES, false>), dim3(blocks), dim3(64 * WAVES), 0, a);
     BYHIP_LAUNCHED("attn_chunk");
     launch("attn_join", (attn_join<32 * WAVES, DIM, 1>), dim3(blocks, 16), dim3(256), 0, a);

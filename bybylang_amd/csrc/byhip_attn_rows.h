@@ -137,7 +137,7 @@ struct Rows {
             if constexpr (CT == BYHIP_F16) {  // the row's largest value to [2^14, 2^15)
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
-                shift = fp16_range_shift(top);
+                shift = query_shift(top);
             }
 #pragma unroll
             for (int st = 0; st < STEPS; ++st)
