@@ -235,6 +235,19 @@ __device__ __forceinline__ void split_terms(float x, typename Half8<CT>::one (&t
 // to [2^14, 2^15). At most 2^100, so that scale / 2^shift stays a normal number (0 times a masked score of -infinity would be NaN):
 // rows of zeros, and rows below 2^-86, whose terms then end at 2^-125 or so, far below what a weight can show.
 __device__ __forceinline__ int query_shift(float top) { return min(fp16_range_shift(top), 100); }
+// Value f of a row of queries, times 2^shift, as terms. A value too small for the first fp16 term still has its sign there (the second
+// takes it back), for a product with an infinite key.
+template <int CT, int NP>
+__device__ __forceinline__ void query_terms(float f, int shift, typename Half8<CT>::one (&t)[NP]) {
+    const float x = ldexpf(f, shift);
+    split_terms<CT, NP>(x, t);
+    if constexpr (CT == BYHIP_F16 && NP == 2) {
+        if ((float)t[0] == 0.0f && f != 0.0f) {
+            t[0] = (_Float16)copysignf(0x1p-24f, f);
+            t[1] = (_Float16)(x - (float)t[0]);
+        }
+    }
+}
 constexpr float kLeastScale = 0x1p-20f;  // smaller scales (and those that are not positive) are applied before the masks
 
 // Two 16-bit values, those that are not finite (all exponent bits `exp` set) as 0.

@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         typename Half8<CT>::one t[NP];
-                        split_terms<CT, NP>(ldexpf(f[e], shift), t);
+                        query_terms<CT, NP>(f[e], shift, t);
 #pragma unroll
                         for (int i = 0; i < NP; ++i) q[i][st][e] = t[i];
                     }
@@ -536,9 +536,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 for (int p = NP - 1; p >= 0; --p) o[k % DT] = mfma32(x, wt[p][k / DT], o[k % DT]);
             }
         };
+        const auto careful_scores = [&](int i) INLINE {  // S^T = K Q^T, infinite keys with the queries' first terms alone, which have their signs
+            if constexpr (EARLY) load_batch(i);
+            unrolled<0, NK>([&](auto k) INLINE {
+                constexpr int E = decltype(k)::value;
+                const vec x = k_operand(k_tile(i), E);
+                const uint4 v = __builtin_bit_cast(uint4, x);
+                const vec y = __builtin_bit_cast(vec, make_uint4(finite_only(v.x, kExp), finite_only(v.y, kExp), finite_only(v.z, kExp), finite_only(v.w, kExp)));
+                if constexpr (E / 2 == 0) sc[E % 2] = (f16v)(0.0f);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) sc[E % 2] = mfma32(p ? y : x, q[p][E / 2], sc[E % 2]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
         // Values that are not finite spoil the sums of rows that do not see them (0 times infinity), and of rows that do where
-        // weights have several terms (infinity less infinity). That shows in the sums, so the tiles are not searched for them: a block
-        // whose sums are not finite works through them once more, carefully, adding such values only where they are seen.
+        // weights have several terms (infinity less infinity), as infinite keys do where queries have. That shows in the sums,
+        // so the tiles are not searched for them: a block whose sums are not finite works through them once more, carefully,
+        // adding such values only where they are seen.
         bool careful = false;
         for (;;) {
             m = -INFINITY;
@@ -579,7 +593,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
                 products(v_tile(i), 0, 0, Index<1>{}, Index<0>{});
             } else {
                 for (int i = 0; i < n; ++i) {
-                    products(0, k_tile(i), i, Index<0>{}, Index<1>{});
+                    if constexpr (NP > 1) careful_scores(i);
+                    else products(0, k_tile(i), i, Index<0>{}, Index<1>{});
                     weights(i);
                     odd_values(i);
                 }

@@ -22,6 +22,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "byhip_attn.h"
 
@@ -38,6 +39,7 @@ struct Rows {
     typedef typename Half8<CT>::vec vec;
     static constexpr int STEPS = DIM / 32, V = DIM / 16;
     static constexpr float kShift = CT == BYHIP_F16 ? 7.0f : 0.0f;  // log2 of the weights' factor
+    static constexpr uint32_t kExp = CT == BYHIP_F16 ? 0x7C00u : 0x7F80u;
     typedef uint32_t KTile[2][STEPS][4];
     typedef uint32_t VTile[8][V / 2];
 
@@ -49,6 +51,7 @@ struct Rows {
     uint32_t kmask[STEPS];     // 0 for those past the end
     float slope, factor;       // factor: scale (and the row's power of two), with log2 e unless EXTRA
     float inv_cap;
+    bool valid;                // this lane's row exists
     vec q[NP][STEPS];
     float m, l;                // reference (log2) of row c; this lane's sum of weights
     f4 o[V];
@@ -107,7 +110,7 @@ struct Rows {
         s = seq_info(a, b);
         head = h;
         const int row = rt * kRows + c;
-        const bool valid = row < s.rows;
+        valid = row < s.rows;
         const int token = valid ? row / a.group : 0, hq = h * a.group + (valid ? row % a.group : 0);
         pos = s.first_pos + token;
         slope = EXTRA && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
@@ -144,7 +147,7 @@ struct Rows {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     typename Half8<CT>::one t[NP];
-                    split_terms<CT, NP>(ldexpf(x[st][e], shift), t);
+                    query_terms<CT, NP>(x[st][e], shift, t);
 #pragma unroll
                     for (int p = 0; p < NP; ++p) q[p][st][e] = t[p];
                 }
@@ -168,14 +171,24 @@ struct Rows {
         }
         inv_cap = EXTRA && a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
         factor = ldexpf(EXTRA ? a.scale : a.scale * kLog2e, -shift);
+    }
+    __device__ __forceinline__ void clear() {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
         for (int t = 0; t < V; ++t) o[t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
     }
+    __device__ __forceinline__ bool finite() const {  // whether all sums of the wave's rows are
+        float none = 0.0f;  // NaN where a sum is infinite or NaN
+#pragma unroll
+        for (int t = 0; t < V; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) none = fmaf(o[t][e], 0.0f, none);
+        return __ballot(none != 0.0f && valid) == 0;
+    }
 
     // One tile of keys j0 ..; `there`: bit j of the keys that exist; `read`: called once k has been read.
-    template <typename F>
+    template <bool CAREFUL, typename F>
     __device__ __forceinline__ void tile(const KTile& k, VTile& v, int j0, uint32_t there, int p0, int p1, F&& read) {
         float x[8];
 #pragma unroll
@@ -184,9 +197,16 @@ struct Rows {
 #pragma unroll
             for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-                for (int st = 0; st < STEPS; ++st)
-                    acc = mfma16(__builtin_bit_cast(vec, make_uint4(k[kb][st][0] & kmask[st], k[kb][st][1] & kmask[st], k[kb][st][2] & kmask[st],
-                                                                    k[kb][st][3] & kmask[st])), q[p][st], acc);
+                for (int st = 0; st < STEPS; ++st) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e] = k[kb][st][e] & kmask[st];
+                        // the further terms of a query may have another sign than it has, or be 0: an infinite key meets the first alone
+                        if (CAREFUL && p) w[e] = finite_only(w[e], kExp);
+                    }
+                    acc = mfma16(__builtin_bit_cast(vec, make_uint4(w[0], w[1], w[2], w[3])), q[p][st], acc);
+                }
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[4 * kb + r] = acc[r] * factor;
         }
@@ -216,7 +236,7 @@ struct Rows {
 #pragma unroll
             for (int t = 0; t < V; ++t) o[t] *= fade;
         }
-        if (!all || NP > 1) spare(v, see, there);
+        if (CAREFUL || !all) spare(v, see, there);
         const float base = m == -INFINITY ? 0.0f : m - kShift;
         vec w[NP];
 #pragma unroll
@@ -241,7 +261,7 @@ struct Rows {
     }
 
     // A hidden value that is not finite would spoil the sums (0 times infinity), and so would one that is seen where
-    // weights have several terms: values of keys that do not exist are cleared, others that are not finite are taken out of V and
+    // weights have several terms (CAREFUL): values of keys that do not exist are cleared, others that are not finite are taken out of V and
     // added to the rows that see them.
     __device__ __forceinline__ void spare(VTile& v, uint32_t see, uint32_t there) {
 #pragma unroll
@@ -250,7 +270,6 @@ struct Rows {
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) v[i][e] &= keep;
         }
-        constexpr uint32_t kExp = CT == BYHIP_F16 ? 0x7C00u : 0x7F80u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             uint32_t odd = 0;
@@ -357,18 +376,15 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
         // while one is worked on
         typename Rows<CT, NP, DIM, EXTRA>::KTile ka, kb;
         typename Rows<CT, NP, DIM, EXTRA>::VTile v;
-        int t = t0 + wave;
-        uint32_t rows = 0, next = 0, there = 0, next_there = 0;
-        if (t < t1) rows = r.key_row(b, range.key(t), there);
-        if (t + kWaves < t1) next = r.key_row(b, range.key(t + kWaves), next_there);
-        if (t < t1) r.load_k(ka, rows);
-        const auto step = [&](auto& cur, auto& ahead) {
-            constexpr bool kOneTile = DIM > 128 || (DIM > 64 && NP > 1);  // registers for one tile of keys: the next one's follow its last use
+        int t;
+        uint32_t rows, next, there, next_there;
+        const auto step = [&](auto& cur, auto& ahead, auto careful) __attribute__((always_inline)) {
+            constexpr bool kOneTile = DIM > 128 || (DIM > 64 && NP > 1) || decltype(careful)::value;  // registers for one tile of keys: the next one's follow its last use
             r.load_v(v, rows);
             uint32_t after = 0, after_there = 0;
             if (t + 2 * kWaves < t1) after = r.key_row(b, range.key(t + 2 * kWaves), after_there);
             if (!kOneTile && t + kWaves < t1) r.load_k(ahead, next);
-            r.tile(cur, v, range.key(t), there, p0, p1, [&] {
+            r.template tile<decltype(careful)::value>(cur, v, range.key(t), there, p0, p1, [&] {
                 if (kOneTile) r.load_k(cur, next);  // row 0 after the last tile
             });
             rows = next;
@@ -377,11 +393,25 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
             next_there = after_there;
             t += kWaves;
         };
-        while (t < t1) {
-            step(ka, kb);
-            if (DIM > 128 || (DIM > 64 && NP > 1)) continue;
-            if (t >= t1) break;
-            step(kb, ka);
+        const auto walk = [&](auto careful) __attribute__((always_inline)) {
+            r.clear();
+            t = t0 + wave;
+            rows = next = there = next_there = 0;
+            if (t < t1) rows = r.key_row(b, range.key(t), there);
+            if (t + kWaves < t1) next = r.key_row(b, range.key(t + kWaves), next_there);
+            if (t < t1) r.load_k(ka, rows);
+            while (t < t1) {
+                step(ka, kb, careful);
+                if (DIM > 128 || (DIM > 64 && NP > 1) || decltype(careful)::value) continue;
+                if (t >= t1) break;
+                step(kb, ka, careful);
+            }
+        };
+        // Values that are not finite, and infinite keys, spoil the sums of rows whose weights and queries have several terms. That
+        // shows in the sums, so the tiles are not searched for them: a wave whose sums are not finite walks once more, carefully.
+        walk(std::false_type{});
+        if constexpr (NP > 1) {
+            if (!r.finite()) walk(std::true_type{});
         }
 
         // 4. the waves' sums join in LDS

@@ -1,8 +1,10 @@
-"""byhip_paged_attention at the ends of its numbers: empty and tiny queries."""
+"""byhip_paged_attention at the ends of its numbers: empty and tiny queries, keys of
+-infinity."""
 import numpy as np
 import pytest
 
 from bybylang_amd import _abi
+from paged_ref import attention, close, from_bits, to_bits
 from test_attn_gpu import Case
 
 pytestmark = pytest.mark.gpu
@@ -18,3 +20,37 @@ def test_empty_and_tiny_queries(hip, new, ct, scale, value):
     c = Case(hip, [230], [new], 4, 2, 128, 32, ct, F32, F32, seed=20, scale=scale)
     c.q[::2] = np.float32(value) * np.sign(c.q[::2])
     c.check()
+
+
+@pytest.mark.parametrize("new", [1, 20, 200])
+@pytest.mark.parametrize("D", [20, 64, 128, 256])
+@pytest.mark.parametrize("ct,qt,ot", [(F16, F32, F32), (BF16, F32, F32), (F16, F16, F32), (F16, F16, F16), (BF16, BF16, BF16)])
+def test_keys_of_minus_infinity_have_no_weight(hip, new, D, ct, qt, ot):
+    c = Case(hip, [260], [new], 4, 2, D, 16, ct, qt, ot, seed=21)
+    rows = from_bits(c.q, qt)
+    rows[:, 5::D] = np.abs(rows[:, 5::D]) + 2.0**-9
+    rows[:, 9::D] = -2.0**-45 if qt == F32 else -2.0**-9  # 2^-45: below half of fp16's least value in its row's scale
+    c.q = to_bits(rows, qt)
+    inf = to_bits(np.array([np.inf, -np.inf]), ct)
+    low = np.zeros(260, bool)
+    for j, d, s in ((3, 5, 1), (40, 5, 1), (41, 9, 0), (59, 5, 1)):
+        c.kv[0][c.table[0, j // 16], :, j % 16, d] = inf[s]
+        low[j] = True
+    got = c.run()
+    q = from_bits(c.q, qt).reshape(-1, 4, D)
+    k, v, there = c.sequence(0)
+    k = np.where(np.isfinite(k), k, 0)
+    out, mean, size, flat = attention(q, k, v, float(np.float32(c.scale)), 0, 0, None, 0, ~low)
+    slack = (2 * np.sqrt(D) * 2.0**-24 * size + 4e-6 + np.sqrt(260) * 2.0**-22) * (mean + np.abs(out))
+    if F32 not in (qt, ot):
+        slack = slack + {F16: 2.0**-11, BF16: 2.0**-8}[ct] * mean + (2.0**-25 * flat if ct == F16 else 0)
+    close(got, out, ot, slack)
+
+
+def test_rows_whose_scores_are_all_minus_infinity(hip):
+    for new in (1, 20, 200):
+        for ct in (F16, BF16):
+            c = Case(hip, [230], [new], 4, 2, 64, 16, ct, F32, F32, seed=22)
+            c.q[:, 7::64] = np.abs(c.q[:, 7::64]) + 1
+            c.kv[0][..., 7] = to_bits(np.array([-np.inf]), ct)[0]
+            assert np.all(c.run() == 0)
