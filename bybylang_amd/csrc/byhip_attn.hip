@@ -70,7 +70,10 @@ __global__ __launch_bounds__(256) void attn_general(AttnArgs a) {
             const int l = __ffsll((unsigned long long)left) - 1;
             const float wj = __shfl(w, l, 64);
             const size_t rj = (size_t)__shfl((long long)row, l, 64);
-            for (int d = lane; d < D; d += 64) acc[d] = fmaf(wj, load1<CT>(a.c.v, rj * D + d), acc[d]);
+            for (int d = lane; d < D; d += 64) {
+                const float v = load1<CT>(a.c.v, rj * D + d);
+                acc[d] = wj == 0.0f && !(fabsf(v) < INFINITY) ? acc[d] + v : fmaf(wj, v, acc[d]);  // no weight is 0, it may only round to it
+            }
         }
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;

@@ -1,5 +1,5 @@
-"""byhip_paged_attention at the ends of its numbers: empty and tiny queries, keys of
--infinity."""
+"""byhip_paged_attention at the ends of its numbers: empty and tiny queries, infinite keys
+and values that are seen."""
 import numpy as np
 import pytest
 
@@ -54,3 +54,20 @@ def test_rows_whose_scores_are_all_minus_infinity(hip):
             c.q[:, 7::64] = np.abs(c.q[:, 7::64]) + 1
             c.kv[0][..., 7] = to_bits(np.array([-np.inf]), ct)[0]
             assert np.all(c.run() == 0)
+
+
+@pytest.mark.parametrize("new", [1, 20, 200])
+@pytest.mark.parametrize("D", [20, 64, 128, 256])
+@pytest.mark.parametrize("ct,qt", [(F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)])
+def test_infinite_values_show_however_small_their_weight(hip, new, D, ct, qt):
+    """A key that is seen has a weight above 0: an infinite value of it is the sum."""
+    c = Case(hip, [300], [new], 2, 1, D, 16, ct, qt, qt, seed=23, scale=1.0)
+    c.q = to_bits(np.abs(from_bits(c.q, qt)) + 0.5, qt)
+    top = from_bits(c.q, qt).reshape(-1, 2, D).sum(-1)
+    at = lambda j: (c.table[0, j // 16], slice(None), j % 16)  # noqa: E731
+    c.kv[0][at(37)] = to_bits(np.full((1, D), -240.0 / top.min()), ct)  # a score at least 120 below the others'
+    c.kv[0][at(38)] = to_bits(np.full((1, D), 120.0 / top.min()), ct)
+    c.kv[1][at(37)] = to_bits(np.where(np.arange(D) == 7, np.inf, np.where(np.arange(D) == 8, -np.inf, 1.0))[None], ct)
+    got = c.run()
+    assert np.all(got[..., 7] == np.inf) and np.all(got[..., 8] == -np.inf)
+    assert np.all(np.isfinite(np.delete(got, [7, 8], -1)))
