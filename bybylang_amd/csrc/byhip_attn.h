@@ -61,7 +61,8 @@ __device__ __forceinline__ bool sees(const AttnArgs& a, const SeqInfo& s, int po
 // The same for 32 keys j0 .. as bits, of those `there`. Formed without branches.
 __device__ __forceinline__ uint32_t low_bits(int n) { return (uint32_t)((1ull << max(0, min(n, 32))) - 1); }
 __device__ __forceinline__ uint32_t seen_keys(const AttnArgs& a, const SeqInfo& s, int pos, int j0, uint32_t there) {
-    const uint32_t gone = a.window > 0 ? low_bits(pos - a.window + 1 - j0) : 0u;
+    const int back = pos - j0;  // positions may lie below 0, so what a window near 2^31 leaves is not formed first
+    const uint32_t gone = a.window > 0 && back >= a.window ? low_bits(back - a.window + 1) : 0u;
     return there & ((low_bits(pos + 1 - j0) & ~gone) | low_bits(s.prefix - j0));
 }
 
@@ -71,7 +72,7 @@ template <int T>
 struct TileRange {
     int prefix_tiles, start, tiles;
     __device__ __forceinline__ TileRange(const AttnArgs& a, const SeqInfo& s, int p0, int p1) {
-        start = a.window > 0 ? max(0, p0 - a.window + 1) / T * T : 0;
+        start = a.window > 0 && p0 >= a.window ? (p0 - a.window + 1) / T * T : 0;
         const int end = max(0, max(min(s.len, p1 + 1), s.prefix));
         start = min(start, end / T * T);
         prefix_tiles = min((s.prefix + T - 1) / T, start / T);

@@ -1,5 +1,5 @@
-"""byhip_paged_attention at the ends of its numbers: empty and tiny queries, infinite keys
-and values that are seen."""
+"""byhip_paged_attention at the ends of its numbers: empty and tiny queries, infinite keys and values that
+are seen, windows near 2^31."""
 import numpy as np
 import pytest
 
@@ -71,3 +71,15 @@ def test_infinite_values_show_however_small_their_weight(hip, new, D, ct, qt):
     got = c.run()
     assert np.all(got[..., 7] == np.inf) and np.all(got[..., 8] == -np.inf)
     assert np.all(np.isfinite(np.delete(got, [7, 8], -1)))
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 4, 2**31 - 40])
+@pytest.mark.parametrize("prefix", [None, [30]])
+@pytest.mark.parametrize("beside", [0, 199])
+def test_windows_near_the_largest_number(hip, window, prefix, beside):
+    """More rows than tokens, so that the first rows' positions lie below 0: no window of this size hides a key."""
+    c = Case(hip, [130], [130], 2, 1, 64, 16, F16, F32, F32, seed=24, window=window, prefix=None if prefix is None else prefix + [0] * beside)
+    c.lens, c.new = [100] + [0] * beside, c.new + [0] * beside
+    c.table = np.concatenate([c.table, np.full((beside, c.table.shape[1]), -1, np.int32)])
+    c.starts = np.concatenate([c.starts, np.full(beside, c.starts[-1], np.int32)])
+    c.check()
