@@ -88,8 +88,11 @@ class PagedDecoder:
             ok &= g.sessionPagedAttention(gbHip, self.q_rot, self.heads, self.attn, cache, self.batch, self.a)
             ok &= g.sessionMatmulQ4(gbHip, self.a, wo, self.o, T)
             ok &= g.sessionNormBlock(gbHip, self.o, T, E, None, None, self.h, 1.0, self.h, norm, self.y)
+        self._taken(ok)
+
+    def _taken(self, ok: bool) -> None:
         if not ok:
-            raise _abi.HipUnsupported("PagedDecoder: an operator does not take these sizes")
+            raise _abi.HipUnsupported(f"PagedDecoder: an operator does not take these sizes ({g.sessionGetLastError(gbHip)})")
 
     def forward(self, x, counts) -> np.ndarray:
         self.set_rows(counts)
@@ -112,14 +115,14 @@ class PagedDecoder:
     def fork(self, parents, rows) -> None:
         self._set(self.some, np.asarray(parents, np.int32))
         self._set(self.others, np.asarray(rows, np.int32))
-        g.sessionCacheFork(gbHip, self.pool, self.some, self.others, len(rows))
+        self._taken(g.sessionCacheFork(gbHip, self.pool, self.some, self.others, len(rows)))
 
     def free(self, rows) -> None:
         self._set(self.some, np.asarray(rows, np.int32))
-        g.sessionCacheFree(gbHip, self.pool, self.some, len(rows))
+        self._taken(g.sessionCacheFree(gbHip, self.pool, self.some, len(rows)))
 
     def compact(self) -> None:
-        g.sessionCacheCompact(gbHip, self.pool)
+        self._taken(g.sessionCacheCompact(gbHip, self.pool))
 
     def lengths(self) -> np.ndarray:
         return g.sessionRead(gbHip, self.lens, self.slots).view(np.int32)

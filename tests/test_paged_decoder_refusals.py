@@ -1,0 +1,18 @@
+"""PagedDecoder says so when an operator does not take a call (no GPU: the session's procs are replaced)."""
+import pytest
+
+from bybylang_amd import _abi, gpubackend as g
+from bybylang_amd.paged_decoder import PagedDecoder
+
+
+@pytest.mark.parametrize("proc,call", [("sessionCacheFork", lambda d: d.fork([0], [1])), ("sessionCacheFree", lambda d: d.free([1])),
+                                       ("sessionCacheCompact", lambda d: d.compact())])
+def test_a_call_that_is_not_taken_raises(monkeypatch, proc, call):
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.pool = d.some = d.others = None
+    monkeypatch.setattr(d, "_set", lambda handle, values: None, raising=False)
+    monkeypatch.setattr(g, proc, lambda *a: True)
+    call(d)
+    monkeypatch.setattr(g, proc, lambda *a: False)
+    with pytest.raises(_abi.HipUnsupported, match="does not take"):
+        call(d)
