@@ -52,13 +52,14 @@ __device__ __forceinline__ void phase_barrier() {
 
 // 16 bytes per lane from memory to LDS byte `to` + 16 lane. Written as assembly because the compiler makes every later LDS
 // read wait for such loads, which here belong to tiles still ahead; it has no output register, phase_barrier waits for
-// it, and a wait of the compiler's own that counts it among its loads only waits longer.
+// it, and a wait of the compiler's own that counts it among its loads only waits longer. m0 (the LDS address) is an operand, so that
+// the compiler knows what it holds; the s_nop is the wait state between its write and the load.
 __device__ __forceinline__ void load_to_lds(const void* p, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(to) : "memory");
 }
 // The same for 4 bytes per lane.
 __device__ __forceinline__ void word_to_lds(const void* p, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(to) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "{m0}"(to) : "memory");
 }
 
 template <int I> struct Index { static constexpr int value = I; };
