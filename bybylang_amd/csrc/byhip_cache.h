@@ -105,7 +105,8 @@ __device__ __forceinline__ void store_vec(void* p, size_t i, const float (&v)[VE
 
 // Whether rows of dtype at p with this stride can be moved four values at a time.
 inline bool aligned4(const void* p, size_t stride, int dtype) {
-    return stride % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * dtype_bytes(dtype)) == 0;
+    const size_t bytes = 4 * dtype_bytes(dtype);  // 0: no dtype, which check_rows refuses
+    return bytes && stride % 4 == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0;
 }
 
 }  // namespace byhip

@@ -229,8 +229,8 @@ extern "C" int byhip_norm_block(const void* x, size_t x_stride, int x_dtype, int
         if (!h && !pre) fail("byhip: norm_block without an output");
         NormArgs a{};
         a.M = M; a.N = N; a.res_scale = res_scale;
-        int vec = aligned4(x, x_stride, x_dtype);
         check_rows(x, M, N, x_stride, x_dtype, "block output");
+        int vec = aligned4(x, x_stride, x_dtype);
         if (!dtype_bytes(h_dtype)) fail("byhip: residual dtype %d", h_dtype);
         if (res) { check_rows(res, M, N, res_stride, h_dtype, "residual"); vec = vec && aligned4(res, res_stride, h_dtype); }
         if (h) { check_rows(h, M, N, h_stride, h_dtype, "residual output"); vec = vec && aligned4(h, h_stride, h_dtype); }
