@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kPlanThreads) void cache_grow_plan(PoolArgs p, cons
     const int have = bad ? 0 : max(0, p.lens[row]);
     const long long want = (long long)have + more;
     int* mine = p.table + (size_t)(bad ? 0 : row) * p.stride;
-    const bool too_long = !bad && more > 0 && want > (long long)p.stride * p.page_size;
+    const bool too_long = !bad && more > 0 && want > min((long long)p.stride * p.page_size, 0x7FFFFFFFLL);
     const bool grows = !bad && !too_long && more > 0;
     int last = -1;  // the partly filled page it would append to
     if (grows && have % p.page_size) last = mine[have / p.page_size];
