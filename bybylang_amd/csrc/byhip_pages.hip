@@ -400,6 +400,8 @@ int byhip_cache_grow(const byhip_kv_pool* pool, const int* rows, const int* add,
         check_span(add, (size_t)n * 4, "token counts");
         if ((size_t)a.p.pages * 4 > kWorkspaceBytes - kListBytes)
             unsupported("byhip: a pool of %d pages is more than the library's workspace plans for", a.p.pages);
+        if ((long long)n * (a.p.stride + 1LL) > 0x7FFFFFFF)  // the plan adds up the pages that the slots ask for
+            unsupported("byhip: %d slots of %d pages in one call: more pages than 31 bits count", n, a.p.stride);
         const MoveList l = small_list();
         int* free_list = reinterpret_cast<int*>(static_cast<char*>(workspace()) + kListBytes);
         launch("cache_grow_plan", cache_grow_plan, dim3(1), dim3(kPlanThreads), 0, a.p, rows, add, n, free_list, l);

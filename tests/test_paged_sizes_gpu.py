@@ -31,3 +31,11 @@ def test_lengths_past_31_bits_are_refused(hip):
     assert b["refs"].read(np.int32).tolist() == [1]
     table = b["table"].read(np.int32).reshape(4, -1)
     assert table[3, 0] == 0 and (table >= 0).sum() == 1
+
+
+def test_more_pages_than_are_counted_are_refused(hip):
+    b, p = pool(hip, [0], 4, 16)
+    far = Elsewhere()
+    wide = hip.KvPool(p.keep[1], b["refs"], far, 2**21, far, 1024, b["status"])  # 1024 slots that may ask for 2^31 pages
+    with pytest.raises(_abi.HipUnsupported, match="1024 slots of 2097152 pages"):
+        hip.cache_grow(wide, far, far, 1024)
