@@ -153,6 +153,8 @@ extern "C" int byhip_paged_attention(const void* q, size_t q_stride, int q_dtype
         if (heads <= 0 || heads % a.c.kv_heads) fail("byhip: %d heads over %d key heads", heads, a.c.kv_heads);
         if (q_dtype != BYHIP_F32 && (q_dtype == BYHIP_F16 || q_dtype == BYHIP_BF16) && q_dtype != cache->dtype)
             unsupported("byhip: 16-bit queries have the cache's dtype (%d, cache %d)", q_dtype, cache->dtype);
+        if ((long long)a.s.rows * (heads / a.c.kv_heads) > 0x7FFFFFFF)  // the kernels count a key head's rows in 31 bits
+            unsupported("byhip: attention of %d rows of %d heads over %d key heads in one call", a.s.rows, heads, a.c.kv_heads);
         const size_t width = (size_t)heads * a.c.dim;
         check_rows(q, a.s.rows, width, q_stride, q_dtype, "queries");
         check_rows(out, a.s.rows, width, out_stride, out_dtype, "attention output");

@@ -39,3 +39,9 @@ def test_more_pages_than_are_counted_are_refused(hip):
     wide = hip.KvPool(p.keep[1], b["refs"], far, 2**21, far, 1024, b["status"])  # 1024 slots that may ask for 2^31 pages
     with pytest.raises(_abi.HipUnsupported, match="1024 slots of 2097152 pages"):
         hip.cache_grow(wide, far, far, 1024)
+
+
+def test_more_rows_than_are_counted_are_refused(hip):
+    far, ints = Elsewhere(), hip.DeviceBuffer.from_array(np.zeros(8, np.int32))
+    with pytest.raises(_abi.HipUnsupported, match="268435457 rows of 16 heads over 2"):
+        hip.paged_attention(far, 128, F16, 16, hip.Attn(0.1), hip.KvCache(far, far, F16, 2, 4, 2, 8), hip.KvBatch(ints, 4, ints, ints, 1, 2**28 + 1), far, 128, F16)
