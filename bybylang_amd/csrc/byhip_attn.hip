@@ -11,6 +11,9 @@
 namespace byhip {
 namespace {
 
+__device__ uint4 g_zeros;  // AttnArgs::zeros: zero from the start, so there is no write for a stream to wait for
+void* zeros = nullptr;     // its address
+
 constexpr int kGeneralMaxDim = 2048;  // queries and sums of 4 waves in 64 KB of LDS
 
 // One wave per row and head, 64 keys at a time, a key per lane for the scores and a value per lane for the
@@ -110,7 +113,7 @@ bool takes(const AttnArgs& a) {
 
 void launch_tiled(AttnArgs a) {
     a.joins = static_cast<int4*>(attn_workspace());
-    a.zeros = static_cast<char*>(attn_workspace()) + kAttnWorkspaceBytes;
+    a.zeros = zeros;
     a.part = reinterpret_cast<float*>(static_cast<char*>(attn_workspace()) + kAttnJoinBytes);
     const bool precise = a.q_dtype == BYHIP_F32 || a.out_dtype == BYHIP_F32, f16 = a.cache_dtype == BYHIP_F16;
     // The lengths are on the device: one sequence has all rows; as many rows as sequences are decoding; else
@@ -137,6 +140,12 @@ void launch_tiled(AttnArgs a) {
 }
 
 }  // namespace
+
+void attn_setup() {
+    BYHIP_HIP(hipGetSymbolAddress(&zeros, HIP_SYMBOL(g_zeros)));
+    if (!zeros) fail("byhip: attention's zeros have no device address");
+}
+
 }  // namespace byhip
 
 using namespace byhip;

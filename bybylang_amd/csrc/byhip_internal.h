@@ -81,11 +81,13 @@ int compute_units();
 // stream uses it in stream order.
 constexpr size_t kWorkspaceBytes = 32u << 20;
 void* workspace();
-// The same for the partial results of attention over a paged cache; 256 zero bytes follow it.
+// The same for the partial results of attention over a paged cache.
 constexpr size_t kAttnWorkspaceBytes = (size_t)80 << 20;
 void* attn_workspace();
 // Takes the device address of byhip_q4_matmul_static's scratch array on `device` (current).
 void static_scratch_setup(int device);
+// Takes the device address of attention's zero bytes.
+void attn_setup();
 // Whether a session (or a recording) is open.
 bool session_open();
 // Properties of the initialised device.

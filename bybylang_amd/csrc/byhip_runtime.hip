@@ -279,13 +279,13 @@ int byhip_init(int device) {
         BYHIP_HIP(hipDeviceGetAttribute(&khz, hipDeviceAttributeWallClockRate, device));
         s.realtime_hz = khz * 1e3;
         BYHIP_HIP(hipMalloc(&s.workspace, kWorkspaceBytes));
-        BYHIP_HIP(hipMalloc(&s.attn_workspace, kAttnWorkspaceBytes + 256));
-        BYHIP_HIP(hipMemset(static_cast<char*>(s.attn_workspace) + kAttnWorkspaceBytes, 0, 256));
+        BYHIP_HIP(hipMalloc(&s.attn_workspace, kAttnWorkspaceBytes));
         BYHIP_HIP(hipMalloc(reinterpret_cast<void**>(&s.flags), 64 * sizeof(int)));
         g_alloc_count.fetch_add(3);
         BYHIP_HIP(hipHostMalloc(reinterpret_cast<void**>(&s.gate), sizeof(int), hipHostMallocCoherent));
         *s.gate = 0;
         static_scratch_setup(device);
+        attn_setup();
         s.device = device;
         s.inited = true;
     });
