@@ -81,7 +81,8 @@ int compute_units();
 // stream uses it in stream order.
 constexpr size_t kWorkspaceBytes = 32u << 20;
 void* workspace();
-// The same for the partial results of attention over a paged cache.
+// The same for the partial results of attention over a paged cache, allocated by the first call that needs it (which may be part of
+// a recording), so that programs without attention do not hold it.
 constexpr size_t kAttnWorkspaceBytes = (size_t)80 << 20;
 void* attn_workspace();
 // Takes the device address of byhip_q4_matmul_static's scratch array on `device` (current).

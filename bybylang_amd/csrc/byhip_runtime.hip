@@ -30,7 +30,7 @@ struct State {
     hipDeviceProp_t prop{};
     std::unordered_map<const void*, Alloc> allocs;
     void* workspace = nullptr;  // kWorkspaceBytes, allocated by byhip_init, kept until exit
-    void* attn_workspace = nullptr;  // kAttnWorkspaceBytes, the same
+    void* attn_workspace = nullptr;  // kAttnWorkspaceBytes, allocated by the first call that needs it, kept until exit
     // session
     bool session_open = false;
     std::vector<void*> deferred_frees;
@@ -123,7 +123,6 @@ void enter_compute() {
 hipStream_t stream() { return st().stream; }
 int compute_units() { return st().prop.multiProcessorCount; }
 void* workspace() { return st().workspace; }
-void* attn_workspace() { return st().attn_workspace; }
 bool session_open() { return st().session_open || st().recording; }
 bool keeping_launches() { return st().recording && st().direct_open; }
 void keep_launch(Relaunch l) { st().kept.push_back(std::move(l)); }
@@ -159,6 +158,21 @@ void* device_alloc(size_t bytes) {
     std::lock_guard<std::recursive_mutex> lk(s.mu);
     s.allocs[p].bytes = bytes;
     return p;
+}
+
+void* attn_workspace() {
+    State& s = st();
+    std::lock_guard<std::recursive_mutex> lk(s.mu);
+    if (!s.attn_workspace) {
+        // An open capture of this thread refuses allocations, which are no part of it, unless the mode is relaxed.
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        BYHIP_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+        const hipError_t e = hipMalloc(&s.attn_workspace, kAttnWorkspaceBytes);
+        BYHIP_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+        BYHIP_HIP(e);
+        g_alloc_count.fetch_add(1);
+    }
+    return s.attn_workspace;
 }
 
 void device_free(void* p) {
@@ -279,9 +293,8 @@ int byhip_init(int device) {
         BYHIP_HIP(hipDeviceGetAttribute(&khz, hipDeviceAttributeWallClockRate, device));
         s.realtime_hz = khz * 1e3;
         BYHIP_HIP(hipMalloc(&s.workspace, kWorkspaceBytes));
-        BYHIP_HIP(hipMalloc(&s.attn_workspace, kAttnWorkspaceBytes));
         BYHIP_HIP(hipMalloc(reinterpret_cast<void**>(&s.flags), 64 * sizeof(int)));
-        g_alloc_count.fetch_add(3);
+        g_alloc_count.fetch_add(2);
         BYHIP_HIP(hipHostMalloc(reinterpret_cast<void**>(&s.gate), sizeof(int), hipHostMallocCoherent));
         *s.gate = 0;
         static_scratch_setup(device);
