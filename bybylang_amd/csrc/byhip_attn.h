@@ -43,11 +43,11 @@ struct SeqInfo {
 
 __device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, int b) {
     SeqInfo s;
-    const int from = a.s.starts[b], to = a.s.starts[b + 1];
+    const int from = a.s.starts[b], to = a.s.starts[b + 1], len = a.s.lens[b], granted = rows_granted(a.s, b);  // loads that wait for each other cost a call 1 us
     const int n = from >= 0 && to <= a.s.rows ? max(0, to - from) : 0;  // rows outside the call's are no rows
-    const bool room = has_room(a.s, b, n);
-    s.first_pos = (room ? a.s.lens[b] : 0) - n;
-    s.len = room ? max(0, seq_len(a.s, a.c, b)) : 0;
+    const int held = n <= granted ? len : 0;
+    s.first_pos = held - n;
+    s.len = max(0, in_table(a.s, a.c, held));
     s.prefix = a.prefix ? max(0, min(a.prefix[b], s.len)) : 0;
     const long long rows = (long long)n * a.group;
     s.rows = rows < a.min_rows || rows > a.max_rows ? 0 : (int)rows;

@@ -394,13 +394,15 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
             next_there = after_there;
             t += kWaves;
         };
-        const auto walk = [&](auto careful) __attribute__((always_inline)) {
+        const auto start = [&]() __attribute__((always_inline)) {
             r.clear();
             t = t0 + wave;
             rows = next = there = next_there = 0;
             if (t < t1) rows = r.key_row(b, range.key(t), there);
             if (t + kWaves < t1) next = r.key_row(b, range.key(t + kWaves), next_there);
             if (t < t1) r.load_k(ka, rows);
+        };
+        const auto walk = [&](auto careful) __attribute__((always_inline)) {
             while (t < t1) {
                 step(ka, kb, careful);
                 if (DIM > 128 || (DIM > 64 && NP > 1) || decltype(careful)::value) continue;
@@ -412,15 +414,23 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
         // as infinite keys do where queries have. That shows in the sums, so full tiles are not searched for them: a wave whose
         // sums are not finite walks once more, carefully. (Two copies of the loop where weights have several terms: 437 us from
         // 504 with a search of every tile, 4 x 65536 keys of 8 heads of 256 values, bf16; one copy where they have one, whose
-        // loop for 128 values would spill registers beside another: 210 us and 223, 64 sequences of up to 8192 keys.)
+        // loop for 128 values would spill registers beside another: 210 us and 223, 64 sequences of up to 8192 keys. The look at
+        // the sums costs a call of one row 0.4 us; behind the waves' join, one look for the block, 1.0.)
+        start();
         if constexpr (NP == 1) {
-            for (r.again = false;; r.again = true) {
+            r.again = false;
+            for (;;) {
                 walk(std::false_type{});
                 if (r.again || r.finite()) break;
+                r.again = true;
+                start();
             }
         } else {
             walk(std::false_type{});
-            if (!r.finite()) walk(std::true_type{});
+            if (!r.finite()) {
+                start();
+                walk(std::true_type{});
+            }
         }
 
         // 4. the waves' sums join in LDS

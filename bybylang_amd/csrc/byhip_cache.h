@@ -29,16 +29,15 @@ BatchArgs batch_args(const byhip_kv_batch* b);
 // Rows of `width` values, `stride` elements apart: the span the caller's buffer must hold.
 void check_rows(const void* p, size_t rows, size_t width, size_t stride, int dtype, const char* what);
 
-// Tokens of sequence b that its table can hold at most.
-__device__ __forceinline__ int seq_len(const BatchArgs& s, const CacheArgs& c, int b) {
+// The tokens of a sequence of `len` that its table has columns for.
+__device__ __forceinline__ int in_table(const BatchArgs& s, const CacheArgs& c, int len) {
     const long long room = (long long)s.stride * c.page_size;
-    const int len = s.lens[b];
     return len > room ? (int)room : len;
 }
 
-// Whether sequence b has room for the n rows that it brings: those of a refused cache_grow have no position, or they would be
-// placed over the tokens before them.
-__device__ __forceinline__ bool has_room(const BatchArgs& s, int b, int n) { return !s.granted || s.granted[b] >= n; }
+// The rows that sequence b has room for at most: those of a refused cache_grow have no position, or they would be placed over the
+// tokens before them.
+__device__ __forceinline__ int rows_granted(const BatchArgs& s, int b) { return s.granted ? s.granted[b] : 0x7FFFFFFF; }
 
 // The sequence of row t: the number of entries of starts[1 .. batch] that are <= t, `batch` when t belongs to
 // none. The 64 lanes of a wave look at 64 entries at a time, so 4096 sequences take two dependent loads.

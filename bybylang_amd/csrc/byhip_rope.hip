@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void rope_append(RopeArgs a, int units, int he
     const int b = find_sequence(a.s.starts, a.s.batch, t);
     if (b >= a.s.batch) return;
     const int from = a.s.starts[b], to = a.s.starts[b + 1], pos = a.s.lens[b] - to + t;
-    if (pos < 0 || from < 0 || to > a.s.rows || !has_room(a.s, b, to - from)) return;  // rows outside the call's are no rows
+    if (pos < 0 || from < 0 || to > a.s.rows || to - from > rows_granted(a.s, b)) return;  // rows outside the call's are no rows
     // the token's place in the pages
     size_t place = 0;
     bool in_cache = false;
