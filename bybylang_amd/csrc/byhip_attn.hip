@@ -99,7 +99,9 @@ void launch_general(const AttnArgs& a) {
 // Rows per key head from which attn_chunk reads a sequence. attn_rows reads its keys once per 16 rows; attn_chunk reads them once
 // per 256 but starts 10 us later, which is 56 MB at attn_rows' rate. 16 sequences of 4096 keys, 8 key heads of 128 values (268 MB),
 // 16 rows: 64 us with attn_rows, 68 with attn_chunk; 32 rows: 100 and 68; one sequence of 600 keys, 32 rows: 15 and 25. With fp32
-// rows, whose terms attn_chunk multiplies for 128 rows at least, 32 rows take 110 and 117 on bf16 (256 values: 240 and 403).
+// rows, whose terms attn_chunk multiplies for 128 rows at least, 32 rows take 108 and 117 on bf16 (256 values: 204 and 403).
+// The lengths are on the device, so the rule goes by the keys that the tables have room for: where they are much wider than their
+// sequences, 17 to 32 rows go to attn_chunk for less (that one sequence of 600 keys in a table for 32000: 26 us).
 int chunk_rows(const AttnArgs& a, bool precise) {
     const double bytes = (double)a.s.batch * key_room(a) * a.c.kv_heads * a.c.dim * 4.0;  // keys and values there is room for
     return !precise && bytes >= 56e6 ? 17 : 33;

@@ -16,11 +16,16 @@
 // order, so that blocks on one XCD read the same head's keys through its L2.
 //
 // What bounds it: the two phases of a tile, products and exponentials, which two waves per SIMD run in turn. 4096 rows x 16384
-// keys, 32 heads of 128 values, bf16: 0.94 to 1.05 ms by the clock of the card, 920 to 1020 TFLOP/s, matrix instructions busy 49% of the cycles. With 64 values the
-// exponentials outweigh the products (4 x 700 rows x 4000 keys: 138 us, 455 TFLOP/s; capped 180 us).
+// keys, 32 heads of 128 values, bf16: 0.94 to 1.05 ms by the clock of the card, 920 to 1020 TFLOP/s, matrix instructions busy 47 to 49% of the cycles. With 64 values the
+// exponentials outweigh the products (4 x 700 rows x 4000 keys, 24 heads: 117 us, 538 TFLOP/s; capped 169 us).
 //
 // fp32 queries or outputs: two fp16 or three bf16 terms of queries and weights, a matrix instruction each, in blocks of 4
-// waves with twice the registers (30 x 255 rows x 2048 keys, 128 values: 91 us in bf16, 239 in fp32 on a bf16 cache).
+// waves with twice the registers (30 x 255 rows x 2048 keys, 8 heads of 128 values: 94 us in bf16, 224 in fp32 on a bf16 cache). With
+// 16-bit rows on both sides a weight is rounded once to the cache's type, as in attn_rows.
+//
+// Registers: heads of up to 128 values keep all vectors but 2 to 8 (fp32 forms: all); of 129 to 256 values 71 to 78 go to memory, 300
+// of fp32 on fp16, 652 to 684 of fp32 on bf16 (4 x 700 rows x 4000 keys, 24 heads of 256: 411 us, 826, 1768), and every
+// form keeps 150 to 390 scalars in vector lanes.
 #pragma once
 
 #include <algorithm>
@@ -33,9 +38,13 @@ namespace {
 #define INLINE __attribute__((always_inline))
 constexpr int kChunkKeys = 64;
 constexpr int kXcds = 8;
-// What cutting an item costs the blocks that share it, in key tiles: the part's way to the workspace and back.
+// What cutting an item costs the blocks that share it, in key tiles: the part's way to the workspace and back. (30 prompts of 255 rows x
+// 1024 keys of 64 values: 135 us, with 4 150; 18 steps beside 6 prompts in a window: 64 us, with 16 77. It is too little for one prompt
+// of 1000 rows: 77 us, with 16 44.)
 constexpr int kCutTiles = 8;
-// Key tiles a block should at least get before another one takes part.
+// Key tiles a block should at least get before another one takes part. (100 rows x 2000 keys: 50 us, with 2 55, with 8 55; 3 prompts
+// in fp32 59 us, with 8 65. It is too little where one item goes to hundreds of blocks, whose parts then take the join longer:
+// 64 rows x 30000 keys of one key head 170 us, with 16 84.)
 constexpr int kShareTiles = 4;
 
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
@@ -165,8 +174,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_chunk(AttnArgs a) 
     }
     const long long per_head = uniform(units_before[NT]), total = per_head * a.c.kv_heads;
     const long long items = (long long)all_row_tiles * a.c.kv_heads;
-    // Whole items where the fullest block then has no more than with equal shares and their cuts (64 values, 255 rows x 1024
-    // keys: 240 items whole 47 us, cut 62; 264 items 71 and 64; 4 x 2100 rows x 4000 keys, 288 items: 182 and 129).
+    // Whole items where the fullest block then has no more than with equal shares and their cuts (8 heads of 64 values, 255 rows x
+    // 1024 keys: 240 items whole 46 us, cut 61; 264 items 68 and 63; 4 x 2100 rows x 4000 keys, 288 items: 155 and 119).
     const bool whole = (items + gridDim.x - 1) / gridDim.x * uniform(longest) <= max((long long)kShareTiles, total / gridDim.x) + kCutTiles;
     const long long blocks = min((long long)gridDim.x, whole ? items : max(1LL, total / kShareTiles));
     int w = blockIdx.x;

@@ -11,14 +11,16 @@
 // 2^8, so most tiles exchange nothing between lanes at all. fp16 weights carry a factor 2^7 so that small ones stay clear
 // of fp16's subnormals.
 //
-// What bounds it: bytes (32 sequences of up to 8192 keys, bf16: 205 us for 1.15 GB, 5.6 TB/s; 2 of 131072, fp32 on fp16:
-// 190 us, 5.4 TB/s). Each key and value is read once per 16 rows, so the work is divided by keys, not by
+// What bounds it: bytes (64 sequences of 300 to 8192 keys, a row each, bf16: 205 us for 1.15 GB, 5.6 TB/s; 2 of up to 131072,
+// fp32 on fp16: 186 us for 1.02 GB, 5.5 TB/s). Each key and value is read once per 16 rows, so the work is divided by keys, not by
 // sequences: all (head, sequence, row tile) items are laid end to end in tiles of 32 keys and every block takes
 // an equal run of them, whatever the lengths. A block therefore holds the end of one item and the start of another; their
 // parts go to the workspace and attn_join adds them.
 //
 // fp32 queries or outputs: the queries as two fp16 terms (scaled per row to fp16's range) or three bf16 terms, the
-// weights likewise, one matrix instruction per term; the memory still bounds it.
+// weights likewise, one matrix instruction per term; the memory still bounds it. With 16-bit rows on both sides a weight is
+// rounded once to the cache's type, in which the matrix instruction takes it: the output is then off from 64 bits by 1.1 (fp16) to 1.4
+// times (bf16) what its own rounding leaves, and a caller who needs less asks for fp32 output.
 #pragma once
 
 #include <algorithm>
@@ -301,8 +303,9 @@ struct Rows {
     }
 };
 
-// Blocks resident per CU: two, but one where 256 registers per lane would not hold a tile (heads of 256 values at one sequence
-// of 65536 keys x 4: 373 us with one, 754 with two; fp32 473 and 1631).
+// Blocks resident per CU: two, but one where 256 registers per lane would not hold a tile (heads of 129 to 256 values; 4 sequences
+// of 65536 keys, 8 key heads of 256, 2.15 GB: 372 us with one, 754 with two; fp32 398 and 1631). With one, 2 to 6 registers of the
+// 16-bit forms still go to memory, 43 to 48 of fp32 on fp16, 100 of fp32 on bf16; no other form spills any.
 constexpr int rows_blocks(int dim) { return dim > 128 ? 1 : 2; }
 
 template <int CT, int NP, int DIM, bool EXTRA>
@@ -412,9 +415,9 @@ __global__ __launch_bounds__(256, rows_blocks(DIM)) void attn_rows(AttnArgs a) {
         };
         // Values that are not finite spoil the sums of rows where a weight is rounded to 0 (0 times infinity), or has several terms,
         // as infinite keys do where queries have. That shows in the sums, so full tiles are not searched for them: a wave whose
-        // sums are not finite walks once more, carefully. (Two copies of the loop where weights have several terms: 437 us from
-        // 504 with a search of every tile, 4 x 65536 keys of 8 heads of 256 values, bf16; one copy where they have one, whose
-        // loop for 128 values would spill registers beside another: 210 us and 223, 64 sequences of up to 8192 keys. The look at
+        // sums are not finite walks once more, carefully. (Two copies of the loop where weights have several terms: 398 us from
+        // 504 with a search of every tile, 4 x 65536 keys of 8 heads of 256 values, fp32 on bf16; one copy where they have one, whose
+        // loop for 128 values would spill registers beside another: 205 us and 223, 64 sequences of up to 8192 keys. The look at
         // the sums costs a call of one row 0.4 us; behind the waves' join, one look for the block, 1.0.)
         start();
         if constexpr (NP == 1) {

@@ -179,9 +179,10 @@ __global__ __launch_bounds__(1024) void norm_block_long(NormArgs a) {
 template <int XT, int HT>
 void launch_norm(const NormArgs& a) {
     // Values per thread: many rows fill the card by themselves, and 16 per thread cost the fewest barriers per value (4099 x 5120
-    // layer norms, 252 MB: 67 us, with 8 per thread 74); few rows take all the threads they can have (32 x 4096: 4.8 us, with 16 per
+    // layer norms, 252 MB, half of what they read in the Infinity Cache: 67 us, with 8 per thread 74; all of it from memory 78 us, 3.2
+    // TB/s); few rows take all the threads they can have (32 x 4096: 4.8 us, with 16 per
     // thread 5.2). What bounds the many is rows in flight: two rows a block that share the weights' loads took 103 us, the
-    // weights' loads ahead of the sums 80, for the registers that they hold.
+    // weights' loads ahead of the sums 80 (both against the 67), for the registers that they hold.
     const bool few = a.M <= 2 * compute_units();
     const long long fours = ((long long)a.N + 3) / 4;
     const int ch = fours <= (few ? 1024 : 64) ? 1 : fours <= (few ? 2048 : 128) ? 2 : fours <= 4096 ? 4 : 8;

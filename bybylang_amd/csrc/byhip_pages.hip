@@ -5,7 +5,8 @@
 // host round trip, and can be recorded. What has to be decided in order (which free page goes to whom, which
 // of several sharers keeps a page) is decided by one block with prefix sums, so the outcome never depends on
 // scheduling; the bytes then move in one copy kernel over all layers, at the rate of a plain copy (841 MB of live pages
-// in 163 us, 5.2 TB/s; the planning blocks 8 to 10 us, a chain of reads and prefix sums).
+// in 163 us, 5.2 TB/s; the planning blocks 8 to 10 us, a chain of reads and prefix sums; a grow of many slots, which
+// compares them in pairs, 11 us for 64, 23 for 256, 80 for 1024).
 #include <algorithm>
 
 #include "byhip_cache.h"

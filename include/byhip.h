@@ -327,8 +327,9 @@ enum byhip_rope_scaling {
     BYHIP_ROPE_LINEAR = 1,  /* the same over `factor` (position interpolation) */
     BYHIP_ROPE_BASE = 2,    /* base * factor^(rot_dim / (rot_dim - 2)): the slowest pair slows by `factor` */
     BYHIP_ROPE_PARTS = 3    /* pairs that turn fewer than `slow` times in original_len positions slow by
-                             * `factor`, those of more than `fast` turns stay, a linear ramp between;
-                             * magnitude 0.1 ln(factor) + 1 */
+                             * `factor`, those of more than `fast` turns stay, a ramp linear in the turns between;
+                             * magnitude 0.1 ln(factor) + 1. (A model that was trained with a ramp linear in the
+                             * pair's index needs steps of the caller's own.) */
 };
 /* Rotary positions of the first rot_dim values of a head (even; the others pass through): steps[i] (device,
  * rot_dim / 2) is pair i's turn per position in units of 2^-64 of a whole turn, so that position * step
