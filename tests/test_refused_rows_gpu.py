@@ -100,6 +100,51 @@ def test_more_rows_than_were_granted(hip):
     assert np.all(out[:3] == 0) and np.all(out[3:] != 0)
 
 
+@pytest.mark.parametrize("new", [1, 20])
+def test_many_sequences(hip, new):
+    """More sequences than one launch counts, every third one refused."""
+    B, D = 1100, 64
+    g = synth.rng(8390)
+    up = hip.DeviceBuffer.from_array
+    kv = [to_bits(g.standard_normal((2 * B, 1, 16, D)), F16) for _ in range(2)]
+    got = np.where(np.arange(B) % 3 == 0, new - 1, new).astype(np.int32)
+    lens = np.full(B, 24, np.int32)
+    q = g.standard_normal((B * new, D)).astype(np.float32)
+    out, rot, both = up(np.full(q.shape, 5, np.float32)), up(np.full(q.shape, 7, np.float32)), [up(a) for a in kv]
+    starts, table = up((np.arange(B + 1) * new).astype(np.int32)), up(np.arange(2 * B, dtype=np.int32))
+    cache = hip.KvCache(*both, F16, 2 * B, 16, 1, D)
+    batch = hip.KvBatch(table, 2, starts, up(lens), B, B * new, up(got))
+    qk = up(q)
+    hip.paged_attention(qk, D, F32, 1, hip.Attn(D ** -0.5), cache, batch, out, D, F32)
+    y = out.read(np.float32).reshape(B, new, D)
+    full = hip.KvBatch(table, 2, starts, up(lens), B, B * new)
+    hip.paged_attention(qk, D, F32, 1, hip.Attn(D ** -0.5), cache, full, out, D, F32)
+    z = out.read(np.float32).reshape(B, new, D)
+    assert np.all(y[::3] == 0) and np.all(z != 0)
+    keep = np.arange(B) % 3 != 0
+    assert np.all(np.abs(y[keep] - z[keep]) <= 4e-6 * (1 + np.abs(z[keep])))  # parts may be cut elsewhere
+    hip.rope_append(qk, D, qk, D, qk, D, F32, 1, None, cache, batch, rot, D, F32)
+    r = rot.read(np.float32).reshape(B, new, D)
+    assert np.all(r[::3] == 7) and np.array_equal(r[keep], q.reshape(B, new, D)[keep])
+    for buf, was in zip(both, kv):
+        now = buf.read(np.float16).reshape(B, 32, D)
+        want = was.reshape(B, 32, D).copy()
+        want[keep, 24 - new:24] = q.reshape(B, new, D)[keep].astype(np.float16)
+        assert np.array_equal(now.view(np.uint16), want.view(np.uint16))
+
+
+def test_short_arrays_are_refused(hip):
+    p = Small(hip, [4, 4, 4], 6, 2)
+    small = p.ints([0, 0])
+    pool = hip.KvPool([p.cache], p.br, p.bt, 2, p.bl, 3, p.bs, small)
+    with pytest.raises(_abi.HipBackendError, match="granted tokens needs 12"):
+        hip.cache_grow(pool, p.ints([0]), p.ints([1]), 1)
+    z = p.up(np.zeros(512, np.float32))
+    batch = hip.KvBatch(p.bt, 2, p.ints([0, 1, 2, 3]), p.bl, 3, 3, small)
+    with pytest.raises(_abi.HipBackendError, match="granted tokens needs 12"):
+        hip.paged_attention(z, 64, F32, 1, hip.Attn(0.1), p.cache, batch, z, 64, F32)
+
+
 def cache_bytes(gb, d):  # noqa: F811
     n = d.caches[0].value
     halves = n.pages * n.kv_heads * n.page_size * n.head_dim
