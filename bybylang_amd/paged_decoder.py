@@ -113,6 +113,8 @@ class PagedDecoder:
         return g.sessionLastRecording(gbHip)
 
     def fork(self, parents, rows) -> None:
+        if len(parents) != len(rows):
+            raise ValueError(f"{len(rows)} forks of {len(parents)} parents")
         self._set(self.some, np.asarray(parents, np.int32))
         self._set(self.others, np.asarray(rows, np.int32))
         self._taken(g.sessionCacheFork(gbHip, self.pool, self.some, self.others, len(rows)))

@@ -16,3 +16,14 @@ def test_a_call_that_is_not_taken_raises(monkeypatch, proc, call):
     monkeypatch.setattr(g, proc, lambda *a: False)
     with pytest.raises(_abi.HipUnsupported, match="does not take"):
         call(d)
+
+
+def test_forks_without_a_parent_each_are_refused(monkeypatch):
+    """The call would have taken the parents of the fork before it."""
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.pool = d.some = d.others = None
+    monkeypatch.setattr(d, "_set", lambda handle, values: None, raising=False)
+    monkeypatch.setattr(g, "sessionCacheFork", lambda *a: pytest.fail("forked"))
+    for parents, rows in (([0], [1, 2]), ([0, 3], [1]), ([], [1])):
+        with pytest.raises(ValueError, match="forks of"):
+            d.fork(parents, rows)
