@@ -78,6 +78,8 @@ class PagedDecoder:
         """The blocks over the rows of self.x, to self.y; the slots' sequences are longer by their rows afterwards, unless
         there is no room for them."""
         T, E = self.rows, self.width
+        if T == 0:
+            return
         ok = g.sessionCacheGrow(gbHip, self.pool, self.all_rows, self.add, self.slots)
         ok &= g.sessionNormBlock(gbHip, self.x, T, E, None, None, None, 1.0, self.h, self.norms[0], self.y)
         for (wq, wk, wv, wo), cache, norm in zip(self.layers, self.caches, self.norms[1:]):

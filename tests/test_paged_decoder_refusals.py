@@ -27,3 +27,11 @@ def test_forks_without_a_parent_each_are_refused(monkeypatch):
     for parents, rows in (([0], [1, 2]), ([0, 3], [1]), ([], [1])):
         with pytest.raises(ValueError, match="forks of"):
             d.fork(parents, rows)
+
+
+def test_a_step_without_rows_does_nothing(monkeypatch):
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.rows, d.width, d.pool, d.all_rows, d.add, d.slots = 0, 8, None, None, None, 2
+    for proc in ("sessionCacheGrow", "sessionNormBlock", "sessionMatmulQ4"):
+        monkeypatch.setattr(g, proc, lambda *a: pytest.fail("queued"))
+    d.encode()
