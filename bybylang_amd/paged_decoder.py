@@ -109,7 +109,11 @@ class PagedDecoder:
         """Keeps a step of the rows last set as a recording; it has been run once."""
         if not g.sessionBeginRecording(gbHip):
             raise _abi.HipBackendError(g.sessionGetLastError(gbHip))
-        self.encode()
+        try:
+            self.encode()
+        except _abi.HipBackendError:
+            g.sessionRecoverQueue(gbHip)
+            raise
         if not g.sessionEnd(gbHip):
             raise _abi.HipBackendError(g.sessionGetLastError(gbHip))
         return g.sessionLastRecording(gbHip)

@@ -35,3 +35,18 @@ def test_a_step_without_rows_does_nothing(monkeypatch):
     for proc in ("sessionCacheGrow", "sessionNormBlock", "sessionMatmulQ4"):
         monkeypatch.setattr(g, proc, lambda *a: pytest.fail("queued"))
     d.encode()
+
+
+def test_a_step_that_cannot_be_recorded_leaves_no_recording_open(monkeypatch):
+    d = PagedDecoder.__new__(PagedDecoder)
+    calls = []
+
+    def encode():
+        raise _abi.HipUnsupported("not taken")
+    monkeypatch.setattr(d, "encode", encode, raising=False)
+    monkeypatch.setattr(g, "sessionBeginRecording", lambda b: True)
+    monkeypatch.setattr(g, "sessionRecoverQueue", lambda b: calls.append("recovered"))
+    monkeypatch.setattr(g, "sessionEnd", lambda b: pytest.fail("kept"))
+    with pytest.raises(_abi.HipUnsupported):
+        d.record()
+    assert calls == ["recovered"]
