@@ -449,7 +449,7 @@ def sessionCacheFree(backend: GpuBackend, pool, rows: SessionHandle, n: int) -> 
 
 
 def sessionCacheGrow(backend: GpuBackend, pool, rows: SessionHandle, add: SessionHandle, n: int) -> bool:
-    """Room for add[i] more tokens in slot rows[i] (negative: that many are dropped)."""
+    """Room for add[i] more tokens in slot rows[i] (negative: that many are dropped); the pool's `granted` says what each got."""
     _require_hip(backend)
     return _encoded(load().byhip_cache_grow(pool.ref, rows.hipHandle, add.hipHandle, n), "sessionCacheGrow")
 
