@@ -14,10 +14,12 @@ BYHIP_OK = 0
 BYHIP_UNSUPPORTED = 1
 BYHIP_ERROR = -1
 
-F32, F16, BF16, MXFP4_KM = 0, 1, 2, 3
+F32, F16, BF16, MXFP4_KM, MXFP8_KM = 0, 1, 2, 3, 4
 ROPE_HALVES, ROPE_PAIRS = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
 NORM_RMS, NORM_LAYER = 0, 1
+MOE_SOFTMAX, MOE_SIGMOID = 0, 1
+MOE_GATHER, MOE_SCATTER, MOE_SWIGLU = 1, 2, 4
 
 
 class HipBackendError(RuntimeError):
@@ -72,6 +74,15 @@ class KvPool(C.Structure):
 
 class Norm(C.Structure):
     _fields_ = [("kind", C.c_int), ("eps", C.c_float), ("weight", C.c_void_p), ("bias", C.c_void_p)]
+
+
+class MoePlan(C.Structure):
+    _fields_ = [("tokens", C.c_int), ("top_k", C.c_int), ("experts", C.c_int), ("plan", C.c_void_p)]
+
+
+class MoeRouter(C.Structure):
+    _fields_ = [("score", C.c_int), ("bias", C.c_void_p), ("groups", C.c_int), ("top_groups", C.c_int),
+                ("group_by", C.c_int), ("renorm", C.c_int), ("scale", C.c_float)]
 
 
 _VP, _SZ, _I, _U8P, _FP = C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p
@@ -143,6 +154,13 @@ SIGNATURES = {
     "byhip_cache_copy": (_I, [C.POINTER(KvPool), _VP, _VP, _I]),
     "byhip_norm_block": (_I, [_VP, _SZ, _I, _I, _I, C.POINTER(Norm), _VP, _SZ, _VP, _SZ, C.c_float,
                               _VP, _SZ, _I, C.POINTER(Norm), _VP, _SZ, _I]),
+    "byhip_mx_quantize": (_I, [_VP, _SZ, _I, _I, _I, _VP, _I]),
+    "byhip_mx_matmul": (_I, [_VP, _I, _U8P, _I, _I, _I, _I, _VP, _SZ, _I]),
+    "byhip_moe_plan_bytes": (C.c_ulonglong, [_I, _I, _I]),
+    "byhip_moe_route": (_I, [_VP, _SZ, _I, C.POINTER(MoeRouter), C.POINTER(MoePlan), _VP, _FP]),
+    "byhip_moe_plan_ids": (_I, [_VP, C.POINTER(MoePlan)]),
+    "byhip_moe_matmul": (_I, [_VP, _I, _U8P, C.POINTER(MoePlan), _I, _I, _I, _VP, _SZ, _I]),
+    "byhip_moe_combine": (_I, [_VP, _SZ, _I, _I, C.POINTER(MoePlan), _VP, _FP, _VP, _SZ, _I, _VP, _SZ, _I]),
     "byhip_debug_unpack_q4": (_I, [_VP, _U8P, _FP, _FP]),
     "byhip_debug_unpack_fp4km": (_I, [_U8P, _SZ, _FP, _SZ, _I, _I, _U8P, _FP]),
     "byhip_debug_copy": (_I, [_VP, _VP, _SZ]),

@@ -1,0 +1,89 @@
+// byhip_moe.h - products of microscaled rows with matrices in 4 bits, one matrix per expert: arguments and what the kernels share.
+#pragma once
+
+#include "byhip_mx.h"
+
+namespace byhip {
+
+struct MoeArgs {
+    const uint8_t* x;         // values, then scales
+    const uint8_t* xs;
+    const uint8_t* w;         // values of all matrices, then their scales
+    const uint8_t* ws;
+    void* y;
+    uint8_t* ys;              // scales of microscaled outputs
+    const int* order;
+    const int* n_units;       // null: one matrix, rows 0 .. M - 1 in order
+    const MoeUnit* units;
+    size_t y_stride;
+    uint32_t x_bytes, xs_bytes;
+    int M, K, KG, R, N;       // KG = K / 32 groups; R rows per matrix, N outputs
+    int top_k, gather, scatter, unit_rows, strips, y_dtype, vec;
+};
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+// The unit and strip of block b: blocks go to the 8 XCDs in turn, and each XCD takes a run of tiles, so that the strips of an
+// expert (which share its rows) and the units of an expert (which share its matrix) meet in one L2. False: no work.
+__device__ __forceinline__ bool moe_tile(const MoeArgs& a, MoeUnit& u, int& strip) {
+    const int units = a.n_units ? *a.n_units : (a.M + a.unit_rows - 1) / a.unit_rows;
+    const long long tiles = (long long)units * a.strips, per = (tiles + 7) / 8;
+    const long long at = blockIdx.x >> 3, t = (blockIdx.x & 7) * per + at;
+    if (at >= per || t >= tiles) return false;
+    const int i = (int)(t / a.strips);
+    strip = (int)(t % a.strips);
+    if (a.n_units) {
+        u = a.units[i];
+    } else {
+        u.expert = 0;
+        u.first = i * a.unit_rows;
+        u.rows = min(a.unit_rows, a.M - u.first);
+    }
+    return true;
+}
+// Row of x, and of y, of the plan's row r.
+__device__ __forceinline__ int moe_x_row(const MoeArgs& a, int r) { return a.gather ? a.order[r] / a.top_k : r; }
+__device__ __forceinline__ int moe_y_row(const MoeArgs& a, int r) { return a.scatter ? a.order[r] : r; }
+
+// silu(g) u
+__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// Four neighbouring outputs n .. n + 3 of y's row.
+__device__ __forceinline__ void moe_store4(const MoeArgs& a, size_t row, int n, const float (&v)[4]) {
+    const size_t at = row * a.y_stride + n;
+    if (a.vec && n + 4 <= a.N) {
+        store_vec<4>(a.y, at, v, a.y_dtype);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < a.N) {
+                const float one[1] = {v[e]};
+                store_vec<1>(a.y, at + e, one, a.y_dtype);
+            }
+    }
+}
+
+__device__ __forceinline__ bool is_mx_out(int dtype) { return dtype == BYHIP_MXFP8_KM || dtype == BYHIP_MXFP4_KM; }
+
+// Eight values of group G of y's row (elements j .. j + 3 and j + 16 ..) whose largest magnitude over the group has these
+// bits, and with `scale` the group's scale byte.
+__device__ __forceinline__ void store_group(const MoeArgs& a, size_t row, int G, int j, bool scale, uint32_t mag, const float (&lo)[4],
+                                            const float (&hi)[4]) {
+    uint8_t* y = static_cast<uint8_t*>(a.y);
+    uint32_t byte, out[2];
+    if (a.y_dtype == BYHIP_MXFP8_KM) {
+        byte = mx_scale<BYHIP_MXFP8_KM>(mag);
+        mx_pack8<BYHIP_MXFP8_KM>(lo, hi, byte, out);
+        mx_store8<BYHIP_MXFP8_KM>(y, row, a.N, G, j, out);
+    } else {
+        byte = mx_scale<BYHIP_MXFP4_KM>(mag);
+        mx_pack8<BYHIP_MXFP4_KM>(lo, hi, byte, out);
+        mx_store8<BYHIP_MXFP4_KM>(y, row, a.N, G, j, out);
+    }
+    if (scale) a.ys[row * (a.N / 32) + G] = (uint8_t)byte;
+}
+
+void launch_moe_rows(const MoeArgs& a, int x_format, bool glu, int max_units);
+
+}  // namespace byhip

@@ -1,0 +1,78 @@
+// byhip_moe.hip - entry points of the products of microscaled rows: with one matrix, and with each row's expert's.
+#include "byhip_moe.h"
+
+namespace byhip {
+namespace {
+
+// What both calls check; rows: x's rows, y_rows: y's.
+MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts, size_t rows, size_t y_rows, int K, int N, bool glu,
+                     void* y, size_t y_stride, int y_dtype) {
+    if (K <= 0 || N <= 0) fail("byhip: a product of rows of %d values with %d outputs", K, N);
+    MoeArgs a{};
+    a.K = K; a.KG = K / 32; a.N = N;
+    const long long R = glu ? 2ll * N : N;
+    check_mx(x, rows, K, x_format, "rows of a product");
+    // Offsets inside the rows and inside one matrix are 32-bit; strips may pass a matrix's last row.
+    if (mx_values(rows, K, x_format) >= 1ull << 31) fail("byhip: %zu rows of %d values: a product takes less than 2 GiB of them", rows, K);
+    if (R > INT32_MAX / 2 || (unsigned long long)(R + 512) * K / 2 >= 1ull << 31) fail("byhip: a matrix of %lld rows of %d values", R, K);
+    a.R = (int)R;
+    check_mx(w, (size_t)experts * R, K, BYHIP_MXFP4_KM, "matrices of a product");
+    if (is_mx(y_dtype)) {
+        check_mx(y, y_rows, N, y_dtype, "product");
+        if (y_stride != (size_t)N) fail("byhip: product of %d values: microscaled rows have no stride of their own (%zu)", N, y_stride);
+        a.ys = static_cast<uint8_t*>(y) + mx_values(y_rows, N, y_dtype);
+    } else {
+        check_rows(y, y_rows, N, y_stride, y_dtype, "product");
+        a.vec = aligned4(y, y_stride, y_dtype);
+    }
+    a.x = static_cast<const uint8_t*>(x);
+    a.x_bytes = (uint32_t)mx_values(rows, K, x_format);
+    a.xs = a.x + a.x_bytes;
+    a.xs_bytes = (uint32_t)(rows * a.KG);
+    a.w = w;
+    a.ws = w + mx_values((size_t)experts * R, K, BYHIP_MXFP4_KM);
+    a.y = y; a.y_stride = y_stride; a.y_dtype = y_dtype;
+    return a;
+}
+
+}  // namespace
+}  // namespace byhip
+
+using namespace byhip;
+
+extern "C" {
+
+int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K, int N, int flags, void* y, size_t y_stride,
+                    int y_dtype) {
+    return guard([&] {
+        enter_compute();
+        if (M < 0) fail("byhip: a product of %d rows", M);
+        if (flags & ~BYHIP_MOE_SWIGLU) fail("byhip: product flags %d without a plan", flags);
+        const bool glu = flags & BYHIP_MOE_SWIGLU;
+        MoeArgs a = product_args(x, x_format, w, 1, M, M, K, N, glu, y, y_stride, y_dtype);
+        if (M == 0) return;
+        a.M = M; a.top_k = 1;
+        a.unit_rows = moe_unit_rows(M, 1);
+        note_device_write(y);
+        launch_moe_rows(a, x_format, glu, (M + a.unit_rows - 1) / a.unit_rows);
+    });
+}
+
+int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_moe_plan* plan, int K, int N, int flags, void* y,
+                     size_t y_stride, int y_dtype) {
+    return guard([&] {
+        enter_compute();
+        const MoePlan p = moe_plan_args(plan);
+        if (flags & ~(BYHIP_MOE_GATHER | BYHIP_MOE_SCATTER | BYHIP_MOE_SWIGLU)) fail("byhip: product flags %d", flags);
+        const bool glu = flags & BYHIP_MOE_SWIGLU, gather = flags & BYHIP_MOE_GATHER;
+        MoeArgs a = product_args(x, x_format, w, p.experts, gather ? p.tokens : p.rows, p.rows, K, N, glu, y, y_stride, y_dtype);
+        if (p.rows == 0) return;
+        a.order = p.order; a.n_units = p.n_units; a.units = p.units;
+        a.top_k = p.top_k; a.gather = gather; a.scatter = (flags & BYHIP_MOE_SCATTER) != 0;
+        a.unit_rows = p.unit_rows;
+        note_device_write(y);
+        launch_moe_rows(a, x_format, glu, p.max_units);
+    });
+}
+
+}  // extern "C"

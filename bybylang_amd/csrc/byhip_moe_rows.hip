@@ -1,0 +1,210 @@
+// byhip_moe_rows.hip - few rows per expert (gfx950): products that read each matrix once, in units of up to 64 rows.
+//
+// Bound by the matrices' bytes. A block takes a strip of a matrix (64 of its rows) and one unit's rows; its four waves share
+// out the values' axis in windows of 512 and add their sums in LDS at the end. A wave loads its window of the
+// strip in 16-byte pieces straight into the operands of v_mfma_scale_f32_16x16x128_f8f6f4, 16 KB in flight before the first
+// product, and the rows' values beside it (they come from L2: every strip of the expert reads them).
+//
+// Operands (checked on the device): the matrix is the first, in 4 bits: lane (c, g) = (l % 16, l / 16) holds the 32 values of
+// block g of row c. Rows in 4 bits are the same. Rows in 8 bits: lane (c, g) holds two pieces of 16 values, those of
+// half g % 2 of blocks g / 2 and 2 + g / 2; scales go by block for both, lane (c, g)'s being block g's. Which 32 values of the
+// window are block g of a step is free as long as both operands agree: step s takes group 4 g + s of the window's 16, so
+// that a lane's four scale bytes lie in one word. The result: lane (c, g) holds row c of x, matrix rows 4 g .. 4 g + 3.
+//
+// Sums are fp32. What the instructions add in one go is exact with rows in 4 bits; with rows in 8 bits they align eight neighbouring
+// products to the largest and cut each off 13 bits below its exponent (measured: 4.5e-6 of a random product's norm at any length, a
+// 6000th of what the rows' own rounding to 8 bits is off by, so that products in 16 bits at half the rate would buy nothing).
+#include "byhip_moe.h"
+
+namespace byhip {
+namespace {
+
+constexpr int kWaves = 4;
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ v4u load16(rsrc_t r, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
+
+// The scale bytes of groups G .. G + 3 of a row that starts at `row` (kOutOfRange: none), 0 for those past its KG groups: a byte
+// of the next row might be a NaN's.
+__device__ __forceinline__ uint32_t load_scales(rsrc_t r, uint32_t row, int G, int KG) {
+    if ((KG & 3) == 0) return buf_load4(r, row == kOutOfRange || G >= KG ? kOutOfRange : row + G);
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, row == kOutOfRange || G + i >= KG ? kOutOfRange : row + G + i, 0, 0) << (8 * i);
+    return v;
+}
+
+template <int XF, int S>
+__device__ __forceinline__ f4v product(v8i w, v8i x, f4v c, int sw, int sx) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, XF == BYHIP_MXFP8_KM ? 0 : 4, S, sw, S, sx);
+}
+
+// MT blocks of 16 rows, NF blocks of 16 matrix rows (GLU: two of gates, two of ups).
+template <int XF, int MT, int NF, bool GLU>
+__global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
+    static_assert(!GLU || NF == 4, "gates and ups");
+    __shared__ float4 part[kWaves][NF * MT][64];
+    MoeUnit u;
+    int strip;
+    if (!moe_tile(a, u, strip)) return;
+    constexpr bool eight = XF == BYHIP_MXFP8_KM;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const uint32_t kb = (uint32_t)a.K / 2, xb = eight ? (uint32_t)a.K : kb;
+    const rsrc_t wr = make_rsrc(a.w + (size_t)u.expert * a.R * kb, (uint32_t)a.R * kb);
+    const rsrc_t wsr = make_rsrc(a.ws + (size_t)u.expert * a.R * a.KG, (uint32_t)a.R * a.KG);
+    const rsrc_t xr = make_rsrc(a.x, a.x_bytes), xsr = make_rsrc(a.xs, a.xs_bytes);
+    const int n0 = strip * (GLU ? 32 : 16 * NF);
+    int n[NF];  // this lane's row of each block of the matrix
+#pragma unroll
+    for (int f = 0; f < NF; ++f) n[f] = GLU ? (f >> 1) * a.N + n0 + 16 * (f & 1) + c : n0 + 16 * f + c;
+    const int windows = (a.KG + 15) / 16;
+
+    for (int m0 = 0; m0 < u.rows; m0 += 16 * MT) {
+        uint32_t x_at[MT], xs_at[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int i = m0 + 16 * m + c;
+            const int row = i < u.rows ? moe_x_row(a, u.first + i) : -1;
+            x_at[m] = row < 0 ? kOutOfRange : (uint32_t)row * xb;
+            xs_at[m] = row < 0 ? kOutOfRange : (uint32_t)row * a.KG;
+        }
+        f4v acc[NF][MT];
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                acc[f][m] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+                // A product whose addend is the constant 0 may be given a result that overlaps its operands, which it then misreads:
+                // the zeros stay in registers.
+                asm volatile("" : "+v"(acc[f][m]));
+            }
+        for (int W = w; W < windows; W += kWaves) {
+            const int G = 16 * W + 4 * g;  // the lane's first group of the matrix
+            v4u wv[NF][4];
+            uint32_t ws[NF];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    wv[f][s] = load16(wr, n[f] < a.R && G + s < a.KG ? (uint32_t)n[f] * kb + 16 * (G + s) : kOutOfRange);
+                ws[f] = load_scales(wsr, n[f] < a.R ? (uint32_t)n[f] * a.KG : kOutOfRange, G, a.KG);
+            }
+            uint32_t xs[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xs[m] = load_scales(xsr, xs_at[m], G, a.KG);
+            auto step = [&](auto Sc) {
+                constexpr int S = decltype(Sc)::value;
+                v8i xv[MT];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    xv[m] = v8i{0, 0, 0, 0, 0, 0, 0, 0};
+                    if constexpr (eight) {
+                        const int g0 = 16 * W + 4 * (g >> 1) + S, g1 = g0 + 8;
+                        const v4u p = load16(xr, x_at[m] != kOutOfRange && g0 < a.KG ? x_at[m] + 32 * g0 + 16 * (g & 1) : kOutOfRange);
+                        const v4u q = load16(xr, x_at[m] != kOutOfRange && g1 < a.KG ? x_at[m] + 32 * g1 + 16 * (g & 1) : kOutOfRange);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { xv[m][e] = (int)p[e]; xv[m][4 + e] = (int)q[e]; }
+                    } else {
+                        const v4u p = load16(xr, x_at[m] != kOutOfRange && G + S < a.KG ? x_at[m] + 16 * (G + S) : kOutOfRange);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) xv[m][e] = (int)p[e];
+                    }
+                }
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    const v8i wf = {(int)wv[f][S][0], (int)wv[f][S][1], (int)wv[f][S][2], (int)wv[f][S][3], 0, 0, 0, 0};
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[f][m] = product<XF, S>(wf, xv[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                }
+            };
+            step(std::integral_constant<int, 0>{});
+            step(std::integral_constant<int, 1>{});
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
+        }
+        __syncthreads();  // the sums of the rows before are read
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) part[w][f * MT + m][lane] = make_float4(acc[f][m][0], acc[f][m][1], acc[f][m][2], acc[f][m][3]);
+        __syncthreads();
+        auto whole = [&](int f, int m, float (&v)[4]) {
+            v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                const float4 p = part[i][f * MT + m][lane];
+                v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+            }
+        };
+        if constexpr (GLU) {
+            for (int m = w; m < MT; m += kWaves) {
+                const int i = m0 + 16 * m + c;
+                float gate[4], up[4], h[2][4];
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    whole(f, m, gate);
+                    whole(2 + f, m, up);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) h[f][e] = swiglu(gate[e], up[e]);
+                }
+                const bool there = i < u.rows;
+                const size_t row = there ? moe_y_row(a, u.first + i) : 0;
+                if (is_mx_out(a.y_dtype)) {
+                    uint32_t mag = mag8(h[0], h[1]);
+                    mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+                    mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+                    if (there) store_group(a, row, strip, 4 * g, g == 0, mag, h[0], h[1]);
+                } else if (there) {
+                    moe_store4(a, row, n0 + 4 * g, h[0]);
+                    moe_store4(a, row, n0 + 16 + 4 * g, h[1]);
+                }
+            }
+        } else if (is_mx_out(a.y_dtype)) {
+            for (int p = w; p < MT * NF / 2; p += kWaves) {
+                const int m = p / (NF / 2), q = p % (NF / 2), i = m0 + 16 * m + c;
+                float h[2][4];
+                whole(2 * q, m, h[0]);
+                whole(2 * q + 1, m, h[1]);
+                uint32_t mag = mag8(h[0], h[1]);
+                mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+                mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+                if (i < u.rows && n0 + 32 * q < a.N) store_group(a, moe_y_row(a, u.first + i), n0 / 32 + q, 4 * g, g == 0, mag, h[0], h[1]);
+            }
+        } else {
+            for (int p = w; p < MT * NF; p += kWaves) {
+                const int m = p / NF, f = p % NF, i = m0 + 16 * m + c;
+                float v[4];
+                whole(f, m, v);
+                if (i < u.rows) moe_store4(a, moe_y_row(a, u.first + i), n0 + 16 * f + 4 * g, v);
+            }
+        }
+    }
+}
+
+template <int XF>
+void launch_rows(const MoeArgs& a, bool glu, const dim3& grid) {
+    const dim3 block(64 * kWaves);
+#define BYHIP_ROWS(MT)                                                                                      \
+    (glu ? launch("moe_rows", (moe_rows<XF, MT, 4, true>), grid, block, 0, a) : launch("moe_rows", (moe_rows<XF, MT, 4, false>), grid, block, 0, a))
+    if (a.unit_rows <= 16) BYHIP_ROWS(1);
+    else if (a.unit_rows <= 32) BYHIP_ROWS(2);
+    else BYHIP_ROWS(4);
+#undef BYHIP_ROWS
+    BYHIP_LAUNCHED("moe_rows");
+}
+
+}  // namespace
+
+void launch_moe_rows(const MoeArgs& args, int x_format, bool glu, int max_units) {
+    MoeArgs a = args;
+    const int wide = glu ? 32 : 64;
+    a.strips = (a.N + wide - 1) / wide;
+    const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;
+    if (blocks >= 1ll << 31) fail("byhip: a product of %d units of %d strips", max_units, a.strips);
+    const dim3 grid((unsigned)blocks);
+    if (x_format == BYHIP_MXFP8_KM) launch_rows<BYHIP_MXFP8_KM>(a, glu, grid);
+    else launch_rows<BYHIP_MXFP4_KM>(a, glu, grid);
+}
+
+}  // namespace byhip

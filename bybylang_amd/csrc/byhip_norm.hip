@@ -7,7 +7,7 @@
 // of 1024 threads pass over x again for each sum.
 #include <algorithm>
 
-#include "byhip_cache.h"
+#include "byhip_mx.h"
 
 namespace byhip {
 namespace {
@@ -23,6 +23,7 @@ struct NormArgs {
     int has_post, has_pre, N, y_dtype, h_dtype, vec;
     long long M;
     float res_scale;
+    uint8_t* y_scales;
 };
 
 // Sums over the block's threads, the same value in every thread. One barrier each: successive sums use the halves of `red`
@@ -66,8 +67,17 @@ __device__ __forceinline__ void write4(void* p, size_t row, int i, int N, int ve
     }
 }
 
-// One norm over the row held in v (columns 4 (threads c + thread) ..).
-template <int CH>
+// First column of chunk c of thread tid. Microscaled rows are written eight values at a time that lie next to each other in
+// their order: elements 4 t .. 4 t + 3 of a group and the four 16 further on, in chunks 2 c and 2 c + 1.
+template <bool MX>
+__device__ __forceinline__ int column(int c, int tid, int threads) {
+    if constexpr (!MX) return 4 * (threads * c + tid);
+    const int u = threads * (c >> 1) + tid;
+    return 32 * (u >> 2) + 4 * (u & 3) + 16 * (c & 1);
+}
+
+// One norm over the row held in v.
+template <int CH, bool MX = false>
 __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n, int N, int vec, int tid, BlockSum& block_sum) {
     const int TH = blockDim.x;
     float mean = 0.0f;
@@ -84,13 +94,13 @@ __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n,
     for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float d = 4 * (TH * c + tid) + e < N ? v[c][e] - mean : 0.0f;
+            const float d = column<MX>(c, tid, TH) + e < N ? v[c][e] - mean : 0.0f;
             s += d * d;
         }
     const float f = 1.0f / sqrtf(block_sum(s) / N + n.eps);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int i = 4 * (TH * c + tid);
+        const int i = column<MX>(c, tid, TH);
         float w[4] = {1.0f, 1.0f, 1.0f, 1.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (n.weight) read4<BYHIP_F32>(n.weight, 0, i, N, vec, w);
         if (n.bias) read4<BYHIP_F32>(n.bias, 0, i, N, vec, b);
@@ -99,7 +109,25 @@ __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n,
     }
 }
 
-template <int XT, int HT, int CH>
+// The row in v as microscaled values: 4 lanes hold a group.
+template <int FMT, int CH>
+__device__ __forceinline__ void write_mx(const NormArgs& a, size_t row, int tid, int TH, const float (&v)[CH][4]) {
+#pragma unroll
+    for (int c = 0; c + 1 < CH; c += 2) {
+        const int u = TH * (c >> 1) + tid, G = u >> 2;
+        uint32_t m = mag8(v[c], v[c + 1]);
+        m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+        if (32 * G >= a.N) continue;
+        const uint32_t byte = mx_scale<FMT>(m);
+        uint32_t out[2];
+        mx_pack8<FMT>(v[c], v[c + 1], byte, out);
+        mx_store8<FMT>(static_cast<uint8_t*>(a.y), row, a.N, G, 4 * (u & 3), out);
+        if ((u & 3) == 0) a.y_scales[row * (a.N / 32) + G] = (uint8_t)byte;
+    }
+}
+
+template <int XT, int HT, int CH, bool MX = false>
 __global__ __launch_bounds__(1024) void norm_block(NormArgs a) {
     __shared__ float red[2][16];
     BlockSum block_sum{red};
@@ -107,15 +135,15 @@ __global__ __launch_bounds__(1024) void norm_block(NormArgs a) {
     const size_t row = blockIdx.x;
     float v[CH][4], r[CH][4];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) read4<XT>(a.x, row * a.x_stride, 4 * (TH * c + tid), a.N, a.vec, v[c]);
+    for (int c = 0; c < CH; ++c) read4<XT>(a.x, row * a.x_stride, column<MX>(c, tid, TH), a.N, a.vec, v[c]);
     if (a.res) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) read4<HT>(a.res, row * a.res_stride, 4 * (TH * c + tid), a.N, a.vec, r[c]);
+        for (int c = 0; c < CH; ++c) read4<HT>(a.res, row * a.res_stride, column<MX>(c, tid, TH), a.N, a.vec, r[c]);
     }
-    if (a.has_post) norm_row<CH>(v, a.post, a.N, a.vec, tid, block_sum);
+    if (a.has_post) norm_row<CH, MX>(v, a.post, a.N, a.vec, tid, block_sum);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int i = 4 * (TH * c + tid);
+        const int i = column<MX>(c, tid, TH);
         if (a.gate) {
             float g[4];
             read4<BYHIP_F32>(a.gate, row * a.gate_stride, i, a.N, a.vec, g);
@@ -131,9 +159,31 @@ __global__ __launch_bounds__(1024) void norm_block(NormArgs a) {
         if (a.h) write4(a.h, row * a.h_stride, i, a.N, a.vec, v[c], HT);
     }
     if (!a.has_pre) return;
-    norm_row<CH>(v, a.pre, a.N, a.vec, tid, block_sum);
+    norm_row<CH, MX>(v, a.pre, a.N, a.vec, tid, block_sum);
+    if constexpr (MX) {
+        if (a.y_dtype == BYHIP_MXFP8_KM) write_mx<BYHIP_MXFP8_KM, CH>(a, row, tid, TH, v);
+        else write_mx<BYHIP_MXFP4_KM, CH>(a, row, tid, TH, v);
+    } else {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) write4(a.y, row * a.y_stride, 4 * (TH * c + tid), a.N, a.vec, v[c], a.y_dtype);
+        for (int c = 0; c < CH; ++c) write4(a.y, row * a.y_stride, column<MX>(c, tid, TH), a.N, a.vec, v[c], a.y_dtype);
+    }
+}
+
+// One value per lane of 32 neighbours (a half wave) that are a group: its byte, or with the lane 16 further on its byte of two.
+template <int FMT>
+__device__ __forceinline__ void write_mx1(const NormArgs& a, size_t row, int i, float v) {
+    uint32_t m = mag_bits(v);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    const uint32_t byte = mx_scale<FMT>(m);
+    const float z = byte == 255u ? 0.0f : v * mx_inverse(byte), far = __shfl_xor(z, 16);
+    const int G = i >> 5, j = i & 31;
+    uint8_t* y = static_cast<uint8_t*>(a.y);
+    if constexpr (FMT == BYHIP_MXFP8_KM)
+        y[row * a.N + 32 * G + 2 * (j & 15) + (j >> 4)] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(z, z, 0, false);
+    else if (j < 16)
+        y[row * (a.N / 2) + 16 * G + j] = (uint8_t)__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, z, far, 1.0f, 0);
+    if (j == 0) a.y_scales[row * (a.N / 32) + G] = (uint8_t)byte;
 }
 
 // Rows of any length: each sum walks over x (and res) again. h may be res's rows, so it is written last.
@@ -172,7 +222,10 @@ __global__ __launch_bounds__(1024) void norm_block_long(NormArgs a) {
         const float yv[1] = {(v - mean2) * f2 * (a.has_pre && a.pre.weight ? a.pre.weight[i] : 1.0f) +
                              (a.has_pre && a.pre.bias ? a.pre.bias[i] : 0.0f)};
         if (a.h) store_vec<1>(a.h, row * a.h_stride + i, hv, HT);
-        if (a.has_pre) store_vec<1>(a.y, row * a.y_stride + i, yv, a.y_dtype);
+        if (!a.has_pre) continue;
+        if (a.y_dtype == BYHIP_MXFP8_KM) write_mx1<BYHIP_MXFP8_KM>(a, row, i, yv[0]);
+        else if (a.y_dtype == BYHIP_MXFP4_KM) write_mx1<BYHIP_MXFP4_KM>(a, row, i, yv[0]);
+        else store_vec<1>(a.y, row * a.y_stride + i, yv, a.y_dtype);
     }
 }
 
@@ -188,6 +241,15 @@ void launch_norm(const NormArgs& a) {
     const int ch = fours <= (few ? 1024 : 64) ? 1 : fours <= (few ? 2048 : 128) ? 2 : fours <= 4096 ? 4 : 8;
     const long long threads = ((fours + ch - 1) / ch + 63) / 64 * 64;
     const dim3 grid(a.M), block((unsigned)threads);
+    if (a.has_pre && is_mx(a.y_dtype) && threads <= 1024) {
+        // Two chunks at least, so that a thread holds eight values of a group.
+        const dim3 two((unsigned)(((fours + 1) / 2 + 63) / 64 * 64));
+        if (ch <= 2) launch("norm_block", (norm_block<XT, HT, 2, true>), grid, two, 0, a);
+        else if (ch == 4) launch("norm_block", (norm_block<XT, HT, 4, true>), grid, block, 0, a);
+        else launch("norm_block", (norm_block<XT, HT, 8, true>), grid, block, 0, a);
+        BYHIP_LAUNCHED("norm_block");
+        return;
+    }
     if (threads > 1024) launch("norm_block_long", (norm_block_long<XT, HT>), grid, dim3(1024), 0, a);
     else if (ch == 1) launch("norm_block", (norm_block<XT, HT, 1>), grid, block, 0, a);
     else if (ch == 2) launch("norm_block", (norm_block<XT, HT, 2>), grid, block, 0, a);
@@ -245,8 +307,14 @@ extern "C" int byhip_norm_block(const void* x, size_t x_stride, int x_dtype, int
         if (pre) {
             check_norm(pre, N, "pre", vec);
             a.pre = *pre; a.has_pre = 1;
-            check_rows(y, M, N, y_stride, y_dtype, "normed output");
-            vec = vec && aligned4(y, y_stride, y_dtype);
+            if (is_mx(y_dtype)) {
+                check_mx(y, M, N, y_dtype, "normed output");
+                if (y_stride != (size_t)N) fail("byhip: normed output of %d values: microscaled rows have no stride of their own (%zu)", N, y_stride);
+                a.y_scales = static_cast<uint8_t*>(y) + mx_values(M, N, y_dtype);
+            } else {
+                check_rows(y, M, N, y_stride, y_dtype, "normed output");
+                vec = vec && aligned4(y, y_stride, y_dtype);
+            }
         }
         if (M == 0) return;
         a.x = x; a.gate = gate; a.res = res; a.h = h; a.y = y; a.vec = vec;

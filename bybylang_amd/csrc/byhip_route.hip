@@ -1,0 +1,618 @@
+// byhip_route.hip - routing to experts (gfx950): scores, the best of them per token, and the plan that orders the
+// assignments by expert; and the sum of a token's rows afterwards.
+//
+// A wave routes a token: lane l holds the experts V l .. V l + V - 1 and the best of those not yet chosen, its head, so that a
+// round of the selection looks at 64 heads and only the winner's lane looks for its next. Keys are compared as whole numbers with floats' order (0: not a choice); keys that are
+// sums with a bias, or ranked by groups' sums, are formed in 64 bits, where their heads' 32-bit roundings tie the 64-bit
+// values decide.
+//
+// The plan is a stable counting sort. A wave takes 64 assignments at a time and finds each one's rank among those of the same
+// expert from ballots over the id's bits, so no atomic's order has a say in the result.
+#include "byhip_mx.h"
+
+namespace byhip {
+namespace {
+
+struct RouteArgs {
+    const void* logits;
+    const float* bias;
+    size_t stride;
+    int T, E, k, score, groups, top_groups, group_by, renorm, vec;
+    float scale;
+    int* ids;
+    float* weights;
+};
+
+// fp32 in an order of whole numbers: every number and infinity above 1, NaN 1, and 0 left for what is no choice.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // -0 as 0
+    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 1u;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+
+// Orders a wave's LDS accesses: what its lanes wrote before is what its lanes read after.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    return v;
+}
+__device__ __forceinline__ float wave_maxf(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ double wave_sumd(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ double lane_d(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// The choices of token t by this wave. WIDE: keys in 64 bits (`group` holds E of them in LDS where groups are ranked).
+template <int DT, int V, bool WIDE>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* group, int* ids_out) {
+    const int lane = threadIdx.x & 63, e0 = lane * V;
+    const size_t row = (size_t)t * a.stride;
+    float x[V];
+    if (a.vec && V >= 4 && e0 + V <= a.E) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            float four[4];
+            load_vec<DT, 4>(a.logits, row + e0 + i, four);
+#pragma unroll
+            for (int q = 0; q < 4 && i + q < V; ++q) x[i + q] = four[q];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = e0 + i < a.E ? load1<DT>(a.logits, row + e0 + i) : -INFINITY;
+    }
+    // Softmax: exp(x - top) / sum. A logit of +infinity leaves weight to its like only; where all are -infinity, none has any.
+    float top = 0.0f, sum = 1.0f;
+    double sum_d = 1.0;
+    const bool soft = a.score == BYHIP_MOE_SOFTMAX;
+    auto lift = [&](float v) { return v == top ? 0.0f : v - top; };
+    if (soft) {
+        top = -INFINITY;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < V; ++i) { top = fmaxf(top, x[i]); nan = nan || x[i] != x[i]; }
+        top = wave_maxf(top);
+        float s = 0.0f;
+        double sd = 0.0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (e0 + i >= a.E) continue;
+            if constexpr (WIDE) sd += exp((double)(x[i] == top ? 0.0 : (double)x[i] - (double)top));
+            else s += expf(lift(x[i]));
+        }
+        if constexpr (WIDE) { sum_d = wave_sumd(sd); sum = (float)sum_d; }
+        else sum = wave_sum(s);
+        if (top == -INFINITY && !__any(nan)) { sum = INFINITY; sum_d = (double)INFINITY; }
+    }
+    auto score_f = [&](float v) { return soft ? expf(lift(v)) / sum : 1.0f / (1.0f + expf(-v)); };
+    auto score_d = [&](float v) {
+        return soft ? exp(v == top ? 0.0 : (double)v - (double)top) / sum_d : 1.0 / (1.0 + exp(-(double)v));
+    };
+
+    uint32_t key[V];
+    double wide[WIDE ? V : 1];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if constexpr (WIDE) {
+            double c = -(double)INFINITY;
+            if (e0 + i < a.E) c = score_d(x[i]) + (a.bias ? (double)a.bias[e0 + i] : 0.0);
+            wide[i] = c;
+            key[i] = e0 + i < a.E ? order_key((float)c) : 0u;
+        } else {
+            key[i] = e0 + i < a.E ? order_key(x[i]) : 0u;
+        }
+    }
+    if (a.groups > 1) {
+        const int size = a.E / a.groups;
+        uint64_t in;
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (e0 + i < a.E) group[e0 + i] = wide[i] == wide[i] ? wide[i] : -(double)INFINITY;
+            wave_sync();
+            double one = -(double)INFINITY, two = -(double)INFINITY;
+            if (lane < a.groups)
+                for (int i = 0; i < size; ++i) {
+                    const double c = group[lane * size + i];
+                    if (c > one) { two = one; one = c; }
+                    else if (c > two) two = c;
+                }
+            const double worth = a.group_by == 2 && size > 1 ? one + two : one;
+            int above = 0;
+            for (int g = 0; g < a.groups; ++g) {
+                const double o = lane_d(worth, g);
+                above += o > worth || (o == worth && g < lane);
+            }
+            in = __ballot(lane < a.groups && above < a.top_groups);
+            wave_sync();
+        } else {
+            uint32_t* keys = reinterpret_cast<uint32_t*>(group);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (e0 + i < a.E) keys[e0 + i] = key[i];
+            wave_sync();
+            uint32_t worth = 0;
+            if (lane < a.groups)
+                for (int i = 0; i < size; ++i) worth = max(worth, keys[lane * size + i]);
+            int above = 0;
+            for (int g = 0; g < a.groups; ++g) {
+                const uint32_t o = __builtin_amdgcn_readlane((int)worth, g);
+                above += o > worth || (o == worth && g < lane);
+            }
+            in = __ballot(lane < a.groups && above < a.top_groups);
+            wave_sync();
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (e0 + i >= a.E || !((in >> ((e0 + i) / size)) & 1)) key[i] = 0u;
+    }
+    // Rounds: the largest head; of several, in 64 bits the largest, then the lowest index (the lowest lane).
+    float mine = 0.0f, total = 0.0f;
+    int mine_id = 0;
+    uint32_t head = 0;
+    double head_wide = 0.0;
+    int at = 0;
+    auto find_head = [&] {
+        head = key[0];
+        at = 0;
+        if constexpr (WIDE) head_wide = wide[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) {
+            bool over = key[i] > head;
+            if constexpr (WIDE) over = over || (key[i] == head && wide[i] > head_wide);
+            head = over ? key[i] : head;
+            at = over ? i : at;
+            if constexpr (WIDE) head_wide = over ? wide[i] : head_wide;
+        }
+    };
+    find_head();
+    for (int j = 0; j < a.k; ++j) {
+        const uint32_t best = wave_max(head);
+        uint64_t who = __ballot(head == best);
+        if constexpr (WIDE) {
+            if (__popcll(who) > 1 && best > 1u) {
+                const double c = head == best ? head_wide : -(double)INFINITY;
+                double m = c;
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+                who = __ballot(head == best && c == m);
+            }
+        }
+        const int win = __ffsll((unsigned long long)who) - 1;
+        const int pick = __builtin_amdgcn_readlane(at, win);
+        float logit = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) logit = at == i ? x[i] : logit;
+        logit = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, logit), win));
+        if (lane == (j & 63)) { mine_id = win * V + pick; mine = logit; }
+        if (lane == win) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = i == pick ? 0u : key[i];
+            find_head();
+        }
+        // 64 choices at most are held; the weights of more are formed in a second turn (below).
+        if ((j & 63) == 63 || j + 1 == a.k) {
+            const int first = j & ~63, n = j - first + 1;
+            if (lane < n) {
+                float s;
+                if constexpr (WIDE) s = (float)score_d(mine);
+                else s = score_f(mine);
+                total += s;
+                ids_out[first + lane] = mine_id;
+                a.ids[(size_t)t * a.k + first + lane] = mine_id;
+                mine = s;
+                if (a.k > 64 || !a.renorm) a.weights[(size_t)t * a.k + first + lane] = s * (a.renorm ? 1.0f : a.scale);
+            }
+        }
+    }
+    if (a.renorm) {
+        total = wave_sum(total);
+        const float f = total == 0.0f ? 0.0f : a.scale / total;
+        if (a.k <= 64) {
+            if (lane < a.k) a.weights[(size_t)t * a.k + lane] = total == 0.0f ? 0.0f : mine * f;
+        } else {
+            for (int i = lane; i < a.k; i += 64) a.weights[(size_t)t * a.k + i] *= f;
+        }
+    }
+}
+
+constexpr int kTokensPerBlock = 4;
+
+template <int DT, int V, bool WIDE>
+__global__ __launch_bounds__(64 * kTokensPerBlock) void moe_route(RouteArgs a) {
+    __shared__ double group[kTokensPerBlock][WIDE ? 64 * V : 32 * V];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.x * kTokensPerBlock + w;
+    if (t >= a.T) return;
+    route_token<DT, V, WIDE>(a, t, group[w], a.ids + (size_t)t * a.k);
+}
+
+// ── the plan ──
+
+// Lanes below this one, and this one's peers: the lanes whose id is the same (bits of an id below 2^BITS; `live` lanes only).
+__device__ __forceinline__ uint64_t same_id(int id, bool live) {
+    uint64_t m = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < 10; ++b) {
+        const bool bit = (id >> b) & 1;
+        const uint64_t set = __ballot(bit);
+        m &= bit ? set : ~set;
+    }
+    return m;
+}
+__device__ __forceinline__ int rank_below(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// Assignments lo .. hi - 1 in `waves` equal stretches of whole 64s; this wave's.
+__device__ __forceinline__ void stretch(int lo, int hi, int waves, int w, int& from, int& to) {
+    const int each = ((hi - lo + waves - 1) / waves + 63) & ~63;
+    from = min(hi, lo + each * w);
+    to = min(hi, from + each);
+}
+
+// How many assignments of its stretch each expert gets, added to the wave's counts.
+__device__ __forceinline__ void count_ids(const int* ids, int from, int to, int E, int* counts) {
+    const int lane = threadIdx.x & 63;
+    for (int i = from + lane; i < to; i += 64) {
+        const int id = ids[i];
+        if ((unsigned)id < (unsigned)E) atomicAdd(&counts[id], 1);
+    }
+}
+
+// Places the stretch's assignments: next[e] is where the wave's next assignment of expert e goes.
+__device__ __forceinline__ void place_ids(const int* ids, int from, int to, int E, int* next, int* order) {
+    const int lane = threadIdx.x & 63;
+    for (int i0 = from; i0 < to; i0 += 64) {
+        const int i = i0 + lane;
+        int id = i < to ? ids[i] : -1;
+        const bool live = (unsigned)id < (unsigned)E;
+        id = live ? id : 0;
+        const uint64_t peers = same_id(id, live);
+        const int rank = rank_below(peers);
+        if (live) order[next[id] + rank] = i;
+        wave_sync();
+        if (live && rank == 0) next[id] += __popcll(peers);
+        wave_sync();
+    }
+}
+
+// Exclusive prefix sums of v over the block's threads (1024 at most), and the total.
+__device__ __forceinline__ int block_prefix(int v, int* part, int& total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int n = __shfl_up(s, o);
+        if (lane >= o) s += n;
+    }
+    __syncthreads();
+    if (lane == 63) part[w] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int i = 0; i < waves; ++i) {
+        before += i < w ? part[i] : 0;
+        total += part[i];
+    }
+    return before + s - v;
+}
+
+// Offsets and units from expert e's count (thread e's; 0 past E), and where e starts.
+__device__ __forceinline__ int write_units(const MoePlan& p, int count, int* part) {
+    const int e = threadIdx.x;
+    int total, units;
+    const int at = block_prefix(count, part, total);
+    const int first = block_prefix((count + p.unit_rows - 1) / p.unit_rows, part, units);
+    if (e < p.experts) {
+        p.offsets[e] = at;
+        for (int u = 0, r = 0; r < count; ++u, r += p.unit_rows)
+            p.units[first + u] = MoeUnit{e, at + r, min(p.unit_rows, count - r), 0};
+    }
+    if (e == 0) {
+        p.offsets[p.experts] = total;
+        *p.n_units = units;
+    }
+    return at;
+}
+
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+
+// The whole plan in one block: counts per wave and expert, their sums, then the places.
+__device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int* counts, int* part) {
+    const int w = threadIdx.x >> 6, E = p.experts;
+    for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanThreads) counts[i] = 0;
+    __syncthreads();
+    int from, to;
+    stretch(0, p.rows, kPlanWaves, w, from, to);
+    count_ids(ids, from, to, E, counts + w * E);
+    __syncthreads();
+    int sum = 0;
+    if ((int)threadIdx.x < E)
+        for (int i = 0; i < kPlanWaves; ++i) {
+            const int c = counts[i * E + threadIdx.x];
+            counts[i * E + threadIdx.x] = sum;
+            sum += c;
+        }
+    const int at = write_units(p, sum, part);
+    if ((int)threadIdx.x < E)
+        for (int i = 0; i < kPlanWaves; ++i) counts[i * E + threadIdx.x] += at;
+    __syncthreads();
+    place_ids(ids, from, to, E, counts + w * E, p.order);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_one(MoePlan p, const int* ids) {
+    __shared__ int counts[kPlanWaves * kMaxExperts];
+    __shared__ int part[kPlanWaves];
+    plan_block(p, ids, counts, part);
+}
+
+// Many assignments: counts per block of them, the sums over the blocks, then the places.
+constexpr int kCountWaves = 4;
+__global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, const int* ids) {
+    __shared__ int counts[kMaxExperts];
+    const int E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
+    for (int i = threadIdx.x; i < E; i += 64 * kCountWaves) counts[i] = 0;
+    __syncthreads();
+    int from, to;
+    stretch(lo, hi, kCountWaves, threadIdx.x >> 6, from, to);
+    count_ids(ids, from, to, E, counts);
+    __syncthreads();
+    for (int i = threadIdx.x; i < E; i += 64 * kCountWaves) p.counts[(size_t)blockIdx.x * E + i] = counts[i];
+}
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_sums(MoePlan p) {
+    __shared__ int part[kPlanWaves];
+    const int e = threadIdx.x, E = p.experts;
+    int sum = 0;
+    if (e < E)
+        for (int b = 0; b < p.blocks; ++b) sum += p.counts[(size_t)b * E + e];
+    int at = write_units(p, sum, part);
+    if (e < E)
+        for (int b = 0; b < p.blocks; ++b) {
+            const int c = p.counts[(size_t)b * E + e];
+            p.counts[(size_t)b * E + e] = at;
+            at += c;
+        }
+}
+__global__ __launch_bounds__(64 * kCountWaves) void moe_plan_place(MoePlan p, const int* ids) {
+    __shared__ int counts[kCountWaves * kMaxExperts];
+    const int w = threadIdx.x >> 6, E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
+    for (int i = threadIdx.x; i < kCountWaves * E; i += 64 * kCountWaves) counts[i] = 0;
+    __syncthreads();
+    int from, to;
+    stretch(lo, hi, kCountWaves, w, from, to);
+    count_ids(ids, from, to, E, counts + w * E);
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += 64 * kCountWaves) {
+        int at = p.counts[(size_t)blockIdx.x * E + e];
+        for (int i = 0; i < kCountWaves; ++i) {
+            const int c = counts[i * E + e];
+            counts[i * E + e] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    place_ids(ids, from, to, E, counts + w * E, p.order);
+}
+
+void launch_plan(const MoePlan& p, const int* ids) {
+    if (p.blocks <= 4) {
+        launch("moe_plan_one", moe_plan_one, dim3(1), dim3(kPlanThreads), 0, p, ids);
+    } else {
+        launch("moe_plan_count", moe_plan_count, dim3(p.blocks), dim3(64 * kCountWaves), 0, p, ids);
+        launch("moe_plan_sums", moe_plan_sums, dim3(1), dim3(kPlanThreads), 0, p);
+        launch("moe_plan_place", moe_plan_place, dim3(p.blocks), dim3(64 * kCountWaves), 0, p, ids);
+    }
+    BYHIP_LAUNCHED("moe_plan");
+}
+
+template <int DT, int V, bool WIDE>
+void launch_route_v(const RouteArgs& a) {
+    launch("moe_route", (moe_route<DT, V, WIDE>), dim3((a.T + kTokensPerBlock - 1) / kTokensPerBlock), dim3(64 * kTokensPerBlock), 0, a);
+    BYHIP_LAUNCHED("moe_route");
+}
+template <int DT, bool WIDE>
+void launch_route_w(const RouteArgs& a) {
+    if (a.E <= 64) launch_route_v<DT, 1, WIDE>(a);
+    else if (a.E <= 128) launch_route_v<DT, 2, WIDE>(a);
+    else if (a.E <= 256) launch_route_v<DT, 4, WIDE>(a);
+    else if (a.E <= 512) launch_route_v<DT, 8, WIDE>(a);
+    else launch_route_v<DT, 16, WIDE>(a);
+}
+template <int DT>
+void launch_route(const RouteArgs& a) {
+    // Without a bias, and with groups ranked by one key, the logits have the keys' order.
+    if (a.bias || (a.groups > 1 && a.group_by == 2)) launch_route_w<DT, true>(a);
+    else launch_route_w<DT, false>(a);
+}
+
+// ── the sum of a token's rows ──
+
+struct CombineArgs {
+    const void* x;
+    const int* ids;
+    const float* weights;
+    const void* res;
+    void* y;
+    size_t x_stride, res_stride, y_stride;
+    int T, k, E, N, res_dtype, y_dtype, vec;
+};
+
+template <int DT>
+__device__ __forceinline__ void read_cols(const void* p, size_t at, int left, int vec, float (&v)[4]) {
+    if (vec && left >= 4) {
+        load_vec<DT, 4>(p, at, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < left ? load1<DT>(p, at + e) : 0.0f;
+    }
+}
+
+template <int XT>
+__global__ __launch_bounds__(256) void moe_combine(CombineArgs a) {
+    const int n = 4 * (blockIdx.x * 256 + threadIdx.x), left = a.N - n;
+    if (left <= 0) return;
+    for (int t = blockIdx.y; t < a.T; t += gridDim.y) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (a.res) {
+            const size_t at = (size_t)t * a.res_stride + n;
+            if (a.res_dtype == BYHIP_F32) read_cols<BYHIP_F32>(a.res, at, left, a.vec, s);
+            else if (a.res_dtype == BYHIP_F16) read_cols<BYHIP_F16>(a.res, at, left, a.vec, s);
+            else read_cols<BYHIP_BF16>(a.res, at, left, a.vec, s);
+        }
+        const size_t first = (size_t)t * a.k;
+        for (int j = 0; j < a.k; ++j) {
+            if ((unsigned)a.ids[first + j] >= (unsigned)a.E) continue;
+            const float w = a.weights[first + j];
+            float v[4];
+            read_cols<XT>(a.x, (first + j) * a.x_stride + n, left, a.vec, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = fmaf(w, v[e], s[e]);
+        }
+        const size_t at = (size_t)t * a.y_stride + n;
+        if (a.vec && left >= 4) {
+            store_vec<4>(a.y, at, s, a.y_dtype);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < left) {
+                    const float one[1] = {s[e]};
+                    store_vec<1>(a.y, at + e, one, a.y_dtype);
+                }
+        }
+    }
+}
+
+}  // namespace
+
+MoePlan moe_layout(const byhip_moe_plan* p) {
+    if (!p) fail("byhip: null plan");
+    if (p->tokens < 0 || p->experts < 1 || p->experts > kMaxExperts || p->top_k < 1 || p->top_k > p->experts ||
+        (long long)p->tokens * p->top_k >= 1 << 24)
+        fail("byhip: a plan of %d tokens, %d of %d experts each", p->tokens, p->top_k, p->experts);
+    MoePlan m{};
+    m.tokens = p->tokens; m.top_k = p->top_k; m.experts = p->experts;
+    m.rows = p->tokens * p->top_k;
+    m.unit_rows = moe_unit_rows(m.rows, m.experts);
+    m.max_units = m.rows / m.unit_rows + (m.rows < m.experts ? m.rows : m.experts);
+    m.blocks = (m.rows + kPlanBlock - 1) / kPlanBlock;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 15) / 16 * 16; return static_cast<char*>(p->plan) + here; };
+    m.offsets = reinterpret_cast<int*>(take(((size_t)m.experts + 1 + m.rows) * 4));
+    m.order = m.offsets + m.experts + 1;
+    m.n_units = reinterpret_cast<int*>(take(4));
+    m.units = reinterpret_cast<MoeUnit*>(take((size_t)m.max_units * sizeof(MoeUnit)));
+    m.counts = reinterpret_cast<int*>(take((size_t)m.blocks * m.experts * 4));
+    m.bytes = at;
+    return m;
+}
+
+MoePlan moe_plan_args(const byhip_moe_plan* p) {
+    const MoePlan m = moe_layout(p);
+    check_span(p->plan, m.bytes, "plan");
+    if (reinterpret_cast<uintptr_t>(p->plan) % 16) fail("byhip: a plan must be 16-byte aligned");
+    return m;
+}
+
+}  // namespace byhip
+
+using namespace byhip;
+
+extern "C" {
+
+unsigned long long byhip_moe_plan_bytes(int tokens, int top_k, int experts) {
+    unsigned long long bytes = 0;
+    guard([&] {
+        const byhip_moe_plan p{tokens, top_k, experts, nullptr};
+        bytes = moe_layout(&p).bytes;
+    });
+    return bytes;
+}
+
+int byhip_moe_route(const void* logits, size_t stride, int dtype, const byhip_moe_router* router, const byhip_moe_plan* plan,
+                    int* ids, float* weights) {
+    return guard([&] {
+        enter_compute();
+        const MoePlan p = moe_plan_args(plan);
+        if (!router) fail("byhip: null router");
+        const byhip_moe_router& r = *router;
+        if (r.score != BYHIP_MOE_SOFTMAX && r.score != BYHIP_MOE_SIGMOID) fail("byhip: router score %d", r.score);
+        if (r.groups < 1 || r.groups > 64 || p.experts % r.groups || r.top_groups < 1 || r.top_groups > r.groups)
+            fail("byhip: the best %d of %d groups of %d experts", r.top_groups, r.groups, p.experts);
+        if (r.groups > 1 && r.group_by != 1 && r.group_by != 2) fail("byhip: groups by their %d best", r.group_by);
+        if (p.top_k > p.experts / r.groups * r.top_groups)
+            fail("byhip: %d choices among %d experts", p.top_k, p.experts / r.groups * r.top_groups);
+        check_rows(logits, p.tokens, p.experts, stride, dtype, "logits");
+        if (r.bias) check_span(r.bias, (size_t)p.experts * 4, "router bias");
+        if (p.rows) {
+            check_span(ids, (size_t)p.rows * 4, "ids");
+            check_span(weights, (size_t)p.rows * 4, "weights");
+        }
+        note_device_write(plan->plan);
+        if (p.rows) {
+            note_device_write(ids);
+            note_device_write(weights);
+            const RouteArgs a{logits, r.bias, stride, p.tokens, p.experts, p.top_k, r.score, r.groups, r.top_groups,
+                              r.group_by, r.renorm, aligned4(logits, stride, dtype), r.scale, ids, weights};
+            switch (dtype) {
+            case BYHIP_F32: launch_route<BYHIP_F32>(a); break;
+            case BYHIP_F16: launch_route<BYHIP_F16>(a); break;
+            default: launch_route<BYHIP_BF16>(a); break;
+            }
+        }
+        launch_plan(p, ids);
+    });
+}
+
+int byhip_moe_plan_ids(const int* ids, const byhip_moe_plan* plan) {
+    return guard([&] {
+        enter_compute();
+        const MoePlan p = moe_plan_args(plan);
+        if (p.rows) check_span(ids, (size_t)p.rows * 4, "ids");
+        note_device_write(plan->plan);
+        launch_plan(p, ids);
+    });
+}
+
+int byhip_moe_combine(const void* x, size_t x_stride, int x_dtype, int N, const byhip_moe_plan* plan, const int* ids,
+                      const float* weights, const void* res, size_t res_stride, int res_dtype, void* y, size_t y_stride,
+                      int y_dtype) {
+    return guard([&] {
+        enter_compute();
+        const MoePlan p = moe_layout(plan);
+        if (N <= 0) fail("byhip: a sum of rows of %d values", N);
+        check_rows(x, p.rows, N, x_stride, x_dtype, "experts' rows");
+        if (res) check_rows(res, p.tokens, N, res_stride, res_dtype, "residual");
+        check_rows(y, p.tokens, N, y_stride, y_dtype, "summed rows");
+        if (res == y && res && (res_stride != y_stride || res_dtype != y_dtype)) fail("byhip: a residual updated in place needs one stride and dtype");
+        if (p.rows == 0) return;
+        check_span(ids, (size_t)p.rows * 4, "ids");
+        check_span(weights, (size_t)p.rows * 4, "weights");
+        const int vec = aligned4(x, x_stride, x_dtype) && (!res || aligned4(res, res_stride, res_dtype)) && aligned4(y, y_stride, y_dtype);
+        const CombineArgs a{x, ids, weights, res, y, x_stride, res_stride, y_stride, p.tokens, p.top_k, p.experts, N, res_dtype, y_dtype, vec};
+        note_device_write(y);
+        const dim3 grid((N + 1023) / 1024, std::min(p.tokens, 65535));
+        switch (x_dtype) {
+        case BYHIP_F32: launch("moe_combine", moe_combine<BYHIP_F32>, grid, dim3(256), 0, a); break;
+        case BYHIP_F16: launch("moe_combine", moe_combine<BYHIP_F16>, grid, dim3(256), 0, a); break;
+        default: launch("moe_combine", moe_combine<BYHIP_BF16>, grid, dim3(256), 0, a); break;
+        }
+        BYHIP_LAUNCHED("moe_combine");
+    });
+}
+
+}  // extern "C"

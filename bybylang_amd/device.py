@@ -10,7 +10,8 @@ import ctypes as C
 import numpy as np
 
 from . import _abi
-from ._abi import (BF16, F16, F32, MXFP4_KM, NORM_LAYER, NORM_RMS, ROPE_BASE, ROPE_HALVES,
+from ._abi import (BF16, F16, F32, MOE_GATHER, MOE_SCATTER, MOE_SIGMOID, MOE_SOFTMAX, MOE_SWIGLU, MXFP4_KM,
+                   MXFP8_KM, NORM_LAYER, NORM_RMS, ROPE_BASE, ROPE_HALVES,
                    ROPE_LINEAR, ROPE_PAIRS, ROPE_PARTS, ROPE_PLAIN, HipBackendError, HipUnsupported,
                    check, load)
 
@@ -20,7 +21,10 @@ __all__ = ["DeviceBuffer", "Q4Weights", "init", "device_info", "synchronize", "s
            "HipUnsupported", "dtype_code", "np_dtype", "KvCache", "KvBatch", "KvPool", "Rope", "Attn",
            "Norm", "rope_steps", "rope_append", "paged_attention", "cache_fork", "cache_free",
            "cache_grow", "cache_compact", "cache_copy", "norm_block", "ROPE_HALVES", "ROPE_PAIRS",
-           "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_BASE", "ROPE_PARTS", "NORM_RMS", "NORM_LAYER"]
+           "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_BASE", "ROPE_PARTS", "NORM_RMS", "NORM_LAYER",
+           "MXFP8_KM", "mx_bytes", "mx_quantize", "mx_matmul", "MoePlan", "MoeRouter", "moe_plan_bytes", "moe_route",
+           "moe_plan", "moe_matmul", "moe_combine", "MOE_SOFTMAX", "MOE_SIGMOID", "MOE_GATHER", "MOE_SCATTER",
+           "MOE_SWIGLU"]
 
 _NP = {F32: np.float32, F16: np.float16, BF16: np.uint16}
 
@@ -340,3 +344,61 @@ def norm_block(x, x_stride: int, x_dtype: int, M: int, N: int, post: Norm | None
     check(load().byhip_norm_block(x.ptr, x_stride, x_dtype, M, N, _ref(post), _ptr(gate), gate_stride,
                                   _ptr(res), res_stride, res_scale, _ptr(h), h_stride, h_dtype, _ref(pre),
                                   _ptr(y), y_stride, y_dtype), "byhip_norm_block")
+
+
+# ── microscaled rows and experts ────────────────────────────────────────────────────────────
+
+
+def mx_bytes(rows: int, width: int, fmt: int) -> int:
+    """Bytes of `rows` microscaled rows of `width` values (MXFP8_KM or MXFP4_KM), scales included."""
+    return rows * (width if fmt == MXFP8_KM else width // 2) + rows * (width // 32)
+
+
+def mx_quantize(x, x_stride: int, x_dtype: int, M: int, K: int, y, y_format: int) -> None:
+    check(load().byhip_mx_quantize(x.ptr, x_stride, x_dtype, M, K, y.ptr, y_format), "byhip_mx_quantize")
+
+
+def mx_matmul(x, x_format: int, w, M: int, K: int, N: int, flags: int, y, y_stride: int, y_dtype: int) -> None:
+    check(load().byhip_mx_matmul(x.ptr, x_format, w.ptr, M, K, N, flags, y.ptr, y_stride, y_dtype), "byhip_mx_matmul")
+
+
+def moe_plan_bytes(tokens: int, top_k: int, experts: int) -> int:
+    """Bytes of a plan's device buffer; ValueError where the sizes are out of range."""
+    n = load().byhip_moe_plan_bytes(tokens, top_k, experts)
+    if n == 0:
+        raise ValueError(_abi.last_error())
+    return n
+
+
+class MoePlan(_Struct):
+    """Which tokens go to which expert (byhip_moe_plan), over a device buffer of moe_plan_bytes bytes."""
+
+    def __init__(self, plan, tokens: int, top_k: int, experts: int):
+        super().__init__(_abi.MoePlan(tokens, top_k, experts, plan.ptr), plan)
+
+
+class MoeRouter(_Struct):
+    """How logits become choices (byhip_moe_router); bias: fp32 [experts] on the device, or None."""
+
+    def __init__(self, score: int = MOE_SOFTMAX, bias=None, groups: int = 1, top_groups: int = 1, group_by: int = 1,
+                 renorm: bool = True, scale: float = 1.0):
+        super().__init__(_abi.MoeRouter(score, _ptr(bias), groups, top_groups, group_by, int(renorm), scale), bias)
+
+
+def moe_route(logits, stride: int, dtype: int, router: MoeRouter, plan: MoePlan, ids, weights) -> None:
+    check(load().byhip_moe_route(logits.ptr, stride, dtype, router.ref, plan.ref, ids.ptr, weights.ptr), "byhip_moe_route")
+
+
+def moe_plan(ids, plan: MoePlan) -> None:
+    check(load().byhip_moe_plan_ids(ids.ptr, plan.ref), "byhip_moe_plan_ids")
+
+
+def moe_matmul(x, x_format: int, w, plan: MoePlan, K: int, N: int, flags: int, y, y_stride: int, y_dtype: int) -> None:
+    check(load().byhip_moe_matmul(x.ptr, x_format, w.ptr, plan.ref, K, N, flags, y.ptr, y_stride, y_dtype),
+          "byhip_moe_matmul")
+
+
+def moe_combine(x, x_stride: int, x_dtype: int, N: int, plan: MoePlan, ids, weights, res, res_stride: int, res_dtype: int,
+                y, y_stride: int, y_dtype: int) -> None:
+    check(load().byhip_moe_combine(x.ptr, x_stride, x_dtype, N, plan.ref, ids.ptr, weights.ptr, _ptr(res), res_stride,
+                                   res_dtype, y.ptr, y_stride, y_dtype), "byhip_moe_combine")

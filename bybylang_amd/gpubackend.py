@@ -460,6 +460,66 @@ def sessionCacheCompact(backend: GpuBackend, pool) -> bool:
     return _encoded(load().byhip_cache_compact(pool.ref, None, None), "sessionCacheCompact")
 
 
+# ── microscaled rows and experts ────────────────────────────────────────────────────────────
+#
+# As above: fp32 handles of dense rows, microscaled rows and plans in handles of bytes (sessionAllocBytes).
+
+
+def sessionAllocBytes(backend: GpuBackend, nBytes: int) -> SessionHandle:
+    """Scratch of at least nBytes bytes, for microscaled rows, plans and chosen experts."""
+    return sessionAllocScratch(backend, (nBytes + 3) // 4)
+
+
+def sessionNormBlockMx(backend: GpuBackend, x: SessionHandle, M: int, N: int, post, gate: SessionHandle | None,
+                       res: SessionHandle | None, resScale: float, h: SessionHandle | None, pre, y: SessionHandle,
+                       fmt: int) -> bool:
+    """sessionNormBlock with y as microscaled rows of format `fmt`."""
+    _require_hip(backend)
+    ptr = lambda b: None if b is None else b.hipHandle  # noqa: E731
+    return _encoded(load().byhip_norm_block(x.hipHandle, N, _abi.F32, M, N, _opt(post), ptr(gate), N, ptr(res), N,
+                                            resScale, ptr(h), N, _abi.F32, pre.ref, y.hipHandle, N, fmt),
+                    "sessionNormBlockMx")
+
+
+def sessionMxQuantize(backend: GpuBackend, x: SessionHandle, M: int, K: int, y: SessionHandle, fmt: int) -> bool:
+    """y = x as microscaled rows of format `fmt`."""
+    _require_hip(backend)
+    return _encoded(load().byhip_mx_quantize(x.hipHandle, K, _abi.F32, M, K, y.hipHandle, fmt), "sessionMxQuantize")
+
+
+def sessionMxMatmul(backend: GpuBackend, x: SessionHandle, fmt: int, w: SessionHandle, M: int, K: int, N: int,
+                    y: SessionHandle, yFmt: int = _abi.F32, swiglu: bool = False) -> bool:
+    """y = x . w^T of microscaled rows and a matrix in 4 bits."""
+    _require_hip(backend)
+    return _encoded(load().byhip_mx_matmul(x.hipHandle, fmt, w.hipHandle, M, K, N, _abi.MOE_SWIGLU if swiglu else 0, y.hipHandle, N,
+                                           yFmt), "sessionMxMatmul")
+
+
+def sessionMoeRoute(backend: GpuBackend, logits: SessionHandle, router, plan, ids: SessionHandle,
+                    weights: SessionHandle) -> bool:
+    """The experts of each row of logits, their weights, and the plan that orders the rows by expert."""
+    _require_hip(backend)
+    return _encoded(load().byhip_moe_route(logits.hipHandle, plan.value.experts, _abi.F32, router.ref, plan.ref, ids.hipHandle,
+                                           weights.hipHandle), "sessionMoeRoute")
+
+
+def sessionMoeMatmul(backend: GpuBackend, x: SessionHandle, fmt: int, w: SessionHandle, plan, K: int, N: int, flags: int,
+                     y: SessionHandle, yFmt: int = _abi.F32) -> bool:
+    """The plan's rows times their experts' matrices (flags of device.py)."""
+    _require_hip(backend)
+    return _encoded(load().byhip_moe_matmul(x.hipHandle, fmt, w.hipHandle, plan.ref, K, N, flags, y.hipHandle, N, yFmt),
+                    "sessionMoeMatmul")
+
+
+def sessionMoeCombine(backend: GpuBackend, x: SessionHandle, N: int, plan, ids: SessionHandle, weights: SessionHandle,
+                      res: SessionHandle | None, y: SessionHandle) -> bool:
+    """y = res + each token's rows of x by their weights."""
+    _require_hip(backend)
+    return _encoded(load().byhip_moe_combine(x.hipHandle, N, _abi.F32, N, plan.ref, ids.hipHandle, weights.hipHandle,
+                                             None if res is None else res.hipHandle, N, _abi.F32, y.hipHandle, N, _abi.F32),
+                    "sessionMoeCombine")
+
+
 # ── FP4-KM / FP16 tile GEMM (gpubackend.nim:1442-1488) ───────────────────────────────────────
 
 

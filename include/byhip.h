@@ -38,9 +38,12 @@ enum byhip_dtype {
     BYHIP_BF16 = 2,
     /* Activations in the FP4-KM packing of the weights: E2M1 nibbles [M, K/2] (byte j of a
      * 32-value group holds element j low and j + 16 high, session_vm.nim:384-388) followed by one
-     * E8M0 scale byte per group [M, K/32]. Only byhip_mxfp4_gemm and byhip_fp4km_tile_gemm read
-     * it. */
-    BYHIP_MXFP4_KM = 3
+     * E8M0 scale byte per group [M, K/32]. byhip_mxfp4_gemm, byhip_fp4km_tile_gemm and the calls on
+     * microscaled rows read it; byhip_norm_block and those calls write it. */
+    BYHIP_MXFP4_KM = 3,
+    /* The same in 8 bits: e4m3 values [M, K] in the FP4-KM order (byte 2 j of a 32-value group holds element j,
+     * byte 2 j + 1 element j + 16), then the scale bytes [M, K/32]. */
+    BYHIP_MXFP8_KM = 4
 };
 
 typedef struct byhip_device_info {
@@ -423,11 +426,80 @@ typedef struct byhip_norm {
 /* Between two blocks, M rows of N values: h = res_scale * res + gate * post(x), y = pre(h). post NULL: x
  * itself; gate (fp32, gate_stride between rows, 0: one row for all) NULL: 1; res NULL: 0; h NULL: not
  * stored; pre NULL: no y. res and h have h_dtype and may be the same rows. y is formed from h before its rounding.
- * Row strides in elements. */
+ * Row strides in elements. y_dtype may also be BYHIP_MXFP8_KM or BYHIP_MXFP4_KM: y is then one buffer of microscaled rows
+ * as byhip_mx_quantize writes it (N a multiple of 32, y_stride N). */
 int byhip_norm_block(const void* x, size_t x_stride, int x_dtype, int M, int N, const byhip_norm* post,
                      const float* gate, size_t gate_stride, const void* res, size_t res_stride,
                      float res_scale, void* h, size_t h_stride, int h_dtype, const byhip_norm* pre, void* y,
                      size_t y_stride, int y_dtype);
+
+/* ── Microscaled rows and experts ─────────────────────────────────────────
+ * No counterpart in the reference.
+ *
+ * Microscaled rows (BYHIP_MXFP8_KM, BYHIP_MXFP4_KM): M rows of K values, K a multiple of 32; all values' bytes, then all
+ * scale bytes, in one buffer aligned to 16 bytes. What these calls write: a group's scale is 2^e with the least
+ * e (-127 or more) for which its largest magnitude is at most 448 2^e (8 bits) or 6 2^e (4 bits), its values are
+ * rounded to the nearest, ties to even, so that none is clipped. A group that holds a NaN or an infinity gets the
+ * scale byte 255, which stands for NaN. Matrices have the same form in 4 bits, one row per output. */
+
+/* M rows of K values of x (F32, F16 or BF16, x_stride elements apart) as microscaled rows. */
+int byhip_mx_quantize(const void* x, size_t x_stride, int x_dtype, int M, int K, void* y, int y_format);
+
+/* What a product does with its rows. */
+enum byhip_moe_flags {
+    BYHIP_MOE_GATHER = 1,  /* x holds the tokens' rows (tokens of them); without it the plan's rows, in its order */
+    BYHIP_MOE_SCATTER = 2, /* y's row a is assignment a's; without it y's row i is the plan's row i */
+    BYHIP_MOE_SWIGLU = 4   /* a matrix has 2 N rows, gates then ups: y = silu(gate) * up, silu(v) = v / (1 + exp(-v)) */
+};
+
+/* y [M, N] = x . w^T of microscaled rows and one matrix [N, K] (with BYHIP_MOE_SWIGLU, the only flag it takes,
+ * [2 N, K]); fp32 sums. y_dtype F32, F16, BF16, or microscaled rows again (N a multiple of 32, y_stride N). */
+int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K, int N, int flags, void* y,
+                    size_t y_stride, int y_dtype);
+
+/* Which tokens go to which expert. Assignment a = t * top_k + j is the j-th choice of token t; `plan` is a device
+ * buffer of byhip_moe_plan_bytes bytes aligned to 16, of which int32 offsets [experts + 1] and order [tokens * top_k] come first:
+ * expert e's rows are the assignments order[offsets[e]] .. order[offsets[e + 1] - 1], ascending. The rest is the library's. */
+typedef struct byhip_moe_plan {
+    int tokens, top_k, experts;
+    void* plan;
+} byhip_moe_plan;
+
+/* Bytes of a plan's buffer; 0 where the sizes are out of range (tokens >= 0, 1 <= top_k <= experts <= 1024,
+ * tokens * top_k < 2^24). Needs no device. */
+unsigned long long byhip_moe_plan_bytes(int tokens, int top_k, int experts);
+
+enum byhip_moe_score { BYHIP_MOE_SOFTMAX = 0, BYHIP_MOE_SIGMOID = 1 };
+/* How logits become choices. score = softmax over the experts or sigmoid; key = score + bias (device, fp32
+ * [experts], or NULL). With groups > 1 (at most 64, dividing experts) only the top_groups best groups take part, by the sum
+ * of their group_by (1 or 2) largest keys. The top_k largest keys are chosen, ties to the lowest index; keys
+ * that are NaN come last. Their weights are score (/ the sum over the chosen, with renorm) * scale. A row whose logits are all
+ * -infinity has weights 0. Keys are compared in 64 bits (without a bias as the logits themselves). */
+typedef struct byhip_moe_router {
+    int score;
+    const float* bias;
+    int groups, top_groups, group_by;
+    int renorm;
+    float scale;
+} byhip_moe_router;
+
+/* Routes plan->tokens rows of logits (F32, F16 or BF16, stride elements apart): ids and weights [tokens, top_k] in descending
+ * order of key, and the plan. */
+int byhip_moe_route(const void* logits, size_t stride, int dtype, const byhip_moe_router* router,
+                    const byhip_moe_plan* plan, int* ids, float* weights);
+/* The plan of a caller's own choices [tokens, top_k]. Ids outside 0 .. experts - 1 are left out of it. */
+int byhip_moe_plan_ids(const int* ids, const byhip_moe_plan* plan);
+
+/* The plan's rows times their experts' matrices: w holds `experts` matrices of N rows (2 N with BYHIP_MOE_SWIGLU) as one
+ * matrix of all their rows. y has tokens * top_k rows (microscaled rows too: its scales follow that many rows); those of
+ * assignments that the plan leaves out, and rows past offsets[experts], stay as they were. */
+int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_moe_plan* plan, int K, int N, int flags,
+                     void* y, size_t y_stride, int y_dtype);
+/* y[t] = res[t] + sum over j of weights[t, j] * x[t * top_k + j], in fp32, j ascending; assignments whose id is outside
+ * 0 .. experts - 1 have no part, whatever x holds there. res NULL: 0; res may be y. */
+int byhip_moe_combine(const void* x, size_t x_stride, int x_dtype, int N, const byhip_moe_plan* plan, const int* ids,
+                      const float* weights, const void* res, size_t res_stride, int res_dtype, void* y, size_t y_stride,
+                      int y_dtype);
 
 /* ── Debug (bit-exact unpack checks) ──────────────────────────────────────────────────────── */
 
