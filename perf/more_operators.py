@@ -271,6 +271,7 @@ def _handles(s):
         ints, E = s["plan_buf"].view(torch.int32), c["experts"]
         s["out"] = {"ids": s["ids"], "weights": s["weights"], "offsets": ints[:E + 1], "order": ints[E + 1:E + 1 + s["ids"].numel()]}
     if c["kind"] in ("up", "down"):
+        torch.cuda.synchronize()  # torch's work on memory that the plan's buffer was given is over before the library writes there
         dev.moe_plan(b["ids"], s["plan"])
         dev.synchronize()
         s["out"] = _answer(*_halves(s["y"], c["rows"] * c["top"], c["N"], "mx8")) if c["y"] == "mx8" else {"y": s["y"]}
