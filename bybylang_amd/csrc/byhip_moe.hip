@@ -69,7 +69,7 @@ int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_
         if (p.rows == 0) return;
         a.order = p.order; a.n_units = p.n_units; a.units = p.units;
         a.top_k = p.top_k; a.gather = gather; a.scatter = (flags & BYHIP_MOE_SCATTER) != 0;
-        a.unit_rows = p.unit_rows;
+        a.unit_rows = p.unit_rows; a.experts = p.experts; a.rows = p.rows; a.max_units = p.max_units;
         note_device_write(y);
         launch_moe_rows(a, x_format, glu, p.max_units);
     });

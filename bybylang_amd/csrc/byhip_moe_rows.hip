@@ -11,9 +11,9 @@
 // window are block g of a step is free as long as both operands agree: step s takes group 4 g + s of the window's 16, so
 // that a lane's four scale bytes lie in one word. The result: lane (c, g) holds row c of x, matrix rows 4 g .. 4 g + 3.
 //
-// Sums are fp32. What the instructions add in one go is exact with rows in 4 bits; with rows in 8 bits they align eight neighbouring
-// products to the largest and cut each off 13 bits below its exponent (measured: 4.5e-6 of a random product's norm at any length, a
-// 6000th of what the rows' own rounding to 8 bits is off by, so that products in 16 bits at half the rate would buy nothing).
+// Sums are fp32. What the instructions add in one go is exact with rows in 4 bits; with rows in 8 bits they cut small products off
+// (split_bytes), which leaves 5e-6 to 1e-5 of a product's norm: less than a hundredth of the rounding to 16 bits or fewer that follows.
+// With fp32 outputs (FINE) rows go in two parts, twice the products (in this kernel they wait for memory).
 #include "byhip_moe.h"
 
 namespace byhip {
@@ -41,7 +41,7 @@ __device__ __forceinline__ f4v product(v8i w, v8i x, f4v c, int sw, int sx) {
 }
 
 // MT blocks of 16 rows, NF blocks of 16 matrix rows (GLU: two of gates, two of ups).
-template <int XF, int MT, int NF, bool GLU>
+template <int XF, int MT, int NF, bool GLU, bool FINE>
 __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     static_assert(!GLU || NF == 4, "gates and ups");
     __shared__ float4 part[kWaves][NF * MT][64];
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
             for (int m = 0; m < MT; ++m) xs[m] = load_scales(xsr, xs_at[m], G, a.KG);
             auto step = [&](auto Sc) {
                 constexpr int S = decltype(Sc)::value;
-                v8i xv[MT];
+                v8i xv[MT], small[FINE ? MT : 1];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     xv[m] = v8i{0, 0, 0, 0, 0, 0, 0, 0};
@@ -105,6 +105,10 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
                         const v4u q = load16(xr, x_at[m] != kOutOfRange && g1 < a.KG ? x_at[m] + 32 * g1 + 16 * (g & 1) : kOutOfRange);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) { xv[m][e] = (int)p[e]; xv[m][4 + e] = (int)q[e]; }
+                        if constexpr (FINE) {
+                            const v8i both = xv[m];
+                            split_bytes(both, xv[m], small[m]);
+                        }
                     } else {
                         const v4u p = load16(xr, x_at[m] != kOutOfRange && G + S < a.KG ? x_at[m] + 16 * (G + S) : kOutOfRange);
 #pragma unroll
@@ -115,7 +119,10 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
                 for (int f = 0; f < NF; ++f) {
                     const v8i wf = {(int)wv[f][S][0], (int)wv[f][S][1], (int)wv[f][S][2], (int)wv[f][S][3], 0, 0, 0, 0};
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[f][m] = product<XF, S>(wf, xv[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                    for (int m = 0; m < MT; ++m) {
+                        if constexpr (FINE) acc[f][m] = product<XF, S>(wf, small[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                        acc[f][m] = product<XF, S>(wf, xv[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                    }
                 }
             };
             step(std::integral_constant<int, 0>{});
@@ -182,15 +189,12 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     }
 }
 
-template <int XF>
-void launch_rows(const MoeArgs& a, bool glu, const dim3& grid) {
+template <int XF, bool GLU, bool FINE>
+void launch_rows(const MoeArgs& a, const dim3& grid) {
     const dim3 block(64 * kWaves);
-#define BYHIP_ROWS(MT)                                                                                      \
-    (glu ? launch("moe_rows", (moe_rows<XF, MT, 4, true>), grid, block, 0, a) : launch("moe_rows", (moe_rows<XF, MT, 4, false>), grid, block, 0, a))
-    if (a.unit_rows <= 16) BYHIP_ROWS(1);
-    else if (a.unit_rows <= 32) BYHIP_ROWS(2);
-    else BYHIP_ROWS(4);
-#undef BYHIP_ROWS
+    if (a.unit_rows <= 16) launch("moe_rows", (moe_rows<XF, 1, 4, GLU, FINE>), grid, block, 0, a);
+    else if (a.unit_rows <= 32) launch("moe_rows", (moe_rows<XF, 2, 4, GLU, FINE>), grid, block, 0, a);
+    else launch("moe_rows", (moe_rows<XF, 4, 4, GLU, FINE>), grid, block, 0, a);
     BYHIP_LAUNCHED("moe_rows");
 }
 
@@ -203,8 +207,10 @@ void launch_moe_rows(const MoeArgs& args, int x_format, bool glu, int max_units)
     const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;
     if (blocks >= 1ll << 31) fail("byhip: a product of %d units of %d strips", max_units, a.strips);
     const dim3 grid((unsigned)blocks);
-    if (x_format == BYHIP_MXFP8_KM) launch_rows<BYHIP_MXFP8_KM>(a, glu, grid);
-    else launch_rows<BYHIP_MXFP4_KM>(a, glu, grid);
+    const bool fine = moe_fine(x_format, a.y_dtype);
+    if (x_format == BYHIP_MXFP4_KM) glu ? launch_rows<BYHIP_MXFP4_KM, true, false>(a, grid) : launch_rows<BYHIP_MXFP4_KM, false, false>(a, grid);
+    else if (fine) glu ? launch_rows<BYHIP_MXFP8_KM, true, true>(a, grid) : launch_rows<BYHIP_MXFP8_KM, false, true>(a, grid);
+    else glu ? launch_rows<BYHIP_MXFP8_KM, true, false>(a, grid) : launch_rows<BYHIP_MXFP8_KM, false, false>(a, grid);
 }
 
 }  // namespace byhip

@@ -185,7 +185,7 @@ def check_product(hip, T, k, E, K, N, xf, yt, flags, seed=0, ids=None, pad=0):
         if at.size:
             a = order[at]
             out = a if scatter else at
-            want[out], slack[out] = expected(xv[a // k if gather else at], wv[e], N, K, glu, xf)
+            want[out], slack[out] = expected(xv[a // k if gather else at], wv[e], N, K, glu, xf, yt)
             live[out] = True
     if yt in (MX8, MX4):
         b = N if yt == MX8 else N // 2
@@ -318,6 +318,21 @@ def test_no_tokens(hip):
     assert np.all(z.read(np.float32, 64) == 7)
 
 
+@pytest.mark.parametrize("fill", [0, 1, 0x7F, 0xFF])
+def test_buffer_without_a_plan(hip, fill):
+    """A product with a buffer that no plan was made in writes rows of its own output or none, and reads its operands only."""
+    T, k, E, K, N = 9, 2, 4, 64, 32
+    up = hip.DeviceBuffer.from_array
+    buf = up(np.full(hip.moe_plan_bytes(T, k, E), fill, np.uint8))
+    p = hip.MoePlan(buf, T, k, E)
+    y = up(np.full(T * k * N + 64, 7, np.float32))
+    x, w = up(np.zeros(mx_size(T * k, K, MX8), np.uint8)), up(np.zeros(mx_size(E * N, K, MX4), np.uint8))
+    for flags in (0, GATHER, SCATTER | GATHER):
+        hip.moe_matmul(x, MX8, w, p, K, N, flags, y, N, F32)
+        got = y.read(np.float32)
+        assert np.all((got == 0) | (got == 7)) and np.all(got[T * k * N:] == 7)
+
+
 def test_quantized_rows_through_experts(hip):
     """Rows quantised on the device, routed, multiplied, brought back to 8 bits, multiplied again and summed: each step against 64 bits of what the
     step before left."""
@@ -347,8 +362,8 @@ def test_quantized_rows_through_experts(hip):
     out, oslack = np.zeros((T * k, D)), np.zeros((T * k, D))
     for e in range(E):
         at = np.arange(offsets[e], offsets[e + 1])
-        want[at], slack[at] = expected(xv[order[at] // k], wv1[e], F, D, True, MX8)
-        out[order[at]], oslack[order[at]] = expected(hv[at], wv2[e], D, F, False, MX8)
+        want[at], slack[at] = expected(xv[order[at] // k], wv1[e], F, D, True, MX8, MX8)
+        out[order[at]], oslack[order[at]] = expected(hv[at], wv2[e], D, F, False, MX8, F32)
     agree(h, want, slack, MX8, T * k, F, F)
     close(dn.read(np.float32).reshape(T * k, D), out, F32, oslack)
     terms = out.reshape(T, k, D) * w.read(np.float32).reshape(T, k, 1)
