@@ -35,6 +35,11 @@ MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts,
     return a;
 }
 
+void launch_product(const MoeArgs& a, int x_format, bool glu, int max_units) {
+    if (moe_tiles_take(a)) launch_moe_tiles(a, x_format, glu, max_units);
+    else launch_moe_rows(a, x_format, glu, max_units);
+}
+
 }  // namespace
 }  // namespace byhip
 
@@ -54,7 +59,7 @@ int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K,
         a.M = M; a.top_k = 1;
         a.unit_rows = moe_unit_rows(M, 1);
         note_device_write(y);
-        launch_moe_rows(a, x_format, glu, (M + a.unit_rows - 1) / a.unit_rows);
+        launch_product(a, x_format, glu, (M + a.unit_rows - 1) / a.unit_rows);
     });
 }
 
@@ -71,7 +76,7 @@ int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_
         a.top_k = p.top_k; a.gather = gather; a.scatter = (flags & BYHIP_MOE_SCATTER) != 0;
         a.unit_rows = p.unit_rows; a.experts = p.experts; a.rows = p.rows; a.max_units = p.max_units;
         note_device_write(y);
-        launch_moe_rows(a, x_format, glu, p.max_units);
+        launch_product(a, x_format, glu, p.max_units);
     });
 }
 

@@ -84,7 +84,7 @@ struct MoeUnit {
 // rows share one pass over the expert's matrix.
 inline int moe_unit_rows(long long rows, int experts) {
     const long long mean = (rows + experts - 1) / experts;
-    return mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
 }
 // The plan's buffer: offsets and order (the caller's to read), the number of units and the units, and what the plan's kernels
 // count in (one row of `experts` counts per block of assignments).
