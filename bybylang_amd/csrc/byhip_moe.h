@@ -28,26 +28,33 @@ inline bool moe_fine(int x_format, int y_dtype) { return x_format == BYHIP_MXFP8
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 
-// The unit and strip of block b: blocks go to the 8 XCDs in turn, and each XCD takes a run of tiles, so that the strips of an
-// expert (which share its rows) and the units of an expert (which share its matrix) meet in one L2. False: no work.
-__device__ __forceinline__ bool moe_tile(const MoeArgs& a, MoeUnit& u, int& strip) {
-    const int units = a.n_units ? min(*a.n_units, a.max_units) : (a.M + a.unit_rows - 1) / a.unit_rows;
-    const long long tiles = (long long)units * a.strips, per = (tiles + 7) / 8;
-    const long long at = blockIdx.x >> 3, t = (blockIdx.x & 7) * per + at;
-    if (at >= per || t >= tiles) return false;
-    const int i = (int)(t / a.strips);
-    strip = (int)(t % a.strips);
-    if (a.n_units) {
-        u = a.units[i];
-        // A buffer that no plan was made in names no rows (and no memory but its own).
-        if ((unsigned)u.expert >= (unsigned)a.experts || u.first < 0 || (unsigned)u.rows > (unsigned)a.unit_rows || u.first > a.rows - u.rows) return false;
-    } else {
-        u.expert = 0;
-        u.first = i * a.unit_rows;
-        u.rows = min(a.unit_rows, a.M - u.first);
+// A call's tiles, `strips` per unit: they are shared out to the 8 XCDs (to which blocks go in turn) in runs, so that the strips of an
+// expert, which share its rows, and the units of an expert, which share its matrix, meet in one L2.
+struct MoeTiles {
+    long long tiles, per;
+    __device__ __forceinline__ explicit MoeTiles(const MoeArgs& a) {
+        const int units = a.n_units ? min(*a.n_units, a.max_units) : (a.M + a.unit_rows - 1) / a.unit_rows;
+        tiles = (long long)units * a.strips;
+        per = (tiles + 7) / 8;
     }
-    return true;
-}
+    // The unit and strip of place `at` of this block's XCD. False: no work (or no rows: a buffer that no plan was made in names none, and
+    // no memory but its own).
+    __device__ __forceinline__ bool find(const MoeArgs& a, long long at, MoeUnit& u, int& strip) const {
+        const long long t = (blockIdx.x & 7) * per + at;
+        if (at >= per || t >= tiles) return false;
+        const int i = (int)((uint32_t)t / (uint32_t)a.strips);
+        strip = (int)((uint32_t)t % (uint32_t)a.strips);
+        if (a.n_units) {
+            u = a.units[i];
+            if ((unsigned)u.expert >= (unsigned)a.experts || u.first < 0 || (unsigned)u.rows > (unsigned)a.unit_rows || u.first > a.rows - u.rows) u.rows = u.expert = u.first = 0;
+        } else {
+            u.expert = 0;
+            u.first = i * a.unit_rows;
+            u.rows = min(a.unit_rows, a.M - u.first);
+        }
+        return true;
+    }
+};
 // Row of x, and of y, of the plan's row r. An order that is not the plan's stays inside the rows.
 __device__ __forceinline__ int moe_assignment(const MoeArgs& a, int r) { return (int)min((unsigned)a.order[r], (unsigned)a.rows - 1u); }
 __device__ __forceinline__ int moe_x_row(const MoeArgs& a, int r) { return a.gather ? moe_assignment(a, r) / a.top_k : r; }
@@ -68,8 +75,10 @@ __device__ __forceinline__ void split_bytes(const v8i& bytes, v8i& large, v8i& s
     }
 }
 
-// silu(g) u
-__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) u by the hardware's exp2 and reciprocal, within an ulp each: with the argument's rounding, about (3 + |g|) 2^-24 of the value.
+__device__ __forceinline__ float swiglu(float g, float u) {
+    return g * u * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
+}
 
 // Four neighbouring outputs n .. n + 3 of y's row.
 __device__ __forceinline__ void moe_store4(const MoeArgs& a, size_t row, int n, const float (&v)[4]) {

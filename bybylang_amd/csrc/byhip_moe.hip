@@ -23,7 +23,9 @@ MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts,
         a.ys = static_cast<uint8_t*>(y) + mx_values(y_rows, N, y_dtype);
     } else {
         check_rows(y, y_rows, N, y_stride, y_dtype, "product");
-        a.vec = aligned4(y, y_stride, y_dtype);
+        // 1: four values at a time, 2: 16 bytes at a time
+        const size_t bytes = dtype_bytes(y_dtype);
+        a.vec = !aligned4(y, y_stride, y_dtype) ? 0 : reinterpret_cast<uintptr_t>(y) % 16 == 0 && y_stride * bytes % 16 == 0 ? 2 : 1;
     }
     a.x = static_cast<const uint8_t*>(x);
     a.x_bytes = (uint32_t)mx_values(rows, K, x_format);

@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     __shared__ float4 part[kWaves][NF * MT][64];
     MoeUnit u;
     int strip;
-    if (!moe_tile(a, u, strip)) return;
+    if (!MoeTiles(a).find(a, blockIdx.x >> 3, u, strip)) return;
     constexpr bool eight = XF == BYHIP_MXFP8_KM;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const uint32_t kb = (uint32_t)a.K / 2, xb = eight ? (uint32_t)a.K : kb;

@@ -10,6 +10,8 @@
 // operands. One barrier per pair. The order of the loads inside a row's 128 (or 64) bytes is turned by the row so that no
 // cycle of the operand reads meets a bank twice: 16 lanes read one place of 16 rows, which lie 128 bytes apart (8 bits), two to all 64
 // banks, or 64 bytes apart (4 bits), four to all banks.
+#include <algorithm>
+
 #include "byhip_moe.h"
 
 namespace byhip {
@@ -54,45 +56,120 @@ __device__ __forceinline__ f16v product(v4u w, v8i x, f16v c, int sw, int sx) {
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide, x, c, 4, XF == BYHIP_MXFP8_KM ? 0 : 4, H, sw, H, sx);
 }
 
-template <int XF, bool GLU, bool FINE>
+// Halves of a wave's registers changed over: x becomes (x of the lower lanes, y of the lower lanes), y the same of the upper lanes.
+__device__ __forceinline__ void swap_halves(uint32_t& x, uint32_t& y) {
+    const auto v = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = v[0];
+    y = v[1];
+}
+
+// 32 outputs n .. n + 31 of a row, of which this lane holds 8 b + 4 lq .. + 3 (v[b]) and the lane 32 further on or back the rest: the
+// two change over so that each stores 16 neighbouring bytes (of 16-bit outputs and 8-bit values).
+template <int YT>
+__device__ __forceinline__ void write_block(const MoeArgs& a, bool there, size_t row, int n, int lq, float (&v)[4][4]) {
+    if constexpr (YT == BYHIP_MXFP8_KM || YT == BYHIP_MXFP4_KM) {
+        uint8_t* y = static_cast<uint8_t*>(a.y);
+        uint32_t mag = max(mag8(v[0], v[1]), mag8(v[2], v[3]));
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+        const uint32_t byte = mx_scale<YT>(mag);
+        uint32_t p[2], q[2];
+        mx_pack8<YT>(v[0], v[2], byte, p);
+        mx_pack8<YT>(v[1], v[3], byte, q);
+        swap_halves(p[0], q[0]);
+        if constexpr (YT == BYHIP_MXFP8_KM) swap_halves(p[1], q[1]);
+        if (!there) return;
+        if constexpr (YT == BYHIP_MXFP8_KM) *reinterpret_cast<uint4*>(y + row * a.N + n + 16 * lq) = make_uint4(p[0], p[1], q[0], q[1]);
+        else *reinterpret_cast<uint2*>(y + row * (a.N / 2) + n / 2 + 8 * lq) = make_uint2(p[0], q[0]);
+        if (lq == 0) a.ys[row * (a.N / 32) + n / 32] = (uint8_t)byte;
+    } else if (a.vec == 2 && n + 32 <= a.N) {
+        if constexpr (YT == BYHIP_F32) {
+            if (!there) return;
+            float4* y = reinterpret_cast<float4*>(static_cast<float*>(a.y) + row * a.y_stride + n + 4 * lq);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) y[2 * b] = make_float4(v[b][0], v[b][1], v[b][2], v[b][3]);
+        } else {
+            uint32_t w[4][2];
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    w[b][h] = YT == BYHIP_F16 ? h_bits((_Float16)v[b][2 * h]) | (uint32_t)h_bits((_Float16)v[b][2 * h + 1]) << 16 : f32x2_to_bf16x2_bits(v[b][2 * h], v[b][2 * h + 1]);
+#pragma unroll
+            for (int b = 0; b < 4; b += 2)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) swap_halves(w[b][h], w[b + 1][h]);
+            if (!there) return;
+            uint16_t* y = static_cast<uint16_t*>(a.y) + row * a.y_stride + n + 8 * lq;
+#pragma unroll
+            for (int b = 0; b < 4; b += 2) *reinterpret_cast<uint4*>(y + 8 * b) = make_uint4(w[b][0], w[b][1], w[b + 1][0], w[b + 1][1]);
+        }
+    } else if (there) {
+        for (int b = 0; b < 4; ++b) {
+            float four[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) four[e] = b == 0 ? v[0][e] : b == 1 ? v[1][e] : b == 2 ? v[2][e] : v[3][e];
+            const size_t at = row * a.y_stride + n + 8 * b + 4 * lq;
+            for (int e = 0; e < 4; ++e)
+                if (n + 8 * b + 4 * lq + e < a.N) store_y<YT>(a.y, at + e, e == 0 ? four[0] : e == 1 ? four[1] : e == 2 ? four[2] : four[3]);
+        }
+    }
+}
+
+template <int XF, bool GLU, int YT>
 __global__ __launch_bounds__(256) void moe_tiles(MoeArgs a) {
     typedef Lds<XF> L;
-    constexpr bool eight = L::eight;
+    constexpr bool eight = L::eight, FINE = eight && YT == BYHIP_F32;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::bytes];
+    const MoeTiles tiles(a);
+    const int round = gridDim.x >> 3;
+    int at = blockIdx.x >> 3;
     MoeUnit u;
     int strip;
-    if (!moe_tile(a, u, strip)) return;
+    if (!tiles.find(a, at, u, strip)) return;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wid >> 1, wt = wid & 1, lq = lane >> 5, lc = lane & 31;
     const uint32_t kb = (uint32_t)a.K / 2, xb = eight ? (uint32_t)a.K : kb, KG = (uint32_t)a.KG;
-    const rsrc_t wr = make_rsrc(a.w + (size_t)u.expert * a.R * kb, (uint32_t)a.R * kb);
-    const rsrc_t wsr = make_rsrc(a.ws + (size_t)u.expert * a.R * KG, (uint32_t)a.R * KG);
     const rsrc_t xr = make_rsrc(a.x, a.x_bytes), xsr = make_rsrc(a.xs, a.xs_bytes);
-
-    // The matrix's row of the tile's row R: a wave's 128 are 64 gates and the ups of the same outputs.
-    const int n0 = strip * (GLU ? kTileW / 2 : kTileW);
-    auto matrix_row = [&](int R) {
-        if constexpr (!GLU) return n0 + R;
-        return ((R >> 6) & 1) * a.N + n0 + 64 * (R >> 7) + (R & 63);
-    };
-    // Offsets of this lane's loads: rows of W 64 wid + 8 q + .., rows of X 32 wid + 8 q + ..; a row past the matrix's or the unit's
-    // reads zeros.
     const int drow = lc >> 2;
-    uint32_t wo[8], xo[4];
+
+    // A tile's rows of x for this lane's loads: rows of X 32 wid + 8 q + .. for its values, row 64 wid + lane for its scales; -1 past the
+    // unit's. Asked for a tile ahead.
+    auto ask_rows = [&](const MoeUnit& u, int (&rows)[5]) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const int R = 64 * wid + 8 * q + drow, n = matrix_row(R);
-        wo[q] = n < a.R ? (uint32_t)n * kb + 16u * ((lane & 3) ^ turn64(R & 15)) + 64u * lq : kNoRow;
-    }
+        for (int q = 0; q < 5; ++q) {
+            const int R = q < 4 ? 32 * wid + 8 * q + (eight ? lane >> 3 : drow) : 64 * wid + lane;
+            rows[q] = R >= u.rows ? -1 : a.gather ? a.order[u.first + R] : u.first + R;
+        }
+    };
+    // Where a tile's operands are: offsets of this lane's loads, rows of W 64 wid + 8 q + ..; a row past the matrix's or the unit's reads
+    // zeros.
+    rsrc_t wr, wsr;
+    uint32_t wo[8], xo[4], wso, xso;
+    auto locate = [&](const MoeUnit& u, int strip, const int (&rows)[5]) {
+        wr = make_rsrc(a.w + (size_t)u.expert * a.R * kb, (uint32_t)a.R * kb);
+        wsr = make_rsrc(a.ws + (size_t)u.expert * a.R * KG, (uint32_t)a.R * KG);
+        // The matrix's row of the tile's row R: a wave's 128 are 64 gates and the ups of the same outputs.
+        const int n0 = strip * (GLU ? kTileW / 2 : kTileW);
+        auto matrix_row = [&](int R) {
+            if constexpr (!GLU) return n0 + R;
+            return ((R >> 6) & 1) * a.N + n0 + 64 * (R >> 7) + (R & 63);
+        };
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int R = 32 * wid + 8 * q + (eight ? lane >> 3 : drow);
-        const uint32_t c = eight ? 16u * ((lane & 7) ^ turn128(R & 15)) : 16u * ((lane & 3) ^ turn64(R & 15)) + 64u * lq;
-        xo[q] = R < u.rows ? (uint32_t)moe_x_row(a, u.first + R) * xb + c : kNoRow;
-    }
-    const int swn = matrix_row(64 * wid + lane), sxr = 64 * wid + lane;
-    const uint32_t wso = swn < a.R ? (uint32_t)swn * KG : kNoRow;
-    const uint32_t xso = wid < 2 && sxr < u.rows ? (uint32_t)moe_x_row(a, u.first + sxr) * KG : kNoRow;
+        for (int q = 0; q < 8; ++q) {
+            const int R = 64 * wid + 8 * q + drow, n = matrix_row(R);
+            wo[q] = n < a.R ? (uint32_t)n * kb + 16u * ((lane & 3) ^ turn64(R & 15)) + 64u * lq : kNoRow;
+        }
+        auto x_row = [&](int id) { return a.gather ? min((unsigned)id, (unsigned)a.rows - 1u) / (unsigned)a.top_k : (unsigned)id; };
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int R = 32 * wid + 8 * q + (eight ? lane >> 3 : drow);
+            const uint32_t c = eight ? 16u * ((lane & 7) ^ turn128(R & 15)) : 16u * ((lane & 3) ^ turn64(R & 15)) + 64u * lq;
+            xo[q] = R < u.rows ? x_row(rows[q]) * xb + c : kNoRow;
+        }
+        const int n = matrix_row(64 * wid + lane);
+        wso = n < a.R ? (uint32_t)n * KG : kNoRow;
+        xso = wid < 2 && 64 * wid + lane < u.rows ? x_row(rows[4]) * KG : kNoRow;
+    };
 
     const int nsteps = a.K / kStep;
     // Loads past the last step read it again, or bytes that no step uses.
@@ -144,6 +221,23 @@ __global__ __launch_bounds__(256) void moe_tiles(MoeArgs a) {
         else o.sx[k - 4] = *reinterpret_cast<const uint16_t*>(sbuf + 16 * (kTileW + 64 * wt + 32 * (k - 4) + lc) + 2 * lq + 4 * T);
     };
 
+    int rows[5];
+    ask_rows(u, rows);
+    locate(u, strip, rows);
+    auto region_at = [&](int s) { return lds + ((s >> 1) & 1) * L::region; };
+    auto sbuf_at = [&](int s) { return lds + L::scale_base + ((s >> 2) & 1) * L::scales; };
+    load_scales(0, sbuf_at(0));
+    load_pair(0, region_at(0));
+    load_pair(2, region_at(2));
+    bool more = true;
+    while (more) {
+    // The next tile's unit and rows are asked for now, and its first loads go out before this one's results are written.
+    MoeUnit u1 = u;
+    int strip1 = 0;
+    at += round;
+    more = tiles.find(a, at, u1, strip1);
+    if (more) ask_rows(u1, rows);
+
     f16v acc[4][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -154,25 +248,19 @@ __global__ __launch_bounds__(256) void moe_tiles(MoeArgs a) {
             asm volatile("" : "+v"(acc[i][j]));  // zeros in registers, not a constant addend (byhip_moe_rows.hip)
         }
 
-    auto region_at = [&](int s) { return lds + ((s >> 1) & 1) * L::region; };
-    auto sbuf_at = [&](int s) { return lds + L::scale_base + ((s >> 2) & 1) * L::scales; };
-
     // At the start of step s `cur` holds its operands, and step s + 1's data and scales have landed. Step s reads them into `nxt`. An odd
     // step issues the loads of the pair s + 3, s + 4 into the region of the pair s - 1, s, whose last reads (for step s) were
     // in step s - 1, before the barrier that ended it; at s % 4 = 1 also the scales of period (s + 3) / 4. An even step ends with a
     // wait for all loads and the barrier. The pointers of a step are distinct, and __restrict__ says so: its reads need not wait
     // for its loads.
     Operands<XF> o0, o1;
-    [&](uint8_t* __restrict__ sc, uint8_t* __restrict__ r0, uint8_t* r1) {
-        load_scales(0, sc);
-        load_pair(0, r0);
-        load_pair(2, r1);
-        stage_barrier<kLoads>();
+    [&](const uint8_t* __restrict__ sc, const uint8_t* __restrict__ r0) {
+        stage_barrier<kLoads>();  // the second pair, or what was written after it, may be on its way
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) read_one(o0, r0, 0, k);
 #pragma unroll
         for (int k = 0; k < 6; ++k) read_scale(o0, sc, 0, k);
-    }(sbuf_at(0), region_at(0), region_at(2));
+    }(sbuf_at(0), region_at(0));
 
     auto step = [&](auto Pc, int s, Operands<XF>& cur, Operands<XF>& nxt, uint8_t* __restrict__ dreg, uint8_t* __restrict__ sdst,
                     const uint8_t* __restrict__ src, const uint8_t* __restrict__ ssrc) {
@@ -219,9 +307,19 @@ __global__ __launch_bounds__(256) void moe_tiles(MoeArgs a) {
     if (s + 1 < nsteps) BYHIP_STEP(1, s + 1, o1, o0);
     if (s + 2 < nsteps) BYHIP_STEP(2, s + 2, o0, o1);
 #undef BYHIP_STEP
-    wait_vmcnt<0>();  // no load may land in the LDS of the block that follows
+    // Every wave has read what its products need (the barrier of the last even step), and no load of this tile is left to land
+    // on the next one's.
+    wait_vmcnt<0>();
+    if (more) {
+        locate(u1, strip1, rows);
+        load_scales(0, sbuf_at(0));
+        load_pair(0, region_at(0));
+        load_pair(2, region_at(2));
+    }
+    __builtin_amdgcn_sched_barrier(0);
 
     // Lane (c, g) holds row c of block j of x; register r is matrix row 8 (r / 4) + 4 g + r % 4 of block i.
+    const int n0 = strip * (GLU ? kTileW / 2 : kTileW);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int t = 64 * wt + 32 * j + lc;
@@ -237,25 +335,28 @@ __global__ __launch_bounds__(256) void moe_tiles(MoeArgs a) {
                 for (int e = 0; e < 4; ++e)
                     v[b][e] = GLU ? swiglu(acc[i][j][4 * b + e], acc[GLU ? 2 + i : i][j][4 * b + e]) : acc[i][j][4 * b + e];
             const int n = n0 + (GLU ? 64 : 128) * wn + 32 * i;
-            if (is_mx_out(a.y_dtype)) {
-                uint32_t mag = max(mag8(v[0], v[1]), mag8(v[2], v[3]));
-                mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
-                if (there && n < a.N) {
-                    store_group(a, row, n / 32, 4 * lq, lq == 0, mag, v[0], v[2]);
-                    store_group(a, row, n / 32, 8 + 4 * lq, false, mag, v[1], v[3]);
-                }
-            } else if (there) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) moe_store4(a, row, n + 8 * b + 4 * lq, v[b]);
-            }
+            write_block<YT>(a, there && n < a.N, row, n, lq, v);
         }
     }
+    u = u1;
+    strip = strip1;
+    }  // tiles
 }
 
-template <int XF, bool GLU, bool FINE>
+template <int XF, bool GLU, int YT>
 void launch_tiles(const MoeArgs& a, const dim3& grid) {
-    launch("moe_tiles", (moe_tiles<XF, GLU, FINE>), grid, dim3(256), 0, a);
+    launch("moe_tiles", (moe_tiles<XF, GLU, YT>), grid, dim3(256), 0, a);
     BYHIP_LAUNCHED("moe_tiles");
+}
+template <int XF, bool GLU>
+void launch_tiles_y(const MoeArgs& a, const dim3& grid) {
+    switch (a.y_dtype) {
+    case BYHIP_F32: launch_tiles<XF, GLU, BYHIP_F32>(a, grid); break;
+    case BYHIP_F16: launch_tiles<XF, GLU, BYHIP_F16>(a, grid); break;
+    case BYHIP_BF16: launch_tiles<XF, GLU, BYHIP_BF16>(a, grid); break;
+    case BYHIP_MXFP8_KM: launch_tiles<XF, GLU, BYHIP_MXFP8_KM>(a, grid); break;
+    default: launch_tiles<XF, GLU, BYHIP_MXFP4_KM>(a, grid); break;
+    }
 }
 
 }  // namespace
@@ -269,11 +370,10 @@ void launch_moe_tiles(const MoeArgs& args, int x_format, bool glu, int max_units
     a.strips = (a.N + wide - 1) / wide;
     const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;
     if (blocks >= 1ll << 31) fail("byhip: a product of %d units of %d strips", max_units, a.strips);
-    const dim3 grid((unsigned)blocks);
-    const bool fine = moe_fine(x_format, a.y_dtype);
-    if (x_format == BYHIP_MXFP4_KM) glu ? launch_tiles<BYHIP_MXFP4_KM, true, false>(a, grid) : launch_tiles<BYHIP_MXFP4_KM, false, false>(a, grid);
-    else if (fine) glu ? launch_tiles<BYHIP_MXFP8_KM, true, true>(a, grid) : launch_tiles<BYHIP_MXFP8_KM, false, true>(a, grid);
-    else glu ? launch_tiles<BYHIP_MXFP8_KM, true, false>(a, grid) : launch_tiles<BYHIP_MXFP8_KM, false, false>(a, grid);
+    // One block per CU (its LDS holds one), each going through its XCD's tiles.
+    const dim3 grid((unsigned)std::min<long long>(blocks, compute_units() / 8 * 8));
+    if (x_format == BYHIP_MXFP4_KM) glu ? launch_tiles_y<BYHIP_MXFP4_KM, true>(a, grid) : launch_tiles_y<BYHIP_MXFP4_KM, false>(a, grid);
+    else glu ? launch_tiles_y<BYHIP_MXFP8_KM, true>(a, grid) : launch_tiles_y<BYHIP_MXFP8_KM, false>(a, grid);
 }
 
 }  // namespace byhip
