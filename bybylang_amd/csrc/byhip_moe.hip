@@ -77,6 +77,7 @@ int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_
         a.order = p.order; a.n_units = p.n_units; a.units = p.units;
         a.top_k = p.top_k; a.gather = gather; a.scatter = (flags & BYHIP_MOE_SCATTER) != 0;
         a.unit_rows = p.unit_rows; a.experts = p.experts; a.rows = p.rows; a.max_units = p.max_units;
+        a.per_token = (uint32_t)(((1ull << 32) + p.top_k - 1) / p.top_k);
         note_device_write(y);
         launch_product(a, x_format, glu, p.max_units);
     });

@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256) void moe_combine(CombineArgs a) {
 
 MoePlan moe_layout(const byhip_moe_plan* p) {
     if (!p) fail("byhip: null plan");
-    if (p->tokens < 0 || p->experts < 1 || p->experts > kMaxExperts || p->top_k < 1 || p->top_k > p->experts ||
+    if (p->tokens < 0 || p->experts < 1 || p->experts > kMaxExperts || p->top_k < 1 || p->top_k > p->experts || p->top_k > 256 ||
         (long long)p->tokens * p->top_k >= 1 << 24)
         fail("byhip: a plan of %d tokens, %d of %d experts each", p->tokens, p->top_k, p->experts);
     MoePlan m{};

@@ -467,7 +467,7 @@ typedef struct byhip_moe_plan {
     void* plan;
 } byhip_moe_plan;
 
-/* Bytes of a plan's buffer; 0 where the sizes are out of range (tokens >= 0, 1 <= top_k <= experts <= 1024,
+/* Bytes of a plan's buffer; 0 where the sizes are out of range (tokens >= 0, 1 <= top_k <= experts <= 1024, top_k <= 256,
  * tokens * top_k < 2^24). Needs no device. */
 unsigned long long byhip_moe_plan_bytes(int tokens, int top_k, int experts);
 
