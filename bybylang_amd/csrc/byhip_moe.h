@@ -133,8 +133,7 @@ __device__ __forceinline__ void store_group(const MoeArgs& a, size_t row, int G,
 }
 
 void launch_moe_rows(const MoeArgs& a, int x_format, bool glu, int max_units);
-// Units of 128 rows, K a multiple of 128.
-bool moe_tiles_take(const MoeArgs& a);
+// Units of kTileRows, K a multiple of 128.
 void launch_moe_tiles(const MoeArgs& a, int x_format, bool glu, int max_units);
 
 }  // namespace byhip

@@ -1,4 +1,5 @@
 // byhip_moe.hip - entry points of the products of microscaled rows: with one matrix, and with each row's expert's.
+#include "byhip_gemm.h"
 #include "byhip_moe.h"
 
 namespace byhip {
@@ -37,9 +38,14 @@ MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts,
     return a;
 }
 
-void launch_product(const MoeArgs& a, int x_format, bool glu, int max_units) {
-    if (moe_tiles_take(a)) launch_moe_tiles(a, x_format, glu, max_units);
-    else launch_moe_rows(a, x_format, glu, max_units);
+// Whether tiles take a product: `units` is what can be told on the host of how many of 128 rows it has. They do where their blocks
+// fill the card, from a few rows per expert on (128 experts, K = 2048, 768 outputs of gates and ups, 4 / 6 / 8 / 12 rows each: 41 / 49 / 50
+// / 50 us, moe_rows 36 / 45 / 50 / 62), and with fewer blocks where moe_rows would read the rows again and again (one matrix of 4096 x
+// 4096, 256 / 384 / 512 rows: 32 us each, 32 / 48 / 64 blocks, moe_rows 21 / 32 / 36; 256 rows and 14336 outputs, 112 blocks: 34 for 62).
+bool tiles_take(const MoeArgs& a, bool glu, long long rows, int units, int experts) {
+    const int wide = glu ? 128 : 256;
+    const long long blocks = (long long)units * ((a.N + wide - 1) / wide);
+    return a.K % 128 == 0 && ((blocks >= 256 && rows >= 8ll * experts) || (blocks >= 48 && rows >= 64ll * experts));
 }
 
 }  // namespace
@@ -58,10 +64,21 @@ int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K,
         const bool glu = flags & BYHIP_MOE_SWIGLU;
         MoeArgs a = product_args(x, x_format, w, 1, M, M, K, N, glu, y, y_stride, y_dtype);
         if (M == 0) return;
-        a.M = M; a.top_k = 1;
-        a.unit_rows = moe_unit_rows(M, 1);
         note_device_write(y);
-        launch_product(a, x_format, glu, (M + a.unit_rows - 1) / a.unit_rows);
+        // Rows in 4 bits as byhip_mxfp4_gemm takes them.
+        if (x_format == BYHIP_MXFP4_KM && !glu && !is_mx(y_dtype) && K % 128 == 0 && y_stride == (size_t)N && M > 64) {
+            launch_mxfp4(a.x, a.xs, a.w, a.ws, y, y_dtype, M, K, N);
+            return;
+        }
+        a.M = M; a.top_k = 1;
+        const int tiles = (M + kTileRows - 1) / kTileRows;
+        if (tiles_take(a, glu, M, tiles, 1)) {
+            a.unit_rows = kTileRows;
+            launch_moe_tiles(a, x_format, glu, tiles);
+        } else {
+            a.unit_rows = moe_unit_rows(M, 1);
+            launch_moe_rows(a, x_format, glu, (M + a.unit_rows - 1) / a.unit_rows);
+        }
     });
 }
 
@@ -74,12 +91,20 @@ int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_
         const bool glu = flags & BYHIP_MOE_SWIGLU, gather = flags & BYHIP_MOE_GATHER;
         MoeArgs a = product_args(x, x_format, w, p.experts, gather ? p.tokens : p.rows, p.rows, K, N, glu, y, y_stride, y_dtype);
         if (p.rows == 0) return;
-        a.order = p.order; a.n_units = p.n_units; a.units = p.units;
+        a.order = p.order;
         a.top_k = p.top_k; a.gather = gather; a.scatter = (flags & BYHIP_MOE_SCATTER) != 0;
-        a.unit_rows = p.unit_rows; a.experts = p.experts; a.rows = p.rows; a.max_units = p.max_units;
+        a.experts = p.experts; a.rows = p.rows;
         a.per_token = (uint32_t)(((1ull << 32) + p.top_k - 1) / p.top_k);
         note_device_write(y);
-        launch_product(a, x_format, glu, p.max_units);
+        if (tiles_take(a, glu, p.rows, p.max_tiles, p.experts)) {
+            a.n_units = p.n_units + 1; a.units = p.tiles; a.max_units = p.max_tiles;
+            a.unit_rows = kTileRows;
+            launch_moe_tiles(a, x_format, glu, p.max_tiles);
+        } else {
+            a.n_units = p.n_units; a.units = p.units; a.max_units = p.max_units;
+            a.unit_rows = p.unit_rows;
+            launch_moe_rows(a, x_format, glu, p.max_units);
+        }
     });
 }
 

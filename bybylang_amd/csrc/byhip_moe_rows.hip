@@ -20,6 +20,7 @@ namespace byhip {
 namespace {
 
 constexpr int kWaves = 4;
+
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ v4u load16(rsrc_t r, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
@@ -167,12 +168,12 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
                     moe_store4(a, row, n0 + 16 + 4 * g, h[1]);
                 }
             }
-        } else if (is_mx_out(a.y_dtype)) {
-            for (int p = w; p < MT * NF / 2; p += kWaves) {
-                const int m = p / (NF / 2), q = p % (NF / 2), i = m0 + 16 * m + c;
+        } else if (NF > 1 && is_mx_out(a.y_dtype)) {
+            for (int p = w; p < MT * (NF / 2); p += kWaves) {
+                const int m = p / (NF > 1 ? NF / 2 : 1), q = p % (NF > 1 ? NF / 2 : 1), i = m0 + 16 * m + c;
                 float h[2][4];
                 whole(2 * q, m, h[0]);
-                whole(2 * q + 1, m, h[1]);
+                whole(NF > 1 ? 2 * q + 1 : 0, m, h[1]);
                 uint32_t mag = mag8(h[0], h[1]);
                 mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
                 mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
@@ -189,28 +190,46 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     }
 }
 
-template <int XF, bool GLU, bool FINE>
-void launch_rows(const MoeArgs& a, const dim3& grid) {
-    const dim3 block(64 * kWaves);
-    if (a.unit_rows <= 16) launch("moe_rows", (moe_rows<XF, 1, 4, GLU, FINE>), grid, block, 0, a);
-    else if (a.unit_rows <= 32) launch("moe_rows", (moe_rows<XF, 2, 4, GLU, FINE>), grid, block, 0, a);
-    else launch("moe_rows", (moe_rows<XF, 4, 4, GLU, FINE>), grid, block, 0, a);
+template <int XF, int MT, int NF, bool GLU, bool FINE>
+void launch_rows_as(MoeArgs a, int max_units) {
+    const int wide = GLU ? 32 : 16 * NF;
+    a.strips = (a.N + wide - 1) / wide;
+    const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;
+    if (blocks >= 1ll << 31) fail("byhip: a product of %d units of %d strips", max_units, a.strips);
+    launch("moe_rows", (moe_rows<XF, MT, NF, GLU, FINE>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, a);
     BYHIP_LAUNCHED("moe_rows");
+}
+
+// Strips of 64, 32 or 16 outputs: the widest that gives most CUs a block, for rows are read once per strip (16 rows, K = 4096, N = 4096: 64 strips of
+// 64 9.7 us, 128 of 32 7.4, 256 of 16 5.8; N = 14336: 224 of 64 11.4 us, 448 of 32 12.9). Gates and ups have 32 each. Eight waves per block took as long where
+// one unit's strips are all there is (9.8 us for 10.5 at N = 14336, 9.6 for 9.7), longer elsewhere (33 us for 41, 48 tokens, 128 experts).
+template <int XF, int MT, bool GLU, bool FINE>
+void launch_rows_n(const MoeArgs& a, int max_units) {
+    if constexpr (!GLU) {
+        const long long strips = (a.N + 15) / 16, room = 200;
+        if (strips / 4 * max_units < room) {
+            if (strips / 2 * max_units < room && !is_mx(a.y_dtype)) launch_rows_as<XF, MT, 1, GLU, FINE>(a, max_units);
+            else launch_rows_as<XF, MT, 2, GLU, FINE>(a, max_units);
+            return;
+        }
+    }
+    launch_rows_as<XF, MT, 4, GLU, FINE>(a, max_units);
+}
+
+template <int XF, bool GLU, bool FINE>
+void launch_rows(const MoeArgs& a, int max_units) {
+    if (a.unit_rows <= 16) launch_rows_n<XF, 1, GLU, FINE>(a, max_units);
+    else if (a.unit_rows <= 32) launch_rows_n<XF, 2, GLU, FINE>(a, max_units);
+    else launch_rows_n<XF, 4, GLU, FINE>(a, max_units);
 }
 
 }  // namespace
 
-void launch_moe_rows(const MoeArgs& args, int x_format, bool glu, int max_units) {
-    MoeArgs a = args;
-    const int wide = glu ? 32 : 64;
-    a.strips = (a.N + wide - 1) / wide;
-    const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;
-    if (blocks >= 1ll << 31) fail("byhip: a product of %d units of %d strips", max_units, a.strips);
-    const dim3 grid((unsigned)blocks);
+void launch_moe_rows(const MoeArgs& a, int x_format, bool glu, int max_units) {
     const bool fine = moe_fine(x_format, a.y_dtype);
-    if (x_format == BYHIP_MXFP4_KM) glu ? launch_rows<BYHIP_MXFP4_KM, true, false>(a, grid) : launch_rows<BYHIP_MXFP4_KM, false, false>(a, grid);
-    else if (fine) glu ? launch_rows<BYHIP_MXFP8_KM, true, true>(a, grid) : launch_rows<BYHIP_MXFP8_KM, false, true>(a, grid);
-    else glu ? launch_rows<BYHIP_MXFP8_KM, true, false>(a, grid) : launch_rows<BYHIP_MXFP8_KM, false, false>(a, grid);
+    if (x_format == BYHIP_MXFP4_KM) glu ? launch_rows<BYHIP_MXFP4_KM, true, false>(a, max_units) : launch_rows<BYHIP_MXFP4_KM, false, false>(a, max_units);
+    else if (fine) glu ? launch_rows<BYHIP_MXFP8_KM, true, true>(a, max_units) : launch_rows<BYHIP_MXFP8_KM, false, true>(a, max_units);
+    else glu ? launch_rows<BYHIP_MXFP8_KM, true, false>(a, max_units) : launch_rows<BYHIP_MXFP8_KM, false, false>(a, max_units);
 }
 
 }  // namespace byhip

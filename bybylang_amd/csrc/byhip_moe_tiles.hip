@@ -19,7 +19,7 @@
 namespace byhip {
 namespace {
 
-constexpr int kStep = 128, kTileW = 256, kTileX = 128;
+constexpr int kStep = 128, kTileW = 256, kTileX = kTileRows;
 constexpr uint32_t kNoRow = 0x80000000u;  // past every range here (below 2 GiB), also with a step's offset added
 
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
@@ -267,11 +267,9 @@ void launch_tiles_y(const MoeArgs& a, const dim3& grid) {
 
 }  // namespace
 
-bool moe_tiles_take(const MoeArgs& a) { return a.unit_rows == kTileX && a.K % kStep == 0; }
-
 void launch_moe_tiles(const MoeArgs& args, int x_format, bool glu, int max_units) {
     MoeArgs a = args;
-    if (!moe_tiles_take(a)) fail("byhip: internal: units of %d rows, %d values", a.unit_rows, a.K);
+    if (a.unit_rows != kTileX || a.K % kStep) fail("byhip: internal: units of %d rows, %d values", a.unit_rows, a.K);
     const int wide = glu ? kTileW / 2 : kTileW;
     a.strips = (a.N + wide - 1) / wide;
     const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;

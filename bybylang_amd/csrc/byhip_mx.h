@@ -80,21 +80,25 @@ constexpr int kMaxExperts = 1024;
 struct MoeUnit {
     int expert, first, rows, pad;
 };
-// Rows of a unit. Plan and product choose it by the mean rows per expert, so that most experts fill one unit: a unit's
-// rows share one pass over the expert's matrix.
+// Rows of a unit of moe_rows, by the mean rows per expert, so that most experts fill one: a unit's rows share one pass over the expert's
+// matrix, but 64 rows' own loads cost more than a second pass over it from the cache (64 / 128 / 256 rows, K = N = 4096: units of 32 12.4 / 15.3 /
+// 24.3 us, of 64 16.7 / 17.5 / 22.0). moe_tiles' units have kTileRows.
 inline int moe_unit_rows(long long rows, int experts) {
     const long long mean = (rows + experts - 1) / experts;
-    return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+    return mean <= 16 ? 16 : mean <= 128 ? 32 : 64;
 }
-// The plan's buffer: offsets and order (the caller's to read), the number of units and the units, and what the plan's kernels
-// count in (one row of `experts` counts per block of assignments).
+constexpr int kTileRows = 128;
+// Units at most: an expert leaves one that is not full.
+inline int moe_max_units(int rows, int experts, int unit) { return rows / unit + (rows < experts ? rows : experts); }
+// The plan's buffer: offsets and order (the caller's to read), the numbers of units of both kinds and the units, and what the plan's
+// kernels count in (one row of `experts` counts per block of assignments).
 struct MoePlan {
-    int tokens, top_k, experts, rows, unit_rows, max_units, blocks;
-    int *offsets, *order, *n_units, *counts;
-    MoeUnit* units;
+    int tokens, top_k, experts, rows, unit_rows, max_units, max_tiles, blocks;
+    int *offsets, *order, *n_units, *counts;  // n_units: of units, of tiles
+    MoeUnit *units, *tiles;
     size_t bytes;
 };
-constexpr int kPlanBlock = 4096;  // assignments per block of the plan's kernels
+constexpr int kPlanBlock = 1024;  // assignments per block of the plan's kernels
 MoePlan moe_layout(const byhip_moe_plan* p);  // sizes checked (fail), the buffer not
 MoePlan moe_plan_args(const byhip_moe_plan* p);
 

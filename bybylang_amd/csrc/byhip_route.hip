@@ -8,6 +8,8 @@
 //
 // The plan is a stable counting sort. A wave takes 64 assignments at a time and finds each one's rank among those of the same
 // expert from ballots over the id's bits, so no atomic's order has a say in the result.
+#include <type_traits>
+
 #include "byhip_mx.h"
 
 namespace byhip {
@@ -37,15 +39,26 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-    return v;
+// The value that order_key made a key of (NaN: minus infinity).
+__device__ __forceinline__ float key_value(uint32_t k) {
+    if (k <= 1u) return -INFINITY;
+    return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
-__device__ __forceinline__ float wave_maxf(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+
+// The largest of the lanes' values, all in DPP (a shuffle through LDS would cost ten times the latency).
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    auto step = [&](auto ctrl, auto mask) { v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(mask)::value, 0xF, false)); };
+    typedef std::integral_constant<int, 0xF> All;
+    step(std::integral_constant<int, 0xB1>{}, All{});   // quad_perm [1,0,3,2]
+    step(std::integral_constant<int, 0x4E>{}, All{});   // quad_perm [2,3,0,1]
+    step(std::integral_constant<int, 0x141>{}, All{});  // row_half_mirror
+    step(std::integral_constant<int, 0x140>{}, All{});  // row_mirror
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15 into rows 1 and 3
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31 into rows 2 and 3
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ float lane_sum(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_sum_lane63(v)), 63));
 }
 __device__ __forceinline__ double wave_sumd(double v) {
 #pragma unroll
@@ -82,11 +95,14 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
     const bool soft = a.score == BYHIP_MOE_SOFTMAX;
     auto lift = [&](float v) { return v == top ? 0.0f : v - top; };
     if (soft) {
-        top = -INFINITY;
+        uint32_t most = 0;
         bool nan = false;
 #pragma unroll
-        for (int i = 0; i < V; ++i) { top = fmaxf(top, x[i]); nan = nan || x[i] != x[i]; }
-        top = wave_maxf(top);
+        for (int i = 0; i < V; ++i) {
+            most = max(most, order_key(x[i]));
+            nan = nan || x[i] != x[i];
+        }
+        top = key_value(wave_max(most));
         float s = 0.0f;
         double sd = 0.0;
 #pragma unroll
@@ -96,7 +112,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
             else s += expf(lift(x[i]));
         }
         if constexpr (WIDE) { sum_d = wave_sumd(sd); sum = (float)sum_d; }
-        else sum = wave_sum(s);
+        else sum = lane_sum(s);
         if (top == -INFINITY && !__any(nan)) { sum = INFINITY; sum_d = (double)INFINITY; }
     }
     auto score_f = [&](float v) { return soft ? expf(lift(v)) / sum : 1.0f / (1.0f + expf(-v)); };
@@ -221,7 +237,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
         }
     }
     if (a.renorm) {
-        total = wave_sum(total);
+        total = lane_sum(total);
         const float f = total == 0.0f ? 0.0f : a.scale / total;
         if (a.k <= 64) {
             if (lane < a.k) a.weights[(size_t)t * a.k + lane] = total == 0.0f ? 0.0f : mine * f;
@@ -315,17 +331,21 @@ __device__ __forceinline__ int block_prefix(int v, int* part, int& total) {
 // Offsets and units from expert e's count (thread e's; 0 past E), and where e starts.
 __device__ __forceinline__ int write_units(const MoePlan& p, int count, int* part) {
     const int e = threadIdx.x;
-    int total, units;
+    int total, units, tiles;
     const int at = block_prefix(count, part, total);
     const int first = block_prefix((count + p.unit_rows - 1) / p.unit_rows, part, units);
+    const int first_tile = block_prefix((count + kTileRows - 1) / kTileRows, part, tiles);
     if (e < p.experts) {
         p.offsets[e] = at;
         for (int u = 0, r = 0; r < count; ++u, r += p.unit_rows)
             p.units[first + u] = MoeUnit{e, at + r, min(p.unit_rows, count - r), 0};
+        for (int u = 0, r = 0; r < count; ++u, r += kTileRows)
+            p.tiles[first_tile + u] = MoeUnit{e, at + r, min(kTileRows, count - r), 0};
     }
     if (e == 0) {
         p.offsets[p.experts] = total;
-        *p.n_units = units;
+        p.n_units[0] = units;
+        p.n_units[1] = tiles;
     }
     return at;
 }
@@ -361,7 +381,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_one(MoePlan p, const in
     plan_block(p, ids, counts, part);
 }
 
-// Many assignments: counts per block of them, the sums over the blocks, then the places.
+// Many assignments: counts per block of them, then the places; every block of the second forms the sums it needs from all blocks' counts,
+// which costs less than a launch between.
 constexpr int kCountWaves = 4;
 __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, const int* ids) {
     __shared__ int counts[kMaxExperts];
@@ -374,31 +395,33 @@ __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, co
     __syncthreads();
     for (int i = threadIdx.x; i < E; i += 64 * kCountWaves) p.counts[(size_t)blockIdx.x * E + i] = counts[i];
 }
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_sums(MoePlan p) {
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const int* ids) {
+    __shared__ int counts[kCountWaves * kMaxExperts];
     __shared__ int part[kPlanWaves];
-    const int e = threadIdx.x, E = p.experts;
-    int sum = 0;
-    if (e < E)
-        for (int b = 0; b < p.blocks; ++b) sum += p.counts[(size_t)b * E + e];
-    int at = write_units(p, sum, part);
-    if (e < E)
+    const int w = threadIdx.x >> 6, e = threadIdx.x, E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
+    int from = 0, to = 0;
+    for (int i = threadIdx.x; i < kCountWaves * E; i += kPlanThreads) counts[i] = 0;
+    // Expert e's assignments in all blocks, and in those before this one.
+    int sum = 0, before = 0;
+    if (e < E) {
+#pragma unroll 8
         for (int b = 0; b < p.blocks; ++b) {
             const int c = p.counts[(size_t)b * E + e];
-            p.counts[(size_t)b * E + e] = at;
-            at += c;
+            sum += c;
+            before += b < (int)blockIdx.x ? c : 0;
         }
-}
-__global__ __launch_bounds__(64 * kCountWaves) void moe_plan_place(MoePlan p, const int* ids) {
-    __shared__ int counts[kCountWaves * kMaxExperts];
-    const int w = threadIdx.x >> 6, E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
-    for (int i = threadIdx.x; i < kCountWaves * E; i += 64 * kCountWaves) counts[i] = 0;
+    }
     __syncthreads();
-    int from, to;
-    stretch(lo, hi, kCountWaves, w, from, to);
-    count_ids(ids, from, to, E, counts + w * E);
+    if (w < kCountWaves) {
+        stretch(lo, hi, kCountWaves, w, from, to);
+        count_ids(ids, from, to, E, counts + w * E);
+    }
+    int total, at;
+    if (blockIdx.x == 0) at = write_units(p, sum, part);
+    else at = block_prefix(sum, part, total);
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += 64 * kCountWaves) {
-        int at = p.counts[(size_t)blockIdx.x * E + e];
+    if (e < E) {
+        at += before;
         for (int i = 0; i < kCountWaves; ++i) {
             const int c = counts[i * E + e];
             counts[i * E + e] = at;
@@ -406,7 +429,7 @@ __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_place(MoePlan p, co
         }
     }
     __syncthreads();
-    place_ids(ids, from, to, E, counts + w * E, p.order);
+    if (w < kCountWaves) place_ids(ids, from, to, E, counts + w * E, p.order);
 }
 
 void launch_plan(const MoePlan& p, const int* ids) {
@@ -414,30 +437,52 @@ void launch_plan(const MoePlan& p, const int* ids) {
         launch("moe_plan_one", moe_plan_one, dim3(1), dim3(kPlanThreads), 0, p, ids);
     } else {
         launch("moe_plan_count", moe_plan_count, dim3(p.blocks), dim3(64 * kCountWaves), 0, p, ids);
-        launch("moe_plan_sums", moe_plan_sums, dim3(1), dim3(kPlanThreads), 0, p);
-        launch("moe_plan_place", moe_plan_place, dim3(p.blocks), dim3(64 * kCountWaves), 0, p, ids);
+        launch("moe_plan_place", moe_plan_place, dim3(p.blocks), dim3(kPlanThreads), 0, p, ids);
     }
     BYHIP_LAUNCHED("moe_plan");
 }
 
+// A decode step's tokens, and their plan, in one block and one launch.
+constexpr int kOneTokens = 64, kOneRows = 1024;
 template <int DT, int V, bool WIDE>
-void launch_route_v(const RouteArgs& a) {
+__global__ __launch_bounds__(kPlanThreads) void moe_route_one(RouteArgs a, MoePlan p) {
+    __shared__ double group[kPlanWaves][WIDE ? 64 * V : 32 * V];
+    __shared__ int counts[kPlanWaves * 64 * V];
+    __shared__ int part[kPlanWaves];
+    __shared__ int ids[kOneRows];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int t = w; t < a.T; t += kPlanWaves) route_token<DT, V, WIDE>(a, t, group[w], ids + t * a.k);
+    __syncthreads();
+    plan_block(p, ids, counts, part);
+}
+
+template <int DT, int V, bool WIDE>
+void launch_route_v(const RouteArgs& a, const MoePlan& p) {
+    if constexpr (V <= 4) {
+        // (32 tokens of 128 experts: 6 us, the two launches 10.)
+        if (a.T <= kOneTokens && p.rows <= kOneRows) {
+            launch("moe_route_one", (moe_route_one<DT, V, WIDE>), dim3(1), dim3(kPlanThreads), 0, a, p);
+            BYHIP_LAUNCHED("moe_route_one");
+            return;
+        }
+    }
     launch("moe_route", (moe_route<DT, V, WIDE>), dim3((a.T + kTokensPerBlock - 1) / kTokensPerBlock), dim3(64 * kTokensPerBlock), 0, a);
     BYHIP_LAUNCHED("moe_route");
+    launch_plan(p, a.ids);
 }
 template <int DT, bool WIDE>
-void launch_route_w(const RouteArgs& a) {
-    if (a.E <= 64) launch_route_v<DT, 1, WIDE>(a);
-    else if (a.E <= 128) launch_route_v<DT, 2, WIDE>(a);
-    else if (a.E <= 256) launch_route_v<DT, 4, WIDE>(a);
-    else if (a.E <= 512) launch_route_v<DT, 8, WIDE>(a);
-    else launch_route_v<DT, 16, WIDE>(a);
+void launch_route_w(const RouteArgs& a, const MoePlan& p) {
+    if (a.E <= 64) launch_route_v<DT, 1, WIDE>(a, p);
+    else if (a.E <= 128) launch_route_v<DT, 2, WIDE>(a, p);
+    else if (a.E <= 256) launch_route_v<DT, 4, WIDE>(a, p);
+    else if (a.E <= 512) launch_route_v<DT, 8, WIDE>(a, p);
+    else launch_route_v<DT, 16, WIDE>(a, p);
 }
 template <int DT>
-void launch_route(const RouteArgs& a) {
+void launch_route(const RouteArgs& a, const MoePlan& p) {
     // Without a bias, and with groups ranked by one key, the logits have the keys' order.
-    if (a.bias || (a.groups > 1 && a.group_by == 2)) launch_route_w<DT, true>(a);
-    else launch_route_w<DT, false>(a);
+    if (a.bias || (a.groups > 1 && a.group_by == 2)) launch_route_w<DT, true>(a, p);
+    else launch_route_w<DT, false>(a, p);
 }
 
 // ── the sum of a token's rows ──
@@ -508,14 +553,16 @@ MoePlan moe_layout(const byhip_moe_plan* p) {
     m.tokens = p->tokens; m.top_k = p->top_k; m.experts = p->experts;
     m.rows = p->tokens * p->top_k;
     m.unit_rows = moe_unit_rows(m.rows, m.experts);
-    m.max_units = m.rows / m.unit_rows + (m.rows < m.experts ? m.rows : m.experts);
+    m.max_units = moe_max_units(m.rows, m.experts, m.unit_rows);
+    m.max_tiles = moe_max_units(m.rows, m.experts, kTileRows);
     m.blocks = (m.rows + kPlanBlock - 1) / kPlanBlock;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 15) / 16 * 16; return static_cast<char*>(p->plan) + here; };
     m.offsets = reinterpret_cast<int*>(take(((size_t)m.experts + 1 + m.rows) * 4));
     m.order = m.offsets + m.experts + 1;
-    m.n_units = reinterpret_cast<int*>(take(4));
+    m.n_units = reinterpret_cast<int*>(take(8));
     m.units = reinterpret_cast<MoeUnit*>(take((size_t)m.max_units * sizeof(MoeUnit)));
+    m.tiles = reinterpret_cast<MoeUnit*>(take((size_t)m.max_tiles * sizeof(MoeUnit)));
     m.counts = reinterpret_cast<int*>(take((size_t)m.blocks * m.experts * 4));
     m.bytes = at;
     return m;
@@ -569,12 +616,13 @@ int byhip_moe_route(const void* logits, size_t stride, int dtype, const byhip_mo
             const RouteArgs a{logits, r.bias, stride, p.tokens, p.experts, p.top_k, r.score, r.groups, r.top_groups,
                               r.group_by, r.renorm, aligned4(logits, stride, dtype), r.scale, ids, weights};
             switch (dtype) {
-            case BYHIP_F32: launch_route<BYHIP_F32>(a); break;
-            case BYHIP_F16: launch_route<BYHIP_F16>(a); break;
-            default: launch_route<BYHIP_BF16>(a); break;
+            case BYHIP_F32: launch_route<BYHIP_F32>(a, p); break;
+            case BYHIP_F16: launch_route<BYHIP_F16>(a, p); break;
+            default: launch_route<BYHIP_BF16>(a, p); break;
             }
+        } else {
+            launch_plan(p, ids);
         }
-        launch_plan(p, ids);
     });
 }
 
