@@ -307,45 +307,47 @@ __device__ __forceinline__ void place_ids(const int* ids, int from, int to, int 
     }
 }
 
-// Exclusive prefix sums of v over the block's threads (1024 at most), and the total.
-__device__ __forceinline__ int block_prefix(int v, int* part, int& total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int n = __shfl_up(s, o);
-        if (lane >= o) s += n;
-    }
-    __syncthreads();
-    if (lane == 63) part[w] = s;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int i = 0; i < waves; ++i) {
-        before += i < w ? part[i] : 0;
-        total += part[i];
-    }
-    return before + s - v;
+// Inclusive prefix sums over the lanes, in DPP: within rows of 16 lanes, then across rows.
+__device__ __forceinline__ int lane_prefix(int v) {
+    auto step = [&](auto ctrl, auto mask) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(mask)::value, 0xF, false); };
+    typedef std::integral_constant<int, 0xF> All;
+    step(std::integral_constant<int, 0x111>{}, All{});  // row_shr:1, 2, 4, 8
+    step(std::integral_constant<int, 0x112>{}, All{});
+    step(std::integral_constant<int, 0x114>{}, All{});
+    step(std::integral_constant<int, 0x118>{}, All{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15 into rows 1 and 3
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31 into rows 2 and 3
+    return v;
 }
 
-// Offsets and units from expert e's count (thread e's; 0 past E), and where e starts.
-__device__ __forceinline__ int write_units(const MoePlan& p, int count, int* part) {
-    const int e = threadIdx.x;
-    int total, units, tiles;
-    const int at = block_prefix(count, part, total);
-    const int first = block_prefix((count + p.unit_rows - 1) / p.unit_rows, part, units);
-    const int first_tile = block_prefix((count + kTileRows - 1) / kTileRows, part, tiles);
+// Where expert e (thread e) starts, from its count (0 past E); with `write` also the offsets and the units. Three prefix sums in one go, over as many
+// waves as hold experts; part: 4 ints per wave.
+__device__ __forceinline__ int expert_starts(const MoePlan& p, int count, int4* part, bool write) {
+    const int e = threadIdx.x, lane = e & 63, w = e >> 6, waves = (p.experts + 63) >> 6;
+    const int units = (count + p.unit_rows - 1) / p.unit_rows, tiles = (count + kTileRows - 1) / kTileRows;
+    const int c = lane_prefix(count), u = lane_prefix(units), t = lane_prefix(tiles);
+    __syncthreads();
+    if (lane == 63) part[w] = make_int4(c, u, t, 0);
+    __syncthreads();
+    int4 before = make_int4(0, 0, 0, 0), total = before;
+    for (int i = 0; i < waves; ++i) {
+        const int4 v = part[i];
+        if (i < w) { before.x += v.x; before.y += v.y; before.z += v.z; }
+        total.x += v.x; total.y += v.y; total.z += v.z;
+    }
+    const int at = before.x + c - count;
+    if (!write) return at;
     if (e < p.experts) {
         p.offsets[e] = at;
-        for (int u = 0, r = 0; r < count; ++u, r += p.unit_rows)
-            p.units[first + u] = MoeUnit{e, at + r, min(p.unit_rows, count - r), 0};
-        for (int u = 0, r = 0; r < count; ++u, r += kTileRows)
-            p.tiles[first_tile + u] = MoeUnit{e, at + r, min(kTileRows, count - r), 0};
+        for (int i = 0, r = 0; r < count; ++i, r += p.unit_rows)
+            p.units[before.y + u - units + i] = MoeUnit{e, at + r, min(p.unit_rows, count - r), 0};
+        for (int i = 0, r = 0; r < count; ++i, r += kTileRows)
+            p.tiles[before.z + t - tiles + i] = MoeUnit{e, at + r, min(kTileRows, count - r), 0};
     }
     if (e == 0) {
-        p.offsets[p.experts] = total;
-        p.n_units[0] = units;
-        p.n_units[1] = tiles;
+        p.offsets[p.experts] = total.x;
+        p.n_units[0] = total.y;
+        p.n_units[1] = total.z;
     }
     return at;
 }
@@ -353,7 +355,7 @@ __device__ __forceinline__ int write_units(const MoePlan& p, int count, int* par
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
 // The whole plan in one block: counts per wave and expert, their sums, then the places.
-__device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int* counts, int* part) {
+__device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int* counts, int4* part) {
     const int w = threadIdx.x >> 6, E = p.experts;
     for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanThreads) counts[i] = 0;
     __syncthreads();
@@ -368,7 +370,7 @@ __device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int
             counts[i * E + threadIdx.x] = sum;
             sum += c;
         }
-    const int at = write_units(p, sum, part);
+    const int at = expert_starts(p, sum, part, true);
     if ((int)threadIdx.x < E)
         for (int i = 0; i < kPlanWaves; ++i) counts[i * E + threadIdx.x] += at;
     __syncthreads();
@@ -377,7 +379,7 @@ __device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int
 
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_one(MoePlan p, const int* ids) {
     __shared__ int counts[kPlanWaves * kMaxExperts];
-    __shared__ int part[kPlanWaves];
+    __shared__ int4 part[kPlanWaves];
     plan_block(p, ids, counts, part);
 }
 
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, co
 }
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const int* ids) {
     __shared__ int counts[kCountWaves * kMaxExperts];
-    __shared__ int part[kPlanWaves];
+    __shared__ int4 part[kPlanWaves];
     const int w = threadIdx.x >> 6, e = threadIdx.x, E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
     int from = 0, to = 0;
     for (int i = threadIdx.x; i < kCountWaves * E; i += kPlanThreads) counts[i] = 0;
@@ -416,9 +418,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const 
         stretch(lo, hi, kCountWaves, w, from, to);
         count_ids(ids, from, to, E, counts + w * E);
     }
-    int total, at;
-    if (blockIdx.x == 0) at = write_units(p, sum, part);
-    else at = block_prefix(sum, part, total);
+    int at = expert_starts(p, sum, part, blockIdx.x == 0);
     __syncthreads();
     if (e < E) {
         at += before;
@@ -442,30 +442,10 @@ void launch_plan(const MoePlan& p, const int* ids) {
     BYHIP_LAUNCHED("moe_plan");
 }
 
-// A decode step's tokens, and their plan, in one block and one launch.
-constexpr int kOneTokens = 64, kOneRows = 1024;
-template <int DT, int V, bool WIDE>
-__global__ __launch_bounds__(kPlanThreads) void moe_route_one(RouteArgs a, MoePlan p) {
-    __shared__ double group[kPlanWaves][WIDE ? 64 * V : 32 * V];
-    __shared__ int counts[kPlanWaves * 64 * V];
-    __shared__ int part[kPlanWaves];
-    __shared__ int ids[kOneRows];
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int t = w; t < a.T; t += kPlanWaves) route_token<DT, V, WIDE>(a, t, group[w], ids + t * a.k);
-    __syncthreads();
-    plan_block(p, ids, counts, part);
-}
-
 template <int DT, int V, bool WIDE>
 void launch_route_v(const RouteArgs& a, const MoePlan& p) {
-    if constexpr (V <= 4) {
-        // (32 tokens of 128 experts: 6 us, the two launches 10.)
-        if (a.T <= kOneTokens && p.rows <= kOneRows) {
-            launch("moe_route_one", (moe_route_one<DT, V, WIDE>), dim3(1), dim3(kPlanThreads), 0, a, p);
-            BYHIP_LAUNCHED("moe_route_one");
-            return;
-        }
-    }
+    // (A decode step's tokens and their plan in one block and one launch took longer: 12.4 us for 32 tokens of 128 experts, one CU's work,
+    // where the two launches take 10.)
     launch("moe_route", (moe_route<DT, V, WIDE>), dim3((a.T + kTokensPerBlock - 1) / kTokensPerBlock), dim3(64 * kTokensPerBlock), 0, a);
     BYHIP_LAUNCHED("moe_route");
     launch_plan(p, a.ids);
