@@ -71,6 +71,32 @@ __device__ __forceinline__ double lane_d(double v, int lane) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
+// 1 / y for y >= 1 (also infinity and NaN), within an ulp or two: the hardware's estimate and two steps of Newton's.
+__device__ __forceinline__ double reciprocal(double y) {
+    double r = __builtin_amdgcn_rcp(y);
+    r = fma(r, fma(-y, r, 1.0), r);
+    r = fma(r, fma(-y, r, 1.0), r);
+    return y == (double)INFINITY ? 0.0 : r;
+}
+
+// The two largest of a and b, given those of two sets.
+struct Two {
+    double one, two;
+};
+__device__ __forceinline__ Two merge(Two a, Two b) {
+    const bool over = b.one > a.one;
+    const double low = over ? a.one : b.one, first = over ? b.one : a.one, second = b.two > a.two ? b.two : a.two;
+    return Two{first, low > second ? low : second};
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, false), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ Two dpp_two(Two v) { return Two{dpp_d<CTRL>(v.one), dpp_d<CTRL>(v.two)}; }
+
 // The choices of token t by this wave. WIDE: keys in 64 bits (`group` holds E of them in LDS where groups are ranked).
 template <int DT, int V, bool WIDE>
 __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* group, int* ids_out) {
@@ -103,21 +129,26 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
             nan = nan || x[i] != x[i];
         }
         top = key_value(wave_max(most));
-        float s = 0.0f;
-        double sd = 0.0;
+        if (!WIDE && a.renorm) {
+            sum = __any(nan) ? NAN : 1.0f;  // it falls out of the weights
+        } else {
+            float s = 0.0f;
+            double sd = 0.0;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (e0 + i >= a.E) continue;
-            if constexpr (WIDE) sd += exp((double)(x[i] == top ? 0.0 : (double)x[i] - (double)top));
-            else s += expf(lift(x[i]));
+            for (int i = 0; i < V; ++i) {
+                if (e0 + i >= a.E) continue;
+                if constexpr (WIDE) sd += exp((double)(x[i] == top ? 0.0 : (double)x[i] - (double)top));
+                else s += expf(lift(x[i]));
+            }
+            if constexpr (WIDE) { sum_d = wave_sumd(sd); sum = (float)sum_d; }
+            else sum = lane_sum(s);
         }
-        if constexpr (WIDE) { sum_d = wave_sumd(sd); sum = (float)sum_d; }
-        else sum = lane_sum(s);
         if (top == -INFINITY && !__any(nan)) { sum = INFINITY; sum_d = (double)INFINITY; }
     }
     auto score_f = [&](float v) { return soft ? expf(lift(v)) / sum : 1.0f / (1.0f + expf(-v)); };
+    const double over_sum = soft ? 1.0 / sum_d : 1.0;
     auto score_d = [&](float v) {
-        return soft ? exp(v == top ? 0.0 : (double)v - (double)top) / sum_d : 1.0 / (1.0 + exp(-(double)v));
+        return soft ? exp(v == top ? 0.0 : (double)v - (double)top) * over_sum : reciprocal(1.0 + exp(-(double)v));
     };
 
     uint32_t key[V];
@@ -135,27 +166,50 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
     }
     if (a.groups > 1) {
         const int size = a.E / a.groups;
-        uint64_t in;
+        uint64_t in = 0;  // the groups that take part
+        bool mine_in = false;
+        const int span = size / V;  // lanes per group where they are whole
         if constexpr (WIDE) {
+            const double none = -(double)INFINITY;
+            if (span * V == size && (span & (span - 1)) == 0 && span <= 16) {
+                // The lane's two best, then those of its neighbours of the group: 1, 2, 4, 8 lanes on. (By one lane per group from LDS: 23.4 us for
+                // 19.4, 8191 tokens, 8 groups of 32.)
+                Two best{none, none};
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (e0 + i < a.E) group[e0 + i] = wide[i] == wide[i] ? wide[i] : -(double)INFINITY;
-            wave_sync();
-            double one = -(double)INFINITY, two = -(double)INFINITY;
-            if (lane < a.groups)
-                for (int i = 0; i < size; ++i) {
-                    const double c = group[lane * size + i];
-                    if (c > one) { two = one; one = c; }
-                    else if (c > two) two = c;
+                for (int i = 0; i < V; ++i) best = merge(best, Two{wide[i] == wide[i] ? wide[i] : none, none});
+                if (span > 1) best = merge(best, dpp_two<0xB1>(best));
+                if (span > 2) best = merge(best, dpp_two<0x4E>(best));
+                if (span > 4) best = merge(best, dpp_two<0x141>(best));
+                if (span > 8) best = merge(best, dpp_two<0x140>(best));
+                const double worth = a.group_by == 2 && size > 1 ? best.one + best.two : best.one;
+                const int own = lane / span;
+                int above = 0;
+                for (int g = 0; g < a.groups; ++g) {
+                    const double o = lane_d(worth, g * span);
+                    above += o > worth || (o == worth && g < own);
                 }
-            const double worth = a.group_by == 2 && size > 1 ? one + two : one;
-            int above = 0;
-            for (int g = 0; g < a.groups; ++g) {
-                const double o = lane_d(worth, g);
-                above += o > worth || (o == worth && g < lane);
+                mine_in = above < a.top_groups;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (e0 + i < a.E) group[e0 + i] = wide[i] == wide[i] ? wide[i] : none;
+                wave_sync();
+                double one = none, two = none;
+                if (lane < a.groups)
+                    for (int i = 0; i < size; ++i) {
+                        const double c = group[lane * size + i];
+                        if (c > one) { two = one; one = c; }
+                        else if (c > two) two = c;
+                    }
+                const double worth = a.group_by == 2 && size > 1 ? one + two : one;
+                int above = 0;
+                for (int g = 0; g < a.groups; ++g) {
+                    const double o = lane_d(worth, g);
+                    above += o > worth || (o == worth && g < lane);
+                }
+                in = __ballot(lane < a.groups && above < a.top_groups);
+                wave_sync();
             }
-            in = __ballot(lane < a.groups && above < a.top_groups);
-            wave_sync();
         } else {
             uint32_t* keys = reinterpret_cast<uint32_t*>(group);
 #pragma unroll
@@ -175,7 +229,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
         }
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (e0 + i >= a.E || !((in >> ((e0 + i) / size)) & 1)) key[i] = 0u;
+            if (e0 + i >= a.E || !(mine_in || ((in >> ((e0 + i) / size)) & 1))) key[i] = 0u;
     }
     // Rounds: the largest head; of several, in 64 bits the largest, then the lowest index (the lowest lane).
     float mine = 0.0f, total = 0.0f;
@@ -211,11 +265,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
         }
         const int win = __ffsll((unsigned long long)who) - 1;
         const int pick = __builtin_amdgcn_readlane(at, win);
-        float logit = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) logit = at == i ? x[i] : logit;
-        logit = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, logit), win));
-        if (lane == (j & 63)) { mine_id = win * V + pick; mine = logit; }
+        if (lane == (j & 63)) mine_id = win * V + pick;
         if (lane == win) {
 #pragma unroll
             for (int i = 0; i < V; ++i) key[i] = i == pick ? 0u : key[i];
@@ -225,6 +275,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
         if ((j & 63) == 63 || j + 1 == a.k) {
             const int first = j & ~63, n = j - first + 1;
             if (lane < n) {
+                mine = load1<DT>(a.logits, row + mine_id);
                 float s;
                 if constexpr (WIDE) s = (float)score_d(mine);
                 else s = score_f(mine);
@@ -399,20 +450,30 @@ __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, co
 }
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const int* ids) {
     __shared__ int counts[kCountWaves * kMaxExperts];
+    __shared__ int2 sums[kPlanThreads];
     __shared__ int4 part[kPlanWaves];
     const int w = threadIdx.x >> 6, e = threadIdx.x, E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
     int from = 0, to = 0;
     for (int i = threadIdx.x; i < kCountWaves * E; i += kPlanThreads) counts[i] = 0;
-    // Expert e's assignments in all blocks, and in those before this one.
+    // Expert e's assignments in all blocks, and in those before this one: as many threads per expert as there are, a share of the blocks each.
+    const int room = (E + 63) & ~63, shares = kPlanThreads / room, share = e / room;
     int sum = 0, before = 0;
-    if (e < E) {
+    if (e - share * room < E && share < shares) {
 #pragma unroll 8
-        for (int b = 0; b < p.blocks; ++b) {
-            const int c = p.counts[(size_t)b * E + e];
+        for (int b = share; b < p.blocks; b += shares) {
+            const int c = p.counts[(size_t)b * E + e - share * room];
             sum += c;
             before += b < (int)blockIdx.x ? c : 0;
         }
     }
+    sums[e] = make_int2(sum, before);
+    __syncthreads();
+    sum = before = 0;
+    if (e < E)
+        for (int i = 0; i < shares; ++i) {
+            sum += sums[i * room + e].x;
+            before += sums[i * room + e].y;
+        }
     __syncthreads();
     if (w < kCountWaves) {
         stretch(lo, hi, kCountWaves, w, from, to);
