@@ -14,6 +14,7 @@ import time
 import numpy as np
 
 from . import _abi, device as dev, gpubackend as g
+from .experts import ExpertsBlock, random_matrix
 from .gpubackend import gbHip
 
 
@@ -33,11 +34,12 @@ class PagedDecoder:
     residual stream of `width` values, for up to `slots` sequences of `max_len` tokens and `max_rows` rows a call.
 
     layers: a list of (wq, wk, wv, wo) resident Q4 weights; norms: gammas of the RMS norm before each layer and
-    after the last one."""
+    after the last one; experts: an ExpertsBlock (experts.py) after each layer's attention, or None."""
 
     def __init__(self, layers, norms, width: int, heads: int, kv_heads: int, head_dim: int, slots: int, max_len: int,
                  max_rows: int, pages: int, page_size: int = 32, cache_dtype: int = _abi.F16, eps: float = 1e-5,
-                 rope_base: float = 10000.0, window: int = 0, softcap: float = 0.0):
+                 rope_base: float = 10000.0, window: int = 0, softcap: float = 0.0, experts=None):
+        self.experts = experts or [None] * len(layers)
         self.layers, self.width, self.heads, self.slots, self.max_rows = layers, width, heads, slots, max_rows
         self.stride = -(-max_len // page_size)
         scratch = lambda n: g.sessionAllocScratch(gbHip, n)  # noqa: E731
@@ -82,13 +84,15 @@ class PagedDecoder:
             return
         ok = g.sessionCacheGrow(gbHip, self.pool, self.all_rows, self.add, self.slots)
         ok &= g.sessionNormBlock(gbHip, self.x, T, E, None, None, None, 1.0, self.h, self.norms[0], self.y)
-        for (wq, wk, wv, wo), cache, norm in zip(self.layers, self.caches, self.norms[1:]):
+        for (wq, wk, wv, wo), cache, norm, experts in zip(self.layers, self.caches, self.norms[1:], self.experts):
             ok &= g.sessionMatmulQ4(gbHip, self.y, wq, self.q, T)
             ok &= g.sessionMatmulQ4(gbHip, self.y, wk, self.k, T)
             ok &= g.sessionMatmulQ4(gbHip, self.y, wv, self.v, T)
             ok &= g.sessionRopeAppend(gbHip, self.q, self.k, self.v, self.heads, self.rope, cache, self.batch, self.q_rot)
             ok &= g.sessionPagedAttention(gbHip, self.q_rot, self.heads, self.attn, cache, self.batch, self.a)
             ok &= g.sessionMatmulQ4(gbHip, self.a, wo, self.o, T)
+            if experts is not None:
+                ok &= experts.encode(self.o, T, self.h, self.o)
             ok &= g.sessionNormBlock(gbHip, self.o, T, E, None, None, self.h, 1.0, self.h, norm, self.y)
         self._taken(ok)
 
@@ -155,6 +159,9 @@ def main() -> None:
     p.add_argument("--beams", type=int, default=4)
     p.add_argument("--prompt-len", type=int, default=900)
     p.add_argument("--steps", type=int, default=64)
+    p.add_argument("--experts", type=int, default=0, help="experts after each attention block (0: none)")
+    p.add_argument("--top-k", type=int, default=8)
+    p.add_argument("--inner", type=int, default=1024, help="values inside an expert")
     args = p.parse_args()
     rng = np.random.default_rng(0)
     g.ensureGpuInit(gbHip)
@@ -164,8 +171,11 @@ def main() -> None:
     norms = [np.ones(args.width, np.float32)] * (args.layers + 1)
     slots = args.prompts * args.beams
     max_len = args.prompt_len + args.steps + 2
+    rows, E, F, W = args.prompts * args.prompt_len, args.experts, args.inner, args.width
+    experts = [ExpertsBlock(random_matrix(rng, E, W), random_matrix(rng, 2 * E * F, W), random_matrix(rng, E * W, F), norms[0], W, F, E,
+                            min(args.top_k, E), rows) for _ in layers] if E else None
     d = PagedDecoder(layers, norms, args.width, args.heads, args.kv_heads, args.head_dim, slots, max_len,
-                     args.prompts * args.prompt_len, slots * -(-max_len // 32))
+                     rows, slots * -(-max_len // 32), experts=experts)
     counts = [0] * slots
     counts[::args.beams] = [args.prompt_len - 37 * i for i in range(args.prompts)]
     t = time.perf_counter()

@@ -362,6 +362,8 @@ def test_quantized_rows_through_experts(hip):
     out, oslack = np.zeros((T * k, D)), np.zeros((T * k, D))
     for e in range(E):
         at = np.arange(offsets[e], offsets[e + 1])
+        if not at.size:
+            continue
         want[at], slack[at] = expected(xv[order[at] // k], wv1[e], F, D, True, MX8, MX8)
         out[order[at]], oslack[order[at]] = expected(hv[at], wv2[e], D, F, False, MX8, F32)
     agree(h, want, slack, MX8, T * k, F, F)
