@@ -67,17 +67,8 @@ __device__ __forceinline__ void write4(void* p, size_t row, int i, int N, int ve
     }
 }
 
-// First column of chunk c of thread tid. Microscaled rows are written eight values at a time that lie next to each other in
-// their order: elements 4 t .. 4 t + 3 of a group and the four 16 further on, in chunks 2 c and 2 c + 1.
-template <bool MX>
-__device__ __forceinline__ int column(int c, int tid, int threads) {
-    if constexpr (!MX) return 4 * (threads * c + tid);
-    const int u = threads * (c >> 1) + tid;
-    return 32 * (u >> 2) + 4 * (u & 3) + 16 * (c & 1);
-}
-
-// One norm over the row held in v.
-template <int CH, bool MX = false>
+// One norm over the row held in v (columns 4 (threads c + thread) ..).
+template <int CH>
 __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n, int N, int vec, int tid, BlockSum& block_sum) {
     const int TH = blockDim.x;
     float mean = 0.0f;
@@ -94,13 +85,13 @@ __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n,
     for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float d = column<MX>(c, tid, TH) + e < N ? v[c][e] - mean : 0.0f;
+            const float d = 4 * (TH * c + tid) + e < N ? v[c][e] - mean : 0.0f;
             s += d * d;
         }
     const float f = 1.0f / sqrtf(block_sum(s) / N + n.eps);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int i = column<MX>(c, tid, TH);
+        const int i = 4 * (TH * c + tid);
         float w[4] = {1.0f, 1.0f, 1.0f, 1.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (n.weight) read4<BYHIP_F32>(n.weight, 0, i, N, vec, w);
         if (n.bias) read4<BYHIP_F32>(n.bias, 0, i, N, vec, b);
@@ -109,21 +100,49 @@ __device__ __forceinline__ void norm_row(float (&v)[CH][4], const byhip_norm& n,
     }
 }
 
-// The row in v as microscaled values: 4 lanes hold a group.
+// The lane's value of the lane 4 further on in its 8, or 4 back.
+__device__ __forceinline__ uint32_t other_half(uint32_t v, bool upper) {
+    const uint32_t up = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x104, 0xF, 0xF, false);    // row_shl:4
+    const uint32_t down = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);  // row_shr:4
+    return upper ? down : up;
+}
+
+// The row in v as microscaled values: 8 neighbouring lanes hold a group, and a lane's four elements and those of the lane 4 further on
+// or back take turns in memory. (With a thread's eight values chosen so that they lie next to each other there, reads of 64 bytes at a time
+// cost more than this exchange: 4099 x 5120 64 us.)
 template <int FMT, int CH>
 __device__ __forceinline__ void write_mx(const NormArgs& a, size_t row, int tid, int TH, const float (&v)[CH][4]) {
+    const int t = tid & 7;
+    const bool upper = t & 4;
+    uint8_t* y = static_cast<uint8_t*>(a.y);
 #pragma unroll
-    for (int c = 0; c + 1 < CH; c += 2) {
-        const int u = TH * (c >> 1) + tid, G = u >> 2;
-        uint32_t m = mag8(v[c], v[c + 1]);
-        m = max(m, (uint32_t)__shfl_xor((int)m, 1));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 2));
-        if (32 * G >= a.N) continue;
+    for (int c = 0; c < CH; ++c) {
+        const int i = 4 * (TH * c + tid), G = i >> 5;
+        uint32_t m = max(max(mag_bits(v[c][0]), mag_bits(v[c][1])), max(mag_bits(v[c][2]), mag_bits(v[c][3])));
+        m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));
+        m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));
+        m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));
         const uint32_t byte = mx_scale<FMT>(m);
-        uint32_t out[2];
-        mx_pack8<FMT>(v[c], v[c + 1], byte, out);
-        mx_store8<FMT>(static_cast<uint8_t*>(a.y), row, a.N, G, 4 * (u & 3), out);
-        if ((u & 3) == 0) a.y_scales[row * (a.N / 32) + G] = (uint8_t)byte;
+        const float f = mx_inverse(byte);
+        float z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = byte == 255u ? 0.0f : v[c][e] * f;
+        if constexpr (FMT == BYHIP_MXFP8_KM) {
+            const int low = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+            const uint32_t own = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], low, true), far = other_half(own, upper);
+            // Bytes 0 and 1 of both (the lower lane's first), or 2 and 3.
+            const uint32_t out = upper ? __builtin_amdgcn_perm(own, far, 0x07030602u) : __builtin_amdgcn_perm(far, own, 0x05010400u);
+            if (i < a.N) *reinterpret_cast<uint32_t*>(y + row * a.N + 32 * G + (upper ? 8 * (t - 4) + 4 : 8 * t)) = out;
+        } else {
+            uint32_t own = 0;
+            own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, z[0], 0.0f, 1.0f, 0);
+            own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, z[1], 0.0f, 1.0f, 1);
+            own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, z[2], 0.0f, 1.0f, 2);
+            own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, z[3], 0.0f, 1.0f, 3);
+            const uint32_t far = other_half(own, upper);
+            if (i < a.N && !upper) *reinterpret_cast<uint32_t*>(y + row * (a.N / 2) + 16 * G + 4 * t) = own | far << 4;
+        }
+        if (i < a.N && t == 0) a.y_scales[row * (a.N / 32) + G] = (uint8_t)byte;
     }
 }
 
@@ -135,15 +154,15 @@ __global__ __launch_bounds__(1024) void norm_block(NormArgs a) {
     const size_t row = blockIdx.x;
     float v[CH][4], r[CH][4];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) read4<XT>(a.x, row * a.x_stride, column<MX>(c, tid, TH), a.N, a.vec, v[c]);
+    for (int c = 0; c < CH; ++c) read4<XT>(a.x, row * a.x_stride, 4 * (TH * c + tid), a.N, a.vec, v[c]);
     if (a.res) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) read4<HT>(a.res, row * a.res_stride, column<MX>(c, tid, TH), a.N, a.vec, r[c]);
+        for (int c = 0; c < CH; ++c) read4<HT>(a.res, row * a.res_stride, 4 * (TH * c + tid), a.N, a.vec, r[c]);
     }
-    if (a.has_post) norm_row<CH, MX>(v, a.post, a.N, a.vec, tid, block_sum);
+    if (a.has_post) norm_row<CH>(v, a.post, a.N, a.vec, tid, block_sum);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int i = column<MX>(c, tid, TH);
+        const int i = 4 * (TH * c + tid);
         if (a.gate) {
             float g[4];
             read4<BYHIP_F32>(a.gate, row * a.gate_stride, i, a.N, a.vec, g);
@@ -159,13 +178,13 @@ __global__ __launch_bounds__(1024) void norm_block(NormArgs a) {
         if (a.h) write4(a.h, row * a.h_stride, i, a.N, a.vec, v[c], HT);
     }
     if (!a.has_pre) return;
-    norm_row<CH, MX>(v, a.pre, a.N, a.vec, tid, block_sum);
+    norm_row<CH>(v, a.pre, a.N, a.vec, tid, block_sum);
     if constexpr (MX) {
         if (a.y_dtype == BYHIP_MXFP8_KM) write_mx<BYHIP_MXFP8_KM, CH>(a, row, tid, TH, v);
         else write_mx<BYHIP_MXFP4_KM, CH>(a, row, tid, TH, v);
     } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) write4(a.y, row * a.y_stride, column<MX>(c, tid, TH), a.N, a.vec, v[c], a.y_dtype);
+        for (int c = 0; c < CH; ++c) write4(a.y, row * a.y_stride, 4 * (TH * c + tid), a.N, a.vec, v[c], a.y_dtype);
     }
 }
 
@@ -242,9 +261,8 @@ void launch_norm(const NormArgs& a) {
     const long long threads = ((fours + ch - 1) / ch + 63) / 64 * 64;
     const dim3 grid(a.M), block((unsigned)threads);
     if (a.has_pre && is_mx(a.y_dtype) && threads <= 1024) {
-        // Two chunks at least, so that a thread holds eight values of a group.
-        const dim3 two((unsigned)(((fours + 1) / 2 + 63) / 64 * 64));
-        if (ch <= 2) launch("norm_block", (norm_block<XT, HT, 2, true>), grid, two, 0, a);
+        if (ch == 1) launch("norm_block", (norm_block<XT, HT, 1, true>), grid, block, 0, a);
+        else if (ch == 2) launch("norm_block", (norm_block<XT, HT, 2, true>), grid, block, 0, a);
         else if (ch == 4) launch("norm_block", (norm_block<XT, HT, 4, true>), grid, block, 0, a);
         else launch("norm_block", (norm_block<XT, HT, 8, true>), grid, block, 0, a);
         BYHIP_LAUNCHED("norm_block");
