@@ -1,14 +1,15 @@
 // byhip_moe_rows.hip - few rows per expert (gfx950): products that read each matrix once, in units of up to 64 rows.
 //
 // Bound by the matrices' bytes. A block takes a strip of a matrix (64 of its rows) and one unit's rows; its four waves share
-// out the values' axis in windows of 512 and add their sums in LDS at the end. A wave loads its window of the
+// out the values' axis in windows of 512 (or 256) and add their sums in LDS at the end. A wave loads its window of the
 // strip in 16-byte pieces straight into the operands of v_mfma_scale_f32_16x16x128_f8f6f4, 16 KB in flight before the first
-// product, and the rows' values beside it (they come from L2: every strip of the expert reads them).
+// product, and the rows' values beside it (they come from L2: every strip of the expert reads them). Six waves per SIMD hide the latencies; loads
+// of the first window ahead of the rows' look-up, with the registers they take, cost more than they saved (48 us for 33, 48 tokens, 128 experts).
 //
 // Operands (checked on the device): the matrix is the first, in 4 bits: lane (c, g) = (l % 16, l / 16) holds the 32 values of
 // block g of row c. Rows in 4 bits are the same. Rows in 8 bits: lane (c, g) holds two pieces of 16 values, those of
 // half g % 2 of blocks g / 2 and 2 + g / 2; scales go by block for both, lane (c, g)'s being block g's. Which 32 values of the
-// window are block g of a step is free as long as both operands agree: step s takes group 4 g + s of the window's 16, so
+// window are block g of a step is free as long as both operands agree: step s takes group S g + s of the window's 4 S, so
 // that a lane's four scale bytes lie in one word. The result: lane (c, g) holds row c of x, matrix rows 4 g .. 4 g + 3.
 //
 // Sums are fp32. What the instructions add in one go is exact with rows in 4 bits; with rows in 8 bits they cut small products off
@@ -25,24 +26,27 @@ typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ v4u load16(rsrc_t r, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
 
-// The scale bytes of groups G .. G + 3 of a row that starts at `row` (kOutOfRange: none), 0 for those past its KG groups: a byte
+// The scale bytes of groups G .. G + S - 1 of a row that starts at `row` (kOutOfRange: none), 0 for those past its KG groups: a byte
 // of the next row might be a NaN's.
+template <int S>
 __device__ __forceinline__ uint32_t load_scales(rsrc_t r, uint32_t row, int G, int KG) {
-    if ((KG & 3) == 0) return buf_load4(r, row == kOutOfRange || G >= KG ? kOutOfRange : row + G);
+    const uint32_t at = row == kOutOfRange || G >= KG ? kOutOfRange : row + G;
+    if (S == 4 && (KG & 3) == 0) return buf_load4(r, at);
+    if (S == 2 && (KG & 1) == 0) return buf_load2(r, at);
     uint32_t v = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < S; ++i)
         v |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, row == kOutOfRange || G + i >= KG ? kOutOfRange : row + G + i, 0, 0) << (8 * i);
     return v;
 }
 
-template <int XF, int S>
+template <int XF, int B>  // B: the scales' byte
 __device__ __forceinline__ f4v product(v8i w, v8i x, f4v c, int sw, int sx) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, XF == BYHIP_MXFP8_KM ? 0 : 4, S, sw, S, sx);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, XF == BYHIP_MXFP8_KM ? 0 : 4, B, sw, B, sx);
 }
 
-// MT blocks of 16 rows, NF blocks of 16 matrix rows (GLU: two of gates, two of ups).
-template <int XF, int MT, int NF, bool GLU, bool FINE>
+// MT blocks of 16 rows, NF blocks of 16 matrix rows (GLU: two of gates, two of ups), windows of S steps.
+template <int XF, int MT, int NF, int S, bool GLU, bool FINE>
 __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     static_assert(!GLU || NF == 4, "gates and ups");
     __shared__ float4 part[kWaves][NF * MT][64];
@@ -59,7 +63,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     int n[NF];  // this lane's row of each block of the matrix
 #pragma unroll
     for (int f = 0; f < NF; ++f) n[f] = GLU ? (f >> 1) * a.N + n0 + 16 * (f & 1) + c : n0 + 16 * f + c;
-    const int windows = (a.KG + 15) / 16;
+    const int windows = (a.KG + 4 * S - 1) / (4 * S);
 
     for (int m0 = 0; m0 < u.rows; m0 += 16 * MT) {
         uint32_t x_at[MT], xs_at[MT];
@@ -81,27 +85,27 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
                 asm volatile("" : "+v"(acc[f][m]));
             }
         for (int W = w; W < windows; W += kWaves) {
-            const int G = 16 * W + 4 * g;  // the lane's first group of the matrix
-            v4u wv[NF][4];
+            const int G = 4 * S * W + S * g;  // the lane's first group of the matrix
+            v4u wv[NF][S];
             uint32_t ws[NF];
 #pragma unroll
             for (int f = 0; f < NF; ++f) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
+                for (int s = 0; s < S; ++s)
                     wv[f][s] = load16(wr, n[f] < a.R && G + s < a.KG ? (uint32_t)n[f] * kb + 16 * (G + s) : kOutOfRange);
-                ws[f] = load_scales(wsr, n[f] < a.R ? (uint32_t)n[f] * a.KG : kOutOfRange, G, a.KG);
+                ws[f] = load_scales<S>(wsr, n[f] < a.R ? (uint32_t)n[f] * a.KG : kOutOfRange, G, a.KG);
             }
             uint32_t xs[MT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) xs[m] = load_scales(xsr, xs_at[m], G, a.KG);
+            for (int m = 0; m < MT; ++m) xs[m] = load_scales<S>(xsr, xs_at[m], G, a.KG);
             auto step = [&](auto Sc) {
-                constexpr int S = decltype(Sc)::value;
+                constexpr int T = decltype(Sc)::value;
                 v8i xv[MT], small[FINE ? MT : 1];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     xv[m] = v8i{0, 0, 0, 0, 0, 0, 0, 0};
                     if constexpr (eight) {
-                        const int g0 = 16 * W + 4 * (g >> 1) + S, g1 = g0 + 8;
+                        const int g0 = 4 * S * W + S * (g >> 1) + T, g1 = g0 + 2 * S;
                         const v4u p = load16(xr, x_at[m] != kOutOfRange && g0 < a.KG ? x_at[m] + 32 * g0 + 16 * (g & 1) : kOutOfRange);
                         const v4u q = load16(xr, x_at[m] != kOutOfRange && g1 < a.KG ? x_at[m] + 32 * g1 + 16 * (g & 1) : kOutOfRange);
 #pragma unroll
@@ -111,25 +115,27 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
                             split_bytes(both, xv[m], small[m]);
                         }
                     } else {
-                        const v4u p = load16(xr, x_at[m] != kOutOfRange && G + S < a.KG ? x_at[m] + 16 * (G + S) : kOutOfRange);
+                        const v4u p = load16(xr, x_at[m] != kOutOfRange && G + T < a.KG ? x_at[m] + 16 * (G + T) : kOutOfRange);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) xv[m][e] = (int)p[e];
                     }
                 }
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
-                    const v8i wf = {(int)wv[f][S][0], (int)wv[f][S][1], (int)wv[f][S][2], (int)wv[f][S][3], 0, 0, 0, 0};
+                    const v8i wf = {(int)wv[f][T][0], (int)wv[f][T][1], (int)wv[f][T][2], (int)wv[f][T][3], 0, 0, 0, 0};
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
-                        if constexpr (FINE) acc[f][m] = product<XF, S>(wf, small[m], acc[f][m], (int)ws[f], (int)xs[m]);
-                        acc[f][m] = product<XF, S>(wf, xv[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                        if constexpr (FINE) acc[f][m] = product<XF, T>(wf, small[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                        acc[f][m] = product<XF, T>(wf, xv[m], acc[f][m], (int)ws[f], (int)xs[m]);
                     }
                 }
             };
             step(std::integral_constant<int, 0>{});
             step(std::integral_constant<int, 1>{});
-            step(std::integral_constant<int, 2>{});
-            step(std::integral_constant<int, 3>{});
+            if constexpr (S > 2) {
+                step(std::integral_constant<int, 2>{});
+                step(std::integral_constant<int, 3>{});
+            }
         }
         __syncthreads();  // the sums of the rows before are read
 #pragma unroll
@@ -196,7 +202,12 @@ void launch_rows_as(MoeArgs a, int max_units) {
     a.strips = (a.N + wide - 1) / wide;
     const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;
     if (blocks >= 1ll << 31) fail("byhip: a product of %d units of %d strips", max_units, a.strips);
-    launch("moe_rows", (moe_rows<XF, MT, NF, GLU, FINE>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, a);
+    // Windows of 512 values, or of 256 where those would leave waves without one or with half of one (48 tokens, 128 experts, 2048 outputs, K = 512
+    // / 768 / 1024 / 1408 / 1536: 15.2 / 18.1 / 24.5 / 27.0 / 23.4 us for 18.0 / 21.6 / 25.8 / 29.4 / 24.5; K = 2048: 32.9 for 33.1, and for one
+    // token 7.5 for 6.8. Windows of 128 took longer than those of 256 but for K = 1408, 26.2).
+    const dim3 grid((unsigned)blocks), block(64 * kWaves);
+    if (a.KG > 48) launch("moe_rows", (moe_rows<XF, MT, NF, 4, GLU, FINE>), grid, block, 0, a);
+    else launch("moe_rows", (moe_rows<XF, MT, NF, 2, GLU, FINE>), grid, block, 0, a);
     BYHIP_LAUNCHED("moe_rows");
 }
 

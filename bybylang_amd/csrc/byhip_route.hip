@@ -560,14 +560,23 @@ __global__ __launch_bounds__(256) void moe_combine(CombineArgs a) {
             else if (a.res_dtype == BYHIP_F16) read_cols<BYHIP_F16>(a.res, at, left, a.vec, s);
             else read_cols<BYHIP_BF16>(a.res, at, left, a.vec, s);
         }
+        // Eight rows' loads at a time, then their sums.
         const size_t first = (size_t)t * a.k;
-        for (int j = 0; j < a.k; ++j) {
-            if ((unsigned)a.ids[first + j] >= (unsigned)a.E) continue;
-            const float w = a.weights[first + j];
-            float v[4];
-            read_cols<XT>(a.x, (first + j) * a.x_stride + n, left, a.vec, v);
+        for (int j0 = 0; j0 < a.k; j0 += 8) {
+            float w[8], v[8][4];
+            bool live[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = fmaf(w, v[e], s[e]);
+            for (int j = 0; j < 8; ++j) {
+                live[j] = j0 + j < a.k && (unsigned)a.ids[first + min(j0 + j, a.k - 1)] < (unsigned)a.E;
+                w[j] = a.weights[first + min(j0 + j, a.k - 1)];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (live[j]) read_cols<XT>(a.x, (first + j0 + j) * a.x_stride + n, left, a.vec, v[j]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = live[j] ? fmaf(w[j], v[j][e], s[e]) : s[e];
         }
         const size_t at = (size_t)t * a.y_stride + n;
         if (a.vec && left >= 4) {
