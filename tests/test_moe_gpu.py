@@ -207,6 +207,22 @@ def test_products(hip, xf, T, k, E, K, N, flags, yt):
     check_product(hip, T, k, E, K, N, xf, yt, flags, seed=T)
 
 
+@pytest.mark.parametrize("xf", [MX8, MX4])
+@pytest.mark.parametrize("T,k,E,K,N", [(300, 3, 6, 256, 1056), (1000, 1, 5, 384, 1504), (90, 8, 64, 128, 1056), (2100, 2, 40, 128, 544)])
+@pytest.mark.parametrize("flags,yt", [(GATHER | GLU, MX8), (GATHER | GLU, MX4), (GATHER | GLU | SCATTER, BF16), (SCATTER, F32), (0, F16), (GATHER, MX8)])
+def test_products_in_tiles(hip, xf, T, k, E, K, N, flags, yt):
+    """Blocks enough for moe_tiles, most experts' last one not full."""
+    check_product(hip, T, k, E, K, N, xf, yt, flags, seed=T)
+
+
+@pytest.mark.parametrize("flags,yt", [(GATHER | GLU, MX8), (SCATTER, F32), (GLU | SCATTER, BF16)])
+def test_tiles_with_assignments_left_out(hip, flags, yt):
+    g = synth.rng(3)
+    check_product(hip, 500, 2, 5, 256, 1056, MX8, yt, flags, ids=g.integers(-2, 7, (500, 2)).astype(np.int32), seed=5)
+    check_product(hip, 500, 2, 5, 128, 1056, MX8, yt, flags, ids=np.full((500, 2), 3, np.int32), seed=5)
+    check_product(hip, 500, 2, 5, 128, 1056, MX8, yt, flags, ids=np.full((500, 2), 5, np.int32), seed=5)
+
+
 @pytest.mark.parametrize("T,k,E", [(33, 2, 9), (400, 2, 4)])
 @pytest.mark.parametrize("flags,yt", [(GATHER | GLU, MX8), (SCATTER, F32), (SCATTER, BF16), (GLU | SCATTER, MX4)])
 def test_assignments_left_out(hip, T, k, E, flags, yt):
@@ -297,7 +313,7 @@ def test_refusals(hip):
             (rt, "by their 3 best", {"groups": 2, "group_by": 3}), (rt, "2 choices among 1", {"groups": 8}), (rt, "below its width", {"stride": 7}), (rt, "dtype 4", {"dt": 4}),
             (rt, "logits needs", {"logits": small}), (rt, "bias needs", {"bias": small}), (rt, "ids needs", {"ids": small}), (rt, "weights needs", {"w": small}),
             (rt, "plan needs", {"plan": hip.MoePlan(small, 4, 2, 8)}), (rt, "aligned", {"plan": hip.MoePlan(odd, 2, 2, 8)}), (rt, "a plan of", {"plan": hip.MoePlan(buf, 4, 9, 8)}),
-            (rt, "a plan of", {"plan": hip.MoePlan(buf, 4, 2, 1025)}), (rt, "a plan of", {"plan": hip.MoePlan(buf, -1, 2, 8)}), (rt, "a plan of", {"plan": hip.MoePlan(buf, 2**23, 2, 8)}),
+            (rt, "a plan of", {"plan": hip.MoePlan(buf, 4, 2, 1025)}), (rt, "a plan of", {"plan": hip.MoePlan(buf, 4, 257, 1024)}), (rt, "a plan of", {"plan": hip.MoePlan(buf, -1, 2, 8)}), (rt, "a plan of", {"plan": hip.MoePlan(buf, 2**23, 2, 8)}),
             (mm, "flags 8", {"flags": 8}), (mm, "multiple of 32", {"K": 33}), (mm, "rows of a product needs", {"x": small}), (mm, "matrices .* needs", {"w": small}), (mm, "product needs", {"y": small}),
             (mm, "format 2", {"xf": BF16}), (mm, "multiple of 32", {"N": 40, "ys": 40, "yt": MX4}), (mm, "below its width", {"ys": 16}), (mm, "plan needs", {"plan": hip.MoePlan(small, 4, 2, 8)}),
             (cb, "rows of 0 values", {"N": 0}), (cb, "rows needs", {"x": small}), (cb, "residual needs", {"res": small}), (cb, "summed rows needs", {"y": small}), (cb, "ids needs", {"ids": small}),
@@ -321,7 +337,12 @@ def test_no_tokens(hip):
 @pytest.mark.parametrize("fill", [0, 1, 0x7F, 0xFF])
 def test_buffer_without_a_plan(hip, fill):
     """A product with a buffer that no plan was made in writes rows of its own output or none, and reads its operands only."""
-    T, k, E, K, N = 9, 2, 4, 64, 32
+    for T, K, N in ((9, 64, 32), (400, 128, 2080)):
+        check_no_plan(hip, fill, T, K, N)
+
+
+def check_no_plan(hip, fill, T, K, N):
+    k, E = 2, 4
     up = hip.DeviceBuffer.from_array
     buf = up(np.full(hip.moe_plan_bytes(T, k, E), fill, np.uint8))
     p = hip.MoePlan(buf, T, k, E)

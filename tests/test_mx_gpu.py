@@ -212,11 +212,31 @@ def test_outputs(hip, xf, yt, M, K, N, glu):
     check(hip, M, K, N, xf, yt, glu=glu, seed=yt)
 
 
-@pytest.mark.parametrize("M,K", [(3, 96), (200, 512), (40, 128)])
-def test_nan_groups_reach_their_outputs_only(hip, M, K):
+@pytest.mark.parametrize("xf", [MX8, MX4])
+@pytest.mark.parametrize("K", [128, 256, 384, 512, 640, 896, 1152])
+@pytest.mark.parametrize("glu", [False, True])
+def test_tiles_lengths(hip, xf, K, glu):
+    """Enough blocks of 128 rows and 256 matrix rows for moe_tiles, the last of each not full."""
+    check(hip, 6 * 128 + 5, K, (1025 if glu else 2049) + K % 3, xf, F16 if glu else F32, glu=glu, pad=1, seed=K)
+
+
+@pytest.mark.parametrize("xf", [MX8, MX4])
+@pytest.mark.parametrize("yt", [F32, F16, BF16, MX8, MX4])
+@pytest.mark.parametrize("M,N,pad", [(900, 2080, 0), (1023, 1824, 8), (385, 4128, 5)])
+@pytest.mark.parametrize("glu", [False, True])
+def test_tiles_outputs(hip, xf, yt, M, N, pad, glu):
+    check(hip, M, 256, N if not glu else -(-N // 64) * 32, xf, yt, glu=glu, pad=pad, seed=yt + M)
+
+
+@pytest.mark.parametrize("M,K,N", [(65, 128, 1), (200, 256, 2), (129, 384, 3)])
+def test_narrow_products_of_rows_in_4_bits(hip, M, K, N):
+    check(hip, M, K, N, MX4, F32, seed=N)
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 96, 70), (200, 512, 70), (40, 128, 70), (700, 384, 2100)])
+def test_nan_groups_reach_their_outputs_only(hip, M, K, N):
     """A row's NaN group makes the row NaN, a matrix row's the column, and nothing else; the bytes behind a row are not its own."""
     g = synth.rng(5)
-    N = 70
     up = hip.DeviceBuffer.from_array
     xb, xv = random_rows(g, M, K, MX8)
     wb, wv = random_rows(g, N, K, MX4)
