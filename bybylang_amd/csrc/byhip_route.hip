@@ -372,8 +372,8 @@ __device__ __forceinline__ int lane_prefix(int v) {
 }
 
 // Where expert e (thread e) starts, from its count (0 past E); with `write` also the offsets and the units. Three prefix sums in one go, over as many
-// waves as hold experts; part: 4 ints per wave.
-__device__ __forceinline__ int expert_starts(const MoePlan& p, int count, int4* part, bool write) {
+// waves as hold experts; part: one per wave, where: one per expert.
+__device__ __forceinline__ int expert_starts(const MoePlan& p, int count, int4* part, int4* where, bool write) {
     const int e = threadIdx.x, lane = e & 63, w = e >> 6, waves = (p.experts + 63) >> 6;
     const int units = (count + p.unit_rows - 1) / p.unit_rows, tiles = (count + kTileRows - 1) / kTileRows;
     const int c = lane_prefix(count), u = lane_prefix(units), t = lane_prefix(tiles);
@@ -388,17 +388,27 @@ __device__ __forceinline__ int expert_starts(const MoePlan& p, int count, int4* 
     }
     const int at = before.x + c - count;
     if (!write) return at;
+    auto unit = [&](int e, int at, int count, int rows, int i) { return MoeUnit{e, at + i * rows, min(rows, count - i * rows), 0}; };
+    constexpr int kFew = 4;
+    const int4 mine = make_int4(at, count, before.y + u - units, before.z + t - tiles);
     if (e < p.experts) {
         p.offsets[e] = at;
-        for (int i = 0, r = 0; r < count; ++i, r += p.unit_rows)
-            p.units[before.y + u - units + i] = MoeUnit{e, at + r, min(p.unit_rows, count - r), 0};
-        for (int i = 0, r = 0; r < count; ++i, r += kTileRows)
-            p.tiles[before.z + t - tiles + i] = MoeUnit{e, at + r, min(kTileRows, count - r), 0};
+        where[e] = mine;
+        for (int i = 0; i < min(units, kFew); ++i) p.units[mine.z + i] = unit(e, at, count, p.unit_rows, i);
+        for (int i = 0; i < min(tiles, kFew); ++i) p.tiles[mine.w + i] = unit(e, at, count, kTileRows, i);
     }
     if (e == 0) {
         p.offsets[p.experts] = total.x;
         p.n_units[0] = total.y;
         p.n_units[1] = total.z;
+    }
+    // Experts of more units: a wave writes one's.
+    if (__syncthreads_or(units > kFew)) {
+        for (int x = w; x < p.experts; x += (int)blockDim.x >> 6) {
+            const int4 s = where[x];
+            for (int i = kFew + lane; i * p.unit_rows < s.y; i += 64) p.units[s.z + i] = unit(x, s.x, s.y, p.unit_rows, i);
+            for (int i = kFew + lane; i * kTileRows < s.y; i += 64) p.tiles[s.w + i] = unit(x, s.x, s.y, kTileRows, i);
+        }
     }
     return at;
 }
@@ -406,7 +416,7 @@ __device__ __forceinline__ int expert_starts(const MoePlan& p, int count, int4* 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
 // The whole plan in one block: counts per wave and expert, their sums, then the places.
-__device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int* counts, int4* part) {
+__device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int* counts, int4* part, int4* where) {
     const int w = threadIdx.x >> 6, E = p.experts;
     for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanThreads) counts[i] = 0;
     __syncthreads();
@@ -421,7 +431,7 @@ __device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int
             counts[i * E + threadIdx.x] = sum;
             sum += c;
         }
-    const int at = expert_starts(p, sum, part, true);
+    const int at = expert_starts(p, sum, part, where, true);
     if ((int)threadIdx.x < E)
         for (int i = 0; i < kPlanWaves; ++i) counts[i * E + threadIdx.x] += at;
     __syncthreads();
@@ -430,8 +440,8 @@ __device__ __forceinline__ void plan_block(const MoePlan& p, const int* ids, int
 
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_one(MoePlan p, const int* ids) {
     __shared__ int counts[kPlanWaves * kMaxExperts];
-    __shared__ int4 part[kPlanWaves];
-    plan_block(p, ids, counts, part);
+    __shared__ int4 part[kPlanWaves], where[kMaxExperts];
+    plan_block(p, ids, counts, part, where);
 }
 
 // Many assignments: counts per block of them, then the places; every block of the second forms the sums it needs from all blocks' counts,
@@ -451,7 +461,7 @@ __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, co
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const int* ids) {
     __shared__ int counts[kCountWaves * kMaxExperts];
     __shared__ int2 sums[kPlanThreads];
-    __shared__ int4 part[kPlanWaves];
+    __shared__ int4 part[kPlanWaves], where[kMaxExperts];
     const int w = threadIdx.x >> 6, e = threadIdx.x, E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
     int from = 0, to = 0;
     for (int i = threadIdx.x; i < kCountWaves * E; i += kPlanThreads) counts[i] = 0;
@@ -479,7 +489,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const 
         stretch(lo, hi, kCountWaves, w, from, to);
         count_ids(ids, from, to, E, counts + w * E);
     }
-    int at = expert_starts(p, sum, part, blockIdx.x == 0);
+    int at = expert_starts(p, sum, part, where, blockIdx.x == 0);
     __syncthreads();
     if (e < E) {
         at += before;

@@ -131,7 +131,7 @@ def test_not_finite(hip, score, bias, renorm):
     check_route(hip, T, E, k, score=score, bias=bias, renorm=renorm, x=x)
 
 
-@pytest.mark.parametrize("T,E,k", [(0, 4, 2), (1, 1, 1), (600, 16, 2), (4000, 60, 6), (3000, 1024, 8), (9000, 8, 2), (20000, 1, 1)])
+@pytest.mark.parametrize("T,E,k", [(0, 4, 2), (1, 1, 1), (600, 16, 2), (4000, 60, 6), (3000, 1024, 8), (9000, 8, 2), (20000, 1, 1), (300000, 3, 1)])
 def test_many_tokens(hip, T, E, k):
     g = synth.rng(T)
     x = g.standard_normal((T, E)).astype(np.float32)
