@@ -8,6 +8,7 @@
 //
 // The plan is a stable counting sort. A wave takes 64 assignments at a time and finds each one's rank among those of the same
 // expert from ballots over the id's bits, so no atomic's order has a say in the result.
+#include <algorithm>
 #include <type_traits>
 
 #include "byhip_mx.h"
@@ -548,56 +549,69 @@ struct CombineArgs {
     int T, k, E, N, res_dtype, y_dtype, vec;
 };
 
-template <int DT>
-__device__ __forceinline__ void read_cols(const void* p, size_t at, int left, int vec, float (&v)[4]) {
-    if (vec && left >= 4) {
-        load_vec<DT, 4>(p, at, v);
-    } else {
+template <int DT, int W>
+__device__ __forceinline__ void read_cols(const void* p, size_t at, int left, int vec, float (&v)[W]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = e < left ? load1<DT>(p, at + e) : 0.0f;
+    for (int q = 0; q < W; q += 4) {
+        float four[4];
+        if (vec && left >= W) {
+            load_vec<DT, 4>(p, at + q, four);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) four[e] = q + e < left ? load1<DT>(p, at + q + e) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q + e] = four[e];
     }
 }
 
-template <int XT>
+// W columns per thread: 16 bytes of a row where it is aligned so.
+template <int XT, int W>
 __global__ __launch_bounds__(256) void moe_combine(CombineArgs a) {
-    const int n = 4 * (blockIdx.x * 256 + threadIdx.x), left = a.N - n;
+    const int n = W * (blockIdx.x * 256 + threadIdx.x), left = a.N - n;
     if (left <= 0) return;
     for (int t = blockIdx.y; t < a.T; t += gridDim.y) {
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float s[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) s[e] = 0.0f;
         if (a.res) {
             const size_t at = (size_t)t * a.res_stride + n;
-            if (a.res_dtype == BYHIP_F32) read_cols<BYHIP_F32>(a.res, at, left, a.vec, s);
-            else if (a.res_dtype == BYHIP_F16) read_cols<BYHIP_F16>(a.res, at, left, a.vec, s);
-            else read_cols<BYHIP_BF16>(a.res, at, left, a.vec, s);
+            if (a.res_dtype == BYHIP_F32) read_cols<BYHIP_F32, W>(a.res, at, left, a.vec, s);
+            else if (a.res_dtype == BYHIP_F16) read_cols<BYHIP_F16, W>(a.res, at, left, a.vec, s);
+            else read_cols<BYHIP_BF16, W>(a.res, at, left, a.vec, s);
         }
-        // Eight rows' loads at a time, then their sums.
+        // Four rows' loads at a time, then their sums.
         const size_t first = (size_t)t * a.k;
-        for (int j0 = 0; j0 < a.k; j0 += 8) {
-            float w[8], v[8][4];
-            bool live[8];
+        for (int j0 = 0; j0 < a.k; j0 += 4) {
+            float w[4], v[4][W];
+            bool live[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 live[j] = j0 + j < a.k && (unsigned)a.ids[first + min(j0 + j, a.k - 1)] < (unsigned)a.E;
                 w[j] = a.weights[first + min(j0 + j, a.k - 1)];
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (live[j]) read_cols<XT>(a.x, (first + j0 + j) * a.x_stride + n, left, a.vec, v[j]);
+            for (int j = 0; j < 4; ++j)
+                if (live[j]) read_cols<XT, W>(a.x, (first + j0 + j) * a.x_stride + n, left, a.vec, v[j]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] = live[j] ? fmaf(w[j], v[j][e], s[e]) : s[e];
+                for (int e = 0; e < W; ++e) s[e] = live[j] ? fmaf(w[j], v[j][e], s[e]) : s[e];
         }
         const size_t at = (size_t)t * a.y_stride + n;
-        if (a.vec && left >= 4) {
-            store_vec<4>(a.y, at, s, a.y_dtype);
-        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < left) {
-                    const float one[1] = {s[e]};
-                    store_vec<1>(a.y, at + e, one, a.y_dtype);
-                }
+        for (int q = 0; q < W; q += 4) {
+            const float four[4] = {s[q], s[q + 1], s[q + 2], s[q + 3]};
+            if (a.vec && left >= W) {
+                store_vec<4>(a.y, at + q, four, a.y_dtype);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (q + e < left) {
+                        const float one[1] = {four[e]};
+                        store_vec<1>(a.y, at + q + e, one, a.y_dtype);
+                    }
+            }
         }
     }
 }
@@ -713,11 +727,12 @@ int byhip_moe_combine(const void* x, size_t x_stride, int x_dtype, int N, const 
         const int vec = aligned4(x, x_stride, x_dtype) && (!res || aligned4(res, res_stride, res_dtype)) && aligned4(y, y_stride, y_dtype);
         const CombineArgs a{x, ids, weights, res, y, x_stride, res_stride, y_stride, p.tokens, p.top_k, p.experts, N, res_dtype, y_dtype, vec};
         note_device_write(y);
-        const dim3 grid((N + 1023) / 1024, std::min(p.tokens, 65535));
+        const unsigned blocks = std::min(p.tokens, 65535);
+        const dim3 four((N + 1023) / 1024, blocks), eight((N + 2047) / 2048, blocks);
         switch (x_dtype) {
-        case BYHIP_F32: launch("moe_combine", moe_combine<BYHIP_F32>, grid, dim3(256), 0, a); break;
-        case BYHIP_F16: launch("moe_combine", moe_combine<BYHIP_F16>, grid, dim3(256), 0, a); break;
-        default: launch("moe_combine", moe_combine<BYHIP_BF16>, grid, dim3(256), 0, a); break;
+        case BYHIP_F32: launch("moe_combine", (moe_combine<BYHIP_F32, 4>), four, dim3(256), 0, a); break;
+        case BYHIP_F16: launch("moe_combine", (moe_combine<BYHIP_F16, 8>), eight, dim3(256), 0, a); break;
+        default: launch("moe_combine", (moe_combine<BYHIP_BF16, 8>), eight, dim3(256), 0, a); break;
         }
         BYHIP_LAUNCHED("moe_combine");
     });
