@@ -517,7 +517,7 @@ void launch_plan(const MoePlan& p, const int* ids) {
 template <int DT, int V, bool WIDE>
 void launch_route_v(const RouteArgs& a, const MoePlan& p) {
     // (A decode step's tokens and their plan in one block and one launch took longer: 12.4 us for 32 tokens of 128 experts, one CU's work,
-    // where the two launches take 10.)
+    // where the two launches take 8.)
     launch("moe_route", (moe_route<DT, V, WIDE>), dim3((a.T + kTokensPerBlock - 1) / kTokensPerBlock), dim3(64 * kTokensPerBlock), 0, a);
     BYHIP_LAUNCHED("moe_route");
     launch_plan(p, a.ids);

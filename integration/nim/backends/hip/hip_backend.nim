@@ -23,6 +23,10 @@ const
   BYHIP_F16* = 1.cint
   BYHIP_BF16* = 2.cint
   BYHIP_MXFP4_KM* = 3.cint
+  BYHIP_MXFP8_KM* = 4.cint
+  BYHIP_MOE_GATHER* = 1.cint
+  BYHIP_MOE_SCATTER* = 2.cint
+  BYHIP_MOE_SWIGLU* = 4.cint
 
 # Attention over a paged cache: the descriptors of include/byhip.h, field by field.
 type
@@ -51,6 +55,14 @@ type
     kind*: cint
     eps*: cfloat
     weight*, bias*: pointer
+  ByhipMoePlan* {.bycopy.} = object
+    tokens*, topK*, experts*: cint
+    plan*: pointer
+  ByhipMoeRouter* {.bycopy.} = object
+    score*: cint
+    bias*: pointer
+    groups*, topGroups*, groupBy*, renorm*: cint
+    scale*: cfloat
 
 {.push importc, cdecl, dynlib: HipLib.}
 proc byhip_init*(device: cint): cint
@@ -122,6 +134,18 @@ proc byhip_norm_block*(x: pointer, xStride: csize_t, xDtype, M, N: cint, post: p
                        gate: pointer, gateStride: csize_t, res: pointer, resStride: csize_t,
                        resScale: cfloat, h: pointer, hStride: csize_t, hDtype: cint,
                        pre: ptr ByhipNorm, y: pointer, yStride: csize_t, yDtype: cint): cint
+proc byhip_mx_quantize*(x: pointer, xStride: csize_t, xDtype, M, K: cint, y: pointer, yFormat: cint): cint
+proc byhip_mx_matmul*(x: pointer, xFormat: cint, w: pointer, M, K, N, flags: cint, y: pointer,
+                      yStride: csize_t, yDtype: cint): cint
+proc byhip_moe_plan_bytes*(tokens, topK, experts: cint): culonglong
+proc byhip_moe_route*(logits: pointer, stride: csize_t, dtype: cint, router: ptr ByhipMoeRouter,
+                      plan: ptr ByhipMoePlan, ids, weights: pointer): cint
+proc byhip_moe_plan_ids*(ids: pointer, plan: ptr ByhipMoePlan): cint
+proc byhip_moe_matmul*(x: pointer, xFormat: cint, w: pointer, plan: ptr ByhipMoePlan, K, N, flags: cint,
+                       y: pointer, yStride: csize_t, yDtype: cint): cint
+proc byhip_moe_combine*(x: pointer, xStride: csize_t, xDtype, N: cint, plan: ptr ByhipMoePlan,
+                        ids, weights, res: pointer, resStride: csize_t, resDtype: cint, y: pointer,
+                        yStride: csize_t, yDtype: cint): cint
 {.pop.}
 
 proc hipCheck*(rc: cint, what: string) =
@@ -296,4 +320,44 @@ proc hipSessionCacheGrow*(pool: var ByhipKvPool, rows, add: pointer, n: int): bo
 proc hipSessionCacheCompact*(pool: var ByhipKvPool): bool =
   let rc = byhip_cache_compact(addr pool, nil, nil)
   hipCheck(rc, "sessionCacheCompact")
+  rc == BYHIP_OK
+
+# ── A block of experts on microscaled weights (no counterpart in gpubackend.nim) ─────────────
+
+proc hipSessionNormBlockMx*(x: pointer, M, N: int, post: ptr ByhipNorm, gate, res: pointer,
+                            resScale: float32, h: pointer, pre: ptr ByhipNorm, y: pointer, fmt: cint): bool =
+  ## hipSessionNormBlock with y as microscaled rows
+  let rc = byhip_norm_block(x, csize_t(N), BYHIP_F32, M.cint, N.cint, post, gate, csize_t(N), res,
+                            csize_t(N), resScale.cfloat, h, csize_t(N), BYHIP_F32, pre, y, csize_t(N), fmt)
+  hipCheck(rc, "sessionNormBlockMx")
+  rc == BYHIP_OK
+
+proc hipSessionMxQuantize*(x: pointer, M, K: int, y: pointer, fmt: cint): bool =
+  let rc = byhip_mx_quantize(x, csize_t(K), BYHIP_F32, M.cint, K.cint, y, fmt)
+  hipCheck(rc, "sessionMxQuantize")
+  rc == BYHIP_OK
+
+proc hipSessionMxMatmul*(x: pointer, fmt: cint, w: pointer, M, K, N: int, y: pointer,
+                         yFmt = BYHIP_F32, swiglu = false): bool =
+  let rc = byhip_mx_matmul(x, fmt, w, M.cint, K.cint, N.cint, (if swiglu: BYHIP_MOE_SWIGLU else: 0.cint),
+                           y, csize_t(N), yFmt)
+  hipCheck(rc, "sessionMxMatmul")
+  rc == BYHIP_OK
+
+proc hipSessionMoeRoute*(logits: pointer, router: var ByhipMoeRouter, plan: var ByhipMoePlan,
+                         ids, weights: pointer): bool =
+  let rc = byhip_moe_route(logits, csize_t(plan.experts), BYHIP_F32, addr router, addr plan, ids, weights)
+  hipCheck(rc, "sessionMoeRoute")
+  rc == BYHIP_OK
+
+proc hipSessionMoeMatmul*(x: pointer, fmt: cint, w: pointer, plan: var ByhipMoePlan, K, N: int, flags: cint,
+                          y: pointer, yFmt = BYHIP_F32): bool =
+  let rc = byhip_moe_matmul(x, fmt, w, addr plan, K.cint, N.cint, flags, y, csize_t(N), yFmt)
+  hipCheck(rc, "sessionMoeMatmul")
+  rc == BYHIP_OK
+
+proc hipSessionMoeCombine*(x: pointer, N: int, plan: var ByhipMoePlan, ids, weights, res, y: pointer): bool =
+  let rc = byhip_moe_combine(x, csize_t(N), BYHIP_F32, N.cint, addr plan, ids, weights, res, csize_t(N),
+                             BYHIP_F32, y, csize_t(N), BYHIP_F32)
+  hipCheck(rc, "sessionMoeCombine")
   rc == BYHIP_OK
