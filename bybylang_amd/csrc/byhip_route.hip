@@ -100,7 +100,7 @@ __device__ __forceinline__ Two dpp_two(Two v) { return Two{dpp_d<CTRL>(v.one), d
 
 // The choices of token t by this wave. WIDE: keys in 64 bits (`group` holds E of them in LDS where groups are ranked).
 template <int DT, int V, bool WIDE>
-__device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* group, int* ids_out) {
+__device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* group) {
     const int lane = threadIdx.x & 63, e0 = lane * V;
     const size_t row = (size_t)t * a.stride;
     float x[V];
@@ -281,7 +281,6 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
                 if constexpr (WIDE) s = (float)score_d(mine);
                 else s = score_f(mine);
                 total += s;
-                ids_out[first + lane] = mine_id;
                 a.ids[(size_t)t * a.k + first + lane] = mine_id;
                 mine = s;
                 if (a.k > 64 || !a.renorm) a.weights[(size_t)t * a.k + first + lane] = s * (a.renorm ? 1.0f : a.scale);
@@ -306,7 +305,7 @@ __global__ __launch_bounds__(64 * kTokensPerBlock) void moe_route(RouteArgs a) {
     __shared__ double group[kTokensPerBlock][WIDE ? 64 * V : 32 * V];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.x * kTokensPerBlock + w;
     if (t >= a.T) return;
-    route_token<DT, V, WIDE>(a, t, group[w], a.ids + (size_t)t * a.k);
+    route_token<DT, V, WIDE>(a, t, group[w]);
 }
 
 // ── the plan ──
