@@ -260,12 +260,15 @@ __global__ __launch_bounds__(512, FM <= 2 ? 4 : 2) void gemm_f32_q4(GemmArgs a) 
     load(w[0], 0, 0);
     __builtin_amdgcn_sched_barrier(0);  // the first wait counts on this order
     load(w[1], 1, 1);
-    auto step = [&](int t, auto kc) __attribute__((always_inline)) {
+    // The last one or two steps load nothing and wait for everything: of loads that no step uses the compiler leaves the direct ones only, and a wait that
+    // counts them all would let the activations of the last step be read before they are there.
+    auto step = [&](int t, auto kc, auto tail) __attribute__((always_inline)) {
         constexpr int k = decltype(kc)::value;
-        wait_vmcnt<kLoads>();  // the loads of step t + 1 may stay in flight
+        constexpr bool more = !decltype(tail)::value;
+        wait_vmcnt<more ? kLoads : 0>();  // the loads of step t + 1 may stay in flight
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        load(w[(k + 2) % 3], t + 2, (k + 2) % 3);
+        if constexpr (more) load(w[(k + 2) % 3], t + 2, (k + 2) % 3);
         const float s = __builtin_bit_cast(float, w[k].s), z = ZU ? a.zero_value : __builtin_bit_cast(float, w[k].z);
         const uint8_t* const x = lds + k * S::kBuf + 512 * c;
 #pragma unroll
@@ -294,9 +297,9 @@ __global__ __launch_bounds__(512, FM <= 2 ? 4 : 2) void gemm_f32_q4(GemmArgs a) 
         __builtin_amdgcn_sched_barrier(0);
     };
     int t = 0;
-    for (; t + 3 <= nt; t += 3) static_for<3>([&](auto kc) { step(t + decltype(kc)::value, kc); });
+    for (; t + 3 <= nt; t += 3) static_for<3>([&](auto kc) { step(t + decltype(kc)::value, kc, std::false_type{}); });
     static_for<2>([&](auto kc) {
-        if (t + decltype(kc)::value < nt) step(t + decltype(kc)::value, kc);
+        if (t + decltype(kc)::value < nt) step(t + decltype(kc)::value, kc, std::true_type{});
     });
     wait_vmcnt<0>();
 
