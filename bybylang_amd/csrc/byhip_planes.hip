@@ -322,7 +322,8 @@ __global__ __launch_bounds__(512, FM == 1 || (FM == 2 && F == BFormat::Fp4Km) ? 
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<issued((k + 7) % 8) + issued(k)>();
+        // In the last, guarded steps the compiler leaves out register loads that no step uses: there only the activations' are counted on.
+        wait_vmcnt<decltype(guard)::value ? 2 * kXLoads : issued((k + 7) % 8) + issued(k)>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         if (live) {

@@ -1,6 +1,7 @@
-"""gemm_f32_q4 keeps the loads of a step in flight by counting them. In its last steps nothing follows that would use loads two steps
+"""gemm_f32_q4 and gemm_planes keep the loads of a step or two in flight by counting them. In their last steps nothing follows that would use loads two steps
 ahead; the compiler drops such loads into registers but not those into LDS, so a count of them all lets a barrier pass before the last
-step's activations are in LDS. This reads the compiled kernels: the loop's three barriers leave a step's loads in flight, the two of the last steps none.
+step's activations are in LDS. This reads the compiled kernels: the loop's three barriers leave a step's loads in flight, the two of the last steps none; gemm_planes' eight
+last steps leave no more than the direct loads of two.
 CPU only: it needs the build's objects and binutils."""
 import os
 import re
@@ -40,3 +41,18 @@ def test_last_steps_wait_for_their_activations(tmp_path):
         loads = int(m.group(1)) + 2 + (1 - int(m.group(2)))
         assert sorted(waits) == [0, 0] + [loads] * 3, f"{name}: {waits}"
     assert seen == 8
+
+
+def test_guarded_steps_count_direct_loads_only(tmp_path):
+    path = os.path.join(BUILD, "byhip_planes.hip.o")
+    if not (os.path.exists(path) and shutil.which("objcopy") and os.path.exists(LLVM + "/llvm-objdump")):
+        pytest.skip("the build's objects or binutils are not there")
+    seen = 0
+    for name, waits in barriers(path, tmp_path).items():
+        m = re.search(r"11gemm_planesILNS_\w*?BFormatE\dELi(\d)E", name)
+        if not m:
+            continue
+        seen += 1
+        few = [w for w in waits if w is not None and w <= 2 * int(m.group(1))]
+        assert len(few) >= 8, f"{name}: {waits}"
+    assert seen >= 8
