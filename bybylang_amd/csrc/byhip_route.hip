@@ -120,6 +120,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
     float top = 0.0f, sum = 1.0f;
     double sum_d = 1.0;
     const bool soft = a.score == BYHIP_MOE_SOFTMAX;
+    bool nan_row = false;  // a softmax over a NaN
     auto lift = [&](float v) { return v == top ? 0.0f : v - top; };
     if (soft) {
         uint32_t most = 0;
@@ -130,9 +131,8 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
             nan = nan || x[i] != x[i];
         }
         top = key_value(wave_max(most));
-        if (!WIDE && a.renorm) {
-            sum = __any(nan) ? NAN : 1.0f;  // it falls out of the weights
-        } else {
+        nan_row = __any(nan);
+        if (WIDE || !a.renorm) {  // (it falls out of renormalised weights)
             float s = 0.0f;
             double sd = 0.0;
 #pragma unroll
@@ -144,7 +144,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
             if constexpr (WIDE) { sum_d = wave_sumd(sd); sum = (float)sum_d; }
             else sum = lane_sum(s);
         }
-        if (top == -INFINITY && !__any(nan)) { sum = INFINITY; sum_d = (double)INFINITY; }
+        if (top == -INFINITY && !nan_row) { sum = INFINITY; sum_d = (double)INFINITY; }
     }
     auto score_f = [&](float v) { return soft ? expf(lift(v)) / sum : 1.0f / (1.0f + expf(-v)); };
     const double over_sum = soft ? 1.0 / sum_d : 1.0;
@@ -233,7 +233,6 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
             if (e0 + i >= a.E || !(mine_in || ((in >> ((e0 + i) / size)) & 1))) key[i] = 0u;
     }
     // Rounds: the largest head; of several, in 64 bits the largest, then the lowest index (the lowest lane).
-    float mine = 0.0f, total = 0.0f;
     int mine_id = 0;
     uint32_t head = 0;
     double head_wide = 0.0;
@@ -272,30 +271,59 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
             for (int i = 0; i < V; ++i) key[i] = i == pick ? 0u : key[i];
             find_head();
         }
-        // 64 choices at most are held; the weights of more are formed in a second turn (below).
+        // 64 choices at most are held.
         if ((j & 63) == 63 || j + 1 == a.k) {
-            const int first = j & ~63, n = j - first + 1;
-            if (lane < n) {
-                mine = load1<DT>(a.logits, row + mine_id);
-                float s;
-                if constexpr (WIDE) s = (float)score_d(mine);
-                else s = score_f(mine);
-                total += s;
-                a.ids[(size_t)t * a.k + first + lane] = mine_id;
-                mine = s;
-                if (a.k > 64 || !a.renorm) a.weights[(size_t)t * a.k + first + lane] = s * (a.renorm ? 1.0f : a.scale);
+            const int i = (j & ~63) + lane;
+            if (i <= j) {
+                a.ids[(size_t)t * a.k + i] = mine_id;
+                if (!a.renorm) {
+                    const float v = load1<DT>(a.logits, row + mine_id);
+                    float s;
+                    if constexpr (WIDE) s = (float)score_d(v);
+                    else s = score_f(v);
+                    a.weights[(size_t)t * a.k + i] = s * a.scale;
+                }
             }
         }
     }
-    if (a.renorm) {
-        total = lane_sum(total);
-        const float f = total == 0.0f ? 0.0f : a.scale / total;
-        if (a.k <= 64) {
-            if (lane < a.k) a.weights[(size_t)t * a.k + lane] = total == 0.0f ? 0.0f : mine * f;
-        } else {
-            for (int i = lane; i < a.k; i += 64) a.weights[(size_t)t * a.k + i] *= f;
+    if (!a.renorm) return;
+    // Renormalised: scores of any size over their sum. They are taken relative to e^ref, ref the largest chosen logit (of a sigmoid where that is below 0), so
+    // that the largest is 1/2 or more and neither it nor the sum vanishes where every score does in 32 bits.
+    float v[4];  // choices lane, lane + 64, ..
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        v[c] = -INFINITY;
+        const int i = 64 * c + lane;
+        if (64 * c < a.k && i < a.k) {
+            v[c] = load1<DT>(a.logits, row + (a.k <= 64 ? mine_id : a.ids[(size_t)t * a.k + i]));
+            most = max(most, order_key(v[c]));
         }
     }
+    const float largest = key_value(wave_max(most)), ref = soft ? largest : fminf(largest, 0.0f);
+    auto share = [&](float x) {
+        if constexpr (WIDE) {
+            const double e = x == ref ? 0.0 : (double)x - (double)ref;
+            return (float)(soft ? exp(e) : ref < 0.0f ? exp(e) * reciprocal(1.0 + exp((double)x)) : reciprocal(1.0 + exp(-(double)x)));
+        } else {
+            const float e = x == ref ? 0.0f : x - ref;
+            return soft ? expf(e) : ref < 0.0f ? expf(e) / (1.0f + expf(x)) : 1.0f / (1.0f + expf(-x));
+        }
+    };
+    float total = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (64 * c < a.k && 64 * c + lane < a.k) {
+            v[c] = share(v[c]);
+            total += v[c];
+        }
+    total = nan_row ? NAN : lane_sum(total);
+    // Below e^-708 a score is taken for 0 (64-bit numbers end there), and so are the weights where all are.
+    const float above = soft && largest != -INFINITY ? (largest == top ? 0.0f : largest - top) : largest;
+    const float f = total != total ? total : above < -708.0f ? 0.0f : a.scale / total;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (64 * c < a.k && 64 * c + lane < a.k) a.weights[(size_t)t * a.k + 64 * c + lane] = v[c] * f;
 }
 
 constexpr int kTokensPerBlock = 4;
