@@ -160,7 +160,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
             double c = -(double)INFINITY;
             if (e0 + i < a.E) c = score_d(x[i]) + (a.bias ? (double)a.bias[e0 + i] : 0.0);
             wide[i] = c;
-            key[i] = e0 + i < a.E ? order_key((float)c) : 0u;
+            key[i] = e0 + i < a.E ? order_key(a.bias ? (float)c : x[i]) : 0u;
         } else {
             key[i] = e0 + i < a.E ? order_key(x[i]) : 0u;
         }
@@ -255,7 +255,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
         const uint32_t best = wave_max(head);
         uint64_t who = __ballot(head == best);
         if constexpr (WIDE) {
-            if (__popcll(who) > 1 && best > 1u) {
+            if (a.bias && __popcll(who) > 1 && best > 1u) {
                 const double c = head == best ? head_wide : -(double)INFINITY;
                 double m = c;
 #pragma unroll
