@@ -98,6 +98,12 @@ __device__ __forceinline__ double dpp_d(double v) {
 template <int CTRL>
 __device__ __forceinline__ Two dpp_two(Two v) { return Two{dpp_d<CTRL>(v.one), dpp_d<CTRL>(v.two)}; }
 
+// What a group's two largest keys make it worth: their sum that is no number (infinities of both signs) comes last, as such keys do.
+__device__ __forceinline__ double group_worth(const RouteArgs& a, int size, double one, double two) {
+    const double sum = a.group_by == 2 && size > 1 ? one + two : one;
+    return sum == sum ? sum : -(double)INFINITY;
+}
+
 // The choices of token t by this wave. WIDE: keys in 64 bits (`group` holds E of them in LDS where groups are ranked).
 template <int DT, int V, bool WIDE>
 __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* group) {
@@ -182,7 +188,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
                 if (span > 2) best = merge(best, dpp_two<0x4E>(best));
                 if (span > 4) best = merge(best, dpp_two<0x141>(best));
                 if (span > 8) best = merge(best, dpp_two<0x140>(best));
-                const double worth = a.group_by == 2 && size > 1 ? best.one + best.two : best.one;
+                const double worth = group_worth(a, size, best.one, best.two);
                 const int own = lane / span;
                 int above = 0;
                 for (int g = 0; g < a.groups; ++g) {
@@ -202,7 +208,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, double* g
                         if (c > one) { two = one; one = c; }
                         else if (c > two) two = c;
                     }
-                const double worth = a.group_by == 2 && size > 1 ? one + two : one;
+                const double worth = group_worth(a, size, one, two);
                 int above = 0;
                 for (int g = 0; g < a.groups; ++g) {
                     const double o = lane_d(worth, g);

@@ -476,7 +476,7 @@ enum byhip_moe_score { BYHIP_MOE_SOFTMAX = 0, BYHIP_MOE_SIGMOID = 1 };
 /* How logits become choices. score = softmax over the experts or sigmoid; key = score + bias (device, fp32
  * [experts], or NULL). With groups > 1 (at most 64, dividing experts) only the top_groups best groups take part, by the sum
  * of their group_by (1 or 2) largest keys. The top_k largest keys are chosen, ties to the lowest index; keys
- * that are NaN come last. Their weights are score (/ the sum over the chosen, with renorm) * scale, renormalised ones also where the
+ * and sums that are NaN come last. Their weights are score (/ the sum over the chosen, with renorm) * scale, renormalised ones also where the
  * scores themselves vanish in fp32. Where no chosen logit is above -708 (sigmoid) or less than 708 below the row's largest (softmax), masked
  * rows among them, and in rows of -infinity, renormalised weights are 0. Keys are compared in 64 bits,
  * without a bias as the logits themselves (groups by their two best as sums of 64-bit scores then too). */

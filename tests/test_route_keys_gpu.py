@@ -44,3 +44,20 @@ def test_a_row_with_a_nan_keeps_different_experts(hip, E, groups, top_groups):
         for score in (SOFT, SIG):
             ids, _ = routed(hip, x, F32, 7, score=score, bias=bias, groups=groups, top_groups=top_groups, group_by=2)
             assert all(len(set(r)) == 7 and min(r) >= 0 and max(r) < E for r in ids.tolist())
+
+
+@pytest.mark.parametrize("E,groups", [(32, 4), (60, 4), (256, 8)])
+@pytest.mark.parametrize("at", [0, 1, 3])
+def test_a_group_of_both_infinities(hip, E, groups, at):
+    """A bias that holds +infinity beside -infinity makes a group's sum NaN: that group comes last, and no group more than asked for takes part."""
+    g = synth.rng(E + at)
+    size, k = E // groups, 6
+    b = (0.3 * g.standard_normal(E)).astype(np.float32)
+    b[at * size:(at + 1) * size] = -np.inf
+    b[at * size + 2] = np.inf
+    x = g.standard_normal((9, E)).astype(np.float32)
+    ids, _ = routed(hip, x, F32, k, score=SIG, bias=b, groups=groups, top_groups=2, group_by=2)
+    for t, row in enumerate(x.astype(np.float64)):
+        key = 1 / (1 + np.exp(-row)) + b
+        worth = [-np.inf if i == at else np.sort(key[i * size:(i + 1) * size])[-2:].sum() for i in range(groups)]
+        assert ids[t].tolist() == chosen(row, worth, groups, 2, k, key), t
