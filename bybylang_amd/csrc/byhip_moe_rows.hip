@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     __shared__ float4 part[kWaves][NF * MT][64];
     MoeUnit u;
     int strip;
-    if (!MoeTiles(a).find(a, blockIdx.x >> 3, u, strip)) return;
+    if (!MoeTiles(a).find(a, blockIdx.x >> 3, u, strip) || u.rows == 0) return;
     constexpr bool eight = XF == BYHIP_MXFP8_KM;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const uint32_t kb = (uint32_t)a.K / 2, xb = eight ? (uint32_t)a.K : kb;
@@ -91,151 +91,148 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     for (int f = 0; f < NF; ++f) n[f] = GLU ? (f >> 1) * a.N + n0 + 16 * (f & 1) + c : n0 + 16 * f + c;
     const int windows = (a.KG + 4 * S - 1) / (4 * S);
 
-    for (int m0 = 0; m0 < u.rows; m0 += 16 * MT) {
-        uint32_t x_at[MT], xs_at[MT];
+    uint32_t x_at[MT], xs_at[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int i = 16 * m + c;
+        const int row = i < u.rows ? moe_x_row(a, u.first + i) : -1;
+        x_at[m] = row < 0 ? kOutOfRange : (uint32_t)row * xb;
+        xs_at[m] = row < 0 ? kOutOfRange : (uint32_t)row * a.KG;
+    }
+    f4v acc[NF][MT];
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const int i = m0 + 16 * m + c;
-            const int row = i < u.rows ? moe_x_row(a, u.first + i) : -1;
-            x_at[m] = row < 0 ? kOutOfRange : (uint32_t)row * xb;
-            xs_at[m] = row < 0 ? kOutOfRange : (uint32_t)row * a.KG;
+            acc[f][m] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            // A product whose addend is the constant 0 may be given a result that overlaps its operands, which it then misreads:
+            // the zeros stay in registers.
+            asm volatile("" : "+v"(acc[f][m]));
         }
-        f4v acc[NF][MT];
+    for (int W = w; W < windows; W += kWaves) {
+        const int G = 4 * S * W;  // the window's first group
+        v4u wv[NF][S];
+        Scales<S> wsv[NF];
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
+        for (int f = 0; f < NF; ++f) {
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                wv[f][s] = load16(wr, n[f] < a.R && G + 4 * s + g < a.KG ? (uint32_t)n[f] * kb + 16 * (G + 4 * s + g) : kOutOfRange);
+            wsv[f] = load_scales<S, WORDS>(wsr, n[f] < a.R ? (uint32_t)n[f] * a.KG : kOutOfRange, G, g, a.KG);
+        }
+        Scales<S> xsv[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xsv[m] = load_scales<S, WORDS>(xsr, xs_at[m], G, g, a.KG);
+        // The rows' values go one step ahead of the products where a window has four (48 tokens, 128 experts, 2048 to 768: 31 us for 34; with
+        // two, 768 to 2048: 23.0 for 22.5).
+        constexpr bool ahead = S == 4;
+        auto load_x = [&](int T, v8i (&x)[MT]) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                acc[f][m] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-                // A product whose addend is the constant 0 may be given a result that overlaps its operands, which it then misreads:
-                // the zeros stay in registers.
-                asm volatile("" : "+v"(acc[f][m]));
-            }
-        for (int W = w; W < windows; W += kWaves) {
-            const int G = 4 * S * W;  // the window's first group
-            v4u wv[NF][S];
-            Scales<S> wsv[NF];
+                x[m] = v8i{0, 0, 0, 0, 0, 0, 0, 0};
+                if constexpr (eight) {
+                    const int g0 = G + 4 * T + (g >> 1), g1 = g0 + 2;
+                    const v4u p = load16(xr, x_at[m] != kOutOfRange && g0 < a.KG ? x_at[m] + 32 * g0 + 16 * (g & 1) : kOutOfRange);
+                    const v4u q = load16(xr, x_at[m] != kOutOfRange && g1 < a.KG ? x_at[m] + 32 * g1 + 16 * (g & 1) : kOutOfRange);
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
+                    for (int e = 0; e < 4; ++e) { x[m][e] = (int)p[e]; x[m][4 + e] = (int)q[e]; }
+                } else {
+                    const v4u p = load16(xr, x_at[m] != kOutOfRange && G + 4 * T + g < a.KG ? x_at[m] + 16 * (G + 4 * T + g) : kOutOfRange);
 #pragma unroll
-                for (int s = 0; s < S; ++s)
-                    wv[f][s] = load16(wr, n[f] < a.R && G + 4 * s + g < a.KG ? (uint32_t)n[f] * kb + 16 * (G + 4 * s + g) : kOutOfRange);
-                wsv[f] = load_scales<S, WORDS>(wsr, n[f] < a.R ? (uint32_t)n[f] * a.KG : kOutOfRange, G, g, a.KG);
-            }
-            Scales<S> xsv[MT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) xsv[m] = load_scales<S, WORDS>(xsr, xs_at[m], G, g, a.KG);
-            // The rows' values go one step ahead of the products where a window has four (48 tokens, 128 experts, 2048 to 768: 31 us for 34; with
-            // two, 768 to 2048: 23.0 for 22.5).
-            constexpr bool ahead = S == 4;
-            auto load_x = [&](int T, v8i (&x)[MT]) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    x[m] = v8i{0, 0, 0, 0, 0, 0, 0, 0};
-                    if constexpr (eight) {
-                        const int g0 = G + 4 * T + (g >> 1), g1 = g0 + 2;
-                        const v4u p = load16(xr, x_at[m] != kOutOfRange && g0 < a.KG ? x_at[m] + 32 * g0 + 16 * (g & 1) : kOutOfRange);
-                        const v4u q = load16(xr, x_at[m] != kOutOfRange && g1 < a.KG ? x_at[m] + 32 * g1 + 16 * (g & 1) : kOutOfRange);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) { x[m][e] = (int)p[e]; x[m][4 + e] = (int)q[e]; }
-                    } else {
-                        const v4u p = load16(xr, x_at[m] != kOutOfRange && G + 4 * T + g < a.KG ? x_at[m] + 16 * (G + 4 * T + g) : kOutOfRange);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[m][e] = (int)p[e];
-                    }
+                    for (int e = 0; e < 4; ++e) x[m][e] = (int)p[e];
                 }
-            };
-            v8i xv[2][MT];
-            if constexpr (ahead) load_x(0, xv[0]);
-            uint32_t ws[NF], xs[MT];
-            auto step = [&](auto Sc) {
-                constexpr int T = decltype(Sc)::value;
-                if constexpr (!ahead) load_x(T, xv[T & 1]);
-                else if constexpr (T + 1 < S) load_x(T + 1, xv[(T + 1) & 1]);
-                if constexpr (T == 0) {
-                    if constexpr (ahead) __builtin_amdgcn_sched_barrier(0);  // the loads are out
-#pragma unroll
-                    for (int f = 0; f < NF; ++f) ws[f] = pick_scales<S, WORDS>(wsv[f], G, g, a.KG);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) xs[m] = pick_scales<S, WORDS>(xsv[m], G, g, a.KG);
-                }
-                v8i large[MT], small[FINE ? MT : 1];
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    if constexpr (FINE) split_bytes(xv[T & 1][m], large[m], small[m]);
-                    else large[m] = xv[T & 1][m];
-                }
-#pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    const v8i wf = {(int)wv[f][T][0], (int)wv[f][T][1], (int)wv[f][T][2], (int)wv[f][T][3], 0, 0, 0, 0};
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        if constexpr (FINE) acc[f][m] = product<XF, T>(wf, small[m], acc[f][m], (int)ws[f], (int)xs[m]);
-                        acc[f][m] = product<XF, T>(wf, large[m], acc[f][m], (int)ws[f], (int)xs[m]);
-                    }
-                }
-            };
-            step(std::integral_constant<int, 0>{});
-            step(std::integral_constant<int, 1>{});
-            if constexpr (S > 2) {
-                step(std::integral_constant<int, 2>{});
-                step(std::integral_constant<int, 3>{});
-            }
-        }
-        __syncthreads();  // the sums of the rows before are read
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) part[w][f * MT + m][lane] = make_float4(acc[f][m][0], acc[f][m][1], acc[f][m][2], acc[f][m][3]);
-        __syncthreads();
-        auto whole = [&](int f, int m, float (&v)[4]) {
-            v[0] = v[1] = v[2] = v[3] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kWaves; ++i) {
-                const float4 p = part[i][f * MT + m][lane];
-                v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
             }
         };
-        if constexpr (GLU) {
-            for (int m = w; m < MT; m += kWaves) {
-                const int i = m0 + 16 * m + c;
-                float gate[4], up[4], h[2][4];
+        v8i xv[2][MT];
+        if constexpr (ahead) load_x(0, xv[0]);
+        uint32_t ws[NF], xs[MT];
+        auto step = [&](auto Sc) {
+            constexpr int T = decltype(Sc)::value;
+            if constexpr (!ahead) load_x(T, xv[T & 1]);
+            else if constexpr (T + 1 < S) load_x(T + 1, xv[(T + 1) & 1]);
+            if constexpr (T == 0) {
+                if constexpr (ahead) __builtin_amdgcn_sched_barrier(0);  // the loads are out
 #pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    whole(f, m, gate);
-                    whole(2 + f, m, up);
+                for (int f = 0; f < NF; ++f) ws[f] = pick_scales<S, WORDS>(wsv[f], G, g, a.KG);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) h[f][e] = swiglu(gate[e], up[e]);
-                }
-                const bool there = i < u.rows;
-                const size_t row = there ? moe_y_row(a, u.first + i) : 0;
-                if (is_mx_out(a.y_dtype)) {
-                    uint32_t mag = mag8(h[0], h[1]);
-                    mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
-                    mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
-                    if (there) store_group(a, row, strip, 4 * g, g == 0, mag, h[0], h[1]);
-                } else if (there) {
-                    moe_store4(a, row, n0 + 4 * g, h[0]);
-                    moe_store4(a, row, n0 + 16 + 4 * g, h[1]);
+                for (int m = 0; m < MT; ++m) xs[m] = pick_scales<S, WORDS>(xsv[m], G, g, a.KG);
+            }
+            v8i large[MT], small[FINE ? MT : 1];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if constexpr (FINE) split_bytes(xv[T & 1][m], large[m], small[m]);
+                else large[m] = xv[T & 1][m];
+            }
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const v8i wf = {(int)wv[f][T][0], (int)wv[f][T][1], (int)wv[f][T][2], (int)wv[f][T][3], 0, 0, 0, 0};
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if constexpr (FINE) acc[f][m] = product<XF, T>(wf, small[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                    acc[f][m] = product<XF, T>(wf, large[m], acc[f][m], (int)ws[f], (int)xs[m]);
                 }
             }
-        } else if (NF > 1 && is_mx_out(a.y_dtype)) {
-            for (int p = w; p < MT * (NF / 2); p += kWaves) {
-                const int m = p / (NF > 1 ? NF / 2 : 1), q = p % (NF > 1 ? NF / 2 : 1), i = m0 + 16 * m + c;
-                float h[2][4];
-                whole(2 * q, m, h[0]);
-                whole(NF > 1 ? 2 * q + 1 : 0, m, h[1]);
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        if constexpr (S > 2) {
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) part[w][f * MT + m][lane] = make_float4(acc[f][m][0], acc[f][m][1], acc[f][m][2], acc[f][m][3]);
+    __syncthreads();
+    auto whole = [&](int f, int m, float (&v)[4]) {
+        v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const float4 p = part[i][f * MT + m][lane];
+            v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+        }
+    };
+    if constexpr (GLU) {
+        for (int m = w; m < MT; m += kWaves) {
+            const int i = 16 * m + c;
+            float gate[4], up[4], h[2][4];
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                whole(f, m, gate);
+                whole(2 + f, m, up);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[f][e] = swiglu(gate[e], up[e]);
+            }
+            const bool there = i < u.rows;
+            const size_t row = there ? moe_y_row(a, u.first + i) : 0;
+            if (is_mx_out(a.y_dtype)) {
                 uint32_t mag = mag8(h[0], h[1]);
                 mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
                 mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
-                if (i < u.rows && n0 + 32 * q < a.N) store_group(a, moe_y_row(a, u.first + i), n0 / 32 + q, 4 * g, g == 0, mag, h[0], h[1]);
+                if (there) store_group(a, row, strip, 4 * g, g == 0, mag, h[0], h[1]);
+            } else if (there) {
+                moe_store4(a, row, n0 + 4 * g, h[0]);
+                moe_store4(a, row, n0 + 16 + 4 * g, h[1]);
             }
-        } else {
-            for (int p = w; p < MT * NF; p += kWaves) {
-                const int m = p / NF, f = p % NF, i = m0 + 16 * m + c;
-                float v[4];
-                whole(f, m, v);
-                if (i < u.rows) moe_store4(a, moe_y_row(a, u.first + i), n0 + 16 * f + 4 * g, v);
-            }
+        }
+    } else if (NF > 1 && is_mx_out(a.y_dtype)) {
+        for (int p = w; p < MT * (NF / 2); p += kWaves) {
+            const int m = p / (NF > 1 ? NF / 2 : 1), q = p % (NF > 1 ? NF / 2 : 1), i = 16 * m + c;
+            float h[2][4];
+            whole(2 * q, m, h[0]);
+            whole(NF > 1 ? 2 * q + 1 : 0, m, h[1]);
+            uint32_t mag = mag8(h[0], h[1]);
+            mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+            mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+            if (i < u.rows && n0 + 32 * q < a.N) store_group(a, moe_y_row(a, u.first + i), n0 / 32 + q, 4 * g, g == 0, mag, h[0], h[1]);
+        }
+    } else {
+        for (int p = w; p < MT * NF; p += kWaves) {
+            const int m = p / NF, f = p % NF, i = 16 * m + c;
+            float v[4];
+            whole(f, m, v);
+            if (i < u.rows) moe_store4(a, moe_y_row(a, u.first + i), n0 + 16 * f + 4 * g, v);
         }
     }
 }
@@ -274,6 +271,8 @@ void launch_rows_n(const MoeArgs& a, int max_units) {
 
 template <int XF, bool GLU, bool FINE>
 void launch_rows(const MoeArgs& a, int max_units) {
+    // A block takes all of its unit's rows at once.
+    if (a.unit_rows > 64) fail("byhip: internal: units of %d rows", a.unit_rows);
     if (a.unit_rows <= 16) launch_rows_n<XF, 1, GLU, FINE>(a, max_units);
     else if (a.unit_rows <= 32) launch_rows_n<XF, 2, GLU, FINE>(a, max_units);
     else launch_rows_n<XF, 4, GLU, FINE>(a, max_units);
