@@ -23,9 +23,6 @@ struct MoeArgs {
     uint32_t per_token;       // 2^32 / top_k, rounded up (top_k > 1)
 };
 
-// Whether a call's products keep fp32's precision: what is rounded to 16 bits or fewer afterwards does not need it.
-inline bool moe_fine(int x_format, int y_dtype) { return x_format == BYHIP_MXFP8_KM && y_dtype == BYHIP_F32; }
-
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 

@@ -12,11 +12,10 @@
 // window are block g of a step is free as long as both operands agree: step s takes groups 4 s .. 4 s + 3 of the window's 4 S, so
 // that four lanes read 64 neighbouring bytes of a row (with group S g + s, 16 bytes of each 64 at a time: 37 us, 48 tokens, 128 experts, 2048 to 768, for 31). The result: lane (c, g) holds row c of x, matrix rows 4 g .. 4 g + 3.
 //
-// Sums are fp32. What the instructions add in one go is exact with rows in 4 bits; with rows in 8 bits they cut small products off
-// (split_bytes), which leaves 5e-6 to 1e-5 of a product's norm: less than a hundredth of the rounding to 16 bits or fewer that follows. (Of outputs
-// in 8 bits one in a thousand then takes the step next to its own: 0.0023 of their norm, where the steps' rounding is 0.026. In two parts they would take
-// half as long again in moe_tiles: 4096 tokens, 6 of 64 experts, 2048 to 1408, 242 us for 153.)
-// With fp32 outputs (FINE) rows go in two parts, twice the products (in this kernel they wait for memory).
+// Sums are fp32. What the instructions add in one go is exact with rows in 4 bits; with rows in 8 bits they cut small products off, so those rows go in two
+// parts (split_bytes), twice the products. With outputs of 16 bits or fewer one part would do for most rows (5e-6 to 1e-5 of a product's norm is cut off then), but not for
+// rows whose large terms cancel, and it saves little here (us, one part: 48 tokens, 128 experts, 2048 to 768 31.4 for 29.4, 800 to 2048 with 400 tokens
+// 46 for 37; 1 / 16 / 64 rows of 4096 x 4096 5.1 / 5.8 / 10.8 for 4.8 / 5.5 / 9.9).
 #include "byhip_moe.h"
 
 namespace byhip {
@@ -72,7 +71,7 @@ __device__ __forceinline__ f4v product(v8i w, v8i x, f4v c, int sw, int sx) {
 }
 
 // MT blocks of 16 rows, NF blocks of 16 matrix rows (GLU: two of gates, two of ups), windows of S steps.
-template <int XF, int MT, int NF, int S, bool WORDS, bool GLU, bool FINE>
+template <int XF, int MT, int NF, int S, bool WORDS, bool GLU>
 __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     static_assert(!GLU || NF == 4, "gates and ups");
     __shared__ float4 part[kWaves][NF * MT][64];
@@ -157,10 +156,10 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) xs[m] = pick_scales<S, WORDS>(xsv[m], G, g, a.KG);
             }
-            v8i large[MT], small[FINE ? MT : 1];
+            v8i large[MT], small[eight ? MT : 1];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                if constexpr (FINE) split_bytes(xv[T & 1][m], large[m], small[m]);
+                if constexpr (eight) split_bytes(xv[T & 1][m], large[m], small[m]);
                 else large[m] = xv[T & 1][m];
             }
 #pragma unroll
@@ -168,7 +167,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
                 const v8i wf = {(int)wv[f][T][0], (int)wv[f][T][1], (int)wv[f][T][2], (int)wv[f][T][3], 0, 0, 0, 0};
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    if constexpr (FINE) acc[f][m] = product<XF, T>(wf, small[m], acc[f][m], (int)ws[f], (int)xs[m]);
+                    if constexpr (eight) acc[f][m] = product<XF, T>(wf, small[m], acc[f][m], (int)ws[f], (int)xs[m]);
                     acc[f][m] = product<XF, T>(wf, large[m], acc[f][m], (int)ws[f], (int)xs[m]);
                 }
             }
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_rows(MoeArgs a) {
     }
 }
 
-template <int XF, int MT, int NF, bool GLU, bool FINE>
+template <int XF, int MT, int NF, bool GLU>
 void launch_rows_as(MoeArgs a, int max_units) {
     const int wide = GLU ? 32 : 16 * NF;
     a.strips = (a.N + wide - 1) / wide;
@@ -247,44 +246,42 @@ void launch_rows_as(MoeArgs a, int max_units) {
     // / 768 / 1024 / 1408 / 1536: 15.2 / 18.1 / 24.5 / 27.0 / 23.4 us for 18.0 / 21.6 / 25.8 / 29.4 / 24.5; K = 2048: 32.9 for 33.1, and for one
     // token 7.5 for 6.8. Windows of 128 took longer than those of 256 but for K = 1408, 26.2).
     const dim3 grid((unsigned)blocks), block(64 * kWaves);
-    if (a.KG & 3) launch("moe_rows", (moe_rows<XF, MT, NF, 2, false, GLU, FINE>), grid, block, 0, a);
-    else if (a.KG > 48) launch("moe_rows", (moe_rows<XF, MT, NF, 4, true, GLU, FINE>), grid, block, 0, a);
-    else launch("moe_rows", (moe_rows<XF, MT, NF, 2, true, GLU, FINE>), grid, block, 0, a);
+    if (a.KG & 3) launch("moe_rows", (moe_rows<XF, MT, NF, 2, false, GLU>), grid, block, 0, a);
+    else if (a.KG > 48) launch("moe_rows", (moe_rows<XF, MT, NF, 4, true, GLU>), grid, block, 0, a);
+    else launch("moe_rows", (moe_rows<XF, MT, NF, 2, true, GLU>), grid, block, 0, a);
     BYHIP_LAUNCHED("moe_rows");
 }
 
 // Strips of 64, 32 or 16 outputs: the widest that gives most CUs a block, for rows are read once per strip (16 rows, K = 4096, N = 4096: 64 strips of
 // 64 9.7 us, 128 of 32 7.4, 256 of 16 5.8; N = 14336: 224 of 64 11.4 us, 448 of 32 12.9). Gates and ups have 32 each. Eight waves per block took as long where
 // one unit's strips are all there is (9.8 us for 10.5 at N = 14336, 9.6 for 9.7), longer elsewhere (33 us for 41, 48 tokens, 128 experts).
-template <int XF, int MT, bool GLU, bool FINE>
+template <int XF, int MT, bool GLU>
 void launch_rows_n(const MoeArgs& a, int max_units) {
     if constexpr (!GLU) {
         const long long strips = (a.N + 15) / 16, room = 200;
         if (strips / 4 * max_units < room) {
-            if (strips / 2 * max_units < room && !is_mx(a.y_dtype)) launch_rows_as<XF, MT, 1, GLU, FINE>(a, max_units);
-            else launch_rows_as<XF, MT, 2, GLU, FINE>(a, max_units);
+            if (strips / 2 * max_units < room && !is_mx(a.y_dtype)) launch_rows_as<XF, MT, 1, GLU>(a, max_units);
+            else launch_rows_as<XF, MT, 2, GLU>(a, max_units);
             return;
         }
     }
-    launch_rows_as<XF, MT, 4, GLU, FINE>(a, max_units);
+    launch_rows_as<XF, MT, 4, GLU>(a, max_units);
 }
 
-template <int XF, bool GLU, bool FINE>
+template <int XF, bool GLU>
 void launch_rows(const MoeArgs& a, int max_units) {
     // A block takes all of its unit's rows at once.
     if (a.unit_rows > 64) fail("byhip: internal: units of %d rows", a.unit_rows);
-    if (a.unit_rows <= 16) launch_rows_n<XF, 1, GLU, FINE>(a, max_units);
-    else if (a.unit_rows <= 32) launch_rows_n<XF, 2, GLU, FINE>(a, max_units);
-    else launch_rows_n<XF, 4, GLU, FINE>(a, max_units);
+    if (a.unit_rows <= 16) launch_rows_n<XF, 1, GLU>(a, max_units);
+    else if (a.unit_rows <= 32) launch_rows_n<XF, 2, GLU>(a, max_units);
+    else launch_rows_n<XF, 4, GLU>(a, max_units);
 }
 
 }  // namespace
 
 void launch_moe_rows(const MoeArgs& a, int x_format, bool glu, int max_units) {
-    const bool fine = moe_fine(x_format, a.y_dtype);
-    if (x_format == BYHIP_MXFP4_KM) glu ? launch_rows<BYHIP_MXFP4_KM, true, false>(a, max_units) : launch_rows<BYHIP_MXFP4_KM, false, false>(a, max_units);
-    else if (fine) glu ? launch_rows<BYHIP_MXFP8_KM, true, true>(a, max_units) : launch_rows<BYHIP_MXFP8_KM, false, true>(a, max_units);
-    else glu ? launch_rows<BYHIP_MXFP8_KM, true, false>(a, max_units) : launch_rows<BYHIP_MXFP8_KM, false, false>(a, max_units);
+    if (x_format == BYHIP_MXFP4_KM) glu ? launch_rows<BYHIP_MXFP4_KM, true>(a, max_units) : launch_rows<BYHIP_MXFP4_KM, false>(a, max_units);
+    else glu ? launch_rows<BYHIP_MXFP8_KM, true>(a, max_units) : launch_rows<BYHIP_MXFP8_KM, false>(a, max_units);
 }
 
 }  // namespace byhip

@@ -10,6 +10,11 @@
 // ahead, the next tile's loads out before this one's results) left the matrix unit idle for half of the time: 12000 of a tile's 34000
 // cycles went outside the steps.
 //
+// With rows in 8 bits and outputs of 16 bits or fewer, the instructions' cut (split_bytes) stays: 5e-6 to 1e-5 of a product's norm, less than a hundredth of the
+// rounding that follows. (Of outputs in 8 bits one in a thousand then takes the step next to its own: 0.0023 of their norm, where the steps' rounding is
+// 0.026.) It is more where large terms cancel. In two parts, as with fp32 outputs, they would take half as long again: 4096 tokens, 6 of 64 experts, 2048 to 1408,
+// 242 us for 153.
+//
 // A step's data goes straight into LDS (16 bytes per lane) while the step before multiplies: two slots, one barrier per step. The
 // order of the 16-byte pieces inside a row is turned by the row so that no cycle of the operand reads meets a bank twice.
 #include <algorithm>

@@ -454,9 +454,9 @@ enum byhip_moe_flags {
 };
 
 /* y [M, N] = x . w^T of microscaled rows and one matrix [N, K] (with BYHIP_MOE_SWIGLU, the only flag it takes,
- * [2 N, K]). y_dtype F32, F16, BF16, or microscaled rows again (N a multiple of 32, y_stride N). Sums are fp32; with y in fp32
- * every product enters them with fp32's precision, with other types products of 8-bit rows that are 2^-13 and less of the largest of eight
- * neighbours may be cut off. */
+ * [2 N, K]). y_dtype F32, F16, BF16, or microscaled rows again (N a multiple of 32, y_stride N). Sums are fp32, and every product enters
+ * them with fp32's precision but for one case: 8-bit rows, y not in fp32 and many rows per matrix (dozens). There products that are 2^-13 and less
+ * of the largest of eight neighbours (in memory order) may be cut off; a caller to whom they matter takes y in fp32 and byhip_mx_quantize. */
 int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K, int N, int flags, void* y,
                     size_t y_stride, int y_dtype);
 
