@@ -91,7 +91,7 @@ constexpr int kTileRows = 128;
 // Units at most: an expert leaves one that is not full.
 inline int moe_max_units(int rows, int experts, int unit) { return rows / unit + (rows < experts ? rows : experts); }
 // The plan's buffer: offsets and order (the caller's to read), the numbers of units of both kinds and the units, and what the plan's
-// kernels count in (one row of `experts` counts per block of assignments).
+// kernels count in (one row of `experts` counts per block of assignments, and one of their sums).
 struct MoePlan {
     int tokens, top_k, experts, rows, unit_rows, max_units, max_tiles, blocks;
     int *offsets, *order, *n_units, *counts;  // n_units: of units, of tiles

@@ -478,8 +478,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_one(MoePlan p, const in
     plan_block(p, ids, counts, part, where);
 }
 
-// Many assignments: counts per block of them, then the places; every block of the second forms the sums it needs from all blocks' counts,
-// which costs less than a launch between.
+// Many assignments: counts per block of them, then the places; with few counts every block of the second forms the sums it needs from all blocks' counts,
+// which costs less than a launch between (kSumCounts).
 constexpr int kCountWaves = 4;
 __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, const int* ids) {
     __shared__ int counts[kMaxExperts];
@@ -492,32 +492,74 @@ __global__ __launch_bounds__(64 * kCountWaves) void moe_plan_count(MoePlan p, co
     __syncthreads();
     for (int i = threadIdx.x; i < E; i += 64 * kCountWaves) p.counts[(size_t)blockIdx.x * E + i] = counts[i];
 }
+// Many blocks of them: the counts become each block's first places among its experts' assignments, with all blocks' sums in a row behind them. 64 experts per block, a
+// stretch of the counts' rows per wave.
+constexpr int kSumWaves = 16;
+__global__ __launch_bounds__(64 * kSumWaves) void moe_plan_sums(MoePlan p) {
+    __shared__ int sums[kSumWaves][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, E = p.experts, e = blockIdx.x * 64 + lane;
+    const int each = (p.blocks + kSumWaves - 1) / kSumWaves, lo = min(p.blocks, each * w), hi = min(p.blocks, lo + each);
+    int* const counts = p.counts + (e < E ? e : 0);
+    int sum = 0;
+    if (e < E) {
+#pragma unroll 8
+        for (int b = lo; b < hi; ++b) sum += counts[(size_t)b * E];
+    }
+    sums[w][lane] = sum;
+    __syncthreads();
+    if (e >= E) return;
+    int at = 0, total = 0;
+    for (int i = 0; i < kSumWaves; ++i) {
+        const int v = sums[i][lane];
+        at += i < w ? v : 0;
+        total += v;
+    }
+    if (w == 0) counts[(size_t)p.blocks * E] = total;
+    for (int b = lo; b < hi; b += 8) {
+        int c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = b + i < hi ? counts[(size_t)(b + i) * E] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (b + i < hi) counts[(size_t)(b + i) * E] = at;
+            at += c[i];
+        }
+    }
+}
+template <bool SUMS>  // whether moe_plan_sums has run
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const int* ids) {
     __shared__ int counts[kCountWaves * kMaxExperts];
-    __shared__ int2 sums[kPlanThreads];
+    __shared__ int2 sums[SUMS ? 1 : kPlanThreads];
     __shared__ int4 part[kPlanWaves], where[kMaxExperts];
     const int w = threadIdx.x >> 6, e = threadIdx.x, E = p.experts, lo = blockIdx.x * kPlanBlock, hi = min(p.rows, lo + kPlanBlock);
     int from = 0, to = 0;
     for (int i = threadIdx.x; i < kCountWaves * E; i += kPlanThreads) counts[i] = 0;
-    // Expert e's assignments in all blocks, and in those before this one: as many threads per expert as there are, a share of the blocks each.
-    const int room = (E + 63) & ~63, shares = kPlanThreads / room, share = e / room;
+    // Expert e's assignments in all blocks, and in those before this one.
     int sum = 0, before = 0;
-    if (e - share * room < E && share < shares) {
+    if constexpr (SUMS) {
+        if (e < E) {
+            sum = p.counts[(size_t)p.blocks * E + e];
+            before = p.counts[(size_t)blockIdx.x * E + e];
+        }
+    } else {  // as many threads per expert as there are, a share of the blocks each
+        const int room = (E + 63) & ~63, shares = kPlanThreads / room, share = e / room;
+        if (e - share * room < E && share < shares) {
 #pragma unroll 8
-        for (int b = share; b < p.blocks; b += shares) {
-            const int c = p.counts[(size_t)b * E + e - share * room];
-            sum += c;
-            before += b < (int)blockIdx.x ? c : 0;
+            for (int b = share; b < p.blocks; b += shares) {
+                const int c = p.counts[(size_t)b * E + e - share * room];
+                sum += c;
+                before += b < (int)blockIdx.x ? c : 0;
+            }
         }
+        sums[e] = make_int2(sum, before);
+        __syncthreads();
+        sum = before = 0;
+        if (e < E)
+            for (int i = 0; i < shares; ++i) {
+                sum += sums[i * room + e].x;
+                before += sums[i * room + e].y;
+            }
     }
-    sums[e] = make_int2(sum, before);
-    __syncthreads();
-    sum = before = 0;
-    if (e < E)
-        for (int i = 0; i < shares; ++i) {
-            sum += sums[i * room + e].x;
-            before += sums[i * room + e].y;
-        }
     __syncthreads();
     if (w < kCountWaves) {
         stretch(lo, hi, kCountWaves, w, from, to);
@@ -537,12 +579,21 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_place(MoePlan p, const 
     if (w < kCountWaves) place_ids(ids, from, to, E, counts + w * E, p.order);
 }
 
+// Up to this many counts (blocks times experts) every block sums them all, whose reads grow with the square of the assignments; beyond, a launch sums them once (us, 256 experts,
+// 128 / 256 / 512 / 2048 blocks: 15.2 / 18.7 / 30.5 / 256 by every block, 16.5 / 18.6 / 22.1 / 54 once; 64 experts, 256 blocks 11.2 and 13.5; 1024 experts, 128
+// blocks 28.4 and 23.5).
+constexpr long long kSumCounts = 65536;
 void launch_plan(const MoePlan& p, const int* ids) {
     if (p.blocks <= 4) {
         launch("moe_plan_one", moe_plan_one, dim3(1), dim3(kPlanThreads), 0, p, ids);
     } else {
         launch("moe_plan_count", moe_plan_count, dim3(p.blocks), dim3(64 * kCountWaves), 0, p, ids);
-        launch("moe_plan_place", moe_plan_place, dim3(p.blocks), dim3(kPlanThreads), 0, p, ids);
+        if ((long long)p.blocks * p.experts <= kSumCounts) {
+            launch("moe_plan_place", moe_plan_place<false>, dim3(p.blocks), dim3(kPlanThreads), 0, p, ids);
+        } else {
+            launch("moe_plan_sums", moe_plan_sums, dim3((p.experts + 63) / 64), dim3(64 * kSumWaves), 0, p);
+            launch("moe_plan_place", moe_plan_place<true>, dim3(p.blocks), dim3(kPlanThreads), 0, p, ids);
+        }
     }
     BYHIP_LAUNCHED("moe_plan");
 }
@@ -670,7 +721,7 @@ MoePlan moe_layout(const byhip_moe_plan* p) {
     m.n_units = reinterpret_cast<int*>(take(8));
     m.units = reinterpret_cast<MoeUnit*>(take((size_t)m.max_units * sizeof(MoeUnit)));
     m.tiles = reinterpret_cast<MoeUnit*>(take((size_t)m.max_tiles * sizeof(MoeUnit)));
-    m.counts = reinterpret_cast<int*>(take((size_t)m.blocks * m.experts * 4));
+    m.counts = reinterpret_cast<int*>(take((size_t)(m.blocks + 1) * m.experts * 4));
     m.bytes = at;
     return m;
 }
