@@ -35,30 +35,21 @@ struct MoeTiles {
         tiles = (long long)units * a.strips;
         per = (tiles + 7) / 8;
     }
-    // The unit of place `at` of this block's XCD.
-    __device__ __forceinline__ uint32_t unit(const MoeArgs& a, long long at) const {
-        return (uint32_t)((blockIdx.x & 7) * per + at) / (uint32_t)a.strips;
-    }
-    // Whether there is work at this place; if so its strip, and its unit in order: a buffer that no plan was made in names no rows, and
+    // Whether there is work at this place; if so its unit and strip, in order: a buffer that no plan was made in names no rows, and
     // no memory but its own.
-    __device__ __forceinline__ bool finish(const MoeArgs& a, long long at, MoeUnit& u, int& strip) const {
+    __device__ __forceinline__ bool find(const MoeArgs& a, long long at, MoeUnit& u, int& strip) const {
         const long long t = (blockIdx.x & 7) * per + at;
         if (at >= per || t >= tiles) return false;
+        const uint32_t i = (uint32_t)t / (uint32_t)a.strips;
         strip = (int)((uint32_t)t % (uint32_t)a.strips);
         if (a.n_units) {
+            u = a.units[i];
             if ((unsigned)u.expert >= (unsigned)a.experts || u.first < 0 || (unsigned)u.rows > (unsigned)a.unit_rows || u.first > a.rows - u.rows) u.rows = u.expert = u.first = 0;
         } else {
-            u.expert = 0;
-            u.first = unit(a, at) * a.unit_rows;
+            u = MoeUnit{0, (int)i * a.unit_rows, 0, 0};
             u.rows = min(a.unit_rows, a.M - u.first);
         }
         return true;
-    }
-    __device__ __forceinline__ bool find(const MoeArgs& a, long long at, MoeUnit& u, int& strip) const {
-        if (at >= per || (blockIdx.x & 7) * per + at >= tiles) return false;
-        u = MoeUnit{};
-        if (a.n_units) u = a.units[unit(a, at)];
-        return finish(a, at, u, strip);
     }
 };
 // The token of an assignment: id / top_k, exact for ids below 2^24 and top_k up to 256 (`per_token` = 2^32 / top_k rounded up is off by

@@ -344,17 +344,18 @@ __global__ __launch_bounds__(64 * kTokensPerBlock) void moe_route(RouteArgs a) {
 
 // ── the plan ──
 
-// Lanes below this one, and this one's peers: the lanes whose id is the same (bits of an id below 2^BITS; `live` lanes only).
+// The `live` lanes whose id (below kMaxExperts) is this lane's.
 __device__ __forceinline__ uint64_t same_id(int id, bool live) {
     uint64_t m = __ballot(live);
 #pragma unroll
-    for (int b = 0; b < 10; ++b) {
+    for (int b = 0; 1 << b < kMaxExperts; ++b) {
         const bool bit = (id >> b) & 1;
         const uint64_t set = __ballot(bit);
         m &= bit ? set : ~set;
     }
     return m;
 }
+// How many of these lanes are below this one.
 __device__ __forceinline__ int rank_below(uint64_t m) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }

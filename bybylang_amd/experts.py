@@ -31,7 +31,7 @@ class ExpertsBlock:
         self.weights, self.width, self.inner, self.experts, self.top_k = (router, up, down), width, inner, experts, top_k
         self.norm = dev.Norm(_abi.NORM_RMS, eps, g.sessionUpload(gbHip, norm))
         self.router = dev.MoeRouter(score, None if bias is None else g.sessionUpload(gbHip, bias), groups, top_groups, group_by, renorm, scale)
-        rows = max_rows * top_k
+        self.max_rows, rows = max_rows, max_rows * top_k
         # A plan of fewer tokens may have shorter units, and more of them.
         self.plan_buffer = g.sessionAllocBytes(gbHip, max(dev.moe_plan_bytes(t, top_k, experts) for t in range(1, max_rows + 1)))
         self.xq = g.sessionAllocBytes(gbHip, dev.mx_bytes(max_rows, width, _abi.MXFP8_KM))

@@ -34,12 +34,17 @@ class PagedDecoder:
     residual stream of `width` values, for up to `slots` sequences of `max_len` tokens and `max_rows` rows a call.
 
     layers: a list of (wq, wk, wv, wo) resident Q4 weights; norms: gammas of the RMS norm before each layer and
-    after the last one; experts: an ExpertsBlock (experts.py) after each layer's attention, or None."""
+    after the last one; experts: for each layer an ExpertsBlock (experts.py) after its attention, or None."""
 
     def __init__(self, layers, norms, width: int, heads: int, kv_heads: int, head_dim: int, slots: int, max_len: int,
                  max_rows: int, pages: int, page_size: int = 32, cache_dtype: int = _abi.F16, eps: float = 1e-5,
                  rope_base: float = 10000.0, window: int = 0, softcap: float = 0.0, experts=None):
         self.experts = experts or [None] * len(layers)
+        if len(self.experts) != len(layers):
+            raise ValueError(f"{len(self.experts)} blocks of experts for {len(layers)} layers")
+        for e in self.experts:
+            if e is not None and (e.width != width or e.max_rows < max_rows):
+                raise ValueError(f"a block of experts over {e.max_rows} rows of {e.width} values for {max_rows} rows of {width}")
         self.layers, self.width, self.heads, self.slots, self.max_rows = layers, width, heads, slots, max_rows
         self.stride = -(-max_len // page_size)
         scratch = lambda n: g.sessionAllocScratch(gbHip, n)  # noqa: E731
