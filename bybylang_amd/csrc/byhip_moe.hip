@@ -13,9 +13,9 @@ MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts,
     a.K = K; a.KG = K / 32; a.N = N;
     const long long R = glu ? 2ll * N : N;
     check_mx(x, rows, K, x_format, "rows of a product");
-    // Offsets inside the rows and inside one matrix are 32-bit; strips may pass a matrix's last row.
+    // Offsets inside the rows and inside one matrix are 32-bit.
     if (mx_values(rows, K, x_format) >= 1ull << 31) fail("byhip: %zu rows of %d values: a product takes less than 2 GiB of them", rows, K);
-    if (R > INT32_MAX / 2 || (unsigned long long)(R + 512) * K / 2 >= 1ull << 31) fail("byhip: a matrix of %lld rows of %d values", R, K);
+    if (R > INT32_MAX / 2 || (unsigned long long)R * K / 2 >= 1ull << 31) fail("byhip: a matrix of %lld rows of %d values", R, K);
     a.R = (int)R;
     check_mx(w, (size_t)experts * R, K, BYHIP_MXFP4_KM, "matrices of a product");
     if (is_mx(y_dtype)) {
