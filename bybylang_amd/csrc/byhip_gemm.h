@@ -232,7 +232,8 @@ bool fp4_gemv_ok(const GemmArgs& a);
 void launch_fp4_gemv(const GemmArgs& a);
 
 // Native MXFP4 GEMM (E2M1 x E2M1 with E8M0 block scales): x and w in the FP4-KM packing.
-// K % 128 == 0 is required.
+// K % 128 == 0 is required, and sizes that fit its offsets (mxfp4_fits).
+bool mxfp4_fits(int M, int K, int N);
 void launch_mxfp4(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w,
                   const uint8_t* w_scales, void* y, int y_dtype, int M, int K, int N);
 

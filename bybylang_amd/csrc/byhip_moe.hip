@@ -66,7 +66,7 @@ int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K,
         if (M == 0) return;
         note_device_write(y);
         // Rows in 4 bits as byhip_mxfp4_gemm takes them.
-        if (x_format == BYHIP_MXFP4_KM && !glu && !is_mx(y_dtype) && K % 128 == 0 && y_stride == (size_t)N && M > 64) {
+        if (x_format == BYHIP_MXFP4_KM && !glu && !is_mx(y_dtype) && K % 128 == 0 && y_stride == (size_t)N && M > 64 && mxfp4_fits(M, K, N)) {
             launch_mxfp4(a.x, a.xs, a.w, a.ws, y, y_dtype, M, K, N);
             return;
         }

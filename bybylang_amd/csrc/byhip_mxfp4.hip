@@ -570,13 +570,14 @@ void launch_mxfp4_mid(MxArgs a, GemmArgs out) {
 
 }  // namespace
 
+// Buffer offsets of the rows a tile reaches past M or N (plus the second half of a last pair of steps) must stay below 2^32.
+bool mxfp4_fits(int M, int K, int N) { return (uint64_t)(std::max(M, N) + TM) * (K / 2) + 128 < kOutOfRange; }
+
 void launch_mxfp4(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w,
                   const uint8_t* w_scales, void* y, int y_dtype, int M, int K, int N) {
     if (K % KSTEP != 0) fail("byhip: internal: MXFP4 GEMM needs K %% 128 == 0 (K=%d)", K);
     if (M <= 0 || N <= 0) return;
-    // Buffer offsets of the rows a tile reaches past M or N (plus the second half of a last pair
-    // of steps) must stay below 2^32.
-    if ((uint64_t)(M + TM) * (K / 2) + 128 >= kOutOfRange || (uint64_t)(N + TN) * (K / 2) + 128 >= kOutOfRange)
+    if (!mxfp4_fits(M, K, N))
         fail("byhip: MXFP4 operands above 4 GiB are not supported");
     MxArgs a;
     a.x = x; a.xs = x_scales; a.w = w; a.ws = w_scales; a.y = y;

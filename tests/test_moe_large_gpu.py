@@ -86,3 +86,24 @@ def test_a_matrix_next_to_2_gib_is_taken(hip):
         hip.mx_matmul(z, MX8, z, 1, 2048, 2**21 - 1, 0, z, 2**21 - 1, F32)
     with pytest.raises(_abi.HipBackendError, match="a matrix of 2097152 rows"):
         hip.mx_matmul(z, MX8, z, 1, 2048, 2**21, 0, z, 2**21, F32)
+
+
+def test_rows_of_2_to_the_25_values(hip):
+    """More than 64 rows in 4 bits whose offsets do not fit mxfp4_gemm, but are below 2 GiB."""
+    M, N, K = 65, 1, 2**25
+    kb, kg = K // 2, K // 32
+    x, w = hip.DeviceBuffer(M * (kb + kg)), hip.DeviceBuffer(N * (kb + kg))
+    x.zero(), w.zero()
+    g = synth.rng(1)
+    at = [0, 128, K // 2, K - 128]  # stretches of 128 values
+    xv, wv = np.zeros((M, 512)), np.zeros((N, 512))
+    for i, k in enumerate(at):
+        for buf, rows, v in ((x, M, xv), (w, N, wv)):
+            b, v[:, 128 * i:128 * i + 128] = random_rows(g, rows, 128, MX4)
+            for r in range(rows):
+                buf.upload(b[64 * r:64 * r + 64], r * kb + k // 2)
+                buf.upload(b[64 * rows + 4 * r:64 * rows + 4 * r + 4], rows * kb + r * kg + k // 32)
+    y = hip.DeviceBuffer(M * N * 4)
+    hip.mx_matmul(x, MX4, w, M, K, N, 0, y, N, F32)
+    # 512 terms that are not 0, in any order among zeros
+    close(y.read(np.float32).reshape(M, N), xv @ wv.T, F32, 520 * 2.0**-24 * (np.abs(xv) @ np.abs(wv).T))
