@@ -38,14 +38,17 @@ MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts,
     return a;
 }
 
-// Whether tiles take a product: `units` is what can be told on the host of how many of 128 rows it has. They do where their blocks
-// fill the card, from a few rows per expert on (128 experts, K = 2048, 768 outputs of gates and ups, 4 / 6 / 8 / 12 rows each: 41 / 49 / 50
-// / 50 us, moe_rows 36 / 45 / 50 / 62), and with fewer blocks where moe_rows would read the rows again and again (one matrix of 4096 x
-// 4096, 256 / 384 / 512 rows: 32 us each, 32 / 48 / 64 blocks, moe_rows 21 / 32 / 36; 256 rows and 14336 outputs, 112 blocks: 34 for 62).
-bool tiles_take(const MoeArgs& a, bool glu, long long rows, int units, int experts) {
+// Whether tiles take a product: `units` is what can be told on the host of how many of 128 rows it has. A block of moe_tiles takes its time (30 us at K = 4096, 58 where 8-bit
+// rows go in two parts into fp32) however few of its rows are real, so tiles need blocks enough and, where those do not fill the card, more products than moe_rows does in that
+// time. Few rows per expert (us, moe_tiles / moe_rows; 128 experts, 2048 to 768 outputs of gates and ups, 6 / 8 / 10 / 12 / 24 each: 49 / 50 / 50 / 51 / 53 for
+// 41 / 47 / 52 / 56 / 76; fp32: 16 / 24 / 32 each 77 / 77 / 79 for 65 / 77 / 90; 8 experts, 4096 to 14336, 8 / 12 each: 125 / 127 for 120 / 136). Few blocks (one matrix of 4096 x 4096, 256 / 384
+// / 512 rows: 32 / 33 / 32 for 20 / 36 / 38, fp32 512 / 768 / 1024 rows: 60 / 61 / 61 for 38 / 56 / 72; 14336 x 4096, 64 / 96 / 128 rows: 31 / 32 / 32 for 22 / 32 / 40, fp32 128 / 256:
+// 59 / 62 for 41 / 72; 8 experts, 14336 to 4096, 32 / 64 rows each: 123 / 130 for 98 / 153).
+bool tiles_take(const MoeArgs& a, bool glu, int x_format, long long rows, int units, int experts) {
     const int wide = glu ? 128 : 256;
+    const bool parts = x_format == BYHIP_MXFP8_KM && a.y_dtype == BYHIP_F32;
     const long long blocks = (long long)units * ((a.N + wide - 1) / wide);
-    return a.K % 128 == 0 && ((blocks >= 256 && rows >= 8ll * experts) || (blocks >= 48 && rows >= 64ll * experts));
+    return a.K % 128 == 0 && rows >= (parts ? 24ll : 10ll) * experts && (blocks >= 256 || rows * a.R >= (parts ? 3000000 : 1500000));
 }
 
 }  // namespace
@@ -72,7 +75,7 @@ int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K,
         }
         a.M = M; a.top_k = 1;
         const int tiles = (M + kTileRows - 1) / kTileRows;
-        if (tiles_take(a, glu, M, tiles, 1)) {
+        if (tiles_take(a, glu, x_format, M, tiles, 1)) {
             a.unit_rows = kTileRows;
             launch_moe_tiles(a, x_format, glu, tiles);
         } else {
@@ -96,7 +99,7 @@ int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_
         a.experts = p.experts; a.rows = p.rows;
         a.per_token = (uint32_t)(((1ull << 32) + p.top_k - 1) / p.top_k);
         note_device_write(y);
-        if (tiles_take(a, glu, p.rows, p.max_tiles, p.experts)) {
+        if (tiles_take(a, glu, x_format, p.rows, p.max_tiles, p.experts)) {
             a.n_units = p.n_units + 1; a.units = p.tiles; a.max_units = p.max_tiles;
             a.unit_rows = kTileRows;
             launch_moe_tiles(a, x_format, glu, p.max_tiles);
