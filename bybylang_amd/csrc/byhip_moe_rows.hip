@@ -242,23 +242,24 @@ void launch_rows_as(MoeArgs a, int max_units) {
     a.strips = (a.N + wide - 1) / wide;
     const long long blocks = ((long long)max_units * a.strips + 7) / 8 * 8;
     if (blocks >= 1ll << 31) fail("byhip: a product of %d units of %d strips", max_units, a.strips);
-    // Windows of 512 values, or of 256 where those would leave waves without one or with half of one (48 tokens, 128 experts, 2048 outputs, K = 512
-    // / 768 / 1024 / 1408 / 1536: 15.2 / 18.1 / 24.5 / 27.0 / 23.4 us for 18.0 / 21.6 / 25.8 / 29.4 / 24.5; K = 2048: 32.9 for 33.1, and for one
-    // token 7.5 for 6.8. Windows of 128 took longer than those of 256 but for K = 1408, 26.2).
+    // Windows of 512 values, or of 256 where those would leave waves without one or with half of one (us, 512 / 256: 48 tokens, 128 experts, 2048 outputs, K = 768 / 1024 / 1408 / 1536 /
+    // 2048 / 4096 22.2 / 24.6 / 27.1 / 31.1 / 43.0 / 79.4 for 19.0 / 21.5 / 29.0 / 32.1 / 44.6 / 95.6; one token, K = 1024 / 1536 / 2048 5.1 / 5.6 / 6.9 for 4.7 / 5.7 / 7.2; 256 rows of one
+    // matrix, K = 1024 / 2048 8.6 / 11.7 for 7.7 / 12.7).
     const dim3 grid((unsigned)blocks), block(64 * kWaves);
     if (a.KG & 3) launch("moe_rows", (moe_rows<XF, MT, NF, 2, false, GLU>), grid, block, 0, a);
-    else if (a.KG > 48) launch("moe_rows", (moe_rows<XF, MT, NF, 4, true, GLU>), grid, block, 0, a);
+    else if (a.KG > 40) launch("moe_rows", (moe_rows<XF, MT, NF, 4, true, GLU>), grid, block, 0, a);
     else launch("moe_rows", (moe_rows<XF, MT, NF, 2, true, GLU>), grid, block, 0, a);
     BYHIP_LAUNCHED("moe_rows");
 }
 
-// Strips of 64, 32 or 16 outputs: the widest that gives most CUs a block, for rows are read once per strip (16 rows, K = 4096, N = 4096: 64 strips of
-// 64 9.7 us, 128 of 32 7.4, 256 of 16 5.8; N = 14336: 224 of 64 11.4 us, 448 of 32 12.9). Gates and ups have 32 each. Eight waves per block took as long where
+// Strips of 64, 32 or 16 outputs: the widest that gives half of the CUs a block, for rows are read once per strip (us, K = 4096, strips
+// of 64 / 32 / 16: 16 rows, N = 4096 9.5 / 7.0 / 5.7, N = 4608 - / 7.3 / 8.8, N = 8192 10.3 / 8.3 / 9.4, N = 9216 10.4 / 11.7 / -, N = 14336 11.0 / 12.1 / 15.4; 32 rows, N =
+// 4608 - / 9.7 / 12.9, N = 9216 13.4 / 16.2 / -; one row, N = 4608 - / 6.6 / 6.2). Gates and ups have 32 each. Eight waves per block took as long where
 // one unit's strips are all there is (9.8 us for 10.5 at N = 14336, 9.6 for 9.7), longer elsewhere (33 us for 41, 48 tokens, 128 experts).
 template <int XF, int MT, bool GLU>
 void launch_rows_n(const MoeArgs& a, int max_units) {
     if constexpr (!GLU) {
-        const long long strips = (a.N + 15) / 16, room = 200;
+        const long long strips = (a.N + 15) / 16, room = 130;
         if (strips / 4 * max_units < room) {
             if (strips / 2 * max_units < room && !is_mx(a.y_dtype)) launch_rows_as<XF, MT, 1, GLU>(a, max_units);
             else launch_rows_as<XF, MT, 2, GLU>(a, max_units);

@@ -1,4 +1,4 @@
-"""The forms of moe_rows that decode steps and few rows run on: windows of 512 values (K from 1568 on), whole and partial, strips of 64 outputs whose last is partly empty, gates and
+"""The forms of moe_rows that decode steps and few rows run on: windows of 512 values (K from 1408 on), whole and partial, strips of 64 outputs whose last is partly empty, gates and
 ups, units of 16, 32 and 64 rows, every output type. Bounds as in test_mx_gpu.py, those of fp32 outputs."""
 import functools
 
