@@ -51,6 +51,14 @@ bool tiles_take(const MoeArgs& a, bool glu, int x_format, long long rows, int un
     return a.K % 128 == 0 && rows >= (parts ? 24ll : 10ll) * experts && (blocks >= 256 || rows * a.R >= (parts ? 3000000 : 1500000));
 }
 
+// Whether byhip_mxfp4_gemm's kernels take rows in 4 bits (with dense rows of 32 or 16 bits out): where there are more than one pass of moe_rows takes and products enough
+// (us, mxfp4_gemm / here: 4096 x 4096, 16 / 64 / 80 / 192 / 512 rows 6.8 / 10.0 / 10.5 / 13.4 / 11.3 for 4.8 / 8.4 / 12.1 / 17.2 / 26.1; N = 14336, 16 / 32 / 64 / 256 rows 10.0 / 10.9 / 13.2
+// / 18.9 for 9.3 / 11.1 / 24.4 / 29.2; K = 14336, 8 / 32 / 64 rows 9.7 / 10.9 / 13.3 for 10.2 / 15.4 / 19.8; 2048 x 2048, 64 / 256 rows 7.4 / 10.2 for 4.2 / 6.6). Rows of y
+// that do not lie next to each other stay here.
+bool mxfp4_takes(int M, int K, int N) {
+    return K % 128 == 0 && M > 16 && (double)M * N * K >= 1.3e9 && mxfp4_fits(M, K, N);
+}
+
 }  // namespace
 }  // namespace byhip
 
@@ -68,8 +76,7 @@ int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K,
         MoeArgs a = product_args(x, x_format, w, 1, M, M, K, N, glu, y, y_stride, y_dtype);
         if (M == 0) return;
         note_device_write(y);
-        // Rows in 4 bits as byhip_mxfp4_gemm takes them.
-        if (x_format == BYHIP_MXFP4_KM && !glu && !is_mx(y_dtype) && K % 128 == 0 && y_stride == (size_t)N && M > 64 && mxfp4_fits(M, K, N)) {
+        if (x_format == BYHIP_MXFP4_KM && !glu && !is_mx(y_dtype) && y_stride == (size_t)N && mxfp4_takes(M, K, N)) {
             launch_mxfp4(a.x, a.xs, a.w, a.ws, y, y_dtype, M, K, N);
             return;
         }

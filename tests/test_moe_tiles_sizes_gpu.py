@@ -40,3 +40,10 @@ def test_assignments_left_out(hip, flags, yt):
 @pytest.mark.parametrize("M,N", [(95, 15808), (190, 7904), (120, 12512)])
 def test_few_blocks(hip, yt, M, N):
     check(hip, M, 128, N, MX8, yt, seed=M)
+
+
+@pytest.mark.parametrize("M,K,N", [(33, 2048, 19300), (40, 4096, 8002), (200, 4096, 1701), (300, 2176, 2050), (520, 640, 4001)])
+@pytest.mark.parametrize("yt,pad", [(F32, 0), (F16, 0), (BF16, 0), (BF16, 3)])
+def test_rows_in_4_bits(hip, M, K, N, yt, pad):
+    """Enough products for byhip_mxfp4_gemm's kernels, and the same with rows of y apart, which stay here."""
+    check(hip, M, K, N, MX4, yt, pad=pad, seed=M)
