@@ -19,7 +19,7 @@ ROPE_HALVES, ROPE_PAIRS = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
 NORM_RMS, NORM_LAYER = 0, 1
 MOE_SOFTMAX, MOE_SIGMOID = 0, 1
-MOE_GATHER, MOE_SCATTER, MOE_SWIGLU = 1, 2, 4
+MOE_GATHER, MOE_SCATTER, MOE_SWIGLU, MOE_EXACT = 1, 2, 4, 16
 
 
 class HipBackendError(RuntimeError):

@@ -21,6 +21,7 @@ struct MoeArgs {
     int top_k, gather, scatter, unit_rows, strips, y_dtype, vec;
     int experts, rows, max_units;  // of the plan
     uint32_t per_token;       // 2^32 / top_k, rounded up (top_k > 1)
+    int parts;                // moe_tiles: 8-bit rows in two parts (split_bytes)
 };
 
 typedef int v8i __attribute__((ext_vector_type(8)));

@@ -6,8 +6,9 @@ namespace byhip {
 namespace {
 
 // What both calls check; rows: x's rows, y_rows: y's.
-MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts, size_t rows, size_t y_rows, int K, int N, bool glu,
+MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts, size_t rows, size_t y_rows, int K, int N, int flags,
                      void* y, size_t y_stride, int y_dtype) {
+    const bool glu = flags & BYHIP_MOE_SWIGLU;
     if (K <= 0 || N <= 0) fail("byhip: a product of rows of %d values with %d outputs", K, N);
     MoeArgs a{};
     a.K = K; a.KG = K / 32; a.N = N;
@@ -35,20 +36,20 @@ MoeArgs product_args(const void* x, int x_format, const uint8_t* w, int experts,
     a.w = w;
     a.ws = w + mx_values((size_t)experts * R, K, BYHIP_MXFP4_KM);
     a.y = y; a.y_stride = y_stride; a.y_dtype = y_dtype;
+    a.parts = x_format == BYHIP_MXFP8_KM && (y_dtype == BYHIP_F32 || flags & BYHIP_MOE_EXACT);
     return a;
 }
 
 // Whether tiles take a product: `units` is what can be told on the host of how many of 128 rows it has. A block of moe_tiles takes its time (30 us at K = 4096, 58 where 8-bit
-// rows go in two parts into fp32) however few of its rows are real, so tiles need blocks enough and, where those do not fill the card, more products than moe_rows does in that
+// rows go in two parts) however few of its rows are real, so tiles need blocks enough and, where those do not fill the card, more products than moe_rows does in that
 // time. Few rows per expert (us, moe_tiles / moe_rows; 128 experts, 2048 to 768 outputs of gates and ups, 6 / 8 / 10 / 12 / 24 each: 49 / 50 / 50 / 51 / 53 for
 // 41 / 47 / 52 / 56 / 76; fp32: 16 / 24 / 32 each 77 / 77 / 79 for 65 / 77 / 90; 8 experts, 4096 to 14336, 8 / 12 each: 125 / 127 for 120 / 136). Few blocks (one matrix of 4096 x 4096, 256 / 384
 // / 512 rows: 32 / 33 / 32 for 20 / 36 / 38, fp32 512 / 768 / 1024 rows: 60 / 61 / 61 for 38 / 56 / 72; 14336 x 4096, 64 / 96 / 128 rows: 31 / 32 / 32 for 22 / 32 / 40, fp32 128 / 256:
 // 59 / 62 for 41 / 72; 8 experts, 14336 to 4096, 32 / 64 rows each: 123 / 130 for 98 / 153).
-bool tiles_take(const MoeArgs& a, bool glu, int x_format, long long rows, int units, int experts) {
+bool tiles_take(const MoeArgs& a, bool glu, long long rows, int units, int experts) {
     const int wide = glu ? 128 : 256;
-    const bool parts = x_format == BYHIP_MXFP8_KM && a.y_dtype == BYHIP_F32;
     const long long blocks = (long long)units * ((a.N + wide - 1) / wide);
-    return a.K % 128 == 0 && rows >= (parts ? 24ll : 10ll) * experts && (blocks >= 256 || rows * a.R >= (parts ? 3000000 : 1500000));
+    return a.K % 128 == 0 && rows >= (a.parts ? 24ll : 10ll) * experts && (blocks >= 256 || rows * a.R >= (a.parts ? 3000000 : 1500000));
 }
 
 // Whether byhip_mxfp4_gemm's kernels take rows in 4 bits (with dense rows of 32 or 16 bits out): where there are more than one pass of moe_rows takes and products enough
@@ -71,9 +72,9 @@ int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K,
     return guard([&] {
         enter_compute();
         if (M < 0) fail("byhip: a product of %d rows", M);
-        if (flags & ~BYHIP_MOE_SWIGLU) fail("byhip: product flags %d without a plan", flags);
+        if (flags & ~(BYHIP_MOE_SWIGLU | BYHIP_MOE_EXACT)) fail("byhip: product flags %d without a plan", flags);
         const bool glu = flags & BYHIP_MOE_SWIGLU;
-        MoeArgs a = product_args(x, x_format, w, 1, M, M, K, N, glu, y, y_stride, y_dtype);
+        MoeArgs a = product_args(x, x_format, w, 1, M, M, K, N, flags, y, y_stride, y_dtype);
         if (M == 0) return;
         note_device_write(y);
         if (x_format == BYHIP_MXFP4_KM && !glu && !is_mx(y_dtype) && y_stride == (size_t)N && mxfp4_takes(M, K, N)) {
@@ -82,7 +83,7 @@ int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K,
         }
         a.M = M; a.top_k = 1;
         const int tiles = (M + kTileRows - 1) / kTileRows;
-        if (tiles_take(a, glu, x_format, M, tiles, 1)) {
+        if (tiles_take(a, glu, M, tiles, 1)) {
             a.unit_rows = kTileRows;
             launch_moe_tiles(a, x_format, glu, tiles);
         } else {
@@ -97,16 +98,16 @@ int byhip_moe_matmul(const void* x, int x_format, const uint8_t* w, const byhip_
     return guard([&] {
         enter_compute();
         const MoePlan p = moe_plan_args(plan);
-        if (flags & ~(BYHIP_MOE_GATHER | BYHIP_MOE_SCATTER | BYHIP_MOE_SWIGLU)) fail("byhip: product flags %d", flags);
+        if (flags & ~(BYHIP_MOE_GATHER | BYHIP_MOE_SCATTER | BYHIP_MOE_SWIGLU | BYHIP_MOE_EXACT)) fail("byhip: product flags %d", flags);
         const bool glu = flags & BYHIP_MOE_SWIGLU, gather = flags & BYHIP_MOE_GATHER;
-        MoeArgs a = product_args(x, x_format, w, p.experts, gather ? p.tokens : p.rows, p.rows, K, N, glu, y, y_stride, y_dtype);
+        MoeArgs a = product_args(x, x_format, w, p.experts, gather ? p.tokens : p.rows, p.rows, K, N, flags, y, y_stride, y_dtype);
         if (p.rows == 0) return;
         a.order = p.order;
         a.top_k = p.top_k; a.gather = gather; a.scatter = (flags & BYHIP_MOE_SCATTER) != 0;
         a.experts = p.experts; a.rows = p.rows;
         a.per_token = (uint32_t)(((1ull << 32) + p.top_k - 1) / p.top_k);
         note_device_write(y);
-        if (tiles_take(a, glu, x_format, p.rows, p.max_tiles, p.experts)) {
+        if (tiles_take(a, glu, p.rows, p.max_tiles, p.experts)) {
             a.n_units = p.n_units + 1; a.units = p.tiles; a.max_units = p.max_tiles;
             a.unit_rows = kTileRows;
             launch_moe_tiles(a, x_format, glu, p.max_tiles);

@@ -12,8 +12,8 @@
 //
 // With rows in 8 bits and outputs of 16 bits or fewer, the instructions' cut (split_bytes) stays: 5e-6 to 1e-5 of a product's norm, less than a hundredth of the
 // rounding that follows. (Of outputs in 8 bits one in a thousand then takes the step next to its own: 0.0023 of their norm, where the steps' rounding is
-// 0.026.) It is more where large terms cancel. In two parts, as with fp32 outputs, they would take half as long again: 4096 tokens, 6 of 64 experts, 2048 to 1408,
-// 242 us for 153.
+// 0.026.) It is more where large terms cancel. In two parts, as with fp32 outputs and where the caller asks for it, they take half as long again: 4096 tokens, 6 of 64
+// experts, 2048 to 1408, 246 us for 157.
 //
 // A step's data goes straight into LDS (16 bytes per lane) while the step before multiplies: two slots, one barrier per step. The
 // order of the 16-byte pieces inside a row is turned by the row so that no cycle of the operand reads meets a bank twice.
@@ -109,10 +109,11 @@ __device__ __forceinline__ void write_block(const MoeArgs& a, bool there, size_t
     }
 }
 
-template <int XF, bool GLU, int YT>
+template <int XF, bool GLU, int YT, bool FINE>
 __global__ __launch_bounds__(256, 2) void moe_tiles(MoeArgs a) {
     typedef Lds<XF> L;
-    constexpr bool eight = L::eight, FINE = eight && YT == BYHIP_F32;
+    constexpr bool eight = L::eight;
+    static_assert(eight || !FINE, "rows in 4 bits are exact in one part");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[L::bytes];
     MoeUnit u;
     int strip;
@@ -256,7 +257,9 @@ __global__ __launch_bounds__(256, 2) void moe_tiles(MoeArgs a) {
 
 template <int XF, bool GLU, int YT>
 void launch_tiles(const MoeArgs& a, const dim3& grid) {
-    launch("moe_tiles", (moe_tiles<XF, GLU, YT>), grid, dim3(256), 0, a);
+    constexpr bool eight = XF == BYHIP_MXFP8_KM;
+    if (eight && a.parts) launch("moe_tiles", (moe_tiles<XF, GLU, YT, eight>), grid, dim3(256), 0, a);
+    else launch("moe_tiles", (moe_tiles<XF, GLU, YT, false>), grid, dim3(256), 0, a);
     BYHIP_LAUNCHED("moe_tiles");
 }
 template <int XF, bool GLU>

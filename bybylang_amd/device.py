@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 
 from . import _abi
-from ._abi import (BF16, F16, F32, MOE_GATHER, MOE_SCATTER, MOE_SIGMOID, MOE_SOFTMAX, MOE_SWIGLU, MXFP4_KM,
+from ._abi import (BF16, F16, F32, MOE_EXACT, MOE_GATHER, MOE_SCATTER, MOE_SIGMOID, MOE_SOFTMAX, MOE_SWIGLU, MXFP4_KM,
                    MXFP8_KM, NORM_LAYER, NORM_RMS, ROPE_BASE, ROPE_HALVES,
                    ROPE_LINEAR, ROPE_PAIRS, ROPE_PARTS, ROPE_PLAIN, HipBackendError, HipUnsupported,
                    check, load)
@@ -24,7 +24,7 @@ __all__ = ["DeviceBuffer", "Q4Weights", "init", "device_info", "synchronize", "s
            "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_BASE", "ROPE_PARTS", "NORM_RMS", "NORM_LAYER",
            "MXFP8_KM", "mx_bytes", "mx_quantize", "mx_matmul", "MoePlan", "MoeRouter", "moe_plan_bytes", "moe_route",
            "moe_plan", "moe_matmul", "moe_combine", "MOE_SOFTMAX", "MOE_SIGMOID", "MOE_GATHER", "MOE_SCATTER",
-           "MOE_SWIGLU"]
+           "MOE_SWIGLU", "MOE_EXACT"]
 
 _NP = {F32: np.float32, F16: np.float16, BF16: np.uint16}
 

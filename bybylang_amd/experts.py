@@ -22,15 +22,16 @@ class ExpertsBlock:
     """`experts` experts of `inner` values over rows of `width`, `top_k` per token, for up to `max_rows` rows a call.
 
     router [experts, width], up [experts, 2 inner, width] (gates, then ups, of each expert) and down [experts, width, inner]:
-    handles of matrices in 4 bits. norm: gammas of the RMS norm before the block; bias: fp32 [experts] added to the scores for the choice
-    only, or None."""
+    handles of matrices in 4 bits; rows are 8-bit ones throughout, the router's too. norm: gammas of the RMS norm before the block; bias: fp32 [experts] added to the scores for the choice
+    only, or None. exact: BYHIP_MOE_EXACT of the experts' products."""
 
     def __init__(self, router, up, down, norm, width: int, inner: int, experts: int, top_k: int, max_rows: int, eps: float = 1e-5,
                  score: int = _abi.MOE_SOFTMAX, bias=None, groups: int = 1, top_groups: int = 1, group_by: int = 1, renorm: bool = True,
-                 scale: float = 1.0):
+                 scale: float = 1.0, exact: bool = False):
         self.weights, self.width, self.inner, self.experts, self.top_k = (router, up, down), width, inner, experts, top_k
         self.norm = dev.Norm(_abi.NORM_RMS, eps, g.sessionUpload(gbHip, norm))
         self.router = dev.MoeRouter(score, None if bias is None else g.sessionUpload(gbHip, bias), groups, top_groups, group_by, renorm, scale)
+        self.exact = _abi.MOE_EXACT * exact
         self.max_rows, rows = max_rows, max_rows * top_k
         # A plan of fewer tokens may have shorter units, and more of them.
         self.plan_buffer = g.sessionAllocBytes(gbHip, max(dev.moe_plan_bytes(t, top_k, experts) for t in range(1, max_rows + 1)))
@@ -47,6 +48,6 @@ class ExpertsBlock:
         ok = g.sessionNormBlockMx(gbHip, x, T, D, None, None, h, 1.0, h, self.norm, self.xq, mx8)
         ok &= g.sessionMxMatmul(gbHip, self.xq, mx8, router, T, D, self.experts, self.logits)
         ok &= g.sessionMoeRoute(gbHip, self.logits, self.router, plan, self.ids, self.shares)
-        ok &= g.sessionMoeMatmul(gbHip, self.xq, mx8, up, plan, D, F, _abi.MOE_GATHER | _abi.MOE_SWIGLU, self.mid, mx8)
+        ok &= g.sessionMoeMatmul(gbHip, self.xq, mx8, up, plan, D, F, _abi.MOE_GATHER | _abi.MOE_SWIGLU | self.exact, self.mid, mx8)
         ok &= g.sessionMoeMatmul(gbHip, self.mid, mx8, down, plan, F, D, _abi.MOE_SCATTER, self.rows)
         return ok and g.sessionMoeCombine(gbHip, self.rows, D, plan, self.ids, self.shares, None, out)

@@ -488,11 +488,11 @@ def sessionMxQuantize(backend: GpuBackend, x: SessionHandle, M: int, K: int, y: 
 
 
 def sessionMxMatmul(backend: GpuBackend, x: SessionHandle, fmt: int, w: SessionHandle, M: int, K: int, N: int,
-                    y: SessionHandle, yFmt: int = _abi.F32, swiglu: bool = False) -> bool:
+                    y: SessionHandle, yFmt: int = _abi.F32, swiglu: bool = False, exact: bool = False) -> bool:
     """y = x . w^T of microscaled rows and a matrix in 4 bits."""
     _require_hip(backend)
-    return _encoded(load().byhip_mx_matmul(x.hipHandle, fmt, w.hipHandle, M, K, N, _abi.MOE_SWIGLU if swiglu else 0, y.hipHandle, N,
-                                           yFmt), "sessionMxMatmul")
+    return _encoded(load().byhip_mx_matmul(x.hipHandle, fmt, w.hipHandle, M, K, N, _abi.MOE_SWIGLU * swiglu | _abi.MOE_EXACT * exact,
+                                           y.hipHandle, N, yFmt), "sessionMxMatmul")
 
 
 def sessionMoeRoute(backend: GpuBackend, logits: SessionHandle, router, plan, ids: SessionHandle,

@@ -450,13 +450,14 @@ int byhip_mx_quantize(const void* x, size_t x_stride, int x_dtype, int M, int K,
 enum byhip_moe_flags {
     BYHIP_MOE_GATHER = 1,  /* x holds the tokens' rows (tokens of them); without it the plan's rows, in its order */
     BYHIP_MOE_SCATTER = 2, /* y's row a is assignment a's; without it y's row i is the plan's row i */
-    BYHIP_MOE_SWIGLU = 4   /* a matrix has 2 N rows, gates then ups: y = silu(gate) * up, silu(v) = v / (1 + exp(-v)) */
+    BYHIP_MOE_SWIGLU = 4,  /* a matrix has 2 N rows, gates then ups: y = silu(gate) * up, silu(v) = v / (1 + exp(-v)) */
+    BYHIP_MOE_EXACT = 16   /* every product enters its sum with fp32's precision (below) */
 };
 
-/* y [M, N] = x . w^T of microscaled rows and one matrix [N, K] (with BYHIP_MOE_SWIGLU, the only flag it takes,
- * [2 N, K]). y_dtype F32, F16, BF16, or microscaled rows again (N a multiple of 32, y_stride N). Sums are fp32, and every product enters
+/* y [M, N] = x . w^T of microscaled rows and one matrix [N, K] (with BYHIP_MOE_SWIGLU [2 N, K]; it takes that flag and
+ * BYHIP_MOE_EXACT). y_dtype F32, F16, BF16, or microscaled rows again (N a multiple of 32, y_stride N). Sums are fp32, and every product enters
  * them with fp32's precision but for one case: 8-bit rows, y not in fp32 and many rows per matrix (dozens). There products that are 2^-13 and less
- * of the largest of eight neighbours (in memory order) may be cut off; a caller to whom they matter takes y in fp32 and byhip_mx_quantize. */
+ * of the largest of eight neighbours (in memory order) may be cut off, unless BYHIP_MOE_EXACT asks for them, at up to 1.6 times the time. */
 int byhip_mx_matmul(const void* x, int x_format, const uint8_t* w, int M, int K, int N, int flags, void* y,
                     size_t y_stride, int y_dtype);
 

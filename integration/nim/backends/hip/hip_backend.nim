@@ -27,6 +27,7 @@ const
   BYHIP_MOE_GATHER* = 1.cint
   BYHIP_MOE_SCATTER* = 2.cint
   BYHIP_MOE_SWIGLU* = 4.cint
+  BYHIP_MOE_EXACT* = 16.cint
 
 # Attention over a paged cache: the descriptors of include/byhip.h, field by field.
 type
@@ -338,9 +339,9 @@ proc hipSessionMxQuantize*(x: pointer, M, K: int, y: pointer, fmt: cint): bool =
   rc == BYHIP_OK
 
 proc hipSessionMxMatmul*(x: pointer, fmt: cint, w: pointer, M, K, N: int, y: pointer,
-                         yFmt = BYHIP_F32, swiglu = false): bool =
-  let rc = byhip_mx_matmul(x, fmt, w, M.cint, K.cint, N.cint, (if swiglu: BYHIP_MOE_SWIGLU else: 0.cint),
-                           y, csize_t(N), yFmt)
+                         yFmt = BYHIP_F32, swiglu = false, exact = false): bool =
+  let flags = (if swiglu: BYHIP_MOE_SWIGLU else: 0.cint) or (if exact: BYHIP_MOE_EXACT else: 0.cint)
+  let rc = byhip_mx_matmul(x, fmt, w, M.cint, K.cint, N.cint, flags, y, csize_t(N), yFmt)
   hipCheck(rc, "sessionMxMatmul")
   rc == BYHIP_OK
 

@@ -1,5 +1,5 @@
-"""Products of 8-bit rows with few rows per matrix (moe_rows) enter sums with fp32's precision whatever the output's type, so that sums whose large terms cancel keep the
-small ones.
+"""Products of 8-bit rows enter sums with fp32's precision whatever the output's type, with few rows per matrix (moe_rows) always, with many (moe_tiles) where the caller asks
+for it, so that sums whose large terms cancel keep the small ones.
 
 Each eight neighbours of a row here (in memory order, which the instructions add first) hold 448, -448 under equal matrix values and six values below 1/2. The pair's
 products cancel exactly, so the bound is that of fp32 outputs (test_mx_gpu.py) for the six alone; a cut 13 bits below the pair's products would leave next to
@@ -14,7 +14,7 @@ from test_mx_gpu import agree, expected, mx_size
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = _abi.F32, _abi.F16, _abi.BF16
-GATHER, SCATTER, GLU = _abi.MOE_GATHER, _abi.MOE_SCATTER, _abi.MOE_SWIGLU
+GATHER, SCATTER, GLU, EXACT = _abi.MOE_GATHER, _abi.MOE_SCATTER, _abi.MOE_SWIGLU, _abi.MOE_EXACT
 
 
 def cancelling(g, M, R, K):
@@ -41,8 +41,33 @@ def test_one_matrix(hip, M, K, N, yt, glu):
     agree(y.read(np.uint8, n), want, slack, yt, M, N, N)
 
 
-@pytest.mark.parametrize("T,k,E,K,N", [(3, 2, 8, 2048, 64), (40, 4, 16, 512, 96)])
-@pytest.mark.parametrize("flags,yt", [(GATHER | GLU, MX8), (SCATTER, BF16), (0, F16)])
+@pytest.mark.parametrize("yt", [F16, BF16, MX8, MX4])
+@pytest.mark.parametrize("glu", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1541, 256, 2112)])
+def test_tiles(hip, M, K, N, yt, glu):
+    N = N // 2 if glu else N
+    g = synth.rng(K)
+    (xb, xv), (wb, wv) = cancelling(g, M, 2 * N if glu else N, K)
+    n = mx_size(M, N, yt) if yt in (MX8, MX4) else M * N * 2
+    y = hip.DeviceBuffer(n)
+    hip.mx_matmul(hip.DeviceBuffer.from_array(xb), MX8, hip.DeviceBuffer.from_array(wb), M, K, N, (GLU if glu else 0) | EXACT, y, N, yt)
+    want, slack = expected(xv, wv, N, K, glu, MX8, F32)
+    agree(y.read(np.uint8, n), want, slack, yt, M, N, N)
+
+
+def test_flags(hip):
+    """4-bit rows are exact as they are and take the flag too; the next bit is refused."""
+    g = synth.rng(2)
+    (xb, xv), (wb, wv) = random_rows(g, 3, 64, MX4), random_rows(g, 32, 64, MX4)
+    x, w, y = hip.DeviceBuffer.from_array(xb), hip.DeviceBuffer.from_array(wb), hip.DeviceBuffer(3 * 32 * 4)
+    hip.mx_matmul(x, MX4, w, 3, 64, 32, EXACT, y, 32, F32)
+    agree(y.read(np.uint8), *expected(xv, wv, 32, 64, False, MX4, F32), F32, 3, 32, 32)
+    with pytest.raises(_abi.HipBackendError, match="flags 32"):
+        hip.mx_matmul(x, MX4, w, 3, 64, 32, 32, y, 32, F32)
+
+
+@pytest.mark.parametrize("T,k,E,K,N", [(3, 2, 8, 2048, 64), (40, 4, 16, 512, 96), (900, 2, 3, 128, 1696)])
+@pytest.mark.parametrize("flags,yt", [(GATHER | GLU | EXACT, MX8), (SCATTER | EXACT, BF16), (EXACT, F16), (GATHER | GLU | EXACT, MX4)])
 def test_experts(hip, T, k, E, K, N, flags, yt):
     g = synth.rng(T)
     R = 2 * N if flags & GLU else N
@@ -53,7 +78,7 @@ def test_experts(hip, T, k, E, K, N, flags, yt):
     buf = hip.DeviceBuffer(hip.moe_plan_bytes(T, k, E))
     p = hip.MoePlan(buf, T, k, E)
     hip.moe_plan(up(ids), p)
-    n = mx_size(T * k, N, yt) if yt == MX8 else T * k * N * 2
+    n = mx_size(T * k, N, yt) if yt in (MX8, MX4) else T * k * N * 2
     y = hip.DeviceBuffer(n)
     hip.moe_matmul(up(xb), MX8, up(wb), p, K, N, flags, y, N, yt)
     offsets, order = plan(ids, E)

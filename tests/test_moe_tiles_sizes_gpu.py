@@ -30,6 +30,12 @@ def test_fp32_experts(hip, T, k, E, K, N, flags):
     check_product(hip, T, k, E, K, N, MX8, F32, flags, seed=T)
 
 
+@pytest.mark.parametrize("yt", [F16, MX8, MX4])
+@pytest.mark.parametrize("flags", [GATHER | GLU, SCATTER])
+def test_exact_experts(hip, flags, yt):
+    check_product(hip, 700, 3, 6, 256, 1568, MX8, yt, flags | _abi.MOE_EXACT, seed=1)
+
+
 @pytest.mark.parametrize("flags,yt", [(SCATTER, F32), (GLU | SCATTER, BF16), (GATHER | GLU, MX8)])
 def test_assignments_left_out(hip, flags, yt):
     g = synth.rng(3)
