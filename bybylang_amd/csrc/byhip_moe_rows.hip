@@ -3,7 +3,7 @@
 // Bound by the matrices' bytes. A block takes a strip of a matrix (64 of its rows) and one unit's rows; its four waves share
 // out the values' axis in windows of 512 (or 256) and add their sums in LDS at the end. A wave loads its window of the
 // strip in 16-byte pieces straight into the operands of v_mfma_scale_f32_16x16x128_f8f6f4, 16 KB in flight before the first
-// product, and the rows' values beside it (they come from L2: every strip of the expert reads them). Five waves per SIMD hide the latencies; loads
+// product, and the rows' values beside it (they come from L2: every strip of the expert reads them). Three waves per SIMD (six or seven with strips of 16) hide the latencies; loads
 // of the first window ahead of the rows' look-up, with the registers they take, cost more than they saved (48 us for 33, 48 tokens, 128 experts).
 //
 // Operands (checked on the device): the matrix is the first, in 4 bits: lane (c, g) = (l % 16, l / 16) holds the 32 values of
@@ -14,7 +14,7 @@
 //
 // Sums are fp32. What the instructions add in one go is exact with rows in 4 bits; with rows in 8 bits they cut small products off, so those rows go in two
 // parts (split_bytes), twice the products. With outputs of 16 bits or fewer one part would do for most rows (5e-6 to 1e-5 of a product's norm is cut off then), but not for
-// rows whose large terms cancel, and it saves little here (us, one part: 48 tokens, 128 experts, 2048 to 768 31.4 for 29.4, 800 to 2048 with 400 tokens
+// rows whose large terms cancel, and it saves little here (us, two parts for one: 48 tokens, 128 experts, 2048 to 768 31.4 for 29.4, 800 to 2048 with 400 tokens
 // 46 for 37; 1 / 16 / 64 rows of 4096 x 4096 5.1 / 5.8 / 10.8 for 4.8 / 5.5 / 9.9).
 #include "byhip_moe.h"
 

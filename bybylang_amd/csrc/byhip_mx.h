@@ -81,8 +81,9 @@ struct MoeUnit {
     int expert, first, rows, pad;
 };
 // Rows of a unit of moe_rows, by the mean rows per expert, so that most experts fill one: a unit's rows share one pass over the expert's
-// matrix, but 64 rows' own loads cost more than a second pass over it from the cache (64 / 128 / 256 rows, K = N = 4096: units of 32 12.4 / 15.3 /
-// 24.3 us, of 64 16.7 / 17.5 / 22.0). moe_tiles' units have kTileRows.
+// matrix, but 64 rows' own loads cost more than a second pass over it from the cache (us, one matrix of 4096 x 4096, 16 / 24 / 32 rows: units of 16 6.0 / 8.4 / 8.4, of 32 6.9 / 7.4 / 7.9;
+// 64 / 128 / 256 rows: units of 32 10.5 / 14.4 / 22.4, of 64 12.4 / 14.8 / 19.3; 16 experts, 2080 to 2048 gates and ups, 8 / 16 rows each: units of 16 21.6 / 28.0, of 32 24.9 / 28.5;
+// 128 / 192 rows each: of 32 82 / 117, of 64 82 / 105). moe_tiles' units have kTileRows.
 inline int moe_unit_rows(long long rows, int experts) {
     const long long mean = (rows + experts - 1) / experts;
     return mean <= 16 ? 16 : mean <= 128 ? 32 : 64;

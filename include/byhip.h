@@ -441,7 +441,8 @@ int byhip_norm_block(const void* x, size_t x_stride, int x_dtype, int M, int N, 
  * e (-127 or more) for which its largest magnitude is at most 448 2^e (8 bits) or 6 2^e (4 bits), its values are
  * rounded to the nearest, ties to even, so that none is clipped. A group that holds a NaN or an infinity gets the
  * scale byte 255, which stands for NaN. Matrices have the same form in 4 bits, one row per output. A product takes rows and
- * matrices (each expert's) of less than 2 GiB of values. */
+ * matrices (each expert's) of less than 2 GiB of values. What a call writes overlaps nothing that it reads, unless it is said
+ * to. */
 
 /* M rows of K values of x (F32, F16 or BF16, x_stride elements apart) as microscaled rows. */
 int byhip_mx_quantize(const void* x, size_t x_stride, int x_dtype, int M, int K, void* y, int y_format);

@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 
 from bybylang_amd import synth
+from bybylang_amd import _abi
+from test_experts_block_gpu import gb  # noqa: F401
 from test_moe_gpu import new_plan, read_plan
 
 pytestmark = pytest.mark.gpu
@@ -11,6 +13,10 @@ pytestmark = pytest.mark.gpu
 def check(hip, T, k, E, ids):
     buf, p = new_plan(hip, T, k, E)
     hip.moe_plan(hip.DeviceBuffer.from_array(ids), p)
+    agree(buf, T, k, E, ids)
+
+
+def agree(buf, T, k, E, ids):
     offsets, order = read_plan(buf, T, k, E)
     flat = ids.reshape(-1)
     key = np.where((flat >= 0) & (flat < E), flat, E)
@@ -38,9 +44,30 @@ def test_all_in_one_expert(hip):
     check(hip, 300000, 1, 300, np.full((300000, 1), -1, np.int32))
 
 
+@pytest.mark.parametrize("direct", [0, 1])
+@pytest.mark.parametrize("T,E", [(70000, 1024), (9000, 40)])
+def test_recorded(hip, gb, direct, T, E):  # noqa: F811
+    """A recorded plan follows the ids of each replay, with a plan of another size between."""
+    _abi.check(_abi.load().byhip_session_set_direct_replay(direct))
+    g = synth.rng(T)
+    all_ids = [g.integers(0, E, (T, 1)).astype(np.int32) for _ in range(3)]
+    ids = hip.DeviceBuffer.from_array(all_ids[0])
+    buf, p = new_plan(hip, T, 1, E)
+    assert gb.sessionBeginRecording(gb.gbHip)
+    hip.moe_plan(ids, p)
+    assert gb.sessionEnd(gb.gbHip)
+    step = gb.sessionLastRecording(gb.gbHip)
+    for turn in range(2):
+        for now in all_ids:
+            ids.upload(now)
+            check(hip, 5000, 2, 30, g.integers(0, 30, (5000, 2)).astype(np.int32))
+            assert gb.sessionReplay(gb.gbHip, step, 1)
+            agree(buf, T, 1, E, now)
+    gb.sessionFreeRecording(gb.gbHip, step)
+
+
 def test_units_of_a_large_plan(hip):
     """The products' units cover each expert's rows: outputs of ones count their inputs."""
-    from bybylang_amd import _abi
     T, E, K, N = 200000, 50, 32, 32
     ids = (synth.rng(5).integers(0, E, (T, 1))).astype(np.int32)
     up = hip.DeviceBuffer.from_array
